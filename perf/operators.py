@@ -72,7 +72,8 @@ def draw(rng):
     batch = _log(rng, 1, 64)
     # No case costs more than the listed ones: a bound on cached tokens and on (row, token) pairs.
     high = _log(rng, 16, 131072)
-    high = max(1, min(high, 500_000 // batch, (1 << 28) // (batch * q_high * kv_heads * shared)))
+    high = max(1, min(high, min(500_000, 3_200_000 // kv_heads) // batch,
+                      (1 << 28) // (batch * q_high * kv_heads * shared)))
     return {"kind": "attend", "batch": batch, "low": rng.randint(1, high), "high": high,
             "empty": rng.choice([0, 0, 1]) if batch > 1 else 0, "q_low": q_low, "q_high": q_high,
             "heads": kv_heads * shared, "kv_heads": kv_heads, "head_dim": rng.choice([64, 128]), "dtype": dtype,
