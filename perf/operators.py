@@ -68,12 +68,13 @@ def draw(rng):
     kv_heads = rng.choice([1, 2, 4, 8, 12])
     shared = rng.choice([1, 2, 4, 7, 8, 16])
     q_high = rng.choice([1, 1, 1, _log(rng, 2, 16), _log(rng, 17, 512)])
-    q_low = q_high if q_high == 1 or rng.random() < 0.3 else rng.randint(1, q_high)
     batch = _log(rng, 1, 64)
-    # No case costs more than the listed ones: a bound on cached tokens and on (row, token) pairs.
+    # No case costs more than the listed ones: bounds on rows, on cached tokens and on (row, token) pairs.
+    q_high = min(q_high, max(1, 700_000 // (batch * kv_heads * shared)))
+    q_low = q_high if q_high == 1 or rng.random() < 0.3 else rng.randint(1, q_high)
     high = _log(rng, 16, 131072)
     high = max(1, min(high, min(500_000, 3_200_000 // kv_heads) // batch,
-                      (1 << 28) // (batch * q_high * kv_heads * shared)))
+                      160_000_000 // (batch * q_high * kv_heads * shared)))
     return {"kind": "attend", "batch": batch, "low": rng.randint(1, high), "high": high,
             "empty": rng.choice([0, 0, 1]) if batch > 1 else 0, "q_low": q_low, "q_high": q_high,
             "heads": kv_heads * shared, "kv_heads": kv_heads, "head_dim": rng.choice([64, 128]), "dtype": dtype,
