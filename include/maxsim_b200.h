@@ -272,6 +272,97 @@ int msb_pack_signs_device(const float* x, int64_t n, int32_t dim, uint8_t* bits,
 int msb_docs_topk_device_noalloc(msb_docs* docs, const float* query, int32_t batch, int32_t query_tokens, int32_t k,
                                  const msb_score_opts* opts, float* out_scores, int64_t* out_ids, void* stream);
 
+/* ---- 4-bit key/value cache and 4-bit weights ----------------------------
+ * Operators of a reader model that answers from retrieved passages, in the
+ * code format of the int4 corpora (no counterpart in the reference).  All
+ * pointers are device pointers on `device`, work is enqueued on `stream`
+ * without synchronising, nothing is allocated, and calls can be captured into
+ * a graph.  Sizes are checked on the host; what device arrays hold (slots,
+ * page ids, lengths, offsets) is bounds-checked by the kernels. */
+#define MSB_TYPE_F32 0
+#define MSB_TYPE_F16 1
+#define MSB_TYPE_BF16 2
+
+/* Pages of page_size (a power of two, 16 to 1024) tokens.  A vector is one
+ * token's key or value of one head: head_dim (64, 128 or 256) codes in
+ * [-7, 7], even dimension in the low nibble, and an fp32 scale.  codes
+ * [num_pages, kv_heads, page_size, head_dim / 2], 16-byte aligned; scales
+ * [num_pages, kv_heads, page_size].  Slot s is token s % page_size of page
+ * s / page_size. */
+typedef struct msb_kv4_cache {
+  uint8_t* k_codes;
+  float* k_scales;
+  uint8_t* v_codes;
+  float* v_scales;
+  int64_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t device;
+} msb_kv4_cache;
+
+/* Quantises keys and values [tokens, kv_heads, head_dim] (fp32, fp16 or bf16;
+ * strides in elements, dimensions contiguous) into slots[tokens]: per vector
+ * scale = fl(max|x| * fl(1/7)) (0 -> 1), code = clip(rint(x / scale), -7, 7).
+ * A vector with an element that is not finite stores scale NaN and codes 0.  A slot outside the cache is not written
+ * (-1 skips a token); a slot given twice holds one of the two, scale and codes
+ * possibly mixed. */
+int msb_kv4_append_device(const msb_kv4_cache* cache, const void* keys, const void* values, int32_t type,
+                          int64_t tokens, int64_t key_token_stride, int64_t key_head_stride,
+                          int64_t value_token_stride, int64_t value_head_stride, const int64_t* slots, void* stream);
+/* Reads slots back: code * scale, rounded once to `type`, into contiguous
+ * [tokens, kv_heads, head_dim] arrays; zeros for a slot outside the cache. */
+int msb_kv4_read_device(const msb_kv4_cache* cache, const int64_t* slots, int64_t tokens, int32_t type, void* keys,
+                        void* values, void* stream);
+
+/* Attention of query rows over the cache.  Sequence b has lengths[b] cached
+ * tokens (page_table[b, j / page_size] holds token j) and query rows
+ * query_offsets[b] .. query_offsets[b + 1], its last positions; NULL offsets:
+ * one row each (rows == batch).  Row i sees tokens j < lengths[b], with
+ * `causal` those up to its own position lengths[b] - n + i, with `window` > 0
+ * the last `window` of these.  Query heads share key/value heads in groups of
+ * heads / kv_heads.  A row that sees nothing gives zeros (lse -inf).  A token
+ * on a page outside the cache is not seen.  Rows that no sequence owns, or
+ * past max_query_rows of one, are not written.  fp16 or bf16; softmax
+ * statistics and sums in fp32. */
+typedef struct msb_kv4_attend_args {
+  const void* query;            /* [rows, heads, head_dim], strides in elements */
+  int64_t query_row_stride;
+  int64_t query_head_stride;
+  int64_t rows;
+  const int32_t* page_table;    /* [batch, max_pages], rows page_table_stride apart */
+  int64_t page_table_stride;
+  const int32_t* lengths;       /* [batch] */
+  const int32_t* query_offsets; /* [batch + 1] or NULL */
+  void* out;                    /* [rows, heads, head_dim] */
+  float* lse;                   /* [rows, heads] natural log-sum-exp, or NULL */
+  void* workspace;              /* msb_kv4_attend_workspace_bytes, 16-byte aligned; one call at a time */
+  int64_t workspace_bytes;
+  int32_t batch;
+  int32_t max_pages;
+  int32_t max_query_rows;
+  int32_t heads;
+  int32_t type;
+  int32_t causal;
+  int32_t window;
+  float scale;
+} msb_kv4_attend_args;
+int msb_kv4_attend_workspace_bytes(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, int64_t* bytes);
+int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream);
+
+/* Weights [n, k] as int4 codes [n, k / 2] with one bfloat16 scale per row and
+ * `group` (32, 64 or 128) inputs, [n, ceil(k / group)]; k a multiple of 8.
+ * msb_w4_pack_device lays them out once for the product kernel, into buffers
+ * of the sizes msb_w4_packed_bytes names. */
+int msb_w4_packed_bytes(int64_t n, int64_t k, int32_t group, int64_t* code_bytes, int64_t* scale_bytes);
+int msb_w4_pack_device(const uint8_t* codes, const void* scales, int64_t n, int64_t k, int32_t group,
+                       void* packed_codes, void* packed_scales, void* stream);
+/* y [rows, n] = x [rows, k] W^T + bias: fp16 or bf16 in and out, summed in fp32
+ * (strides of x and y rows in elements; bias [n] of the same type, or NULL). */
+int msb_w4_product_device(const void* packed_codes, const void* packed_scales, int64_t n, int64_t k, int32_t group,
+                          const void* x, int64_t x_stride, int64_t rows, const void* bias, void* y, int64_t y_stride,
+                          int32_t type, int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,9 +3,11 @@
 Drop-in for the reference ``maxsim`` package's GPU path: the same public names
 (``Index``/``Corpus``, ``Reranker``, ``SearchResult``, ``pack_signs``,
 ``to_device``, ``score``, ``maxsim``, ``topk_maxsim``, the residual cascade
-API) over ``libmaxsim_b200.so``.  ``maxsim_b200._maxsim_cuda`` reproduces the
-reference's native extension module and can be installed as
-``maxsim._maxsim_cuda``.
+API) over ``libmaxsim_b200.so``; beside it, for a reader model that answers
+from what was retrieved, a key/value cache in the same 4-bit codes
+(``Int4KVCache``) and products with 4-bit weights (``Int4Linear``).
+``maxsim_b200._maxsim_cuda`` reproduces the reference's native extension module
+and can be installed as ``maxsim._maxsim_cuda``.
 
 Importing the package loads the CUDA library; it fails loudly when the library
 has not been built -- there is no CPU fallback.
@@ -43,6 +45,7 @@ from maxsim_b200.experimental import (
 )
 from maxsim_b200.sdk import MODE_PRESETS, Corpus, CorpusMemoryReport, Index, Reranker, SearchResult
 from maxsim_b200.loader import load_reranker, load_resident_corpus
+from maxsim_b200.generation import Int4KVCache, Int4Linear
 
 __all__ = [
     "PackedDocs",
@@ -84,4 +87,6 @@ __all__ = [
     "binary_prefix_score",
     "binary_residual_score",
     "binary_cascade_topk",
+    "Int4KVCache",
+    "Int4Linear",
 ]

@@ -29,6 +29,9 @@ ARRAY_CODES = 0
 ARRAY_TOKEN_SCALES = 1
 ARRAY_RESIDUAL_CODES = 2
 ARRAY_RESIDUAL_TOKEN_SCALES = 3
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
 QUERY_F32 = 0
 QUERY_I8 = 1
 REDUCER_IDS = {"maxsim": 0, "weighted_maxsim": 1, "topk2": 2, "topk4": 3, "smoothsim": 4}
@@ -64,6 +67,45 @@ class DocsInfo(ctypes.Structure):
         ("device", ctypes.c_int32),
         ("resident_bytes", ctypes.c_int64),
         ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+    ]
+
+
+class Kv4AttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", ctypes.c_void_p),
+        ("query_row_stride", ctypes.c_int64),
+        ("query_head_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("query_offsets", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("max_query_rows", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
     ]
 
 
@@ -108,6 +150,16 @@ SIGNATURES = {
     "msb_quantize_query_int8_device": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp]),
     "msb_pack_int4_device": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _vp, ctypes.POINTER(_f32), _vp]),
     "msb_pack_signs_device": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp]),
+    "msb_kv4_append_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64,
+                                             _vp, _vp]),
+    "msb_kv4_read_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), _vp, _i64, _i32, _vp, _vp, _vp]),
+    "msb_kv4_attend_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs),
+                                                      ctypes.POINTER(_i64)]),
+    "msb_kv4_attend_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs), _vp]),
+    "msb_w4_packed_bytes": (ctypes.c_int, [_i64, _i64, _i32, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
+    "msb_w4_pack_device": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "msb_w4_product_device": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32,
+                                             _vp]),
 }
 
 

@@ -14,6 +14,7 @@
 
 #include "../../include/maxsim_b200.h"
 #include "common.cuh"
+#include "quant4.cuh"
 
 namespace msb {
 void launch_simt_scan(const DocsView&, const QueryView&, const ReduceView&, const TargetsView&, bool, float*,
@@ -46,6 +47,12 @@ void launch_popc_scan(const DocsView&, const QueryView&, const ReduceView&, cons
 void launch_expand_codes8(const uint8_t* codes, int64_t num_tokens, uint8_t* out, cudaStream_t);
 void launch_expand_binary8(const uint8_t* codes, int64_t num_tokens, uint8_t* out, cudaStream_t);
 void launch_expand_codes16(const uint8_t* codes, int64_t num_tokens, uint16_t* out, cudaStream_t);
+void launch_kv4_append(const Kv4View&, const Kv4Append&, cudaStream_t);
+void launch_kv4_read(const Kv4View&, const Kv4Read&, cudaStream_t);
+size_t kv4_attend_workspace_bytes(const Kv4View&, const Kv4Attend&);
+void launch_kv4_attend(const Kv4View&, const Kv4Attend&, cudaStream_t);
+void launch_w4_pack(const uint8_t*, const uint16_t*, int64_t, int64_t, int, uint8_t*, uint16_t*, cudaStream_t);
+void launch_w4_product(const W4View&, const W4Product&, cudaStream_t);
 void set_tc_row_replicas(int on);
 int get_tc_row_replicas();
 
@@ -1450,3 +1457,195 @@ extern "C" int msb_docs_topk_device_noalloc(msb_docs* h, const float* query, int
     launch_topk_rows(scores, h->num_docs, batch, h->num_docs, k, nullptr, false, out_scores, out_ids, s);
   });
 }
+
+// ---------------------------------------------------------------------------
+// 4-bit key/value cache and 4-bit weights
+// ---------------------------------------------------------------------------
+namespace {
+
+Kv4View kv4_view(const msb_kv4_cache* c) {
+  if (!c) throw InvalidArgument("cache is NULL");
+  if (!c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales) throw InvalidArgument("a cache array is NULL");
+  if (c->num_pages < 1 || c->kv_heads < 1) throw InvalidArgument("num_pages and kv_heads must be positive");
+  if (c->num_pages > (int64_t{1} << 31) - 1) throw InvalidArgument("num_pages must be below 2^31");
+  if (c->kv_heads > 65535) throw InvalidArgument("kv_heads must be at most 65535");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    throw InvalidArgument("head_dim must be 64, 128 or 256");
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+    throw InvalidArgument("page_size must be a power of two from 16 to 1024");
+  if ((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15)
+    throw InvalidArgument("cache codes must be 16-byte aligned");
+  Kv4View v{};
+  v.codes[0] = c->k_codes;
+  v.codes[1] = c->v_codes;
+  v.scales[0] = c->k_scales;
+  v.scales[1] = c->v_scales;
+  v.num_pages = c->num_pages;
+  for (v.page_shift = 4; (1 << v.page_shift) < c->page_size;) ++v.page_shift;
+  v.heads = c->kv_heads;
+  v.dim = c->head_dim;
+  return v;
+}
+
+int element_type(int32_t type, bool f32) {
+  if (type == MSB_TYPE_F16) return kElemF16;
+  if (type == MSB_TYPE_BF16) return kElemBF16;
+  if (type == MSB_TYPE_F32 && f32) return kElemF32;
+  throw InvalidArgument(f32 ? "type must be fp32, fp16 or bf16" : "type must be fp16 or bf16");
+}
+
+Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
+  if (!a) throw InvalidArgument("arguments are NULL");
+  if (a->rows < 0 || a->batch < 0 || a->max_pages < 0 || a->max_query_rows < 0)
+    throw InvalidArgument("sizes must not be negative");
+  if (a->rows > (int64_t{1} << 31) - 1) throw InvalidArgument("rows must be below 2^31");
+  if (a->heads < 1 || a->heads % c.heads) throw InvalidArgument("heads must be a positive multiple of kv_heads");
+  if ((static_cast<int64_t>(a->max_pages) << c.page_shift) > (int64_t{1} << 31) - 1)
+    throw InvalidArgument("max_pages * page_size must be below 2^31");
+  if (!a->query_offsets && a->rows != a->batch) throw InvalidArgument("without query_offsets rows must equal batch");
+  if (!(a->scale > 0.0F) || !std::isfinite(a->scale)) throw InvalidArgument("scale must be finite and > 0");
+  if (a->window < 0) throw InvalidArgument("window must not be negative");
+  if (a->window > 0 && !a->causal) throw InvalidArgument("window needs causal");
+  Kv4Attend r{};
+  r.type = element_type(a->type, false);
+  r.query = a->query;
+  r.q_row_stride = a->query_row_stride;
+  r.q_head_stride = a->query_head_stride;
+  r.rows = a->rows;
+  r.heads = a->heads;
+  r.page_table = a->page_table;
+  r.table_stride = a->page_table_stride;
+  r.max_pages = a->max_pages;
+  r.lengths = a->lengths;
+  r.offsets = a->query_offsets;
+  r.batch = a->batch;
+  r.max_rows = a->query_offsets ? a->max_query_rows : 1;
+  r.scale = a->scale;
+  r.causal = a->causal != 0;
+  r.window = a->window;
+  r.out = a->out;
+  r.lse = a->lse;
+  r.workspace = a->workspace;
+  r.workspace_bytes = a->workspace_bytes > 0 ? static_cast<size_t>(a->workspace_bytes) : 0;
+  return r;
+}
+
+void check_w4(int64_t n, int64_t k, int32_t group) {
+  if (n < 1 || k < 8 || k % 8) throw InvalidArgument("n must be positive and k a positive multiple of 8");
+  if (group != 32 && group != 64 && group != 128) throw InvalidArgument("group must be 32, 64 or 128");
+  if (n > (int64_t{1} << 31) - 64 || k > (int64_t{1} << 31) - 64) throw InvalidArgument("n and k must be below 2^31");
+}
+
+}  // namespace
+
+extern "C" {
+
+int msb_kv4_append_device(const msb_kv4_cache* cache, const void* keys, const void* values, int32_t type,
+                          int64_t tokens, int64_t key_token_stride, int64_t key_head_stride,
+                          int64_t value_token_stride, int64_t value_head_stride, const int64_t* slots, void* stream) {
+  return guarded([&] {
+    const Kv4View v = kv4_view(cache);
+    Kv4Append a{};
+    a.type = element_type(type, true);
+    if (tokens < 0) throw InvalidArgument("tokens must not be negative");
+    if (tokens == 0) return;
+    if (!keys || !values || !slots) throw InvalidArgument("NULL argument");
+    a.x[0] = keys;
+    a.x[1] = values;
+    a.token_stride[0] = key_token_stride;
+    a.token_stride[1] = value_token_stride;
+    a.head_stride[0] = key_head_stride;
+    a.head_stride[1] = value_head_stride;
+    a.slots = slots;
+    a.tokens = tokens;
+    DeviceGuard g(cache->device);
+    launch_kv4_append(v, a, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_kv4_read_device(const msb_kv4_cache* cache, const int64_t* slots, int64_t tokens, int32_t type, void* keys,
+                        void* values, void* stream) {
+  return guarded([&] {
+    const Kv4View v = kv4_view(cache);
+    Kv4Read a{};
+    a.type = element_type(type, true);
+    if (tokens < 0) throw InvalidArgument("tokens must not be negative");
+    if (tokens == 0) return;
+    if (!keys || !values || !slots) throw InvalidArgument("NULL argument");
+    a.out[0] = keys;
+    a.out[1] = values;
+    a.slots = slots;
+    a.tokens = tokens;
+    DeviceGuard g(cache->device);
+    launch_kv4_read(v, a, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_kv4_attend_workspace_bytes(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, int64_t* bytes) {
+  return guarded([&] {
+    if (!bytes) throw InvalidArgument("NULL argument");
+    const Kv4View v = kv4_view(cache);
+    DeviceGuard g(cache->device);
+    *bytes = static_cast<int64_t>(kv4_attend_workspace_bytes(v, kv4_attend(v, args)));
+  });
+}
+
+int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream) {
+  return guarded([&] {
+    const Kv4View v = kv4_view(cache);
+    const Kv4Attend a = kv4_attend(v, args);
+    if (a.rows == 0 || a.batch == 0) return;
+    if (!a.query || !a.lengths || !a.out || (a.max_pages > 0 && !a.page_table)) throw InvalidArgument("NULL argument");
+    DeviceGuard g(cache->device);
+    if (a.workspace_bytes < kv4_attend_workspace_bytes(v, a)) throw InvalidArgument("workspace is too small");
+    launch_kv4_attend(v, a, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_w4_packed_bytes(int64_t n, int64_t k, int32_t group, int64_t* code_bytes, int64_t* scale_bytes) {
+  return guarded([&] {
+    check_w4(n, k, group);
+    if (!code_bytes || !scale_bytes) throw InvalidArgument("NULL argument");
+    *code_bytes = ((n + 15) / 16) * ((k + 63) / 64) * 512;
+    *scale_bytes = ((n + 15) / 16) * ((k + group - 1) / group) * 32;
+  });
+}
+
+int msb_w4_pack_device(const uint8_t* codes, const void* scales, int64_t n, int64_t k, int32_t group,
+                       void* packed_codes, void* packed_scales, void* stream) {
+  return guarded([&] {
+    check_w4(n, k, group);
+    if (!codes || !scales || !packed_codes || !packed_scales) throw InvalidArgument("NULL argument");
+    launch_w4_pack(codes, static_cast<const uint16_t*>(scales), n, k, group, static_cast<uint8_t*>(packed_codes),
+                   static_cast<uint16_t*>(packed_scales), static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_w4_product_device(const void* packed_codes, const void* packed_scales, int64_t n, int64_t k, int32_t group,
+                          const void* x, int64_t x_stride, int64_t rows, const void* bias, void* y, int64_t y_stride,
+                          int32_t type, int32_t device, void* stream) {
+  return guarded([&] {
+    check_w4(n, k, group);
+    W4Product p{};
+    p.type = element_type(type, false);
+    if (rows < 0) throw InvalidArgument("rows must not be negative");
+    if (rows == 0) return;
+    if (!packed_codes || !packed_scales || !x || !y) throw InvalidArgument("NULL argument");
+    W4View w{};
+    w.codes = static_cast<const uint8_t*>(packed_codes);
+    w.scales = static_cast<const uint16_t*>(packed_scales);
+    w.n = n;
+    w.k = k;
+    w.group = group;
+    p.x = x;
+    p.x_stride = x_stride;
+    p.rows = rows;
+    p.bias = bias;
+    p.y = y;
+    p.y_stride = y_stride;
+    DeviceGuard g(device);
+    launch_w4_product(w, p, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,120 @@
+// What the kernels of the 4-bit key/value cache and of the 4-bit weights share: element types, the cache's
+// addressing and the host-side argument blocks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace msb {
+
+enum ElementType : int { kElemF32 = 0, kElemF16 = 1, kElemBF16 = 2 };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Pages of `page_size` (a power of two) tokens: codes [pages, heads, page_size, dim / 2], scales
+// [pages, heads, page_size].  Slot s is token s % page_size of page s / page_size.
+struct Kv4View {
+  uint8_t* codes[2];   // keys, values
+  float* scales[2];
+  int64_t num_pages;
+  int page_shift;      // log2(page_size)
+  int heads;
+  int dim;
+  // Index of a token's vector of one head, in vectors (64 bits: caches pass 2^31 vectors and 4 GB).
+  __host__ __device__ __forceinline__ int64_t vector(int64_t page, int head, int at) const {
+    return (((page * heads) + head) << page_shift) + at;
+  }
+};
+
+struct Kv4Append {
+  const void* x[2];           // keys, values [tokens, heads, dim]
+  int64_t token_stride[2];    // in elements
+  int64_t head_stride[2];
+  const int64_t* slots;       // [tokens]; outside the cache: not written
+  int64_t tokens;
+  int type;
+};
+
+struct Kv4Read {
+  void* out[2];               // [tokens, heads, dim], contiguous
+  const int64_t* slots;       // outside the cache: zeros
+  int64_t tokens;
+  int type;
+};
+
+struct Kv4Attend {
+  const void* query;          // [rows, heads, dim]
+  int64_t q_row_stride, q_head_stride;
+  int64_t rows;               // query rows of all sequences
+  int heads;                  // query heads, a multiple of the cache's
+  const int32_t* page_table;  // [batch, max_pages]
+  int64_t table_stride;
+  int max_pages;
+  const int32_t* lengths;     // [batch] cached tokens
+  const int32_t* offsets;     // [batch + 1] rows of each sequence, or nullptr: one row each
+  int batch;
+  int max_rows;               // the most rows of one sequence
+  float scale;
+  int causal;
+  int window;                 // 0: none
+  void* out;                  // [rows, heads, dim], contiguous
+  float* lse;                 // [rows, heads] or nullptr
+  void* workspace;
+  size_t workspace_bytes;
+  int type;
+};
+
+// One sequence of an attention call, with what the device arrays say held to what the call can read:
+// lengths to the table's pages, rows to the query's rows and the announced maximum.
+struct Kv4Sequence {
+  int64_t row0;
+  int rows;
+  int length;
+};
+__device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page_shift, int b) {
+  Kv4Sequence s;
+  const int64_t most = static_cast<int64_t>(a.max_pages) << page_shift;
+  s.length = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(a.lengths[b]), most)));
+  if (a.offsets == nullptr) {
+    s.row0 = b;
+    s.rows = 1;
+  } else {
+    const int64_t lo = max(0, a.offsets[b]);
+    const int64_t hi = min(static_cast<int64_t>(a.offsets[b + 1]), a.rows);
+    s.row0 = lo;
+    s.rows = static_cast<int>(max(static_cast<int64_t>(0), min(hi - lo, static_cast<int64_t>(a.max_rows))));
+  }
+  return s;
+}
+
+struct W4View {
+  const uint8_t* codes;       // packed, see w4.cu
+  const uint16_t* scales;     // bfloat16 bits [row tiles, groups, 16]
+  int64_t n;
+  int64_t k;
+  int group;
+};
+
+struct W4Product {
+  const void* x;              // [rows, k]
+  int64_t x_stride;
+  int64_t rows;
+  const void* bias;           // [n] or nullptr
+  void* y;                    // [rows, n]
+  int64_t y_stride;
+  int type;
+};
+
+}  // namespace msb
