@@ -28,6 +28,7 @@
 //   A segment cut by a range's end leaves partial sums in the workspace (at most two per block), which
 //   kv4_join_kernel adds in a fixed order; it is launched early (programmatic dependent launch).
 #include <algorithm>
+#include <atomic>
 
 #include "quant4.cuh"
 
@@ -37,6 +38,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStep = 32;              // tokens a warp takes at a time
 constexpr int kTile = kWarps * kStep;  // tokens of one unit of the work line
+constexpr int kExponents = 110;        // powers of two that scales and queries are brought back from
 constexpr float kLift = 8.0F;          // references lie 2^8 below the maximum: probabilities of 2^-22 are normal in fp16
 
 template <class T>
@@ -76,19 +78,20 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[kWords], const uint8_t*
   }
 }
 
-// fp16 pair 72 + code of nibbles i and i + 4 of a word.
+// Nibbles kI and kI + 4 of a word as the fp16 pair 72 + code.
 template <int kI>
 __device__ __forceinline__ uint32_t codes_plus72(uint32_t w) {
-  const uint32_t at = kI == 0 ? w << 4 : w >> (4 * kI - 4);
   uint32_t r;
-  asm("lop3.b32 %0, %1, 0x00f000f0, 0x54805480, 0x6a;" : "=r"(r) : "r"(at));  // (a & b) ^ c
+  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0x6a;"  // (a & b) ^ c
+      : "=r"(r)
+      : "r"(kI == 0 ? w << 4 : w >> (4 * kI - 4)), "r"(0x54805480u));
   return r;
 }
+// The same pair, exact.
 template <int kI>
 __device__ __forceinline__ uint32_t codes_exact(uint32_t w) {
-  const uint32_t v = codes_plus72<kI>(w);
   uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x54805480u));  // 0x5480 is 72
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(codes_plus72<kI>(w)), "r"(0x54805480u));
   return r;
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -96,6 +99,22 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// kN consecutive elements as fp32.
+template <int kN, class T>
+__device__ __forceinline__ void load_row(float (&x)[kN], const T* p, bool aligned) {
+  if (aligned) {
+#pragma unroll
+    for (int d = 0; d < kN; d += 8) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + d);
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[d + i] = to_f32(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int d = 0; d < kN; ++d) x[d] = to_f32(p[d]);
+  }
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -121,7 +140,7 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // Exponent of a scale (the e of 2^(e + [0, 1))), held to +-110.
 __device__ __forceinline__ float scale_exponent(float s) {
   const int e = static_cast<int>((__float_as_uint(s) >> 23) & 255) - 127;
-  return static_cast<float>(max(-110, min(110, e)));
+  return static_cast<float>(max(-kExponents, min(kExponents, e)));
 }
 
 // The work line: units of kTile tokens of every (sequence, key/value head, row block).
@@ -130,10 +149,11 @@ struct Line {
   int shared;       // query heads per cache head
   int block_rows;   // rows of a row block
   int page_shift;
+  int aligned;      // query rows of every head start on 16 bytes
 };
 struct SequenceWork {
   Kv4Sequence q;
-  int begin;        // first token that a row may see, down to a multiple of 16
+  int begin;        // first token that a row may see, down to a multiple of kStep
   int tiles;        // units of one segment
   int blocks;       // row blocks
   __device__ __forceinline__ int64_t units(const Line& l) const {
@@ -144,25 +164,25 @@ __device__ __forceinline__ SequenceWork sequence_work(const Kv4Attend& a, const 
   SequenceWork w;
   w.q = kv4_sequence(a, l.page_shift, b);
   w.begin = 0;
-  if (a.window > 0) w.begin = max(0, max(0, w.q.length - w.q.rows) - a.window + 1) & ~15;
+  if (a.window > 0) w.begin = max(0, max(0, w.q.length - w.q.rows) - a.window + 1) & ~(kStep - 1);
   // A sequence of no tokens keeps one empty unit: its rows are written as zeros.
   w.tiles = max(1, (w.q.length - w.begin + kTile - 1) / kTile);
   w.blocks = (w.q.rows * l.shared + l.block_rows - 1) / l.block_rows;
   return w;
 }
 
-// Units of all sequences, and those before sequence b: every thread of the block gets both.  kWarps * 32
-// sequences at a time.
+// Units of all sequences, and those before sequence b: every thread of the block gets both.  as many
+// sequences at a time as the block has threads.
 struct Place {
   int64_t total;
   int64_t before;   // units before the found sequence
   int sequence;
 };
 // Finds the sequence that holds unit (range start) `first(total)`, or sums up to sequence `want` if want >= 0.
-template <class F>
+template <int kWarpsHere, class F>
 __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, int want, F first, int64_t* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int kBlock = kWarps * 32;
+  constexpr int kBlock = kWarpsHere * 32;
   int64_t mine = 0, total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kBlock) {
     mine = b0 + threadIdx.x < a.batch ? sequence_work(a, l, b0 + threadIdx.x).units(l) : 0;
@@ -174,7 +194,7 @@ __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, i
   __syncthreads();
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += scratch[w];
+  for (int w = 0; w < kWarpsHere; ++w) total += scratch[w];
   Place p{total, 0, want >= 0 ? want : a.batch};
   const int64_t target = want >= 0 ? -1 : first(total);
   int64_t carry = 0;
@@ -188,24 +208,24 @@ __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, i
     }
     __syncthreads();
     if (lane == 31) scratch[warp] = upto;
-    if (threadIdx.x == 0) scratch[kWarps] = -1;
+    if (threadIdx.x == 0) scratch[kWarpsHere] = -1;
     __syncthreads();
     int64_t base = carry, chunk = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kWarpsHere; ++w) {
       if (w < warp) base += scratch[w];
       chunk += scratch[w];
     }
     const int64_t before = base + upto - mine;
     const bool hit = want >= 0 ? b0 + static_cast<int>(threadIdx.x) == want : target >= before && target < before + mine;
     if (hit) {
-      scratch[kWarps] = before;
-      scratch[kWarps + 1] = b0 + threadIdx.x;
+      scratch[kWarpsHere] = before;
+      scratch[kWarpsHere + 1] = b0 + threadIdx.x;
     }
     __syncthreads();
-    if (scratch[kWarps] >= 0) {
-      p.before = scratch[kWarps];
-      p.sequence = static_cast<int>(scratch[kWarps + 1]);
+    if (scratch[kWarpsHere] >= 0) {
+      p.before = scratch[kWarpsHere];
+      p.sequence = static_cast<int>(scratch[kWarpsHere + 1]);
       break;
     }
     carry += chunk;
@@ -224,8 +244,13 @@ __device__ __forceinline__ int64_t range_of(int64_t total, int64_t u, int64_t n)
 // Partial sums of one segment's row block: rows x dim unnormalised outputs, then (reference, sum) per row.
 __host__ __device__ constexpr int partial_floats(int rows, int dim) { return rows * dim + 2 * rows; }
 
+// Resident blocks per SM that the registers are held to (128 threads, 65,536 registers).
+__host__ __device__ constexpr int resident_blocks(int dim, int tiles) {
+  return dim == 256 ? 2 : dim == 128 ? (tiles == 1 ? 4 : 2) : (tiles == 1 ? 4 : 3);
+}
+
 template <class T, int kDim, int kTiles>
-__global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4Attend a, Line line) {
+__global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv4_attend_kernel(Kv4View c, Kv4Attend a, Line line) {
   constexpr int kRows = 8 * kTiles;      // rows of a row block
   constexpr int kKeyWords = kDim / 32;   // of one token, per lane
   constexpr int kValueWords = kDim / 64;
@@ -237,7 +262,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4A
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
 
   const int64_t block = blockIdx.x;
-  const Place place = find_place(
+  const Place place = find_place<kWarps>(
       a, line, -1, [&](int64_t total) { return range_start(total, block, ranges(total, gridDim.x)); }, scratch);
   const int64_t n = ranges(place.total, gridDim.x);
 #if __CUDA_ARCH__ >= 900
@@ -266,29 +291,27 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4A
 
     // Queries: lane (g, t) holds row g of each column tile, dimensions t * kDim / 4 and on.
     uint32_t q[kTiles][2 * kKeyWords][2];
-    float lift[kTiles][2];   // -72 sum(q) of columns 2t, 2t + 1
-    float factor[kTiles][2]; // scale * log2(e) * the row's power of two
+    float2 lift[kTiles];     // -72 sum(q) of columns 2t, 2t + 1
+    float2 factor[kTiles];   // scale * log2(e) * the row's power of two
     int last[kTiles][2], first[kTiles][2];  // tokens that columns 2t, 2t + 1 see: first <= j <= last
     int every_last = INT_MAX, every_first = 0, any_last = -1, any_first = INT_MAX;
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int r = row0 + nt * 8 + g;
       float x[kKeyWords * 8], top = 0.0F;
+#pragma unroll
+      for (int d = 0; d < kKeyWords * 8; ++d) x[d] = 0.0F;
       if (r < all_rows) {
         const T* p = static_cast<const T*>(a.query) + (w.q.row0 + r / line.shared) * a.q_row_stride +
                      static_cast<int64_t>(head * line.shared + r % line.shared) * a.q_head_stride + t * (kDim / 4);
-#pragma unroll
-        for (int d = 0; d < kKeyWords * 8; ++d) x[d] = to_f32(p[d]);
-      } else {
-#pragma unroll
-        for (int d = 0; d < kKeyWords * 8; ++d) x[d] = 0.0F;
+        load_row<kKeyWords * 8>(x, p, line.aligned);
       }
 #pragma unroll
       for (int d = 0; d < kKeyWords * 8; ++d) top = fmaxf(top, fabsf(x[d]));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const int e = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      const int e = max(-kExponents, min(kExponents, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
       float sum = 0.0F;
 #pragma unroll
       for (int word = 0; word < kKeyWords; ++word) {
@@ -302,11 +325,13 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4A
       }
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
       sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-      const float up = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      sum *= -72.0F;
+      const float up = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
+      // from the lanes that hold rows 2t, 2t + 1 to the columns' lanes
+      lift[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, sum, 8 * t), __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4));
+      factor[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, up, 8 * t), __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4));
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {  // from the lanes that hold row 2t + k to the column's lanes
-        lift[nt][k] = -72.0F * __shfl_sync(0xFFFFFFFFu, sum, 4 * (2 * t + k));
-        factor[nt][k] = __shfl_sync(0xFFFFFFFFu, up, 4 * (2 * t + k));
+      for (int k = 0; k < 2; ++k) {
         const int rr = row0 + nt * 8 + 2 * t + k;
         first[nt][k] = 0;
         last[nt][k] = INT_MAX;  // rows past the block are not written: no reason to mask for them
@@ -330,67 +355,84 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4A
     }
 
     float o[kOut][kTiles][4];
-    float top[kTiles][2], sum[kTiles][2];
+    float top[kTiles][2];
+    float2 sum[kTiles];
 #pragma unroll
-    for (int i = 0; i < kOut; ++i)
+    for (int nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
-      for (int nt = 0; nt < kTiles; ++nt)
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.0F;
-#pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) top[nt][0] = top[nt][1] = -INFINITY, sum[nt][0] = sum[nt][1] = 0.0F;
+        for (int i = 0; i < kOut; ++i) o[i][nt][k] = 0.0F;
+      top[nt][0] = top[nt][1] = -INFINITY;
+      sum[nt] = make_float2(0.0F, 0.0F);
+    }
 
     // This warp's steps of 32 tokens, those that some row sees.
-    const int from = w.begin + tile0 * kTile, upto = min(w.begin + tile1 * kTile, any_last + 1);
-    int j0 = from + warp * kStep;
+    const int upto = min(w.begin + tile1 * kTile, any_last + 1);
+    int j0 = w.begin + tile0 * kTile + warp * kStep;
     if (any_first > j0) j0 += (any_first - j0) / kTile * kTile;
 
+    const int32_t* pages = a.page_table + b * a.table_stride;
+    const uint8_t* lane_keys = c.codes[0] + g * (kDim / 2) + t * (kDim / 8);
+    const uint8_t* lane_values = c.codes[1] + 2 * t * (kDim / 2) + g * (kDim / 16);
     uint32_t key[2][2][kKeyWords], value[2][4][kValueWords];
     float key_scale[2][2], value_scale[2][2];
-    bool held[2];
-    auto tile_vector = [&](int j, bool& ok) -> int64_t {
-      ok = false;
-      if (j > any_last) return 0;
-      const int page = a.page_table[b * a.table_stride + (j >> c.page_shift)];
-      ok = page >= 0 && page < c.num_pages;
-      return ok ? c.vector(page, head, j & ((1 << c.page_shift) - 1)) : 0;
+    // A 16-token tile's first vector: page p of this head and `at` tokens in, or vector 0 where no page is named.
+    auto page_at = [&](int j) { return j <= any_last ? pages[j >> c.page_shift] : -1; };
+    auto vector_of = [&](int page, int j) {
+      return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages)
+                 ? c.vector(page, head, j & ((1 << c.page_shift) - 1))
+                 : int64_t{0};
     };
+    int page[2], next_page[2];
     int64_t vector[2];
+    const bool two_pages = c.page_shift == 4;  // else 32 aligned tokens lie in one
+    auto ask_pages = [&](int (&p)[2], int j) {
+      p[0] = page_at(j);
+      p[1] = two_pages ? page_at(j + 16) : p[0];
+    };
     auto load_keys = [&](int j) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        vector[i] = tile_vector(j + 16 * i, held[i]);
+        vector[i] = vector_of(page[i], j + 16 * i);
+        const uint8_t* codes = lane_keys + vector[i] * (kDim / 2);
+        const float* ks = c.scales[0] + vector[i] + g;
+        const float* vs = c.scales[1] + vector[i] + g;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          load_words(key[i][k], c.codes[0] + (vector[i] + g + 8 * k) * (kDim / 2) + t * (kDim / 8));
-          key_scale[i][k] = c.scales[0][vector[i] + g + 8 * k];
-          value_scale[i][k] = c.scales[1][vector[i] + g + 8 * k];
+          load_words(key[i][k], codes + k * 8 * (kDim / 2));
+          key_scale[i][k] = __ldg(ks + 8 * k);
+          value_scale[i][k] = __ldg(vs + 8 * k);
         }
       }
     };
     auto load_values = [&]() {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* codes = lane_values + vector[i] * (kDim / 2);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          load_words(value[i][k],
-                     c.codes[1] + (vector[i] + 2 * t + (k & 1) + 8 * (k >> 1)) * (kDim / 2) + g * (kDim / 16));
+        for (int k = 0; k < 4; ++k) load_words(value[i][k], codes + ((k & 1) + 8 * (k >> 1)) * (kDim / 2));
+      }
     };
     if (j0 < upto) {
+      ask_pages(page, j0);
+      ask_pages(next_page, j0 + kTile);
       load_keys(j0);
       load_values();
     }
     for (; j0 < upto; j0 += kTile) {
-      // Scores of the step: s[i][nt][0, 1] of token g, [2, 3] of token g + 8, columns 2t, 2t + 1.
-      float s[2][kTiles][4];
-      float ks[2][2], vs[2][2];
-      bool seen[2];
+      // Scores of the step: s[i][nt][0] of token g, [1] of token g + 8, columns 2t, 2t + 1.
+      float2 s[2][kTiles][2];
+      float2 vs[2][2];
+      bool whole[2], seen[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        float d[kTiles][4];
 #pragma unroll
-        for (int nt = 0; nt < kTiles; ++nt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s[i][nt][k] = lift[nt][k & 1];
+        for (int nt = 0; nt < kTiles; ++nt) {
+          d[nt][0] = d[nt][2] = lift[nt].x;
+          d[nt][1] = d[nt][3] = lift[nt].y;
+        }
 #pragma unroll
         for (int word = 0; word < kKeyWords; ++word) {
           const uint32_t x = key[i][0][word], y = key[i][1][word];
@@ -398,121 +440,116 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4A
           const uint32_t y0 = codes_plus72<0>(y), y1 = codes_plus72<1>(y), y2 = codes_plus72<2>(y), y3 = codes_plus72<3>(y);
 #pragma unroll
           for (int nt = 0; nt < kTiles; ++nt) {
-            mma(s[i][nt], x0, y0, x1, y1, q[nt][2 * word][0], q[nt][2 * word][1]);
-            mma(s[i][nt], x2, y2, x3, y3, q[nt][2 * word + 1][0], q[nt][2 * word + 1][1]);
+            mma(d[nt], x0, y0, x1, y1, q[nt][2 * word][0], q[nt][2 * word][1]);
+            mma(d[nt], x2, y2, x3, y3, q[nt][2 * word + 1][0], q[nt][2 * word + 1][1]);
           }
         }
-        ks[i][0] = key_scale[i][0], ks[i][1] = key_scale[i][1];
-        vs[i][0] = value_scale[i][0], vs[i][1] = value_scale[i][1];
-        seen[i] = held[i];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 ks = make_float2(key_scale[i][k], key_scale[i][k]);
+          vs[i][k] = make_float2(value_scale[i][k], value_scale[i][k]);
+#pragma unroll
+          for (int nt = 0; nt < kTiles; ++nt)
+            s[i][nt][k] = __fmul2_rn(make_float2(d[nt][2 * k], d[nt][2 * k + 1]), __fmul2_rn(factor[nt], ks));
+        }
+        const int j = j0 + 16 * i;
+        seen[i] = static_cast<uint32_t>(page[i]) < static_cast<uint32_t>(c.num_pages);
+        whole[i] = seen[i] && j >= every_first && j + 15 <= every_last;
       }
-      uint32_t p[2][kTiles][2];
-      // Values of this step were loaded with its keys; the next keys are asked for before the softmax.
-      uint32_t now[2][4][kValueWords];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int word = 0; word < kValueWords; ++word) now[i][k][word] = value[i][k][word];
+      // The next step's keys, and the page of the one after it.
+      page[0] = next_page[0];
+      page[1] = next_page[1];
       if (j0 + kTile < upto) {
         load_keys(j0 + kTile);
-        load_values();
+        ask_pages(next_page, j0 + 2 * kTile);
       }
-      float e[2][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        e[i][0] = scale_exponent(vs[i][0]);
-        e[i][1] = scale_exponent(vs[i][1]);
-      }
-#pragma unroll
-      for (int nt = 0; nt < kTiles; ++nt) {
+      const bool masked = !(whole[0] && whole[1]);
+      if (masked) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[i][nt][k] *= ks[i][k >> 1] * factor[nt][k & 1];
-      }
-      bool masked[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = j0 + 16 * i;
-        masked[i] = !seen[i] || j < every_first || j + 15 > every_last;
-        if (masked[i]) {
-#pragma unroll
           for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int at = j + g + 8 * (k >> 1);
-              if (!seen[i] || at < first[nt][k & 1] || at > last[nt][k & 1]) s[i][nt][k] = -INFINITY;
+            for (int k = 0; k < 2; ++k) {
+              const int j = j0 + 16 * i + g + 8 * k;
+              if (!seen[i] || j < first[nt][0] || j > last[nt][0]) s[i][nt][k].x = -INFINITY;
+              if (!seen[i] || j < first[nt][1] || j > last[nt][1]) s[i][nt][k].y = -INFINITY;
             }
-        }
       }
       bool moved = false;
-      float fade[kTiles][2], ref[kTiles][2];
+      float2 fade[kTiles], ref[kTiles];
 #pragma unroll
       for (int nt = 0; nt < kTiles; ++nt) {
+        float2 m = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float m = fmaxf(fmaxf(s[0][nt][k] + e[0][0], s[0][nt][k + 2] + e[0][1]),
-                          fmaxf(s[1][nt][k] + e[1][0], s[1][nt][k + 2] + e[1][1]));
-          m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
-          m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
-          m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-          m = fmaxf(m, top[nt][k]);
-          moved = moved || m > top[nt][k];
-          ref[nt][k] = m == -INFINITY ? 0.0F : m - kLift;
-          fade[nt][k] = fade_to(top[nt][k], m);
-          top[nt][k] = m;
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float e = scale_exponent(vs[i][k].x);
+            const float2 v = __fadd2_rn(s[i][nt][k], make_float2(e, e));
+            m.x = fmaxf(m.x, v.x);
+            m.y = fmaxf(m.y, v.y);
+          }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          m.x = fmaxf(m.x, __shfl_xor_sync(0xFFFFFFFFu, m.x, d));
+          m.y = fmaxf(m.y, __shfl_xor_sync(0xFFFFFFFFu, m.y, d));
         }
+        moved = moved || m.x > top[nt][0] || m.y > top[nt][1];
+        m.x = fmaxf(m.x, top[nt][0]);
+        m.y = fmaxf(m.y, top[nt][1]);
+        ref[nt] = make_float2(m.x == -INFINITY ? 0.0F : kLift - m.x, m.y == -INFINITY ? 0.0F : kLift - m.y);
+        fade[nt] = m;
       }
       if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < kTiles; ++nt) {
-          sum[nt][0] *= fade[nt][0];
-          sum[nt][1] *= fade[nt][1];
+          const float2 m = fade[nt], f = make_float2(fade_to(top[nt][0], m.x), fade_to(top[nt][1], m.y));
+          top[nt][0] = m.x;
+          top[nt][1] = m.y;
+          sum[nt] = __fmul2_rn(sum[nt], f);
 #pragma unroll
-          for (int i = 0; i < kOut; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[i][nt][k] *= fade[nt][k & 1];
+          for (int i = 0; i < kOut; ++i) {
+            const float2 lo = __fmul2_rn(make_float2(o[i][nt][0], o[i][nt][1]), f);
+            const float2 hi = __fmul2_rn(make_float2(o[i][nt][2], o[i][nt][3]), f);
+            o[i][nt][0] = lo.x, o[i][nt][1] = lo.y, o[i][nt][2] = hi.x, o[i][nt][3] = hi.y;
+          }
         }
       }
+      uint32_t p[2][kTiles][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int nt = 0; nt < kTiles; ++nt) {
-          float pv[4];
+        for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float pr = exp2_fast(s[i][nt][k] - ref[nt][k & 1]);
-            sum[nt][k & 1] += pr;
-            pv[k] = pr * vs[i][k >> 1];
+          for (int k = 0; k < 2; ++k) {
+            const float2 x = __fadd2_rn(s[i][nt][k], ref[nt]);
+            const float2 pr = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+            sum[nt] = __fadd2_rn(sum[nt], pr);
+            float2 pv = __fmul2_rn(pr, vs[i][k]);
+            if (masked) {  // an unseen token's scale may be NaN or infinite
+              if (s[i][nt][k].x == -INFINITY) pv.x = 0.0F;
+              if (s[i][nt][k].y == -INFINITY) pv.y = 0.0F;
+            }
+            p[i][nt][k] = transpose8x8(pack_half2(pv.x, pv.y));
           }
-          if (masked[i]) {  // an unseen token's scale may be NaN or infinite
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (s[i][nt][k] == -INFINITY) pv[k] = 0.0F;
-          }
-          p[i][nt][0] = transpose8x8(pack_half2(pv[0], pv[1]));
-          p[i][nt][1] = transpose8x8(pack_half2(pv[2], pv[3]));
-        }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int word = 0; word < kValueWords; ++word) {
-          const uint32_t va = now[i][0][word], vb = now[i][1][word], vc = now[i][2][word], vd = now[i][3][word];
+          const uint32_t va = value[i][0][word], vb = value[i][1][word], vc = value[i][2][word], vd = value[i][3][word];
           const uint32_t x0 = __byte_perm(va, vb, 0x5410), y0 = __byte_perm(va, vb, 0x7632);
           const uint32_t x1 = __byte_perm(vc, vd, 0x5410), y1 = __byte_perm(vc, vd, 0x7632);
 #pragma unroll
-          for (int nib = 0; nib < 4; ++nib) {
-            uint32_t a0, a1, a2, a3;
-            if (nib == 0) a0 = codes_exact<0>(x0), a1 = codes_exact<0>(y0), a2 = codes_exact<0>(x1), a3 = codes_exact<0>(y1);
-            else if (nib == 1) a0 = codes_exact<1>(x0), a1 = codes_exact<1>(y0), a2 = codes_exact<1>(x1), a3 = codes_exact<1>(y1);
-            else if (nib == 2) a0 = codes_exact<2>(x0), a1 = codes_exact<2>(y0), a2 = codes_exact<2>(x1), a3 = codes_exact<2>(y1);
-            else a0 = codes_exact<3>(x0), a1 = codes_exact<3>(y0), a2 = codes_exact<3>(x1), a3 = codes_exact<3>(y1);
-#pragma unroll
-            for (int nt = 0; nt < kTiles; ++nt) mma(o[4 * word + nib][nt], a0, a1, a2, a3, p[i][nt][0], p[i][nt][1]);
+          for (int nt = 0; nt < kTiles; ++nt) {
+            mma(o[4 * word][nt], codes_exact<0>(x0), codes_exact<0>(y0), codes_exact<0>(x1), codes_exact<0>(y1), p[i][nt][0], p[i][nt][1]);
+            mma(o[4 * word + 1][nt], codes_exact<1>(x0), codes_exact<1>(y0), codes_exact<1>(x1), codes_exact<1>(y1), p[i][nt][0], p[i][nt][1]);
+            mma(o[4 * word + 2][nt], codes_exact<2>(x0), codes_exact<2>(y0), codes_exact<2>(x1), codes_exact<2>(y1), p[i][nt][0], p[i][nt][1]);
+            mma(o[4 * word + 3][nt], codes_exact<3>(x0), codes_exact<3>(y0), codes_exact<3>(x1), codes_exact<3>(y1), p[i][nt][0], p[i][nt][1]);
           }
         }
+      }
+      if (j0 + kTile < upto) load_values();
     }
 
     // The warps' parts, joined in the order of the warps.
@@ -520,7 +557,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4A
     for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        float l = sum[nt][k];
+        float l = k ? sum[nt].y : sum[nt].x;
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 4);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 8);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
@@ -584,41 +621,74 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attend_kernel(Kv4View c, Kv4A
   }
 }
 
-// Adds the partial sums of the segments that were cut, in the order of the line.
+// Adds the partial sums of the segments that were cut, in the order of the line.  A thread owns four dimensions of
+// a row; the parts' weights (2 to the distance of their references from the largest) are formed once, so that the
+// loads of the parts do not wait for one another.
+constexpr int kParts = 64;  // parts whose weights are held at a time
 template <class T, int kDim, int kTiles>
-__global__ void __launch_bounds__(kWarps * 32) kv4_join_kernel(Kv4View c, Kv4Attend a, Line line, int64_t blocks) {
-  constexpr int kRows = 8 * kTiles;
-  __shared__ int64_t scratch[kWarps + 2];
+__global__ void __launch_bounds__(2 * kDim * kTiles) kv4_join_kernel(Kv4View c, Kv4Attend a, Line line, int64_t blocks) {
+  constexpr int kRows = 8 * kTiles, kThreads = 2 * kDim * kTiles;  // kRows * kDim / 4
+  __shared__ int64_t scratch[kThreads / 32 + 2];
+  __shared__ float weight[kParts][kRows];
+  __shared__ float stats[2][kRows];
   const int b = blockIdx.x;
-  const Place place = find_place(a, line, b, [](int64_t) { return int64_t{0}; }, scratch);
+  const Place place = find_place<kThreads / 32>(a, line, b, [](int64_t) { return int64_t{0}; }, scratch);
   const SequenceWork w = sequence_work(a, line, b);
+  const int64_t n = ranges(place.total, blocks);
 #if __CUDA_ARCH__ >= 900
   cudaGridDependencySynchronize();
 #endif
-  const int64_t n = ranges(place.total, blocks);
   for (int64_t segment = blockIdx.y; segment < static_cast<int64_t>(c.heads) * w.blocks; segment += gridDim.y) {
     const int64_t u0 = place.before + segment * w.tiles, u1 = u0 + w.tiles;
     const int64_t c0 = range_of(place.total, u0, n), c1 = range_of(place.total, u1 - 1, n);
     if (c0 == c1) continue;
     const int head = static_cast<int>(segment / w.blocks), row0 = static_cast<int>(segment % w.blocks) * kRows;
+    // Part k of the segment: the last of the block where the segment starts, the first of the others.
     const float* base = static_cast<const float*>(a.workspace);
-    for (int i = threadIdx.x; i < kRows * kDim; i += kWarps * 32) {
-      const int r = i / kDim, d = i - r * kDim;
-      if (row0 + r >= w.q.rows * line.shared) continue;
-      float m = -INFINITY, l = 0.0F, v = 0.0F;
+    auto part = [&](int64_t k) {
+      return base + (2 * k + (k == c0 ? 1 : 0)) * partial_floats(kRows, kDim);
+    };
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+      float m = -INFINITY, l = 0.0F;
+#pragma unroll 8
+      for (int64_t k = c0; k <= c1; ++k) m = fmaxf(m, part(k)[kRows * kDim + 2 * threadIdx.x]);
+#pragma unroll 8
       for (int64_t k = c0; k <= c1; ++k) {
-        // Where the segment starts, it is the block's last; elsewhere its first.
-        const float* p = base + (2 * k + (range_start(place.total, k, n) <= u0 ? 1 : 0)) * partial_floats(kRows, kDim);
-        const float pm = p[kRows * kDim + 2 * r], pl = p[kRows * kDim + 2 * r + 1];
-        const float next = fmaxf(m, pm);
-        const float f0 = fade_to(m, next), f1 = fade_to(pm, next);
-        l = l * f0 + pl * f1;
-        v = v * f0 + p[i] * f1;
-        m = next;
+        const float2 s = *reinterpret_cast<const float2*>(part(k) + kRows * kDim + 2 * threadIdx.x);
+        l += s.y * fade_to(s.x, m);
       }
+      stats[0][threadIdx.x] = m;
+      stats[1][threadIdx.x] = l;
+    }
+    __syncthreads();
+    const int r = threadIdx.x / (kDim / 4), d = threadIdx.x % (kDim / 4) * 4;
+    float4 v = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+    for (int64_t k0 = c0; k0 <= c1; k0 += kParts) {
+      const int parts = static_cast<int>(min(static_cast<int64_t>(kParts), c1 - k0 + 1));
+      for (int i = threadIdx.x; i < parts * kRows; i += kThreads)
+        weight[i / kRows][i % kRows] = fade_to(part(k0 + i / kRows)[kRows * kDim + 2 * (i % kRows)], stats[0][i % kRows]);
+      __syncthreads();
+#pragma unroll 8
+      for (int k = 0; k < parts; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(part(k0 + k) + r * kDim + d);
+        const float f = weight[k][r];
+        v.x += f * x.x;
+        v.y += f * x.y;
+        v.z += f * x.z;
+        v.w += f * x.w;
+      }
+      __syncthreads();
+    }
+    if (row0 + r < w.q.rows * line.shared) {
+      const float l = stats[1][r], inv = l == 0.0F ? 0.0F : 1.0F / l;
       const int64_t row = (w.q.row0 + (row0 + r) / line.shared) * a.heads + head * line.shared + (row0 + r) % line.shared;
-      static_cast<T*>(a.out)[row * kDim + d] = from_f32<T>(l == 0.0F ? 0.0F : v / l);
-      if (a.lse && d == 0) a.lse[row] = log_sum(m, l);
+      T* out = static_cast<T*>(a.out) + row * kDim + d;
+      out[0] = from_f32<T>(v.x * inv);
+      out[1] = from_f32<T>(v.y * inv);
+      out[2] = from_f32<T>(v.z * inv);
+      out[3] = from_f32<T>(v.w * inv);
+      if (a.lse && d == 0) a.lse[row] = log_sum(stats[0][r], l);
     }
   }
 }
@@ -627,7 +697,17 @@ struct Shape {
   int tiles;        // column tiles of 8 rows
   int64_t blocks;   // blocks of the main kernel
 };
-constexpr int kResident = 148 * 4;
+int sm_count() {
+  static std::atomic<int> known{0};
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    int dev = 0;
+    check(cudaGetDevice(&dev), "get device");
+    check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "SM count");
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 Shape shape_of(const Kv4View& c, const Kv4Attend& a) {
   const int shared = a.heads / c.heads;
@@ -637,13 +717,15 @@ Shape shape_of(const Kv4View& c, const Kv4Attend& a) {
   const int64_t most = static_cast<int64_t>(a.max_pages) << c.page_shift;
   const int64_t units = std::max<int64_t>(1, (most + kTile - 1) / kTile) * a.batch * c.heads *
                         ((rows + 8 * s.tiles - 1) / (8 * s.tiles));
-  s.blocks = std::max<int64_t>(1, std::min<int64_t>(kResident, units));
+  s.blocks = std::max<int64_t>(1, std::min<int64_t>(sm_count() * resident_blocks(c.dim, s.tiles), units));
   return s;
 }
 
 template <class T, int kDim, int kTiles>
 void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStream_t stream) {
-  const Line line{c.heads, a.heads / c.heads, 8 * kTiles, c.page_shift};
+  const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
+                          static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
+  const Line line{c.heads, a.heads / c.heads, 8 * kTiles, c.page_shift, (starts & 15) == 0};
   kv4_attend_kernel<T, kDim, kTiles><<<static_cast<unsigned>(s.blocks), kWarps * 32, 0, stream>>>(c, a, line);
   count_launch();
   check(cudaGetLastError(), "launch cache attention kernel");
@@ -651,7 +733,7 @@ void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
   const int64_t segments = c.heads * ((static_cast<int64_t>(a.max_rows) * line.shared + line.block_rows - 1) / line.block_rows);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.batch), static_cast<unsigned>(std::min<int64_t>(segments, 65535)));
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(2 * kDim * kTiles);
   cfg.stream = stream;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
