@@ -287,7 +287,7 @@ int msb_docs_topk_device_noalloc(msb_docs* docs, const float* query, int32_t bat
  * token's key or value of one head: head_dim (64, 128 or 256) codes in
  * [-7, 7], even dimension in the low nibble, and an fp32 scale.  codes
  * [num_pages, kv_heads, page_size, head_dim / 2], 16-byte aligned; scales
- * [num_pages, kv_heads, page_size].  Slot s is token s % page_size of page
+ * [num_pages, kv_heads, page_size], 16-byte aligned.  Slot s is token s % page_size of page
  * s / page_size. */
 typedef struct msb_kv4_cache {
   uint8_t* k_codes;

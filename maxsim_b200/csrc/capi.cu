@@ -1469,12 +1469,14 @@ Kv4View kv4_view(const msb_kv4_cache* c) {
   if (c->num_pages < 1 || c->kv_heads < 1) throw InvalidArgument("num_pages and kv_heads must be positive");
   if (c->num_pages > (int64_t{1} << 31) - 1) throw InvalidArgument("num_pages must be below 2^31");
   if (c->kv_heads > 65535) throw InvalidArgument("kv_heads must be at most 65535");
+  if (c->num_pages * c->kv_heads > (int64_t{1} << 31) - 1) throw InvalidArgument("num_pages * kv_heads must be below 2^31");
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
     throw InvalidArgument("head_dim must be 64, 128 or 256");
   if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
     throw InvalidArgument("page_size must be a power of two from 16 to 1024");
-  if ((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15)
-    throw InvalidArgument("cache codes must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes) |
+       reinterpret_cast<uintptr_t>(c->k_scales) | reinterpret_cast<uintptr_t>(c->v_scales)) & 15)
+    throw InvalidArgument("cache arrays must be 16-byte aligned");
   Kv4View v{};
   v.codes[0] = c->k_codes;
   v.codes[1] = c->v_codes;

@@ -39,40 +39,29 @@ constexpr int kWarps = 4;
 constexpr int kStep = 32;              // tokens a warp takes at a time
 constexpr int kTile = kWarps * kStep;  // tokens of one unit of the work line
 constexpr int kExponents = 110;        // powers of two that scales and queries are brought back from
+constexpr int kStages = 3;             // steps in a warp's ring: one worked on, two on their way
 constexpr float kLift = 8.0F;          // references lie 2^8 below the maximum: probabilities of 2^-22 are normal in fp16
 
-template <class T>
-__device__ __forceinline__ T load_stream(const void* p);
-template <>
-__device__ __forceinline__ uint4 load_stream<uint4>(const void* p) {
-  uint4 r;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-template <>
-__device__ __forceinline__ uint2 load_stream<uint2>(const void* p) {
-  uint2 r;
-  asm("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
-template <>
-__device__ __forceinline__ uint32_t load_stream<uint32_t>(const void* p) {
-  uint32_t r;
-  asm("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
-  return r;
-}
-// kWords consecutive words (a power of two; the address is aligned to their size or to 16 bytes).
+// kWords consecutive words of shared memory (aligned to their size or to 16 bytes).
 template <int kWords>
-__device__ __forceinline__ void load_words(uint32_t (&r)[kWords], const uint8_t* p) {
+__device__ __forceinline__ void load_words(uint32_t (&r)[kWords], const unsigned char* p) {
   if constexpr (kWords == 1) {
-    r[0] = load_stream<uint32_t>(p);
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
   } else if constexpr (kWords == 2) {
-    const uint2 v = load_stream<uint2>(p);
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     r[0] = v.x, r[1] = v.y;
   } else {
 #pragma unroll
     for (int i = 0; i < kWords; i += 4) {
-      const uint4 v = load_stream<uint4>(p + 4 * i);
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
       r[i] = v.x, r[i + 1] = v.y, r[i + 2] = v.z, r[i + 3] = v.w;
     }
   }
@@ -246,8 +235,11 @@ __host__ __device__ constexpr int partial_floats(int rows, int dim) { return row
 
 // Resident blocks per SM that the registers are held to (128 threads, 65,536 registers).
 __host__ __device__ constexpr int resident_blocks(int dim, int tiles) {
-  return dim == 256 ? 2 : dim == 128 ? (tiles == 1 ? 4 : 2) : (tiles == 1 ? 4 : 3);
+  return dim == 256 ? 2 : dim == 128 ? (tiles == 1 ? 4 : 3) : (tiles == 1 ? 5 : 4);
 }
+
+// The warps' rings: codes of keys and values and both scales of kStages steps.
+__host__ __device__ constexpr int ring_bytes(int dim) { return kWarps * kStages * (kStep * dim + 2 * kStep * 4); }
 
 template <class T, int kDim, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv4_attend_kernel(Kv4View c, Kv4Attend a, Line line) {
@@ -255,8 +247,11 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
   constexpr int kKeyWords = kDim / 32;   // of one token, per lane
   constexpr int kValueWords = kDim / 64;
   constexpr int kOut = kDim / 16;        // 16-dimension tiles of the output
-  constexpr int kPitch = kDim + 4;       // floats between rows in shared memory
-  __shared__ float merge[kWarps][kRows * kPitch / 2];
+  constexpr int kHalfPitch = kDim / 2 + 2;          // floats between rows of the warps' sums
+  constexpr int kCodeBytes = kStep * kDim / 2;      // one step's keys, or values
+  constexpr int kStageBytes = 2 * kCodeBytes + 2 * kStep * 4;
+  extern __shared__ __align__(128) unsigned char ring[];
+  float(*merge)[kRows * kHalfPitch] = reinterpret_cast<float(*)[kRows * kHalfPitch]>(ring);  // after the last step
   __shared__ float stats[kWarps][2][kRows];
   __shared__ int64_t scratch[kWarps + 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -373,58 +368,65 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     if (any_first > j0) j0 += (any_first - j0) / kTile * kTile;
 
     const int32_t* pages = a.page_table + b * a.table_stride;
-    const uint8_t* lane_keys = c.codes[0] + g * (kDim / 2) + t * (kDim / 8);
-    const uint8_t* lane_values = c.codes[1] + 2 * t * (kDim / 2) + g * (kDim / 16);
-    uint32_t key[2][2][kKeyWords], value[2][4][kValueWords];
-    float key_scale[2][2], value_scale[2][2];
-    // A 16-token tile's first vector: page p of this head and `at` tokens in, or vector 0 where no page is named.
-    auto page_at = [&](int j) { return j <= any_last ? pages[j >> c.page_shift] : -1; };
-    auto vector_of = [&](int page, int j) {
-      return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages)
-                 ? c.vector(page, head, j & ((1 << c.page_shift) - 1))
-                 : int64_t{0};
-    };
-    int page[2], next_page[2];
-    int64_t vector[2];
     const bool two_pages = c.page_shift == 4;  // else 32 aligned tokens lie in one
-    auto ask_pages = [&](int (&p)[2], int j) {
-      p[0] = page_at(j);
-      p[1] = two_pages ? page_at(j + 16) : p[0];
+    const int page_mask = (1 << c.page_shift) - 1;
+    unsigned char* const stages = ring + warp * (kStages * kStageBytes);
+    const uint32_t lane_stage = static_cast<uint32_t>(__cvta_generic_to_shared(stages)) + lane * 16;
+    const unsigned char* lane_codes[2] = {c.codes[0] + lane * 16, c.codes[1] + lane * 16};
+    const float* lane_scales = (lane & 8 ? c.scales[1] : c.scales[0]) + (lane & 3) * 4;
+    int next_page[2];  // the pages of the next step to be copied, -1 past the last token seen
+    uint32_t seen_queue = 0;  // two bits a step, the oldest lowest: its 16-token tiles lie on pages of the cache
+    auto ask_pages = [&](int j) {
+      next_page[0] = j < upto ? __ldg(pages + (j >> c.page_shift)) : -1;
+      next_page[1] = !two_pages ? next_page[0] : j + 16 < upto ? __ldg(pages + ((j + 16) >> c.page_shift)) : -1;
     };
-    auto load_keys = [&](int j) {
+    // Copies the step at j into a stage; tiles without a page copy the cache's first vectors.
+    auto copy_step = [&](int j, int stage, int slot) {
+      if (j < upto) {
+        const uint32_t dst = lane_stage + stage * kStageBytes;
+        uint32_t bits = 0;
+        int64_t tile[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        vector[i] = vector_of(page[i], j + 16 * i);
-        const uint8_t* codes = lane_keys + vector[i] * (kDim / 2);
-        const float* ks = c.scales[0] + vector[i] + g;
-        const float* vs = c.scales[1] + vector[i] + g;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          load_words(key[i][k], codes + k * 8 * (kDim / 2));
-          key_scale[i][k] = __ldg(ks + 8 * k);
-          value_scale[i][k] = __ldg(vs + 8 * k);
+        for (int i = 0; i < 2; ++i) {
+          const bool ok = static_cast<uint32_t>(next_page[i]) < static_cast<uint32_t>(c.num_pages);
+          bits |= ok ? 1u << i : 0u;
+          const uint32_t index = ok ? static_cast<uint32_t>(next_page[i]) * c.heads + head : 0u;  // below 2^31
+          tile[i] = (static_cast<int64_t>(index) << c.page_shift) + (ok ? (j + 16 * i) & page_mask : 0);
         }
-      }
-    };
-    auto load_values = [&]() {
+        seen_queue |= bits << (2 * slot);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint8_t* codes = lane_values + vector[i] * (kDim / 2);
+        for (int which = 0; which < 2; ++which)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) load_words(value[i][k], codes + ((k & 1) + 8 * (k >> 1)) * (kDim / 2));
+          for (int i = 0; i < 2; ++i) {
+            const uint8_t* src = lane_codes[which] + tile[i] * (kDim / 2);
+#pragma unroll
+            for (int k = 0; k < kDim / 64; ++k)
+              copy16(dst + which * kCodeBytes + i * (kCodeBytes / 2) + k * 512, src + k * 512);
+          }
+        if (lane < 16) copy16(dst + 2 * kCodeBytes, lane_scales + ((lane >> 2) & 1 ? tile[1] : tile[0]));
       }
+      copies_commit();
     };
-    if (j0 < upto) {
-      ask_pages(page, j0);
-      ask_pages(next_page, j0 + kTile);
-      load_keys(j0);
-      load_values();
+    ask_pages(j0);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      copy_step(j0 + i * kTile, i, i);
+      ask_pages(j0 + (i + 1) * kTile);
     }
+    int stage = 0;
     for (; j0 < upto; j0 += kTile) {
+      copies_wait<kStages - 2>();
+      __syncwarp();
+      // Every lane has left the stage of the step before: the copies two steps ahead go there.
+      const unsigned char* here = stages + stage * kStageBytes;
+      const uint32_t seen = seen_queue & 3u;
+      seen_queue >>= 2;
+      copy_step(j0 + (kStages - 1) * kTile, stage == 0 ? kStages - 1 : stage - 1, kStages - 2);
+      ask_pages(j0 + kStages * kTile);
+      stage = stage == kStages - 1 ? 0 : stage + 1;
       // Scores of the step: s[i][nt][0] of token g, [1] of token g + 8, columns 2t, 2t + 1.
       float2 s[2][kTiles][2];
       float2 vs[2][2];
-      bool whole[2], seen[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float d[kTiles][4];
@@ -433,9 +435,12 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
           d[nt][0] = d[nt][2] = lift[nt].x;
           d[nt][1] = d[nt][3] = lift[nt].y;
         }
+        uint32_t key[2][kKeyWords];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) load_words(key[k], here + (16 * i + g + 8 * k) * (kDim / 2) + t * (kDim / 8));
 #pragma unroll
         for (int word = 0; word < kKeyWords; ++word) {
-          const uint32_t x = key[i][0][word], y = key[i][1][word];
+          const uint32_t x = key[0][word], y = key[1][word];
           const uint32_t x0 = codes_plus72<0>(x), x1 = codes_plus72<1>(x), x2 = codes_plus72<2>(x), x3 = codes_plus72<3>(x);
           const uint32_t y0 = codes_plus72<0>(y), y1 = codes_plus72<1>(y), y2 = codes_plus72<2>(y), y3 = codes_plus72<3>(y);
 #pragma unroll
@@ -444,26 +449,17 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
             mma(d[nt], x2, y2, x3, y3, q[nt][2 * word + 1][0], q[nt][2 * word + 1][1]);
           }
         }
+        const float* scales = reinterpret_cast<const float*>(here + 2 * kCodeBytes) + 16 * i + g;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float2 ks = make_float2(key_scale[i][k], key_scale[i][k]);
-          vs[i][k] = make_float2(value_scale[i][k], value_scale[i][k]);
+          const float ks = scales[8 * k], v = scales[kStep + 8 * k];
+          vs[i][k] = make_float2(v, v);
 #pragma unroll
           for (int nt = 0; nt < kTiles; ++nt)
-            s[i][nt][k] = __fmul2_rn(make_float2(d[nt][2 * k], d[nt][2 * k + 1]), __fmul2_rn(factor[nt], ks));
+            s[i][nt][k] = __fmul2_rn(make_float2(d[nt][2 * k], d[nt][2 * k + 1]), __fmul2_rn(factor[nt], make_float2(ks, ks)));
         }
-        const int j = j0 + 16 * i;
-        seen[i] = static_cast<uint32_t>(page[i]) < static_cast<uint32_t>(c.num_pages);
-        whole[i] = seen[i] && j >= every_first && j + 15 <= every_last;
       }
-      // The next step's keys, and the page of the one after it.
-      page[0] = next_page[0];
-      page[1] = next_page[1];
-      if (j0 + kTile < upto) {
-        load_keys(j0 + kTile);
-        ask_pages(next_page, j0 + 2 * kTile);
-      }
-      const bool masked = !(whole[0] && whole[1]);
+      const bool masked = seen != 3u || j0 < every_first || j0 + kStep - 1 > every_last;
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -472,8 +468,9 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int j = j0 + 16 * i + g + 8 * k;
-              if (!seen[i] || j < first[nt][0] || j > last[nt][0]) s[i][nt][k].x = -INFINITY;
-              if (!seen[i] || j < first[nt][1] || j > last[nt][1]) s[i][nt][k].y = -INFINITY;
+              const bool off = !((seen >> i) & 1u);
+              if (off || j < first[nt][0] || j > last[nt][0]) s[i][nt][k].x = -INFINITY;
+              if (off || j < first[nt][1] || j > last[nt][1]) s[i][nt][k].y = -INFINITY;
             }
       }
       bool moved = false;
@@ -535,9 +532,13 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
           }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        uint32_t value[4][kValueWords];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          load_words(value[k], here + kCodeBytes + (16 * i + 2 * t + (k & 1) + 8 * (k >> 1)) * (kDim / 2) + g * (kDim / 16));
 #pragma unroll
         for (int word = 0; word < kValueWords; ++word) {
-          const uint32_t va = value[i][0][word], vb = value[i][1][word], vc = value[i][2][word], vd = value[i][3][word];
+          const uint32_t va = value[0][word], vb = value[1][word], vc = value[2][word], vd = value[3][word];
           const uint32_t x0 = __byte_perm(va, vb, 0x5410), y0 = __byte_perm(va, vb, 0x7632);
           const uint32_t x1 = __byte_perm(vc, vd, 0x5410), y1 = __byte_perm(vc, vd, 0x7632);
 #pragma unroll
@@ -549,8 +550,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
           }
         }
       }
-      if (j0 + kTile < upto) load_values();
     }
+    copies_wait<0>();
 
     // The warps' parts, joined in the order of the warps.
 #pragma unroll
@@ -571,7 +572,6 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     if (!whole)
       partial = static_cast<float*>(a.workspace) + (2 * block + (tile0 == 0 ? 1 : 0)) * partial_floats(kRows, kDim);
     constexpr int kHalf = kDim / 2;      // dimensions of one pass through shared memory
-    constexpr int kHalfPitch = kPitch / 2;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       __syncthreads();
@@ -693,6 +693,18 @@ __global__ void __launch_bounds__(2 * kDim * kTiles) kv4_join_kernel(Kv4View c, 
   }
 }
 
+// Opts a kernel in to its dynamic shared memory, once per device.
+template <auto kernel>
+void allow_shared(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  check(cudaGetDevice(&dev), "get device");
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory of the cache attention kernel");
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 struct Shape {
   int tiles;        // column tiles of 8 rows
   int64_t blocks;   // blocks of the main kernel
@@ -726,7 +738,10 @@ void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
   const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
   const Line line{c.heads, a.heads / c.heads, 8 * kTiles, c.page_shift, (starts & 15) == 0};
-  kv4_attend_kernel<T, kDim, kTiles><<<static_cast<unsigned>(s.blocks), kWarps * 32, 0, stream>>>(c, a, line);
+  constexpr int kShared = ring_bytes(kDim);
+  static_assert(kShared >= static_cast<int>(sizeof(float)) * kWarps * 8 * kTiles * (kDim / 2 + 2), "sums fit the ring");
+  allow_shared<kv4_attend_kernel<T, kDim, kTiles>>(kShared);
+  kv4_attend_kernel<T, kDim, kTiles><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
   count_launch();
   check(cudaGetLastError(), "launch cache attention kernel");
   if ((static_cast<int64_t>(a.max_pages) << c.page_shift) <= kTile) return;  // no segment can be cut

@@ -96,8 +96,8 @@ class Int4KVCache:
         _check_cache_sizes(size, 2 * half)
         if pages < 1 or heads < 1:
             raise ValueError("num_pages and num_kv_heads must be positive")
-        if k_codes.data_ptr() % 16 or v_codes.data_ptr() % 16:
-            raise ValueError("cache codes must be 16-byte aligned")
+        if any(t.data_ptr() % 16 for t in (k_codes, k_scales, v_codes, v_scales)):
+            raise ValueError("cache arrays must be 16-byte aligned")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.device = device
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = pages, heads, size, 2 * half
