@@ -38,7 +38,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStep = 32;              // tokens a warp takes at a time
 constexpr int kTile = kWarps * kStep;  // tokens of one unit of the work line
-constexpr int kExponents = 110;        // powers of two that scales and queries are brought back from
+constexpr float kExponents = 110.0F;   // powers of two that scales and queries are brought back from
 constexpr int kStages = 3;             // steps in a warp's ring: one worked on, two on their way
 constexpr float kLift = 8.0F;          // references lie 2^8 below the maximum: probabilities of 2^-22 are normal in fp16
 
@@ -67,21 +67,25 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[kWords], const unsigned
   }
 }
 
-// Nibbles kI and kI + 4 of a word as the fp16 pair 72 + code.
+// Nibbles kI and kI + 4 of a word as an fp16 pair: 1032 + code (kI even) or 72 + code (kI odd), the nibbles in
+// the last bits of 1024's mantissa or four above the last of 64's.
 template <int kI>
-__device__ __forceinline__ uint32_t codes_plus72(uint32_t w) {
+__device__ __forceinline__ uint32_t codes_raised(uint32_t w) {
+  constexpr uint32_t kMask = kI & 1 ? 0x00f000f0u : 0x000f000fu, kFlip = kI & 1 ? 0x54805480u : 0x64086408u;
   uint32_t r;
-  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0x6a;"  // (a & b) ^ c
-      : "=r"(r)
-      : "r"(kI == 0 ? w << 4 : w >> (4 * kI - 4)), "r"(0x54805480u));
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(kI < 2 ? w : w >> 8), "n"(kMask), "r"(kFlip));  // (a & b) ^ c
   return r;
 }
-// The same pair, exact.
 template <int kI>
 __device__ __forceinline__ uint32_t codes_exact(uint32_t w) {
   uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(codes_plus72<kI>(w)), "r"(0x54805480u));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(codes_raised<kI>(w)), "r"(kI & 1 ? 0x54805480u : 0x64086408u));
   return r;
+}
+// Key codes: the 72 of odd nibbles stays, and the accumulators start at -72 times the sum of their queries.
+template <int kI>
+__device__ __forceinline__ uint32_t codes_key(uint32_t w) {
+  return kI & 1 ? codes_raised<kI>(w) : codes_exact<kI>(w);
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -126,10 +130,16 @@ __device__ __forceinline__ float fade_to(float from, float to) { return from == 
 __device__ __forceinline__ float log_sum(float m, float l) {
   return l == 0.0F ? -INFINITY : (m - kLift + __log2f(l)) * 0.693147181F;
 }
-// Exponent of a scale (the e of 2^(e + [0, 1))), held to +-110.
+// About log2 of a scale, held to +-110 (and so a number where the scale is 0, NaN or infinite).
 __device__ __forceinline__ float scale_exponent(float s) {
-  const int e = static_cast<int>((__float_as_uint(s) >> 23) & 255) - 127;
-  return static_cast<float>(max(-kExponents, min(kExponents, e)));
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fminf(fmaxf(r, -kExponents), kExponents);
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // The work line: units of kTile tokens of every (sequence, key/value head, row block).
@@ -247,11 +257,11 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
   constexpr int kKeyWords = kDim / 32;   // of one token, per lane
   constexpr int kValueWords = kDim / 64;
   constexpr int kOut = kDim / 16;        // 16-dimension tiles of the output
-  constexpr int kHalfPitch = kDim / 2 + 2;          // floats between rows of the warps' sums
+  constexpr int kPitch = kDim + 4;                  // floats between rows of the warps' sums
   constexpr int kCodeBytes = kStep * kDim / 2;      // one step's keys, or values
   constexpr int kStageBytes = 2 * kCodeBytes + 2 * kStep * 4;
   extern __shared__ __align__(128) unsigned char ring[];
-  float(*merge)[kRows * kHalfPitch] = reinterpret_cast<float(*)[kRows * kHalfPitch]>(ring);  // after the last step
+  float(*merge)[kRows * kPitch] = reinterpret_cast<float(*)[kRows * kPitch]>(ring);  // after the last step
   __shared__ float stats[kWarps][2][kRows];
   __shared__ int64_t scratch[kWarps + 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
 
     // Queries: lane (g, t) holds row g of each column tile, dimensions t * kDim / 4 and on.
     uint32_t q[kTiles][2 * kKeyWords][2];
-    float2 lift[kTiles];     // -72 sum(q) of columns 2t, 2t + 1
+    float2 lift[kTiles];     // what columns 2t, 2t + 1 start at (codes_key)
     float2 factor[kTiles];   // scale * log2(e) * the row's power of two
     int last[kTiles][2], first[kTiles][2];  // tokens that columns 2t, 2t + 1 see: first <= j <= last
     int every_last = INT_MAX, every_first = 0, any_last = -1, any_first = INT_MAX;
@@ -305,25 +315,21 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       for (int d = 0; d < kKeyWords * 8; ++d) top = fmaxf(top, fabsf(x[d]));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const int e = max(-kExponents, min(kExponents, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
       const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
-      float sum = 0.0F;
+      float sum[4] = {0.0F, 0.0F, 0.0F, 0.0F};
 #pragma unroll
       for (int word = 0; word < kKeyWords; ++word) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t v = pack_half2(x[8 * word + i] * down, x[8 * word + 4 + i] * down);
-          q[nt][2 * word + (i >> 1)][i & 1] = v;
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-          sum += f.x + f.y;
-        }
+        for (int i = 0; i < 4; ++i)
+          q[nt][2 * word + (i >> 1)][i & 1] = pack_half2(x[8 * word + i] * down, x[8 * word + 4 + i] * down);
+        // -72 (0xD480) times the queries of odd nibbles, summed where the scores will be
+        mma(sum, 0u, 0u, 0xD480D480u, 0xD480D480u, q[nt][2 * word][0], q[nt][2 * word][1]);
+        mma(sum, 0u, 0u, 0xD480D480u, 0xD480D480u, q[nt][2 * word + 1][0], q[nt][2 * word + 1][1]);
       }
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-      sum *= -72.0F;
       const float up = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
       // from the lanes that hold rows 2t, 2t + 1 to the columns' lanes
-      lift[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, sum, 8 * t), __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4));
+      lift[nt] = make_float2(sum[0], sum[1]);
       factor[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, up, 8 * t), __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4));
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -384,26 +390,31 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     auto copy_step = [&](int j, int stage, int slot) {
       if (j < upto) {
         const uint32_t dst = lane_stage + stage * kStageBytes;
-        uint32_t bits = 0;
-        int64_t tile[2];
+        auto tile_of = [&](int i) -> int64_t {
+          if (static_cast<uint32_t>(next_page[i]) >= static_cast<uint32_t>(c.num_pages)) return 0;
+          seen_queue |= (!two_pages ? 3u : 1u << i) << (2 * slot);
+          return (static_cast<int64_t>(static_cast<uint32_t>(next_page[i]) * c.heads + head) << c.page_shift) +
+                 ((j + 16 * i) & page_mask);
+        };
+        const int64_t tile = tile_of(0);
+        const uint8_t* src[2] = {lane_codes[0] + tile * (kDim / 2), lane_codes[1] + tile * (kDim / 2)};
+        if (!two_pages) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bool ok = static_cast<uint32_t>(next_page[i]) < static_cast<uint32_t>(c.num_pages);
-          bits |= ok ? 1u << i : 0u;
-          const uint32_t index = ok ? static_cast<uint32_t>(next_page[i]) * c.heads + head : 0u;  // below 2^31
-          tile[i] = (static_cast<int64_t>(index) << c.page_shift) + (ok ? (j + 16 * i) & page_mask : 0);
+          for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int k = 0; k < kDim / 32; ++k) copy16(dst + which * kCodeBytes + k * 512, src[which] + k * 512);
+          if (lane < 16) copy16(dst + 2 * kCodeBytes, lane_scales + tile + ((lane >> 2) & 1) * 16);
+        } else {
+          const int64_t other = tile_of(1), step = (other - tile) * (kDim / 2);
+#pragma unroll
+          for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int k = 0; k < kDim / 64; ++k) {
+              copy16(dst + which * kCodeBytes + k * 512, src[which] + k * 512);
+              copy16(dst + which * kCodeBytes + kCodeBytes / 2 + k * 512, src[which] + step + k * 512);
+            }
+          if (lane < 16) copy16(dst + 2 * kCodeBytes, lane_scales + ((lane >> 2) & 1 ? other : tile));
         }
-        seen_queue |= bits << (2 * slot);
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint8_t* src = lane_codes[which] + tile[i] * (kDim / 2);
-#pragma unroll
-            for (int k = 0; k < kDim / 64; ++k)
-              copy16(dst + which * kCodeBytes + i * (kCodeBytes / 2) + k * 512, src + k * 512);
-          }
-        if (lane < 16) copy16(dst + 2 * kCodeBytes, lane_scales + ((lane >> 2) & 1 ? tile[1] : tile[0]));
       }
       copies_commit();
     };
@@ -441,8 +452,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
 #pragma unroll
         for (int word = 0; word < kKeyWords; ++word) {
           const uint32_t x = key[0][word], y = key[1][word];
-          const uint32_t x0 = codes_plus72<0>(x), x1 = codes_plus72<1>(x), x2 = codes_plus72<2>(x), x3 = codes_plus72<3>(x);
-          const uint32_t y0 = codes_plus72<0>(y), y1 = codes_plus72<1>(y), y2 = codes_plus72<2>(y), y3 = codes_plus72<3>(y);
+          const uint32_t x0 = codes_key<0>(x), x1 = codes_key<1>(x), x2 = codes_key<2>(x), x3 = codes_key<3>(x);
+          const uint32_t y0 = codes_key<0>(y), y1 = codes_key<1>(y), y2 = codes_key<2>(y), y3 = codes_key<3>(y);
 #pragma unroll
           for (int nt = 0; nt < kTiles; ++nt) {
             mma(d[nt], x0, y0, x1, y1, q[nt][2 * word][0], q[nt][2 * word][1]);
@@ -473,28 +484,28 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
               if (off || j < first[nt][1] || j > last[nt][1]) s[i][nt][k].y = -INFINITY;
             }
       }
+      float2 raise[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float e = scale_exponent(vs[i][k].x);
+          raise[i][k] = make_float2(e, e);
+        }
       bool moved = false;
       float2 fade[kTiles], ref[kTiles];
 #pragma unroll
       for (int nt = 0; nt < kTiles; ++nt) {
-        float2 m = make_float2(-INFINITY, -INFINITY);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float e = scale_exponent(vs[i][k].x);
-            const float2 v = __fadd2_rn(s[i][nt][k], make_float2(e, e));
-            m.x = fmaxf(m.x, v.x);
-            m.y = fmaxf(m.y, v.y);
-          }
+        const float2 v0 = __fadd2_rn(s[0][nt][0], raise[0][0]), v1 = __fadd2_rn(s[0][nt][1], raise[0][1]);
+        const float2 v2 = __fadd2_rn(s[1][nt][0], raise[1][0]), v3 = __fadd2_rn(s[1][nt][1], raise[1][1]);
+        float2 m = make_float2(fmax3(v0.x, v1.x, fmaxf(v2.x, v3.x)), fmax3(v0.y, v1.y, fmaxf(v2.y, v3.y)));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
-          m.x = fmaxf(m.x, __shfl_xor_sync(0xFFFFFFFFu, m.x, d));
-          m.y = fmaxf(m.y, __shfl_xor_sync(0xFFFFFFFFu, m.y, d));
+          const float2 other = make_float2(__shfl_xor_sync(0xFFFFFFFFu, m.x, d), __shfl_xor_sync(0xFFFFFFFFu, m.y, d));
+          m.x = d < 16 ? fmaxf(m.x, other.x) : fmax3(m.x, other.x, top[nt][0]);
+          m.y = d < 16 ? fmaxf(m.y, other.y) : fmax3(m.y, other.y, top[nt][1]);
         }
         moved = moved || m.x > top[nt][0] || m.y > top[nt][1];
-        m.x = fmaxf(m.x, top[nt][0]);
-        m.y = fmaxf(m.y, top[nt][1]);
         ref[nt] = make_float2(m.x == -INFINITY ? 0.0F : kLift - m.x, m.y == -INFINITY ? 0.0F : kLift - m.y);
         fade[nt] = m;
       }
@@ -554,6 +565,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     copies_wait<0>();
 
     // The warps' parts, joined in the order of the warps.
+    __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
@@ -562,57 +574,54 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 4);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 8);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
+        const int r = nt * 8 + 2 * t + k;
         if (g == 0) {
-          stats[warp][0][nt * 8 + 2 * t + k] = top[nt][k];
-          stats[warp][1][nt * 8 + 2 * t + k] = l;
+          stats[warp][0][r] = top[nt][k];
+          stats[warp][1][r] = l;
         }
-      }
-    const bool whole = tile0 == 0 && tile1 == w.tiles;
-    float* partial = nullptr;
-    if (!whole)
-      partial = static_cast<float*>(a.workspace) + (2 * block + (tile0 == 0 ? 1 : 0)) * partial_floats(kRows, kDim);
-    constexpr int kHalf = kDim / 2;      // dimensions of one pass through shared memory
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      __syncthreads();
-      // Lanes with g / 4 == half hold dimensions of this half: tile word * 4 + nib of lane g is dimension
-      // g * kDim / 8 + 8 word + nib (and + 4).
-      if ((g >> 2) == half) {
+        // Lane g holds dimensions g * kDim / 8 and on: tile 4 word + nib is 8 word + nib, and + 4.
 #pragma unroll
         for (int word = 0; word < kValueWords; ++word)
 #pragma unroll
-          for (int nib = 0; nib < 4; ++nib)
-#pragma unroll
-            for (int nt = 0; nt < kTiles; ++nt)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                merge[warp][(nt * 8 + 2 * t + (k & 1)) * kHalfPitch + (g & 3) * (kDim / 8) + 8 * word + nib +
-                            4 * (k >> 1)] = o[4 * word + nib][nt][k];
+          for (int hi = 0; hi < 2; ++hi)
+            *reinterpret_cast<float4*>(&merge[warp][r * kPitch + g * (kDim / 8) + 8 * word + 4 * hi]) =
+                make_float4(o[4 * word][nt][2 * hi + k], o[4 * word + 1][nt][2 * hi + k], o[4 * word + 2][nt][2 * hi + k],
+                            o[4 * word + 3][nt][2 * hi + k]);
       }
-      __syncthreads();
-      for (int i = threadIdx.x; i < kRows * kHalf; i += kWarps * 32) {
-        const int r = i / kHalf, d = i - r * kHalf;
-        if (row0 + r >= all_rows) continue;
-        float m = -INFINITY, l = 0.0F, v = 0.0F;
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == w.tiles;
+    float* partial = static_cast<float*>(a.workspace) + (2 * block + (tile0 == 0 ? 1 : 0)) * partial_floats(kRows, kDim);
+    for (int i = threadIdx.x; i < kRows * kDim / 4; i += kWarps * 32) {
+      const int r = i / (kDim / 4), d = i % (kDim / 4) * 4;
+      if (row0 + r >= all_rows) continue;
+      float m = stats[0][0][r], l = 0.0F;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) m = fmaxf(m, stats[k][0][r]);
+      for (int k = 1; k < kWarps; ++k) m = fmaxf(m, stats[k][0][r]);
+      float4 v = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-          const float f = fade_to(stats[k][0][r], m);
-          l += f * stats[k][1][r];
-          v += f * merge[k][r * kHalfPitch + d];
-        }
-        if (whole) {
-          const int64_t row = (w.q.row0 + (row0 + r) / line.shared) * a.heads + head * line.shared + (row0 + r) % line.shared;
-          static_cast<T*>(a.out)[row * kDim + half * kHalf + d] = from_f32<T>(l == 0.0F ? 0.0F : v / l);
-          if (a.lse && half == 0 && d == 0)
-            a.lse[row] = log_sum(m, l);
-        } else {
-          partial[r * kDim + half * kHalf + d] = v;
-          if (half == 0 && d == 0) {
-            partial[kRows * kDim + 2 * r] = m;
-            partial[kRows * kDim + 2 * r + 1] = l;
-          }
+      for (int k = 0; k < kWarps; ++k) {
+        const float f = fade_to(stats[k][0][r], m);
+        const float4 x = *reinterpret_cast<const float4*>(&merge[k][r * kPitch + d]);
+        l += f * stats[k][1][r];
+        v.x += f * x.x;
+        v.y += f * x.y;
+        v.z += f * x.z;
+        v.w += f * x.w;
+      }
+      if (whole) {
+        const float inv = l == 0.0F ? 0.0F : 1.0F / l;
+        const int64_t row = (w.q.row0 + (row0 + r) / line.shared) * a.heads + head * line.shared + (row0 + r) % line.shared;
+        T* out = static_cast<T*>(a.out) + row * kDim + d;
+        out[0] = from_f32<T>(v.x * inv);
+        out[1] = from_f32<T>(v.y * inv);
+        out[2] = from_f32<T>(v.z * inv);
+        out[3] = from_f32<T>(v.w * inv);
+        if (a.lse && d == 0) a.lse[row] = log_sum(m, l);
+      } else {
+        *reinterpret_cast<float4*>(partial + r * kDim + d) = v;
+        if (d == 0) {
+          partial[kRows * kDim + 2 * r] = m;
+          partial[kRows * kDim + 2 * r + 1] = l;
         }
       }
     }
@@ -739,7 +748,7 @@ void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
   const Line line{c.heads, a.heads / c.heads, 8 * kTiles, c.page_shift, (starts & 15) == 0};
   constexpr int kShared = ring_bytes(kDim);
-  static_assert(kShared >= static_cast<int>(sizeof(float)) * kWarps * 8 * kTiles * (kDim / 2 + 2), "sums fit the ring");
+  static_assert(kShared >= static_cast<int>(sizeof(float)) * kWarps * 8 * kTiles * (kDim + 4), "sums fit the ring");
   allow_shared<kv4_attend_kernel<T, kDim, kTiles>>(kShared);
   kv4_attend_kernel<T, kDim, kTiles><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
   count_launch();
