@@ -170,18 +170,26 @@ __device__ __forceinline__ SequenceWork sequence_work(const Kv4Attend& a, const 
   return w;
 }
 
-// Units of all sequences, and those before sequence b: every thread of the block gets both.  as many
-// sequences at a time as the block has threads.
+// The workspace: where each sequence starts on the line ([batch + 1], the last is the line's end), then the blocks'
+// partial sums.
+__host__ __device__ __forceinline__ size_t starts_bytes(int64_t batch) {
+  return (static_cast<size_t>(batch + 1) * sizeof(int64_t) + 127) & ~static_cast<size_t>(127);
+}
+__device__ __forceinline__ float* line_parts(const Kv4Attend& a) {
+  return reinterpret_cast<float*>(static_cast<char*>(a.workspace) + starts_bytes(a.batch));
+}
+
+// Units of all sequences, the sequence that holds unit `first(total)` and the units before it, by all threads of
+// the block, as many sequences at a time as it has threads.  The first block writes the sequences' starts.
 struct Place {
   int64_t total;
-  int64_t before;   // units before the found sequence
+  int64_t before;
   int sequence;
 };
-// Finds the sequence that holds unit (range start) `first(total)`, or sums up to sequence `want` if want >= 0.
-template <int kWarpsHere, class F>
-__device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, int want, F first, int64_t* scratch) {
+template <class F>
+__device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, F first, int64_t* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int kBlock = kWarpsHere * 32;
+  constexpr int kBlock = kWarps * 32;
   int64_t mine = 0, total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kBlock) {
     mine = b0 + threadIdx.x < a.batch ? sequence_work(a, l, b0 + threadIdx.x).units(l) : 0;
@@ -193,9 +201,12 @@ __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, i
   __syncthreads();
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarpsHere; ++w) total += scratch[w];
-  Place p{total, 0, want >= 0 ? want : a.batch};
-  const int64_t target = want >= 0 ? -1 : first(total);
+  for (int w = 0; w < kWarps; ++w) total += scratch[w];
+  Place p{total, 0, a.batch};
+  const int64_t target = first(total);
+  const bool writes = blockIdx.x == 0 && a.workspace != nullptr;
+  int64_t* starts = static_cast<int64_t*>(a.workspace);
+  if (writes && threadIdx.x == 0) starts[a.batch] = total;
   int64_t carry = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kBlock) {
     if (a.batch > kBlock) mine = b0 + threadIdx.x < a.batch ? sequence_work(a, l, b0 + threadIdx.x).units(l) : 0;
@@ -207,25 +218,25 @@ __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, i
     }
     __syncthreads();
     if (lane == 31) scratch[warp] = upto;
-    if (threadIdx.x == 0) scratch[kWarpsHere] = -1;
+    if (threadIdx.x == 0) scratch[kWarps] = -1;
     __syncthreads();
     int64_t base = carry, chunk = 0;
 #pragma unroll
-    for (int w = 0; w < kWarpsHere; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) base += scratch[w];
       chunk += scratch[w];
     }
     const int64_t before = base + upto - mine;
-    const bool hit = want >= 0 ? b0 + static_cast<int>(threadIdx.x) == want : target >= before && target < before + mine;
-    if (hit) {
-      scratch[kWarpsHere] = before;
-      scratch[kWarpsHere + 1] = b0 + threadIdx.x;
+    if (writes && b0 + threadIdx.x < a.batch) starts[b0 + threadIdx.x] = before;
+    if (target >= before && target < before + mine) {
+      scratch[kWarps] = before;
+      scratch[kWarps + 1] = b0 + threadIdx.x;
     }
     __syncthreads();
-    if (scratch[kWarpsHere] >= 0) {
-      p.before = scratch[kWarpsHere];
-      p.sequence = static_cast<int>(scratch[kWarpsHere + 1]);
-      break;
+    if (scratch[kWarps] >= 0) {
+      p.before = scratch[kWarps];
+      p.sequence = static_cast<int>(scratch[kWarps + 1]);
+      if (!writes) break;
     }
     carry += chunk;
   }
@@ -267,8 +278,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
 
   const int64_t block = blockIdx.x;
-  const Place place = find_place<kWarps>(
-      a, line, -1, [&](int64_t total) { return range_start(total, block, ranges(total, gridDim.x)); }, scratch);
+  const Place place = find_place(
+      a, line, [&](int64_t total) { return range_start(total, block, ranges(total, gridDim.x)); }, scratch);
   const int64_t n = ranges(place.total, gridDim.x);
 #if __CUDA_ARCH__ >= 900
   cudaTriggerProgrammaticLaunchCompletion();
@@ -590,7 +601,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       }
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == w.tiles;
-    float* partial = static_cast<float*>(a.workspace) + (2 * block + (tile0 == 0 ? 1 : 0)) * partial_floats(kRows, kDim);
+    float* partial = line_parts(a) + (2 * block + (tile0 == 0 ? 1 : 0)) * partial_floats(kRows, kDim);
     for (int i = threadIdx.x; i < kRows * kDim / 4; i += kWarps * 32) {
       const int r = i / (kDim / 4), d = i % (kDim / 4) * 4;
       if (row0 + r >= all_rows) continue;
@@ -630,74 +641,105 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
   }
 }
 
-// Adds the partial sums of the segments that were cut, in the order of the line.  A thread owns four dimensions of
-// a row; the parts' weights (2 to the distance of their references from the largest) are formed once, so that the
-// loads of the parts do not wait for one another.
-constexpr int kParts = 64;  // parts whose weights are held at a time
+// Adds the partial sums of the segments that were cut.  A warp adds the parts of one output row, or, where
+// segments have many parts, each of a block's kJoinWarps warps adds every kJoinWarps-th of one row's and the first
+// adds the warps' sums: in either case in an order that the cut alone decides.
+constexpr int kJoinWarps = 8;
 template <class T, int kDim, int kTiles>
-__global__ void __launch_bounds__(2 * kDim * kTiles) kv4_join_kernel(Kv4View c, Kv4Attend a, Line line, int64_t blocks) {
-  constexpr int kRows = 8 * kTiles, kThreads = 2 * kDim * kTiles;  // kRows * kDim / 4
-  __shared__ int64_t scratch[kThreads / 32 + 2];
-  __shared__ float weight[kParts][kRows];
-  __shared__ float stats[2][kRows];
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(Kv4View c, Kv4Attend a, Line line, int64_t blocks,
+                                                                  int warps_per_row) {
+  constexpr int kRows = 8 * kTiles, kPer = kDim / 32;
+  __shared__ float sums[kJoinWarps][kDim + 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x;
-  const Place place = find_place<kThreads / 32>(a, line, b, [](int64_t) { return int64_t{0}; }, scratch);
   const SequenceWork w = sequence_work(a, line, b);
-  const int64_t n = ranges(place.total, blocks);
 #if __CUDA_ARCH__ >= 900
   cudaGridDependencySynchronize();
 #endif
-  for (int64_t segment = blockIdx.y; segment < static_cast<int64_t>(c.heads) * w.blocks; segment += gridDim.y) {
-    const int64_t u0 = place.before + segment * w.tiles, u1 = u0 + w.tiles;
-    const int64_t c0 = range_of(place.total, u0, n), c1 = range_of(place.total, u1 - 1, n);
-    if (c0 == c1) continue;
-    const int head = static_cast<int>(segment / w.blocks), row0 = static_cast<int>(segment % w.blocks) * kRows;
-    // Part k of the segment: the last of the block where the segment starts, the first of the others.
-    const float* base = static_cast<const float*>(a.workspace);
-    auto part = [&](int64_t k) {
-      return base + (2 * k + (k == c0 ? 1 : 0)) * partial_floats(kRows, kDim);
-    };
-    __syncthreads();
-    if (threadIdx.x < kRows) {
-      float m = -INFINITY, l = 0.0F;
+  const int64_t* line_starts = reinterpret_cast<const int64_t*>(a.workspace);
+  const int64_t before = line_starts[b], total = line_starts[a.batch], n = ranges(total, blocks);
+  const float* base = line_parts(a);
+  const int rows_per_block = kJoinWarps / warps_per_row, group = warp % warps_per_row;
+  const int64_t rows = static_cast<int64_t>(w.q.rows) * a.heads;
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.y) * rows_per_block; i0 < rows; i0 += static_cast<int64_t>(gridDim.y) * rows_per_block) {
+    // Output row i is query row i / heads, head i % heads.
+    const int64_t i = i0 + warp / warps_per_row;
+    const bool mine = i < rows;
+    const int row = static_cast<int>(mine ? i / a.heads : 0), q_head = static_cast<int>(mine ? i % a.heads : 0);
+    const int r = row * line.shared + q_head % line.shared;
+    const int64_t segment = static_cast<int64_t>(q_head / line.shared) * w.blocks + r / kRows;
+    const int64_t u0 = before + segment * w.tiles, u1 = u0 + w.tiles;
+    const int64_t c0 = range_of(total, u0, n), c1 = range_of(total, u1 - 1, n);
+    float m = -INFINITY, l = 0.0F, v[kPer];
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) v[d] = 0.0F;
+    if (mine && c0 != c1) {
+      // Part k of the segment: the last of the block where the segment starts, the first of the others.
+      const float* first = base + (2 * c0 + 1) * partial_floats(kRows, kDim);
+      const float* other = base + 2 * c0 * partial_floats(kRows, kDim);
+      const int parts = static_cast<int>(c1 - c0) + 1, rr = r % kRows;
+      for (int k0 = group; k0 < parts; k0 += 32 * warps_per_row) {
+        // 32 parts at a time: lane k holds the k-th's reference and sum.
+        const int k = k0 + lane * warps_per_row;
+        const float* p = k == 0 ? first : other + 2 * static_cast<int64_t>(k) * partial_floats(kRows, kDim);
+        float2 st = make_float2(-INFINITY, 0.0F);
+        if (k < parts) st = *reinterpret_cast<const float2*>(p + kRows * kDim + 2 * rr);
+        float next = st.x;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) next = fmaxf(next, __shfl_xor_sync(0xFFFFFFFFu, next, d));
+        next = fmaxf(next, m);
+        const float old = fade_to(m, next), f = fade_to(st.x, next);
+        l *= old;
+        m = next;
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) v[d] *= old;
+        const int here = min(32, (parts - k0 + warps_per_row - 1) / warps_per_row);
 #pragma unroll 8
-      for (int64_t k = c0; k <= c1; ++k) m = fmaxf(m, part(k)[kRows * kDim + 2 * threadIdx.x]);
-#pragma unroll 8
-      for (int64_t k = c0; k <= c1; ++k) {
-        const float2 s = *reinterpret_cast<const float2*>(part(k) + kRows * kDim + 2 * threadIdx.x);
-        l += s.y * fade_to(s.x, m);
+        for (int j = 0; j < here; ++j) {
+          const int64_t at = k0 + static_cast<int64_t>(j) * warps_per_row;
+          const float* x = (at == 0 ? first : other + 2 * at * partial_floats(kRows, kDim)) + rr * kDim + lane * kPer;
+          const float fj = __shfl_sync(0xFFFFFFFFu, f, j);
+          l += fj * __shfl_sync(0xFFFFFFFFu, st.y, j);
+          float e[kPer];
+          if constexpr (kPer == 2) {
+            *reinterpret_cast<float2*>(e) = *reinterpret_cast<const float2*>(x);
+          } else {
+#pragma unroll
+            for (int d = 0; d < kPer; d += 4) *reinterpret_cast<float4*>(e + d) = *reinterpret_cast<const float4*>(x + d);
+          }
+#pragma unroll
+          for (int d = 0; d < kPer; ++d) v[d] += fj * e[d];
+        }
       }
-      stats[0][threadIdx.x] = m;
-      stats[1][threadIdx.x] = l;
     }
-    __syncthreads();
-    const int r = threadIdx.x / (kDim / 4), d = threadIdx.x % (kDim / 4) * 4;
-    float4 v = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-    for (int64_t k0 = c0; k0 <= c1; k0 += kParts) {
-      const int parts = static_cast<int>(min(static_cast<int64_t>(kParts), c1 - k0 + 1));
-      for (int i = threadIdx.x; i < parts * kRows; i += kThreads)
-        weight[i / kRows][i % kRows] = fade_to(part(k0 + i / kRows)[kRows * kDim + 2 * (i % kRows)], stats[0][i % kRows]);
+    if (warps_per_row > 1) {
       __syncthreads();
-#pragma unroll 8
-      for (int k = 0; k < parts; ++k) {
-        const float4 x = *reinterpret_cast<const float4*>(part(k0 + k) + r * kDim + d);
-        const float f = weight[k][r];
-        v.x += f * x.x;
-        v.y += f * x.y;
-        v.z += f * x.z;
-        v.w += f * x.w;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) sums[warp][lane * kPer + d] = v[d];
+      if (lane == 0) sums[warp][kDim] = m, sums[warp][kDim + 1] = l;
+      __syncthreads();
+      if (group != 0) continue;
+      float top = m;
+      for (int k = 1; k < warps_per_row; ++k) top = fmaxf(top, sums[warp + k][kDim]);
+      const float f0 = fade_to(m, top);
+      l *= f0;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) v[d] *= f0;
+      for (int k = 1; k < warps_per_row; ++k) {
+        const float f = fade_to(sums[warp + k][kDim], top);
+        l += f * sums[warp + k][kDim + 1];
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) v[d] += f * sums[warp + k][lane * kPer + d];
       }
-      __syncthreads();
+      m = top;
     }
-    if (row0 + r < w.q.rows * line.shared) {
-      const float l = stats[1][r], inv = l == 0.0F ? 0.0F : 1.0F / l;
-      const int64_t row = (w.q.row0 + (row0 + r) / line.shared) * a.heads + head * line.shared + (row0 + r) % line.shared;
-      T* out = static_cast<T*>(a.out) + row * kDim + d;
-      out[0] = from_f32<T>(v.x * inv);
-      out[1] = from_f32<T>(v.y * inv);
-      out[2] = from_f32<T>(v.z * inv);
-      out[3] = from_f32<T>(v.w * inv);
-      if (a.lse && d == 0) a.lse[row] = log_sum(stats[0][r], l);
+    if (mine && c0 != c1) {
+      const float inv = l == 0.0F ? 0.0F : 1.0F / l;
+      const int64_t at = (w.q.row0 + row) * a.heads + q_head;
+      T* out = static_cast<T*>(a.out) + at * kDim + lane * kPer;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) out[d] = from_f32<T>(v[d] * inv);
+      if (a.lse && lane == 0) a.lse[at] = log_sum(m, l);
     }
   }
 }
@@ -754,17 +796,22 @@ void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
   count_launch();
   check(cudaGetLastError(), "launch cache attention kernel");
   if ((static_cast<int64_t>(a.max_pages) << c.page_shift) <= kTile) return;  // no segment can be cut
+  const int64_t rows = static_cast<int64_t>(a.max_rows) * a.heads;
   const int64_t segments = c.heads * ((static_cast<int64_t>(a.max_rows) * line.shared + line.block_rows - 1) / line.block_rows);
+  // Eight warps a row where a segment has 16 parts or more on average, each adding two or more.
+  const int warps_per_row = s.blocks >= 16 * segments * a.batch ? kJoinWarps : 1;
+  const int64_t blocks_y = (rows * warps_per_row + kJoinWarps - 1) / kJoinWarps;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.batch), static_cast<unsigned>(std::min<int64_t>(segments, 65535)));
-  cfg.blockDim = dim3(2 * kDim * kTiles);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.batch), static_cast<unsigned>(std::min<int64_t>(blocks_y, 65535)));
+  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  check(cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, kDim, kTiles>, c, a, line, s.blocks), "launch cache attention join kernel");
+  check(cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, kDim, kTiles>, c, a, line, s.blocks, warps_per_row),
+        "launch cache attention join kernel");
   count_launch();
 }
 
@@ -787,7 +834,7 @@ size_t kv4_attend_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
   if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0) return 0;
   if ((static_cast<int64_t>(a.max_pages) << c.page_shift) <= kTile) return 0;
   const Shape s = shape_of(c, a);
-  return sizeof(float) * 2 * static_cast<size_t>(s.blocks) * partial_floats(8 * s.tiles, c.dim);
+  return starts_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(s.blocks) * partial_floats(8 * s.tiles, c.dim);
 }
 
 void launch_kv4_attend(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
