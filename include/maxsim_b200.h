@@ -311,7 +311,7 @@ int msb_kv4_append_device(const msb_kv4_cache* cache, const void* keys, const vo
                           int64_t tokens, int64_t key_token_stride, int64_t key_head_stride,
                           int64_t value_token_stride, int64_t value_head_stride, const int64_t* slots, void* stream);
 /* Reads slots back: code * scale, rounded once to `type`, into contiguous
- * [tokens, kv_heads, head_dim] arrays; zeros for a slot outside the cache. */
+ * [tokens, kv_heads, head_dim] arrays on 16-byte boundaries; zeros for a slot outside the cache. */
 int msb_kv4_read_device(const msb_kv4_cache* cache, const int64_t* slots, int64_t tokens, int32_t type, void* keys,
                         void* values, void* stream);
 

@@ -1496,6 +1496,11 @@ int element_type(int32_t type, bool f32) {
   throw InvalidArgument(f32 ? "type must be fp32, fp16 or bf16" : "type must be fp16 or bf16");
 }
 
+void check_tokens(int64_t tokens, const Kv4View& v) {
+  if (tokens < 0) throw InvalidArgument("tokens must not be negative");
+  if (tokens > ((int64_t{1} << 31) - 1) / v.heads) throw InvalidArgument("tokens * kv_heads must be below 2^31");
+}
+
 Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   if (!a) throw InvalidArgument("arguments are NULL");
   if (a->rows < 0 || a->batch < 0 || a->max_pages < 0 || a->max_query_rows < 0)
@@ -1549,7 +1554,7 @@ int msb_kv4_append_device(const msb_kv4_cache* cache, const void* keys, const vo
     const Kv4View v = kv4_view(cache);
     Kv4Append a{};
     a.type = element_type(type, true);
-    if (tokens < 0) throw InvalidArgument("tokens must not be negative");
+    check_tokens(tokens, v);
     if (tokens == 0) return;
     if (!keys || !values || !slots) throw InvalidArgument("NULL argument");
     a.x[0] = keys;
@@ -1571,9 +1576,11 @@ int msb_kv4_read_device(const msb_kv4_cache* cache, const int64_t* slots, int64_
     const Kv4View v = kv4_view(cache);
     Kv4Read a{};
     a.type = element_type(type, true);
-    if (tokens < 0) throw InvalidArgument("tokens must not be negative");
+    check_tokens(tokens, v);
     if (tokens == 0) return;
     if (!keys || !values || !slots) throw InvalidArgument("NULL argument");
+    if ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15)
+      throw InvalidArgument("keys and values must be 16-byte aligned");
     a.out[0] = keys;
     a.out[1] = values;
     a.slots = slots;

@@ -157,6 +157,8 @@ class Int4KVCache:
                 _on(t, name, self.device, out[0].dtype)
                 if t.shape != shape or not t.is_contiguous():
                     raise ValueError(f"{name} must be contiguous with shape {list(shape)}")
+                if t.data_ptr() % 16:
+                    raise ValueError(f"{name} must be 16-byte aligned")
         check(lib.msb_kv4_read_device(self._ref, slots.data_ptr(), shape[0], kind, out[0].data_ptr(), out[1].data_ptr(),
                                       self._stream()))
         return tuple(out)

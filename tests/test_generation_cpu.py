@@ -46,7 +46,7 @@ def test_cache_is_checked_by_every_entry_point(kw, text):
 
 def test_append_and_read_arguments():
     for kw, text in ((dict(keys=None), "NULL"), (dict(slots=None), "NULL"), (dict(type=7), "type must be"),
-                     (dict(tokens=-1), "tokens")):
+                     (dict(tokens=-1), "tokens"), (dict(tokens=1 << 31), "tokens")):
         with pytest.raises(ValueError, match=text):
             check(_append(_cache(), **kw))
     with pytest.raises(ValueError, match="cache is NULL"):

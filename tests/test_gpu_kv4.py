@@ -322,7 +322,7 @@ def test_range_of_bf16(size):
 def test_values_of_very_different_sizes():
     """Scales of values from 1e-6 to 1e6 in one sequence, and zero vectors among small ones."""
     cache = m.Int4KVCache(8, 16, 1, 64)
-    v = _normal((128, 1, 64), 2) * torch.logspace(-6, 6, 128, device="cuda")[torch.randperm(128)].view(-1, 1, 1)
+    v = _normal((128, 1, 64), 2) * torch.logspace(-6, 6, 128, device="cuda")[torch.randperm(128, generator=torch.Generator().manual_seed(9))].view(-1, 1, 1)
     cache.append(_normal((128, 1, 64), 3), v, torch.arange(128, device="cuda"))
     table = torch.arange(8, dtype=torch.int32, device="cuda").view(1, 8)
     q = _normal((1, 4, 64), 4, torch.float16)
