@@ -5,6 +5,9 @@
 Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` into
 ``maxsim_b200/libmaxsim_b200.so`` (static cudart, so the library does not
 depend on which libcudart torch bundles).  nvcc cross-compiles without a GPU.
+``csrc/generation_binding.cpp`` becomes ``maxsim_b200/_generation.so``, the
+Python module between torch and the library's cache and weight operators
+(g++, torch's own headers and libraries).
 """
 
 from __future__ import annotations
@@ -18,6 +21,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmaxsim_b200.so"
+BINDING_SRC = CSRC / "generation_binding.cpp"
+BINDING = PKG / "_generation.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
               "-Xptxas", "-warn-spills"]
@@ -35,10 +40,10 @@ def sources() -> list[Path]:
 
 
 def needs_build() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not BINDING.exists():
         return True
-    mtime = LIB.stat().st_mtime
-    deps = sources() + sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "maxsim_b200.h"]
+    mtime = min(LIB.stat().st_mtime, BINDING.stat().st_mtime)
+    deps = sources() + [BINDING_SRC] + sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "maxsim_b200.h"]
     return any(p.stat().st_mtime > mtime for p in deps if p.exists())
 
 
@@ -70,7 +75,26 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objs), "-cudart", "static"]
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
+    build_binding()
     return LIB
+
+
+def build_binding() -> Path:
+    import sysconfig
+
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{base / 'include'}",
+           f"-I{base / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(BINDING_SRC), "-o", str(tmp), f"-L{base / 'lib'}", f"-L{PKG}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 if __name__ == "__main__":

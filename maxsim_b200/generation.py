@@ -12,20 +12,25 @@ There is no backward pass: codes have no gradient, and these are the operators o
 from __future__ import annotations
 
 import ctypes
-import math
 
-torch = _lib = lib = check = None
+torch = _lib = lib = check = _native = None
 
 
 def _load():
-    """Import torch and the CUDA library, once, when the first object is made (the package imports without them)."""
-    global torch, _lib, lib, check
-    if _lib is None:
+    """Import torch, the CUDA library and the module between them, once, when the first object is made (the package
+    imports without them)."""
+    global torch, _lib, lib, check, _native
+    if _native is None:
         import torch as torch_module
         from maxsim_b200 import _lib as lib_module
 
-        torch, lib, check = torch_module, lib_module.lib, lib_module.check
-        _lib = lib_module
+        try:
+            from maxsim_b200 import _generation
+        except ImportError as error:
+            raise ImportError("maxsim_b200/_generation.so is missing or does not load: build it with "
+                              "`python -m maxsim_b200.build`") from error
+        torch, _lib, lib, check = torch_module, lib_module, lib_module.lib, lib_module.check
+        _native = _generation
 
 
 def _type_id(dtype, allowed="fp32, fp16 or bf16"):
@@ -103,26 +108,11 @@ class Int4KVCache:
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = pages, heads, size, 2 * half
         self._c = _lib.Kv4Cache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), pages,
                                 size, heads, 2 * half, device.index)
-        self._ref = ctypes.byref(self._c)
+        self._address = ctypes.addressof(self._c)
 
     @property
     def resident_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales))
-
-    def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _vectors(self, x, name, tokens=None):
-        _on(x, name, self.device, ndim=3)
-        if x.shape[1] != self.num_kv_heads or x.shape[2] != self.head_dim:
-            raise ValueError(f"{name} must have shape [tokens, {self.num_kv_heads}, {self.head_dim}], got {list(x.shape)}")
-        if tokens is not None and x.shape[0] != tokens:
-            raise ValueError("keys, values and slots must have the same number of tokens")
-        return x if x.stride(2) == 1 else x.contiguous()
-
-    def _slots(self, slots):
-        _on(slots, "slots", self.device, torch.int64, 1)
-        return slots if slots.is_contiguous() else slots.contiguous()
 
     def append(self, keys, values, slots) -> None:
         """Quantise ``keys`` and ``values`` ``[tokens, kv_heads, head_dim]`` (fp32, fp16 or bf16, any token and
@@ -131,37 +121,13 @@ class Int4KVCache:
         Per vector: ``scale = max|x| * fl(1/7)`` (0 becomes 1), ``code = clip(rint(x / scale), -7, 7)``.  A vector with
         a value that is not finite stores scale NaN and codes 0.  A slot outside the cache (-1, say) is skipped; a
         slot must not be given twice in one call."""
-        slots = self._slots(slots)
-        tokens = slots.shape[0]
-        keys, values = self._vectors(keys, "keys", tokens), self._vectors(values, "values", tokens)
-        if keys.dtype != values.dtype:
-            raise ValueError("keys and values must have the same dtype")
-        check(lib.msb_kv4_append_device(self._ref, keys.data_ptr(), values.data_ptr(), _type_id(keys.dtype), tokens,
-                                        keys.stride(0), keys.stride(1), values.stride(0), values.stride(1),
-                                        slots.data_ptr(), self._stream()))
+        _native.append(self._address, keys, values, slots)
 
     def read(self, slots, *, dtype=None, out=None):
         """``(keys, values)`` of int64 ``slots`` as ``[tokens, kv_heads, head_dim]`` of ``dtype`` (bf16 by default):
-        ``code * scale`` rounded once; zeros for a slot outside the cache.  ``out``: a pair of contiguous tensors."""
-        slots = self._slots(slots)
-        shape = (slots.shape[0], self.num_kv_heads, self.head_dim)
-        if out is None:
-            dtype = torch.bfloat16 if dtype is None else dtype
-            kind = _type_id(dtype)
-            out = (torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device))
-        else:
-            kind = _type_id(out[0].dtype)
-            if dtype is not None and dtype != out[0].dtype:
-                raise ValueError("out must have the given dtype")
-            for name, t in zip(("out[0]", "out[1]"), out):
-                _on(t, name, self.device, out[0].dtype)
-                if t.shape != shape or not t.is_contiguous():
-                    raise ValueError(f"{name} must be contiguous with shape {list(shape)}")
-                if t.data_ptr() % 16:
-                    raise ValueError(f"{name} must be 16-byte aligned")
-        check(lib.msb_kv4_read_device(self._ref, slots.data_ptr(), shape[0], kind, out[0].data_ptr(), out[1].data_ptr(),
-                                      self._stream()))
-        return tuple(out)
+        ``code * scale`` rounded once; zeros for a slot outside the cache.  ``out``: a pair of contiguous tensors
+        on 16-byte boundaries."""
+        return _native.read(self._address, slots, dtype, out)
 
     def slots(self, page_table, sequences, positions):
         """int64 slots of ``positions`` of ``sequences`` (tensors of one shape) under ``page_table``."""
@@ -184,65 +150,8 @@ class Int4KVCache:
         Returns ``[rows, heads, head_dim]`` in the query's dtype, with ``return_lse`` also the fp32 natural
         log-sum-exp ``[rows, heads]`` (-inf where nothing is seen), with which results over parts of a context
         can be joined."""
-        device = self.device
-        _on(query, "query", device, ndim=3)
-        kind = _type_id(query.dtype, "fp16 or bf16")
-        rows, heads, dim = query.shape
-        if dim != self.head_dim or heads == 0 or heads % self.num_kv_heads:
-            raise ValueError(f"query must have shape [rows, a multiple of {self.num_kv_heads}, {self.head_dim}], got "
-                             f"{list(query.shape)}")
-        if query.stride(2) != 1:
-            query = query.contiguous()
-        _on(page_table, "page_table", device, torch.int32, 2)
-        _on(lengths, "lengths", device, torch.int32, 1)
-        batch, pages = page_table.shape
-        if lengths.shape[0] != batch:
-            raise ValueError("page_table and lengths must have the same batch")
-        if pages > 1 and page_table.stride(1) != 1:
-            page_table = page_table.contiguous()
-        if not lengths.is_contiguous():
-            lengths = lengths.contiguous()
-        if query_offsets is None:
-            if rows != batch:
-                raise ValueError("without query_offsets, query must have one row per sequence")
-            if max_query_tokens not in (None, 1):
-                raise ValueError("max_query_tokens needs query_offsets")
-            most = 1
-        else:
-            _on(query_offsets, "query_offsets", device, torch.int32, 1)
-            if query_offsets.shape[0] != batch + 1:
-                raise ValueError("query_offsets must have shape [batch + 1]")
-            if not query_offsets.is_contiguous():
-                query_offsets = query_offsets.contiguous()
-            most = rows if max_query_tokens is None else int(max_query_tokens)
-            if most < 0:
-                raise ValueError("max_query_tokens must not be negative")
-        if window is not None and (int(window) < 1 or not causal):
-            raise ValueError("window must be at least 1 and needs causal")
-        scale = dim ** -0.5 if scale is None else float(scale)
-        if not (scale > 0.0 and math.isfinite(scale)):
-            raise ValueError("scale must be finite and > 0")
-        shape = (rows, heads, dim)
-        if out is None:
-            out = torch.empty(shape, dtype=query.dtype, device=device)
-        else:
-            _on(out, "out", device, query.dtype)
-            if out.shape != shape or not out.is_contiguous():
-                raise ValueError(f"out must be contiguous with shape {list(shape)}")
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=device) if return_lse else None
-        args = _lib.Kv4AttendArgs(
-            query.data_ptr(), query.stride(0), query.stride(1), rows, page_table.data_ptr(), page_table.stride(0),
-            lengths.data_ptr(), None if query_offsets is None else query_offsets.data_ptr(), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), None, 0, batch, pages, most, heads, kind, 1 if causal else 0,
-            int(window or 0), scale)
-        ref = ctypes.byref(args)
-        need = ctypes.c_int64()
-        check(lib.msb_kv4_attend_workspace_bytes(self._ref, ref, ctypes.byref(need)))
-        if need.value:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-            args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
-        check(lib.msb_kv4_attend_device(self._ref, ref, self._stream()))
-        return (out, lse) if return_lse else out
+        return _native.attend(self._address, query, page_table, lengths, query_offsets, max_query_tokens, scale, causal,
+                              window, return_lse, out)
 
 
 def _check_cache_sizes(page_size, head_dim):
@@ -250,6 +159,19 @@ def _check_cache_sizes(page_size, head_dim):
         raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
     if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
         raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+
+
+class _Linear(ctypes.Structure):  # as csrc/generation_binding.cpp reads it
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("group", ctypes.c_int32),
+        ("bias_type", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+    ]
 
 
 class Int4Linear:
@@ -289,6 +211,10 @@ class Int4Linear:
             check(lib.msb_w4_pack_device(codes.data_ptr(), scales.data_ptr(), self.out_features, self.in_features,
                                          self.group_size, self._codes.data_ptr(), self._scales.data_ptr(),
                                          torch.cuda.current_stream().cuda_stream))
+        self._c = _Linear(self._codes.data_ptr(), self._scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                          self.out_features, self.in_features, self.group_size,
+                          -1 if bias is None else _type_id(bias.dtype, "fp16 or bf16"), self.device.index)
+        self._address = ctypes.addressof(self._c)
 
     @classmethod
     def from_weight(cls, weight, *, group_size=128, bias=None):
@@ -318,25 +244,4 @@ class Int4Linear:
 
     def __call__(self, x, *, out=None):
         """``x`` ``[..., in]`` (fp16 or bf16) to ``[..., out]``; sums are fp32, rounded once."""
-        _on(x, "x", self.device)
-        kind = _type_id(x.dtype, "fp16 or bf16")
-        if x.dim() < 1 or x.shape[-1] != self.in_features:
-            raise ValueError(f"x must have shape [..., {self.in_features}], got {list(x.shape)}")
-        if self.bias is not None and self.bias.dtype != x.dtype:
-            raise ValueError("bias and x must have the same dtype")
-        lead = x.shape[:-1]
-        rows = x if x.dim() == 2 else x.reshape(-1, self.in_features)
-        if rows.stride(1) != 1:
-            rows = rows.contiguous()
-        if out is None:
-            out = torch.empty(lead + (self.out_features,), dtype=x.dtype, device=self.device)
-        else:
-            _on(out, "out", self.device, x.dtype)
-            if out.shape != lead + (self.out_features,) or not out.is_contiguous():
-                raise ValueError(f"out must be contiguous with shape {list(lead) + [self.out_features]}")
-        check(lib.msb_w4_product_device(
-            self._codes.data_ptr(), self._scales.data_ptr(), self.out_features, self.in_features, self.group_size,
-            rows.data_ptr(), rows.stride(0), rows.shape[0], None if self.bias is None else self.bias.data_ptr(),
-            out.data_ptr(), self.out_features, kind, self.device.index,
-            torch.cuda.current_stream(self.device).cuda_stream))
-        return out
+        return _native.linear(self._address, x, out)
