@@ -33,6 +33,9 @@
 #include "quant4.cuh"
 
 namespace msb {
+bool kv4_chunk_supported(const Kv4View&);
+void launch_kv4_chunk(const Kv4View&, const Kv4Attend&, cudaStream_t);
+
 namespace {
 
 constexpr int kWarps = 4;
@@ -828,10 +831,15 @@ void launch_typed(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
   }
 }
 
+constexpr int kManyRows = 64;
+bool many_rows(const Kv4View& c, const Kv4Attend& a) {
+  return kv4_chunk_supported(c) && static_cast<int64_t>(a.max_rows) * (a.heads / c.heads) >= kManyRows;
+}
+
 }  // namespace
 
 size_t kv4_attend_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
-  if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0) return 0;
+  if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0 || many_rows(c, a)) return 0;
   if ((static_cast<int64_t>(a.max_pages) << c.page_shift) <= kTile) return 0;
   const Shape s = shape_of(c, a);
   return starts_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(s.blocks) * partial_floats(8 * s.tiles, c.dim);
@@ -839,6 +847,10 @@ size_t kv4_attend_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
 
 void launch_kv4_attend(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
   if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0) return;
+  if (many_rows(c, a)) {
+    launch_kv4_chunk(c, a, stream);
+    return;
+  }
   const Shape s = shape_of(c, a);
   if (a.type == kElemF16) launch_typed<__half>(c, a, s, stream);
   else launch_typed<__nv_bfloat16>(c, a, s, stream);

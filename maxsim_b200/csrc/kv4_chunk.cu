@@ -1,0 +1,672 @@
+// Attention of many query rows over the 4-bit key/value cache (prompt chunks), on the 5th-generation tensor cores.
+//
+// The operator and its formulas: kv4_attend.cu.  A block owns one sequence, one key/value head and 256 rows (query
+// tokens times the query heads that share the head), and walks the 128-token tiles that its rows see.
+//   Bound: the exponentials (16 a clock and SM) and the products (two of 128 x 128 x D per 128 rows), about equal at
+//   D = 128; then instruction issue.
+//   Products.  S = Q K^T from shared memory (tcgen05.mma, fp16, 128 x 128 x D, fp32 in tensor memory), O += P V with P
+//   (fp16) read back from tensor memory over S.  The 256 rows are two tiles of 128: while one's softmax runs, the
+//   other's products do.
+//   Operands.  Four warps unpack keys and four unpack values, each code once per block, to exact fp16 integers in the
+//   128-byte-swizzled layout of the products: keys as [token][dimension] (dimensions in the order of a word's nibble
+//   pairs, queries alike), values as [dimension][token] - their nibbles are paired by tokens (byte permutes of two
+//   tokens' words), so nothing is transposed.  Codes are loaded a tile ahead into registers.
+//   Softmax.  A thread owns a row.  Scales of keys and values are fp32 factors of scores and probabilities (they would
+//   lose digits in fp16 operands); the reference is the running maximum of s_j + log2(vs_j) as in kv4_attend.cu,
+//   moved (and the sums rescaled) only when it is passed by 2^8, which fp16 holds.
+// Every wait is bounded; a block that gives up writes NaN rows.
+#include <algorithm>
+#include <atomic>
+#include <climits>
+
+#include "quant4.cuh"
+
+namespace msb {
+namespace {
+
+constexpr int kTokens = 128;         // of a tile
+constexpr int kRowsTile = 128;       // rows of one accumulator
+constexpr int kBlockRows = 256;
+constexpr int kSoftWarps = 8;        // warps 0-3: first row tile, 4-7: second
+constexpr int kKeyWarp0 = 8;         // warps 8-11: keys and the tiles' scales
+constexpr int kValueWarp0 = 12;      // warps 12-15: values
+constexpr int kMmaWarp = 16;
+constexpr int kThreads = 17 * 32;
+constexpr int kStages = 2;
+constexpr float kExponents = 110.0F;
+constexpr float kLift = 4.0F;        // references lie 2^4 below where they were set
+constexpr float kSlack = 8.0F;       // and may be passed by 2^8: probabilities stay below 2^13
+constexpr uint64_t kTimeoutNs = 4000000000ull;
+
+template <int kDim>
+struct Layout {
+  static constexpr int kQBytes = kRowsTile * kDim * 2;         // one row tile
+  static constexpr int kTileBytes = kTokens * kDim * 2;        // one tile of keys, or of values
+  static constexpr int off_q = 0;
+  static constexpr int off_k = off_q + 2 * kQBytes;
+  static constexpr int off_v = off_k + kStages * kTileBytes;
+  static constexpr int off_meta = off_v + kStages * kTileBytes;  // [stage][3][128]: key scales, value scales, their log2
+  static constexpr int off_flags = off_meta + kStages * 3 * kTokens * 4;  // [stage][4]: some token is not seen
+  static constexpr int off_bars = off_flags + kStages * 16;
+  static constexpr int kUsed = off_bars + 24 * 8 + 1024;        // and room to align to 1024
+  // A block takes all of an SM's tensor memory: more than half of its shared memory keeps a second one away.
+  static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ uint64_t global_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+// False when the wait was given up (here or elsewhere in the block).
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t it = 0;; ++it) {
+    if (mbar_try(bar, parity)) return true;
+    if ((it & 7u) == 7u) {
+      if (*abort_flag) return false;
+      if (global_ns() - t0 > kTimeoutNs) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// K-major, 128-byte swizzle: 1024 bytes between groups of 8 rows.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&f)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&f)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(f[0]),
+      "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]), "f"(f[8]), "f"(f[9]), "f"(f[10]),
+      "f"(f[11]), "f"(f[12]), "f"(f[13]), "f"(f[14]), "f"(f[15]), "f"(f[16]), "f"(f[17]), "f"(f[18]), "f"(f[19]),
+      "f"(f[20]), "f"(f[21]), "f"(f[22]), "f"(f[23]), "f"(f[24]), "f"(f[25]), "f"(f[26]), "f"(f[27]), "f"(f[28]),
+      "f"(f[29]), "f"(f[30]), "f"(f[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float scale_exponent(float s) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fminf(fmaxf(r, -kExponents), kExponents);
+}
+__device__ __forceinline__ float fade_to(float from, float to) { return from == to ? 1.0F : exp2_fast(from - to); }
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Nibbles kI and kI + 4 of a word as an exact fp16 pair (kv4_attend.cu).
+template <int kI>
+__device__ __forceinline__ uint32_t codes_exact(uint32_t w) {
+  constexpr uint32_t kMask = kI & 1 ? 0x00f000f0u : 0x000f000fu, kFlip = kI & 1 ? 0x54805480u : 0x64086408u;
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n sub.rn.f16x2 %0, %0, %3;" : "=&r"(r) : "r"(kI < 2 ? w : w >> 8), "n"(kMask), "r"(kFlip));
+  return r;
+}
+// Byte of 16-byte chunk `chunk` of row `row` in a tile of 128-byte rows, 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
+  return static_cast<uint32_t>((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void store16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+template <class T, int kDim>
+__global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4Attend a, int shared, int row_blocks,
+                                                                bool aligned) {
+  using L = Layout<kDim>;
+  extern __shared__ unsigned char raw_smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // Later row blocks see more tokens under a causal mask: they start first.
+  const int64_t per_block = static_cast<int64_t>(a.batch) * c.heads;
+  const int block = row_blocks - 1 - static_cast<int>(blockIdx.x / per_block);
+  const int b = static_cast<int>(blockIdx.x % per_block / c.heads), head = static_cast<int>(blockIdx.x % c.heads);
+  const Kv4Sequence q = kv4_sequence(a, c.page_shift, b);
+  const int64_t all_rows = static_cast<int64_t>(q.rows) * shared, block_row0 = static_cast<int64_t>(block) * kBlockRows;
+  if (block_row0 >= all_rows) return;
+  const int row_count = static_cast<int>(min(static_cast<int64_t>(kBlockRows), all_rows - block_row0));
+  const int tiles_m = row_count > kRowsTile ? 2 : 1;
+  // Tokens that some row of the block sees, and the tiles over them.
+  const int pos0 = q.length - q.rows + static_cast<int>(block_row0 / shared);
+  const int pos1 = q.length - q.rows + static_cast<int>((block_row0 + row_count - 1) / shared);
+  const int any_last = a.causal ? pos1 : q.length - 1;
+  const int any_first = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+  const int begin = any_first & ~15;
+  const int tiles = any_last >= any_first ? (any_last - begin) / kTokens + 1 : 0;
+
+  unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
+  const uint32_t base = smem_u32(smem);
+  float* const meta = reinterpret_cast<float*>(smem + L::off_meta);
+  uint32_t* const flags = reinterpret_cast<uint32_t*>(smem + L::off_flags);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::off_bars);
+  uint64_t* const k_full = bars;           // [stage] keys and scales written
+  uint64_t* const k_empty = bars + 2;      // [stage] products over the keys done
+  uint64_t* const v_full = bars + 4;
+  uint64_t* const v_empty = bars + 6;
+  uint64_t* const meta_empty = bars + 8;   // [stage] scales read by every softmax warp
+  uint64_t* const s_full = bars + 10;      // [row tile] scores ready (and the sums of the tile before)
+  uint64_t* const p_full = bars + 12;      // [row tile] probabilities written
+  uint64_t* const o_full = bars + 14;      // all sums done
+  uint64_t* const q_full = bars + 15;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(bars + 17);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 4);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 4);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&meta_empty[s], 4 * tiles_m);
+    }
+    for (int m = 0; m < 2; ++m) {
+      mbar_init(&s_full[m], 1);
+      mbar_init(&p_full[m], 4);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(q_full, 4 * tiles_m);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // Tensor memory: scores of the row tiles at columns 0 and 128 (probabilities over them), sums at 256 and 384.
+
+  const int32_t* const pages = a.page_table + b * a.table_stride;
+  const int page_mask = (1 << c.page_shift) - 1;
+  // Vector of token j's 16-token group on page p (-1: none), and whether the page is the cache's.
+  auto ask_page = [&](int j) { return j <= any_last ? __ldg(pages + (j >> c.page_shift)) : -1; };
+  auto vector_of = [&](int page, int j) {
+    return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages)
+               ? (static_cast<int64_t>(static_cast<uint32_t>(page) * c.heads + head) << c.page_shift) + (j & page_mask)
+               : int64_t{0};
+  };
+
+  if (warp < kSoftWarps) {
+    // =================== softmax: a thread owns a row ===================
+    const int m = warp >> 2;
+    if (m < tiles_m) {
+      const int r = m * kRowsTile + (warp & 3) * 32 + lane;
+      const int64_t row = block_row0 + r;
+      const bool live = r < row_count;
+      const int64_t out_row = (q.row0 + (live ? row / shared : 0)) * a.heads + head * shared + (live ? row % shared : 0);
+      // The row of the query tile: scaled by a power of two to a maximum in [2^10, 2^11), fp16, in the codes' order.
+      float factor;
+      {
+        const T* x = static_cast<const T*>(a.query) + (q.row0 + (live ? row / shared : 0)) * a.q_row_stride +
+                     (head * shared + (live ? row % shared : 0)) * a.q_head_stride;
+        float top = 0.0F;
+        auto load8 = [&](int d, float (&v)[8]) {
+          if (aligned) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + d));
+            const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = live ? to_f32(e[i]) : 0.0F;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = live ? to_f32(x[d + i]) : 0.0F;
+          }
+        };
+#pragma unroll 4
+        for (int d = 0; d < kDim; d += 8) {
+          float v[8];
+          load8(d, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+        }
+        const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+        const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
+        factor = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
+#pragma unroll 4
+        for (int d = 0; d < kDim; d += 8) {
+          float v[8];
+          load8(d, v);
+          store16(base + L::off_q + m * L::kQBytes + (d >> 6) * (kRowsTile * 128) +
+                      swizzled((warp & 3) * 32 + lane, (d & 63) >> 3),
+                  pack_half2(v[0] * down, v[4] * down), pack_half2(v[1] * down, v[5] * down),
+                  pack_half2(v[2] * down, v[6] * down), pack_half2(v[3] * down, v[7] * down));
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      const float2 factor2 = make_float2(factor, factor);
+      const int pos = q.length - q.rows + static_cast<int>(row / shared);
+      const int last = live ? (a.causal ? pos : q.length - 1) : INT_MAX;
+      const int first = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's quarter of the lanes
+      const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + 256 + m * 128;
+      float top = -INFINITY;
+      float2 sum = make_float2(0.0F, 0.0F);
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int s = i & 1, j0 = begin + i * kTokens;
+        ok = mbar_wait(&k_full[s], (i >> 1) & 1, abort_flag) && mbar_wait(&s_full[m], i & 1, abort_flag);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const float4* const key_scale = reinterpret_cast<const float4*>(meta + s * 3 * kTokens);
+        const float4* const value_scale = key_scale + kTokens / 4;
+        const float4* const raise = value_scale + kTokens / 4;
+        const uint4 flag = *reinterpret_cast<const uint4*>(flags + 4 * s);
+        const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < first ||
+                                                       j0 + kTokens - 1 > last);
+        float best = -INFINITY;
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+          float x[32];
+          tmem_ld32(s_at + 32 * part, x);
+          if (!masked) {
+            float b0 = -INFINITY, b1 = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 ks = key_scale[part * 8 + k], e = raise[part * 8 + k];
+              const float2 u0 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k], x[4 * k + 1]), make_float2(ks.x, ks.y)), factor2,
+                                           make_float2(e.x, e.y));
+              const float2 u1 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k + 2], x[4 * k + 3]), make_float2(ks.z, ks.w)),
+                                           factor2, make_float2(e.z, e.w));
+              b0 = fmax3(b0, u0.x, u0.y);
+              b1 = fmax3(b1, u1.x, u1.y);
+            }
+            best = fmax3(best, b0, b1);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int j = j0 + part * 32 + k;
+              const float ks = meta[s * 3 * kTokens + part * 32 + k], e = meta[(s * 3 + 2) * kTokens + part * 32 + k];
+              if (e != -INFINITY && j >= first && j <= last) best = fmaxf(best, x[k] * ks * factor + e);
+            }
+          }
+        }
+        // best is -inf where the row sees nothing, or nothing but NaN
+        if (__any_sync(0xFFFFFFFFu, best > top + kSlack)) {
+          const float next = fmaxf(top, best), f = fade_to(top, next);
+          top = next;
+          sum = __fmul2_rn(sum, make_float2(f, f));
+          if (i > 0) {
+#pragma unroll
+            for (int part = 0; part < kDim / 32; ++part) {
+              float x[32];
+              tmem_ld32(o_at + 32 * part, x);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[k] *= f;
+              tmem_st32(o_at + 32 * part, x);
+            }
+          }
+        }
+        const float ref = top == -INFINITY ? 0.0F : kLift - top;
+        const float2 ref2 = make_float2(ref, ref);
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+          float x[32];
+          uint32_t p[16];
+          tmem_ld32(s_at + 32 * part, x);
+          if (!masked) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 ks = key_scale[part * 8 + k], vs = value_scale[part * 8 + k];
+              const float2 u0 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k], x[4 * k + 1]), make_float2(ks.x, ks.y)), factor2, ref2);
+              const float2 u1 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k + 2], x[4 * k + 3]), make_float2(ks.z, ks.w)), factor2, ref2);
+              const float2 p0 = make_float2(exp2_fast(u0.x), exp2_fast(u0.y));
+              const float2 p1 = make_float2(exp2_fast(u1.x), exp2_fast(u1.y));
+              sum = __fadd2_rn(sum, __fadd2_rn(p0, p1));
+              const float2 v0 = __fmul2_rn(p0, make_float2(vs.x, vs.y)), v1 = __fmul2_rn(p1, make_float2(vs.z, vs.w));
+              p[2 * k] = pack_half2(v0.x, v0.y);
+              p[2 * k + 1] = pack_half2(v1.x, v1.y);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float v[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int at = part * 32 + k + h, j = j0 + at;
+                const float ks = meta[s * 3 * kTokens + at], vs = meta[(s * 3 + 1) * kTokens + at];
+                const bool seen = meta[(s * 3 + 2) * kTokens + at] != -INFINITY && j >= first && j <= last;
+                const float pr = seen ? exp2_fast(x[k + h] * ks * factor + ref) : 0.0F;
+                sum.x += pr;
+                v[h] = seen ? pr * vs : 0.0F;
+              }
+              p[k / 2] = pack_half2(v[0], v[1]);
+            }
+          }
+          tmem_st16(s_at + 16 * part, p);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&p_full[m]);
+          mbar_arrive(&meta_empty[s]);
+        }
+      }
+      // The row's output.
+      const float l = sum.x + sum.y, inv = l == 0.0F ? 0.0F : 1.0F / l;
+      if (ok && tiles > 0) ok = mbar_wait(o_full, 0, abort_flag);
+      ok = __all_sync(0xFFFFFFFFu, ok) && !*abort_flag;
+      tc_fence_after();
+#pragma unroll
+      for (int part = 0; part < kDim / 32; ++part) {
+        float x[32];
+        if (ok && tiles > 0) tmem_ld32(o_at + 32 * part, x);
+        __align__(16) T e[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) e[k] = from_f32<T>(!ok ? NAN : l == 0.0F ? 0.0F : x[k] * inv);
+        if (live) {
+          T* out = static_cast<T*>(a.out) + out_row * kDim + 32 * part;
+          if ((reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) reinterpret_cast<uint4*>(out)[k] = reinterpret_cast<const uint4*>(e)[k];
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) out[k] = e[k];
+          }
+        }
+      }
+      if (a.lse && live)
+        a.lse[out_row] = !ok ? NAN : l == 0.0F ? -INFINITY : ((top == -INFINITY ? 0.0F : top - kLift) + __log2f(l)) * 0.693147181F;
+    }
+  } else if (warp < kValueWarp0) {
+    // =================== keys: lane (g, t) unpacks 16 bytes t of tokens g, g + 8, .. of its warp's 32 ===================
+    const int kw = warp - kKeyWarp0, g = lane >> 2, t = lane & 3;
+    constexpr int kWords = kDim / 32;   // of a token, per lane
+    uint32_t word[4][kWords];
+    float ks = 0.0F, vs = 0.0F;
+    bool seen = false;
+    int page[2] = {ask_page(begin + 32 * kw), ask_page(begin + 32 * kw + 16)};
+    auto load_tile = [&](int i) {
+      const int j = begin + i * kTokens + 32 * kw;
+      const int64_t v[2] = {vector_of(page[0], j), vector_of(page[1], j + 16)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint8_t* src = c.codes[0] + (v[k >> 1] + 8 * (k & 1) + g) * (kDim / 2) + t * (kDim / 8);
+        if constexpr (kWords == 4) {
+          const uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
+          word[k][0] = u.x, word[k][1] = u.y, word[k][2] = u.z, word[k][3] = u.w;
+        } else {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(src));
+          word[k][0] = u.x, word[k][1] = u.y;
+        }
+      }
+      const int mine = j + lane;
+      const int64_t at = (lane < 16 ? v[0] : v[1]) + (lane & 15);
+      seen = static_cast<uint32_t>(lane < 16 ? page[0] : page[1]) < static_cast<uint32_t>(c.num_pages) &&
+             mine >= any_first && mine <= any_last;
+      ks = __ldg(c.scales[0] + at);
+      vs = __ldg(c.scales[1] + at);
+      page[0] = ask_page(j + kTokens);
+      page[1] = ask_page(j + kTokens + 16);
+    };
+    if (tiles > 0) load_tile(0);
+    for (int i = 0; i < tiles; ++i) {
+      const int s = i & 1;
+      if (i >= kStages) {
+        const uint32_t parity = ((i >> 1) - 1) & 1;
+        const bool ok = mbar_wait(&k_empty[s], parity, abort_flag) && mbar_wait(&meta_empty[s], parity, abort_flag);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      }
+      const uint32_t dst = base + L::off_k + s * L::kTileBytes;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int token = 32 * kw + 8 * k + g;
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
+          // Lanes two apart lie in the two halves of a row: they take their words in another order, off the same banks.
+          const int jj = kWords == 4 ? j ^ (t & 2) : j;
+          uint32_t w = word[k][j];
+          if constexpr (kWords == 4) w = (t & 2) ? word[k][j ^ 2] : w;
+          const int at = t * kWords + jj;  // word of the row
+          store16(dst + (at >> 3) * (kTokens * 128) + swizzled(token, at & 7), codes_exact<0>(w), codes_exact<1>(w),
+                  codes_exact<2>(w), codes_exact<3>(w));
+        }
+      }
+      float* const ms = meta + s * 3 * kTokens + 32 * kw + lane;
+      ms[0] = seen ? ks : 0.0F;
+      ms[kTokens] = seen ? vs : 0.0F;
+      ms[2 * kTokens] = seen ? scale_exponent(vs) : -INFINITY;
+      const uint32_t all = __ballot_sync(0xFFFFFFFFu, seen);
+      if (lane == 0) flags[4 * s + kw] = ~all;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[s]);
+      if (i + 1 < tiles) load_tile(i + 1);
+    }
+  } else if (warp < kMmaWarp) {
+    // =================== values: a lane unpacks 8 tokens x 8 or 16 dimensions ===================
+    const int vw = warp - kValueWarp0;
+    constexpr int kWords = kDim / 64;                       // 8-dimension words of a token, per lane
+    const int group = (vw >> 1) * 8 + (lane & 7);           // its 8 tokens
+    const int piece = (vw & 1) * 4 + (lane >> 3);           // its words: piece * kWords and on
+    uint32_t word[8][kWords];
+    int page = ask_page(begin + (group >> 1) * 16);
+    auto load_tile = [&](int i) {
+      const int j = begin + i * kTokens + (group >> 1) * 16;
+      const uint8_t* src = c.codes[1] + (vector_of(page, j) + 8 * (group & 1)) * (kDim / 2) + piece * (4 * kWords);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if constexpr (kWords == 2) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + k * (kDim / 2)));
+          word[k][0] = u.x, word[k][1] = u.y;
+        } else {
+          word[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * (kDim / 2)));
+        }
+      }
+      page = ask_page(j + kTokens);
+    };
+    if (tiles > 0) load_tile(0);
+    for (int i = 0; i < tiles; ++i) {
+      const int s = i & 1;
+      if (i >= kStages) {
+        const bool ok = mbar_wait(&v_empty[s], ((i >> 1) - 1) & 1, abort_flag);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      }
+      // Row of a dimension: 64 tokens, 128 bytes; this lane's 8 tokens are one 16-byte chunk.
+      const uint32_t dst = base + L::off_v + s * L::kTileBytes + (group >> 3) * (kDim * 128);
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) {
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[k] = __byte_perm(word[2 * k][j], word[2 * k + 1][j], 0x5410);
+          y[k] = __byte_perm(word[2 * k][j], word[2 * k + 1][j], 0x7632);
+        }
+        const int d = (piece * kWords + j) * 8, chunk = group & 7;
+        store16(dst + swizzled(d + 0, chunk), codes_exact<0>(x[0]), codes_exact<0>(x[1]), codes_exact<0>(x[2]), codes_exact<0>(x[3]));
+        store16(dst + swizzled(d + 1, chunk), codes_exact<1>(x[0]), codes_exact<1>(x[1]), codes_exact<1>(x[2]), codes_exact<1>(x[3]));
+        store16(dst + swizzled(d + 2, chunk), codes_exact<2>(x[0]), codes_exact<2>(x[1]), codes_exact<2>(x[2]), codes_exact<2>(x[3]));
+        store16(dst + swizzled(d + 3, chunk), codes_exact<3>(x[0]), codes_exact<3>(x[1]), codes_exact<3>(x[2]), codes_exact<3>(x[3]));
+        store16(dst + swizzled(d + 4, chunk), codes_exact<0>(y[0]), codes_exact<0>(y[1]), codes_exact<0>(y[2]), codes_exact<0>(y[3]));
+        store16(dst + swizzled(d + 5, chunk), codes_exact<1>(y[0]), codes_exact<1>(y[1]), codes_exact<1>(y[2]), codes_exact<1>(y[3]));
+        store16(dst + swizzled(d + 6, chunk), codes_exact<2>(y[0]), codes_exact<2>(y[1]), codes_exact<2>(y[2]), codes_exact<2>(y[3]));
+        store16(dst + swizzled(d + 7, chunk), codes_exact<3>(y[0]), codes_exact<3>(y[1]), codes_exact<3>(y[2]), codes_exact<3>(y[3]));
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[s]);
+      if (i + 1 < tiles) load_tile(i + 1);
+    }
+  } else if (lane == 0 && tiles > 0) {
+    // =================== products: one thread issues ===================
+    constexpr uint32_t kInstrS = (1u << 4) | (static_cast<uint32_t>(kTokens >> 3) << 17) | (8u << 24);
+    constexpr uint32_t kInstrO = (1u << 4) | (static_cast<uint32_t>(kDim >> 3) << 17) | (8u << 24);
+    auto scores = [&](int m, int s) {
+#pragma unroll
+      for (int k = 0; k < kDim / 16; ++k) {  // 16 dimensions: 32 bytes of a 128-byte row
+        const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
+        mma_ss(tmem + m * 128, operand_desc(base + L::off_q + m * L::kQBytes + at),
+               operand_desc(base + L::off_k + s * L::kTileBytes + at), kInstrS, k > 0);
+      }
+    };
+    auto sums = [&](int m, int s, bool add) {
+#pragma unroll
+      for (int k = 0; k < kTokens / 16; ++k) {
+        const uint32_t at = (k >> 2) * (kDim * 128) + (k & 3) * 32;
+        mma_ts(tmem + 256 + m * 128, tmem + m * 128 + 8 * k, operand_desc(base + L::off_v + s * L::kTileBytes + at), kInstrO,
+               add || k > 0);
+      }
+    };
+    bool ok = mbar_wait(q_full, 0, abort_flag) && mbar_wait(&k_full[0], 0, abort_flag);
+    if (ok) {
+      tc_fence_after();
+      for (int m = 0; m < tiles_m; ++m) {
+        scores(m, 0);
+        mma_commit(&s_full[m]);
+      }
+      mma_commit(&k_empty[0]);
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int s = i & 1, next = (i + 1) & 1;
+        ok = mbar_wait(&v_full[s], (i >> 1) & 1, abort_flag);
+        for (int m = 0; m < tiles_m && ok; ++m) {
+          ok = mbar_wait(&p_full[m], i & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          sums(m, s, i > 0);
+          if (m == tiles_m - 1) mma_commit(&v_empty[s]);
+          if (i + 1 < tiles) {
+            if (m == 0) ok = mbar_wait(&k_full[next], ((i + 1) >> 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            scores(m, next);
+            mma_commit(&s_full[m]);
+            if (m == tiles_m - 1) mma_commit(&k_empty[next]);
+          }
+        }
+      }
+      if (ok) mma_commit(o_full);
+    }
+  }
+  __syncwarp();
+  // After a wait was given up, products under way end by themselves: time for that before the tensor memory is freed.
+  if (warp == kMmaWarp && *abort_flag) {
+    const uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 2000000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <auto kernel>
+void allow_shared(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  check(cudaGetDevice(&dev), "get device");
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory of the chunk attention kernel");
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+template <class T, int kDim>
+void launch_dim(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
+  const int shared = a.heads / c.heads;
+  const int64_t row_blocks = (static_cast<int64_t>(a.max_rows) * shared + kBlockRows - 1) / kBlockRows;
+  const int64_t blocks = row_blocks * a.batch * c.heads;
+  if (blocks > INT_MAX) throw InvalidArgument("batch * heads * query rows are too many for one call");
+  const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
+                          static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
+  allow_shared<kv4_chunk_kernel<T, kDim>>(Layout<kDim>::kBytes);
+  kv4_chunk_kernel<T, kDim><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
+      c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
+  count_launch();
+  check(cudaGetLastError(), "launch chunk attention kernel");
+}
+
+template <class T>
+void launch_typed(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
+  if (c.dim == 64) launch_dim<T, 64>(c, a, stream);
+  else launch_dim<T, 128>(c, a, stream);
+}
+
+}  // namespace
+
+// Head dimension 256 would need 768 columns of tensor memory.
+bool kv4_chunk_supported(const Kv4View& c) { return c.dim <= 128; }
+
+void launch_kv4_chunk(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
+  if (a.type == kElemF16) launch_typed<__half>(c, a, stream);
+  else launch_typed<__nv_bfloat16>(c, a, stream);
+}
+
+}  // namespace msb
