@@ -28,14 +28,15 @@ constexpr int kTokens = 128;         // of a tile
 constexpr int kRowsTile = 128;       // rows of one accumulator
 constexpr int kBlockRows = 256;
 constexpr int kSoftWarps = 8;        // warps 0-3: first row tile, 4-7: second
-constexpr int kKeyWarp0 = 8;         // warps 8-11: keys and the tiles' scales
-constexpr int kValueWarp0 = 12;      // warps 12-15: values
-constexpr int kMmaWarp = 16;
-constexpr int kThreads = 17 * 32;
+constexpr int kUnpackWarp0 = 8;      // warps 8-11: keys, the tiles' scales, values
+constexpr int kMmaWarp = 12;
+constexpr int kThreads = 13 * 32;
 constexpr int kStages = 2;
 constexpr float kExponents = 110.0F;
-constexpr float kLift = 4.0F;        // references lie 2^4 below where they were set
-constexpr float kSlack = 8.0F;       // and may be passed by 2^8: probabilities stay below 2^13
+constexpr float kLift = 4.0F;        // a reference is set 2^4 below the largest p vs seen
+constexpr float kMostP = 16384.0F;   // and kept while p vs stays below 2^14, which fp16 holds
+constexpr int kMetaPitch = 20;       // floats of the 16 columns (of 64) that one lane in four reads
+constexpr int kMetaFloats = 2 * 4 * kMetaPitch;
 constexpr uint64_t kTimeoutNs = 4000000000ull;
 
 template <int kDim>
@@ -45,9 +46,10 @@ struct Layout {
   static constexpr int off_q = 0;
   static constexpr int off_k = off_q + 2 * kQBytes;
   static constexpr int off_v = off_k + kStages * kTileBytes;
-  static constexpr int off_meta = off_v + kStages * kTileBytes;  // [stage][3][128]: key scales, value scales, their log2
-  static constexpr int off_flags = off_meta + kStages * 3 * kTokens * 4;  // [stage][4]: some token is not seen
-  static constexpr int off_bars = off_flags + kStages * 16;
+  static constexpr int off_meta = off_v + kStages * kTileBytes;  // [stage][3]: key scales, value scales, their log2
+  static constexpr int off_flags = off_meta + kStages * 3 * kMetaFloats * 4;  // [stage][4]: some token is not seen
+  static constexpr int off_rows = off_flags + kStages * 16;      // [256] factors, then references; [256] sums
+  static constexpr int off_bars = off_rows + 2 * kBlockRows * 4;
   static constexpr int kUsed = off_bars + 24 * 8 + 1024;        // and room to align to 1024
   // A block takes all of an SM's tensor memory: more than half of its shared memory keeps a second one away.
   static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
@@ -76,7 +78,10 @@ __device__ __forceinline__ uint64_t global_ns() {
 }
 // False when the wait was given up (here or elsewhere in the block).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_try(bar, parity)) return true;
+  // A try sleeps in hardware until the phase ends or a while has passed; the clock, slow to read, comes after some.
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i)
+    if (mbar_try(bar, parity)) return true;
   const uint64_t t0 = global_ns();
   for (uint32_t it = 0;; ++it) {
     if (mbar_try(bar, parity)) return true;
@@ -97,21 +102,31 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
   return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1) << 16) |
          (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Issued by the one lane whose `leader` is not 0, in converged code: operands stay warp-uniform.
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r;
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&f)[32]) {
   uint32_t r[32];
@@ -127,9 +142,25 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&f)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&f)[32]) {
+// 16 lanes x 64 columns: thread t receives, for j = 0..7, columns 8j + 2 (t % 4) + {0, 1} of lane t / 4 in f[4j],
+// f[4j + 1] and of lane t / 4 + 8 in f[4j + 2], f[4j + 3].
+__device__ __forceinline__ void tmem_ld16x64(uint32_t taddr, float (&f)[32]) {
+  uint32_t r[32];
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16x64(uint32_t taddr, const float (&f)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(f[0]),
       "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]), "f"(f[8]), "f"(f[9]), "f"(f[10]),
       "f"(f[11]), "f"(f[12]), "f"(f[13]), "f"(f[14]), "f"(f[15]), "f"(f[16]), "f"(f[17]), "f"(f[18]), "f"(f[19]),
@@ -137,11 +168,22 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&f)[32]) 
       "f"(f[29]), "f"(f[30]), "f"(f[31]), "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+// 16 lanes x 32 columns: thread t holds, for j = 0..7, column 4j + t % 4 of lane t / 4 in r[2j], of t / 4 + 8 in r[2j + 1]:
+// the fp16 pairs of what tmem_ld16x64 gave.
+__device__ __forceinline__ void tmem_st16x32(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x128b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      " tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -181,6 +223,70 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
 }
 __device__ __forceinline__ void store16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Where column `c` of a tile keeps its scale: the 16 of each 64 columns that one lane reads lie together.
+__device__ __forceinline__ int meta_at(int c) {
+  return (c >> 6) * (4 * kMetaPitch) + ((c >> 1) & 3) * kMetaPitch + ((c >> 3) & 7) * 2 + (c & 1);
+}
+
+// What a thread keeps of its two rows of a 16-lane half.
+struct Rows {
+  float2 factor[2];   // scale * log2(e) * the row's power of two, twice
+  float2 ref[2];      // 2^-(reference), as an exponent, twice
+  float2 sum[2];      // of p, the thread's columns
+  int first[2], last[2];
+};
+
+// Scores (f: two rows x 16 columns) to probabilities times value scales, fp16 pairs; the largest into `most`.
+template <bool kMasked>
+__device__ __forceinline__ void probabilities(const float (&f)[32], const float* meta, int j0, const Rows& rows, uint32_t (&p)[16],
+                                              float2 (&add)[2], float (&most)[2]) {
+  add[0] = add[1] = make_float2(0.0F, 0.0F);
+  most[0] = most[1] = 0.0F;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const float4 ks4 = *reinterpret_cast<const float4*>(meta + 2 * j);
+    const float4 vs4 = *reinterpret_cast<const float4*>(meta + kMetaFloats + 2 * j);
+    float4 e4 = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+    if (kMasked) e4 = *reinterpret_cast<const float4*>(meta + 2 * kMetaFloats + 2 * j);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 ks = h ? make_float2(ks4.z, ks4.w) : make_float2(ks4.x, ks4.y);
+      const float2 vs = h ? make_float2(vs4.z, vs4.w) : make_float2(vs4.x, vs4.y);
+      const float2 e = h ? make_float2(e4.z, e4.w) : make_float2(e4.x, e4.y);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int at = 4 * (j + h) + 2 * r;
+        const float2 x = __ffma2_rn(__fmul2_rn(make_float2(f[at], f[at + 1]), ks), rows.factor[r], rows.ref[r]);
+        float2 pr = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+        float2 pv = __fmul2_rn(pr, vs);
+        if (kMasked) {
+          const int c = j0 + 8 * (j + h);
+          if (e.x == -INFINITY || c < rows.first[r] || c > rows.last[r]) pr.x = pv.x = 0.0F;
+          if (e.y == -INFINITY || c + 1 < rows.first[r] || c + 1 > rows.last[r]) pr.y = pv.y = 0.0F;
+        }
+        add[r] = __fadd2_rn(add[r], pr);
+        most[r] = fmax3(most[r], pv.x, pv.y);
+        p[2 * (j + h) + r] = pack_half2(pv.x, pv.y);
+      }
+    }
+  }
+}
+// The largest s + log2(vs) of the thread's seen columns, per row; -inf where there are none (or nothing but NaN).
+__device__ __forceinline__ void references(const float (&f)[32], const float* meta, int j0, const Rows& rows, float (&best)[2]) {
+  best[0] = best[1] = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float ks = meta[2 * j + k], e = meta[2 * kMetaFloats + 2 * j + k];
+      const int c = j0 + 8 * j + k;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        if (e != -INFINITY && c >= rows.first[r] && c <= rows.last[r])
+          best[r] = fmaxf(best[r], f[4 * j + 2 * r + k] * ks * rows.factor[r].x + e);
+    }
 }
 
 template <class T, int kDim>
@@ -307,14 +413,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
       }
-      const float2 factor2 = make_float2(factor, factor);
-      const int pos = q.length - q.rows + static_cast<int>(row / shared);
-      const int last = live ? (a.causal ? pos : q.length - 1) : INT_MAX;
-      const int first = live && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      // From here to the output a thread works on two rows of each 16-lane half of its warp's 32: lane / 4 and + 8,
+      // 32 of a tile's columns, so that a column's scales serve four rows.
+      float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + (warp & 3) * 32;
+      float* const row_sum = row_factor + kBlockRows;
+      row_factor[lane] = factor;
+      __syncwarp();
+      Rows half[2];
+      float top[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int mine = 16 * h + 8 * k + (lane >> 2), at = m * kRowsTile + (warp & 3) * 32 + mine;
+          const int pos = q.length - q.rows + static_cast<int>((block_row0 + at) / shared);
+          half[h].factor[k] = make_float2(row_factor[mine], row_factor[mine]);
+          half[h].ref[k] = half[h].sum[k] = make_float2(0.0F, 0.0F);
+          half[h].last[k] = at < row_count ? (a.causal ? pos : q.length - 1) : INT_MAX;
+          half[h].first[k] = at < row_count && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+          top[h][k] = -INFINITY;
+        }
+      const int every_last = min(min(half[0].last[0], half[0].last[1]), min(half[1].last[0], half[1].last[1]));
+      const int every_first = max(max(half[0].first[0], half[0].first[1]), max(half[1].first[0], half[1].first[1]));
       const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's quarter of the lanes
       const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + 256 + m * 128;
-      float top = -INFINITY;
-      float2 sum = make_float2(0.0F, 0.0F);
       bool ok = true;
       for (int i = 0; i < tiles && ok; ++i) {
         const int s = i & 1, j0 = begin + i * kTokens;
@@ -324,92 +446,67 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           break;
         }
         tc_fence_after();
-        const float4* const key_scale = reinterpret_cast<const float4*>(meta + s * 3 * kTokens);
-        const float4* const value_scale = key_scale + kTokens / 4;
-        const float4* const raise = value_scale + kTokens / 4;
         const uint4 flag = *reinterpret_cast<const uint4*>(flags + 4 * s);
-        const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < first ||
-                                                       j0 + kTokens - 1 > last);
-        float best = -INFINITY;
+        const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < every_first ||
+                                                       j0 + kTokens - 1 > every_last);
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+          const float* const my_meta = meta + s * 3 * kMetaFloats + part * (4 * kMetaPitch) + (lane & 3) * kMetaPitch;
+          const int my_j0 = j0 + 64 * part + 2 * (lane & 3);
 #pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          float x[32];
-          tmem_ld32(s_at + 32 * part, x);
-          if (!masked) {
-            float b0 = -INFINITY, b1 = -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t half_lanes = static_cast<uint32_t>(h) << 20;  // 16 lanes on
+            float x[32], most[2];
+            float2 add[2];
+            uint32_t p[16];
+            tmem_ld16x64(s_at + half_lanes + 64 * part, x);
+            if (masked) probabilities<true>(x, my_meta, my_j0, half[h], p, add, most);
+            else probabilities<false>(x, my_meta, my_j0, half[h], p, add, most);
+            // A row without a reference yet, or one whose reference has become too low (an infinite p among it).
+            const bool low = top[h][0] == -INFINITY || top[h][1] == -INFINITY || most[0] > kMostP || most[1] > kMostP;
+            if (__any_sync(0xFFFFFFFFu, low)) {
+              tmem_wait_st();  // what was written before is read below
+              float best[2];
+              references(x, my_meta, my_j0, half[h], best);
+              float2 fade[2];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float4 ks = key_scale[part * 8 + k], e = raise[part * 8 + k];
-              const float2 u0 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k], x[4 * k + 1]), make_float2(ks.x, ks.y)), factor2,
-                                           make_float2(e.x, e.y));
-              const float2 u1 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k + 2], x[4 * k + 3]), make_float2(ks.z, ks.w)),
-                                           factor2, make_float2(e.z, e.w));
-              b0 = fmax3(b0, u0.x, u0.y);
-              b1 = fmax3(b1, u1.x, u1.y);
-            }
-            best = fmax3(best, b0, b1);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int j = j0 + part * 32 + k;
-              const float ks = meta[s * 3 * kTokens + part * 32 + k], e = meta[(s * 3 + 2) * kTokens + part * 32 + k];
-              if (e != -INFINITY && j >= first && j <= last) best = fmaxf(best, x[k] * ks * factor + e);
-            }
-          }
-        }
-        // best is -inf where the row sees nothing, or nothing but NaN
-        if (__any_sync(0xFFFFFFFFu, best > top + kSlack)) {
-          const float next = fmaxf(top, best), f = fade_to(top, next);
-          top = next;
-          sum = __fmul2_rn(sum, make_float2(f, f));
-          if (i > 0) {
-#pragma unroll
-            for (int part = 0; part < kDim / 32; ++part) {
-              float x[32];
-              tmem_ld32(o_at + 32 * part, x);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] *= f;
-              tmem_st32(o_at + 32 * part, x);
-            }
-          }
-        }
-        const float ref = top == -INFINITY ? 0.0F : kLift - top;
-        const float2 ref2 = make_float2(ref, ref);
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          float x[32];
-          uint32_t p[16];
-          tmem_ld32(s_at + 32 * part, x);
-          if (!masked) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float4 ks = key_scale[part * 8 + k], vs = value_scale[part * 8 + k];
-              const float2 u0 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k], x[4 * k + 1]), make_float2(ks.x, ks.y)), factor2, ref2);
-              const float2 u1 = __ffma2_rn(__fmul2_rn(make_float2(x[4 * k + 2], x[4 * k + 3]), make_float2(ks.z, ks.w)), factor2, ref2);
-              const float2 p0 = make_float2(exp2_fast(u0.x), exp2_fast(u0.y));
-              const float2 p1 = make_float2(exp2_fast(u1.x), exp2_fast(u1.y));
-              sum = __fadd2_rn(sum, __fadd2_rn(p0, p1));
-              const float2 v0 = __fmul2_rn(p0, make_float2(vs.x, vs.y)), v1 = __fmul2_rn(p1, make_float2(vs.z, vs.w));
-              p[2 * k] = pack_half2(v0.x, v0.y);
-              p[2 * k + 1] = pack_half2(v1.x, v1.y);
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float v[2];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int at = part * 32 + k + h, j = j0 + at;
-                const float ks = meta[s * 3 * kTokens + at], vs = meta[(s * 3 + 1) * kTokens + at];
-                const bool seen = meta[(s * 3 + 2) * kTokens + at] != -INFINITY && j >= first && j <= last;
-                const float pr = seen ? exp2_fast(x[k + h] * ks * factor + ref) : 0.0F;
-                sum.x += pr;
-                v[h] = seen ? pr * vs : 0.0F;
+              for (int k = 0; k < 2; ++k) {
+                best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 1));
+                best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 2));
+                const float next = fmaxf(top[h][k], best[k]), f = fade_to(top[h][k], next);
+                fade[k] = make_float2(f, f);
+                top[h][k] = next;
+                const float ref = next == -INFINITY ? 0.0F : kLift - next;
+                half[h].ref[k] = make_float2(ref, ref);
+                half[h].sum[k] = __fmul2_rn(half[h].sum[k], fade[k]);
               }
-              p[k / 2] = pack_half2(v[0], v[1]);
+              if (i > 0) {  // the sums of the tiles before
+#pragma unroll 1
+                for (int d = 0; d < kDim; d += 64) {
+                  float o[32];
+                  tmem_ld16x64(o_at + half_lanes + d, o);
+#pragma unroll
+                  for (int k = 0; k < 32; ++k) o[k] *= fade[(k >> 1) & 1].x;
+                  tmem_st16x64(o_at + half_lanes + d, o);
+                }
+              }
+              if (part > 0) {  // and the probabilities of the columns before
+                uint32_t w[16];
+                tmem_ld16x32(s_at + half_lanes, w);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  const __half2 v = *reinterpret_cast<const __half2*>(&w[k]);
+                  const float2 f = __half22float2(v);
+                  w[k] = pack_half2(f.x * fade[k & 1].x, f.y * fade[k & 1].x);
+                }
+                tmem_st16x32(s_at + half_lanes, w);
+              }
+              probabilities<true>(x, my_meta, my_j0, half[h], p, add, most);
             }
+            half[h].sum[0] = __fadd2_rn(half[h].sum[0], add[0]);
+            half[h].sum[1] = __fadd2_rn(half[h].sum[1], add[1]);
+            tmem_st16x32(s_at + half_lanes + 32 * part, p);
           }
-          tmem_st16(s_at + 16 * part, p);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -419,8 +516,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           mbar_arrive(&meta_empty[s]);
         }
       }
+      // Back to a row a thread.
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float l = half[h].sum[k].x + half[h].sum[k].y;
+          l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+          l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+          if ((lane & 3) == 0) {
+            row_sum[16 * h + 8 * k + (lane >> 2)] = l;
+            row_factor[16 * h + 8 * k + (lane >> 2)] = top[h][k];
+          }
+        }
+      __syncwarp();
+      const float l = row_sum[lane], reference = row_factor[lane];
       // The row's output.
-      const float l = sum.x + sum.y, inv = l == 0.0F ? 0.0F : 1.0F / l;
+      const float inv = l == 0.0F ? 0.0F : 1.0F / l;
       if (ok && tiles > 0) ok = mbar_wait(o_full, 0, abort_flag);
       ok = __all_sync(0xFFFFFFFFu, ok) && !*abort_flag;
       tc_fence_after();
@@ -443,18 +555,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         }
       }
       if (a.lse && live)
-        a.lse[out_row] = !ok ? NAN : l == 0.0F ? -INFINITY : ((top == -INFINITY ? 0.0F : top - kLift) + __log2f(l)) * 0.693147181F;
+        a.lse[out_row] = !ok ? NAN : l == 0.0F ? -INFINITY : ((reference == -INFINITY ? 0.0F : reference - kLift) + __log2f(l)) * 0.693147181F;
     }
-  } else if (warp < kValueWarp0) {
-    // =================== keys: lane (g, t) unpacks 16 bytes t of tokens g, g + 8, .. of its warp's 32 ===================
-    const int kw = warp - kKeyWarp0, g = lane >> 2, t = lane & 3;
-    constexpr int kWords = kDim / 32;   // of a token, per lane
+  } else if (warp < kMmaWarp) {
+    // =================== unpacking ===================
+    // Keys: lane (g, t) takes 16 bytes t (at D = 128) of tokens g, g + 8, .. of its warp's 32.
+    const int uw = warp - kUnpackWarp0, g = lane >> 2, t = lane & 3;
+    constexpr int kWords = kDim / 32;                       // of a token, per lane
     uint32_t word[4][kWords];
     float ks = 0.0F, vs = 0.0F;
     bool seen = false;
-    int page[2] = {ask_page(begin + 32 * kw), ask_page(begin + 32 * kw + 16)};
-    auto load_tile = [&](int i) {
-      const int j = begin + i * kTokens + 32 * kw;
+    int page[2] = {ask_page(begin + 32 * uw), ask_page(begin + 32 * uw + 16)};
+    auto load_keys = [&](int i) {
+      const int j = begin + i * kTokens + 32 * uw;
       const int64_t v[2] = {vector_of(page[0], j), vector_of(page[1], j + 16)};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -476,18 +589,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       page[0] = ask_page(j + kTokens);
       page[1] = ask_page(j + kTokens + 16);
     };
-    if (tiles > 0) load_tile(0);
+    // Values: a lane takes 8 tokens and 8 or 16 dimensions.
+    constexpr int kValueWords = kDim / 64;                  // 8-dimension words of a token, per lane
+    const int group = (uw >> 1) * 8 + (lane & 7);           // its 8 tokens
+    const int piece = (uw & 1) * 4 + (lane >> 3);           // its words: piece * kValueWords and on
+    uint32_t value[8][kValueWords];
+    int value_page = ask_page(begin + (group >> 1) * 16);
+    auto load_values = [&](int i) {
+      const int j = begin + i * kTokens + (group >> 1) * 16;
+      const uint8_t* src = c.codes[1] + (vector_of(value_page, j) + 8 * (group & 1)) * (kDim / 2) + piece * (4 * kValueWords);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if constexpr (kValueWords == 2) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + k * (kDim / 2)));
+          value[k][0] = u.x, value[k][1] = u.y;
+        } else {
+          value[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * (kDim / 2)));
+        }
+      }
+      value_page = ask_page(j + kTokens);
+    };
+    if (tiles > 0) {
+      load_keys(0);
+      load_values(0);
+    }
     for (int i = 0; i < tiles; ++i) {
       const int s = i & 1;
+      const uint32_t parity = ((i >> 1) - 1) & 1;
       if (i >= kStages) {
-        const uint32_t parity = ((i >> 1) - 1) & 1;
         const bool ok = mbar_wait(&k_empty[s], parity, abort_flag) && mbar_wait(&meta_empty[s], parity, abort_flag);
         if (!__all_sync(0xFFFFFFFFu, ok)) break;
       }
-      const uint32_t dst = base + L::off_k + s * L::kTileBytes;
+      const uint32_t key_dst = base + L::off_k + s * L::kTileBytes;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int token = 32 * kw + 8 * k + g;
+        const int token = 32 * uw + 8 * k + g;
 #pragma unroll
         for (int j = 0; j < kWords; ++j) {
           // Lanes two apart lie in the two halves of a row: they take their words in another order, off the same banks.
@@ -495,61 +631,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           uint32_t w = word[k][j];
           if constexpr (kWords == 4) w = (t & 2) ? word[k][j ^ 2] : w;
           const int at = t * kWords + jj;  // word of the row
-          store16(dst + (at >> 3) * (kTokens * 128) + swizzled(token, at & 7), codes_exact<0>(w), codes_exact<1>(w),
+          store16(key_dst + (at >> 3) * (kTokens * 128) + swizzled(token, at & 7), codes_exact<0>(w), codes_exact<1>(w),
                   codes_exact<2>(w), codes_exact<3>(w));
         }
       }
-      float* const ms = meta + s * 3 * kTokens + 32 * kw + lane;
+      float* const ms = meta + s * 3 * kMetaFloats + meta_at(32 * uw + lane);
       ms[0] = seen ? ks : 0.0F;
-      ms[kTokens] = seen ? vs : 0.0F;
-      ms[2 * kTokens] = seen ? scale_exponent(vs) : -INFINITY;
+      ms[kMetaFloats] = seen ? vs : 0.0F;
+      ms[2 * kMetaFloats] = seen ? scale_exponent(vs) : -INFINITY;
       const uint32_t all = __ballot_sync(0xFFFFFFFFu, seen);
-      if (lane == 0) flags[4 * s + kw] = ~all;
+      if (lane == 0) flags[4 * s + uw] = ~all;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[s]);
-      if (i + 1 < tiles) load_tile(i + 1);
-    }
-  } else if (warp < kMmaWarp) {
-    // =================== values: a lane unpacks 8 tokens x 8 or 16 dimensions ===================
-    const int vw = warp - kValueWarp0;
-    constexpr int kWords = kDim / 64;                       // 8-dimension words of a token, per lane
-    const int group = (vw >> 1) * 8 + (lane & 7);           // its 8 tokens
-    const int piece = (vw & 1) * 4 + (lane >> 3);           // its words: piece * kWords and on
-    uint32_t word[8][kWords];
-    int page = ask_page(begin + (group >> 1) * 16);
-    auto load_tile = [&](int i) {
-      const int j = begin + i * kTokens + (group >> 1) * 16;
-      const uint8_t* src = c.codes[1] + (vector_of(page, j) + 8 * (group & 1)) * (kDim / 2) + piece * (4 * kWords);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if constexpr (kWords == 2) {
-          const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + k * (kDim / 2)));
-          word[k][0] = u.x, word[k][1] = u.y;
-        } else {
-          word[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * (kDim / 2)));
-        }
-      }
-      page = ask_page(j + kTokens);
-    };
-    if (tiles > 0) load_tile(0);
-    for (int i = 0; i < tiles; ++i) {
-      const int s = i & 1;
+      if (i + 1 < tiles) load_keys(i + 1);
+
       if (i >= kStages) {
-        const bool ok = mbar_wait(&v_empty[s], ((i >> 1) - 1) & 1, abort_flag);
+        const bool ok = mbar_wait(&v_empty[s], parity, abort_flag);
         if (!__all_sync(0xFFFFFFFFu, ok)) break;
       }
       // Row of a dimension: 64 tokens, 128 bytes; this lane's 8 tokens are one 16-byte chunk.
       const uint32_t dst = base + L::off_v + s * L::kTileBytes + (group >> 3) * (kDim * 128);
 #pragma unroll
-      for (int j = 0; j < kWords; ++j) {
+      for (int j = 0; j < kValueWords; ++j) {
         uint32_t x[4], y[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          x[k] = __byte_perm(word[2 * k][j], word[2 * k + 1][j], 0x5410);
-          y[k] = __byte_perm(word[2 * k][j], word[2 * k + 1][j], 0x7632);
+          x[k] = __byte_perm(value[2 * k][j], value[2 * k + 1][j], 0x5410);
+          y[k] = __byte_perm(value[2 * k][j], value[2 * k + 1][j], 0x7632);
         }
-        const int d = (piece * kWords + j) * 8, chunk = group & 7;
+        const int d = (piece * kValueWords + j) * 8, chunk = group & 7;
         store16(dst + swizzled(d + 0, chunk), codes_exact<0>(x[0]), codes_exact<0>(x[1]), codes_exact<0>(x[2]), codes_exact<0>(x[3]));
         store16(dst + swizzled(d + 1, chunk), codes_exact<1>(x[0]), codes_exact<1>(x[1]), codes_exact<1>(x[2]), codes_exact<1>(x[3]));
         store16(dst + swizzled(d + 2, chunk), codes_exact<2>(x[0]), codes_exact<2>(x[1]), codes_exact<2>(x[2]), codes_exact<2>(x[3]));
@@ -562,17 +673,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[s]);
-      if (i + 1 < tiles) load_tile(i + 1);
+      if (i + 1 < tiles) load_values(i + 1);
     }
-  } else if (lane == 0 && tiles > 0) {
-    // =================== products: one thread issues ===================
+  } else if (tiles > 0) {
+    // =================== products: one lane issues ===================
+    const uint32_t leader = elect();
     constexpr uint32_t kInstrS = (1u << 4) | (static_cast<uint32_t>(kTokens >> 3) << 17) | (8u << 24);
     constexpr uint32_t kInstrO = (1u << 4) | (static_cast<uint32_t>(kDim >> 3) << 17) | (8u << 24);
     auto scores = [&](int m, int s) {
 #pragma unroll
       for (int k = 0; k < kDim / 16; ++k) {  // 16 dimensions: 32 bytes of a 128-byte row
         const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
-        mma_ss(tmem + m * 128, operand_desc(base + L::off_q + m * L::kQBytes + at),
+        mma_ss(leader, tmem + m * 128, operand_desc(base + L::off_q + m * L::kQBytes + at),
                operand_desc(base + L::off_k + s * L::kTileBytes + at), kInstrS, k > 0);
       }
     };
@@ -580,38 +692,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
 #pragma unroll
       for (int k = 0; k < kTokens / 16; ++k) {
         const uint32_t at = (k >> 2) * (kDim * 128) + (k & 3) * 32;
-        mma_ts(tmem + 256 + m * 128, tmem + m * 128 + 8 * k, operand_desc(base + L::off_v + s * L::kTileBytes + at), kInstrO,
+        mma_ts(leader, tmem + 256 + m * 128, tmem + m * 128 + 8 * k, operand_desc(base + L::off_v + s * L::kTileBytes + at), kInstrO,
                add || k > 0);
       }
     };
-    bool ok = mbar_wait(q_full, 0, abort_flag) && mbar_wait(&k_full[0], 0, abort_flag);
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0;
+    };
+    bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
     if (ok) {
       tc_fence_after();
       for (int m = 0; m < tiles_m; ++m) {
         scores(m, 0);
-        mma_commit(&s_full[m]);
+        mma_commit(leader, &s_full[m]);
       }
-      mma_commit(&k_empty[0]);
+      mma_commit(leader, &k_empty[0]);
       for (int i = 0; i < tiles && ok; ++i) {
         const int s = i & 1, next = (i + 1) & 1;
-        ok = mbar_wait(&v_full[s], (i >> 1) & 1, abort_flag);
+        ok = wait(&v_full[s], (i >> 1) & 1);
         for (int m = 0; m < tiles_m && ok; ++m) {
-          ok = mbar_wait(&p_full[m], i & 1, abort_flag);
+          ok = wait(&p_full[m], i & 1);
           if (!ok) break;
           tc_fence_after();
           sums(m, s, i > 0);
-          if (m == tiles_m - 1) mma_commit(&v_empty[s]);
+          if (m == tiles_m - 1) mma_commit(leader, &v_empty[s]);
           if (i + 1 < tiles) {
-            if (m == 0) ok = mbar_wait(&k_full[next], ((i + 1) >> 1) & 1, abort_flag);
+            if (m == 0) ok = wait(&k_full[next], ((i + 1) >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
             scores(m, next);
-            mma_commit(&s_full[m]);
-            if (m == tiles_m - 1) mma_commit(&k_empty[next]);
+            mma_commit(leader, &s_full[m]);
+            if (m == tiles_m - 1) mma_commit(leader, &k_empty[next]);
           }
         }
       }
-      if (ok) mma_commit(o_full);
+      if (ok) mma_commit(leader, o_full);
     }
   }
   __syncwarp();
