@@ -1506,6 +1506,7 @@ Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   if (a->rows < 0 || a->batch < 0 || a->max_pages < 0 || a->max_query_rows < 0)
     throw InvalidArgument("sizes must not be negative");
   if (a->rows > (int64_t{1} << 31) - 1) throw InvalidArgument("rows must be below 2^31");
+  if (a->heads > 0 && a->rows > ((int64_t{1} << 31) - 1) / a->heads) throw InvalidArgument("rows * heads must be below 2^31");
   if (a->heads < 1 || a->heads % c.heads) throw InvalidArgument("heads must be a positive multiple of kv_heads");
   if ((static_cast<int64_t>(a->max_pages) << c.page_shift) > (int64_t{1} << 31) - 1)
     throw InvalidArgument("max_pages * page_size must be below 2^31");

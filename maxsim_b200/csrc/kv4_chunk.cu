@@ -33,8 +33,8 @@ constexpr int kMmaWarp = 12;
 constexpr int kThreads = 13 * 32;
 constexpr int kStages = 2;
 constexpr float kExponents = 110.0F;
-constexpr float kLift = 4.0F;        // a reference is set 2^4 below the largest p vs seen
-constexpr float kMostP = 16384.0F;   // and kept while p vs stays below 2^14, which fp16 holds
+constexpr float kLift = 2.0F;        // a reference is set 2^2 below the largest p vs seen
+constexpr float kMostP = 60000.0F;   // and kept while p vs stays in fp16
 constexpr int kMetaPitch = 20;       // floats of the 16 columns (of 64) that one lane in four reads
 constexpr int kMetaFloats = 2 * 4 * kMetaPitch;
 constexpr uint64_t kTimeoutNs = 4000000000ull;
@@ -143,20 +143,31 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&f)[32]) {
   for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
 }
 // 16 lanes x 64 columns: thread t receives, for j = 0..7, columns 8j + 2 (t % 4) + {0, 1} of lane t / 4 in f[4j],
-// f[4j + 1] and of lane t / 4 + 8 in f[4j + 2], f[4j + 3].
-__device__ __forceinline__ void tmem_ld16x64(uint32_t taddr, float (&f)[32]) {
-  uint32_t r[32];
+// f[4j + 1] and of lane t / 4 + 8 in f[4j + 2], f[4j + 3] - when tmem_arrived has returned.
+__device__ __forceinline__ void tmem_ask16x64(uint32_t taddr, float (&f)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]),
+        "=f"(f[8]), "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]),
+        "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]), "=f"(f[21]), "=f"(f[22]), "=f"(f[23]),
+        "=f"(f[24]), "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]), "=f"(f[31])
       : "r"(taddr)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_arrived(float (&f)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]),
+        "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]), "+f"(f[12]), "+f"(f[13]), "+f"(f[14]), "+f"(f[15]),
+        "+f"(f[16]), "+f"(f[17]), "+f"(f[18]), "+f"(f[19]), "+f"(f[20]), "+f"(f[21]), "+f"(f[22]), "+f"(f[23]),
+        "+f"(f[24]), "+f"(f[25]), "+f"(f[26]), "+f"(f[27]), "+f"(f[28]), "+f"(f[29])
+      :
+      : "memory");
+  asm volatile("" : "+f"(f[30]), "+f"(f[31])::"memory");
+}
+__device__ __forceinline__ void tmem_ld16x64(uint32_t taddr, float (&f)[32]) {
+  tmem_ask16x64(taddr, f);
+  tmem_arrived(f);
 }
 __device__ __forceinline__ void tmem_st16x64(uint32_t taddr, const float (&f)[32]) {
   asm volatile(
@@ -235,7 +246,8 @@ struct Rows {
   float2 factor[2];   // scale * log2(e) * the row's power of two, twice
   float2 ref[2];      // 2^-(reference), as an exponent, twice
   float2 sum[2];      // of p, the thread's columns
-  int first[2], last[2];
+  int last[2];        // the last token seen
+  int window;         // and how many up to it (INT_MAX: all)
 };
 
 // Scores (f: two rows x 16 columns) to probabilities times value scales, fp16 pairs; the largest into `most`.
@@ -263,8 +275,8 @@ __device__ __forceinline__ void probabilities(const float (&f)[32], const float*
         float2 pv = __fmul2_rn(pr, vs);
         if (kMasked) {
           const int c = j0 + 8 * (j + h);
-          if (e.x == -INFINITY || c < rows.first[r] || c > rows.last[r]) pr.x = pv.x = 0.0F;
-          if (e.y == -INFINITY || c + 1 < rows.first[r] || c + 1 > rows.last[r]) pr.y = pv.y = 0.0F;
+          if (e.x == -INFINITY || c > rows.last[r] || rows.last[r] - c >= rows.window) pr.x = pv.x = 0.0F;
+          if (e.y == -INFINITY || c + 1 > rows.last[r] || rows.last[r] - c - 1 >= rows.window) pr.y = pv.y = 0.0F;
         }
         add[r] = __fadd2_rn(add[r], pr);
         most[r] = fmax3(most[r], pv.x, pv.y);
@@ -284,13 +296,13 @@ __device__ __forceinline__ void references(const float (&f)[32], const float* me
       const int c = j0 + 8 * j + k;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        if (e != -INFINITY && c >= rows.first[r] && c <= rows.last[r])
+        if (e != -INFINITY && c <= rows.last[r] && rows.last[r] - c < rows.window)
           best[r] = fmaxf(best[r], f[4 * j + 2 * r + k] * ks * rows.factor[r].x + e);
     }
 }
 
 template <class T, int kDim>
-__global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4Attend a, int shared, int row_blocks,
+__global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4Attend a, uint32_t shared, int row_blocks,
                                                                 bool aligned) {
   using L = Layout<kDim>;
   extern __shared__ unsigned char raw_smem[];
@@ -300,9 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   const int block = row_blocks - 1 - static_cast<int>(blockIdx.x / per_block);
   const int b = static_cast<int>(blockIdx.x % per_block / c.heads), head = static_cast<int>(blockIdx.x % c.heads);
   const Kv4Sequence q = kv4_sequence(a, c.page_shift, b);
-  const int64_t all_rows = static_cast<int64_t>(q.rows) * shared, block_row0 = static_cast<int64_t>(block) * kBlockRows;
+  const uint32_t all_rows = static_cast<uint32_t>(q.rows) * shared, block_row0 = static_cast<uint32_t>(block) * kBlockRows;  // below 2^31
   if (block_row0 >= all_rows) return;
-  const int row_count = static_cast<int>(min(static_cast<int64_t>(kBlockRows), all_rows - block_row0));
+  const int row_count = static_cast<int>(min(static_cast<uint32_t>(kBlockRows), all_rows - block_row0));
   const int tiles_m = row_count > kRowsTile ? 2 : 1;
   // Tokens that some row of the block sees, and the tiles over them.
   const int pos0 = q.length - q.rows + static_cast<int>(block_row0 / shared);
@@ -369,45 +381,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
     // =================== softmax: a thread owns a row ===================
     const int m = warp >> 2;
     if (m < tiles_m) {
-      const int r = m * kRowsTile + (warp & 3) * 32 + lane;
-      const int64_t row = block_row0 + r;
-      const bool live = r < row_count;
-      const int64_t out_row = (q.row0 + (live ? row / shared : 0)) * a.heads + head * shared + (live ? row % shared : 0);
-      // The row of the query tile: scaled by a power of two to a maximum in [2^10, 2^11), fp16, in the codes' order.
-      float factor;
+      float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + (warp & 3) * 32;
+      float* const row_sum = row_factor + kBlockRows;
+      // The warp's 32 rows of the query tile, 8 dimensions a lane: scaled by a power of two to a maximum in
+      // [2^10, 2^11), fp16, in the codes' order.
+      constexpr int kRowLanes = kDim / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 32 / kRowsAtOnce;
       {
-        const T* x = static_cast<const T*>(a.query) + (q.row0 + (live ? row / shared : 0)) * a.q_row_stride +
-                     (head * shared + (live ? row % shared : 0)) * a.q_head_stride;
-        float top = 0.0F;
-        auto load8 = [&](int d, float (&v)[8]) {
-          if (aligned) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + d));
-            const T* e = reinterpret_cast<const T*>(&u);
+        uint4 x[kLoads];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = live ? to_f32(e[i]) : 0.0F;
-          } else {
+        for (int k = 0; k < kLoads; ++k) {
+          const int r = m * kRowsTile + (warp & 3) * 32 + k * kRowsAtOnce + lane / kRowLanes;
+          x[k] = make_uint4(0, 0, 0, 0);
+          if (r < row_count) {
+            const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
+            const T* src = static_cast<const T*>(a.query) + (q.row0 + token) * a.q_row_stride +
+                           static_cast<int64_t>(head * shared + in_group) * a.q_head_stride + (lane % kRowLanes) * 8;
+            if (aligned) {
+              x[k] = __ldg(reinterpret_cast<const uint4*>(src));
+            } else {
+              __align__(16) T e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = live ? to_f32(x[d + i]) : 0.0F;
+              for (int i = 0; i < 8; ++i) e[i] = src[i];
+              x[k] = *reinterpret_cast<const uint4*>(e);
+            }
           }
-        };
-#pragma unroll 4
-        for (int d = 0; d < kDim; d += 8) {
-          float v[8];
-          load8(d, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
         }
-        const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
-        const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
-        factor = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
-#pragma unroll 4
-        for (int d = 0; d < kDim; d += 8) {
-          float v[8];
-          load8(d, v);
-          store16(base + L::off_q + m * L::kQBytes + (d >> 6) * (kRowsTile * 128) +
-                      swizzled((warp & 3) * 32 + lane, (d & 63) >> 3),
-                  pack_half2(v[0] * down, v[4] * down), pack_half2(v[1] * down, v[5] * down),
-                  pack_half2(v[2] * down, v[6] * down), pack_half2(v[3] * down, v[7] * down));
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+          const T* const v = reinterpret_cast<const T*>(&x[k]);
+          float top = 0.0F;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_f32(v[i])));
+#pragma unroll
+          for (int d = 1; d < kRowLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+          const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+          const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
+          const int r = (warp & 3) * 32 + k * kRowsAtOnce + lane / kRowLanes, piece = lane % kRowLanes;
+          store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled(r, piece & 7),
+                  pack_half2(to_f32(v[0]) * down, to_f32(v[4]) * down), pack_half2(to_f32(v[1]) * down, to_f32(v[5]) * down),
+                  pack_half2(to_f32(v[2]) * down, to_f32(v[6]) * down), pack_half2(to_f32(v[3]) * down, to_f32(v[7]) * down));
+          if (piece == 0)
+            row_factor[k * kRowsAtOnce + lane / kRowLanes] =
+                a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
         }
         fence_proxy_async();
         __syncwarp();
@@ -415,10 +430,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       }
       // From here to the output a thread works on two rows of each 16-lane half of its warp's 32: lane / 4 and + 8,
       // 32 of a tile's columns, so that a column's scales serve four rows.
-      float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + (warp & 3) * 32;
-      float* const row_sum = row_factor + kBlockRows;
-      row_factor[lane] = factor;
-      __syncwarp();
       Rows half[2];
       float top[2][2];
 #pragma unroll
@@ -426,15 +437,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int mine = 16 * h + 8 * k + (lane >> 2), at = m * kRowsTile + (warp & 3) * 32 + mine;
-          const int pos = q.length - q.rows + static_cast<int>((block_row0 + at) / shared);
+          // Rows past the last do as it does: what they compute is not written.
+          const int pos = q.length - q.rows + static_cast<int>((block_row0 + min(at, row_count - 1)) / shared);
           half[h].factor[k] = make_float2(row_factor[mine], row_factor[mine]);
           half[h].ref[k] = half[h].sum[k] = make_float2(0.0F, 0.0F);
-          half[h].last[k] = at < row_count ? (a.causal ? pos : q.length - 1) : INT_MAX;
-          half[h].first[k] = at < row_count && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+          half[h].last[k] = a.causal ? pos : q.length - 1;
+          half[h].window = a.window > 0 ? a.window : INT_MAX;
           top[h][k] = -INFINITY;
         }
       const int every_last = min(min(half[0].last[0], half[0].last[1]), min(half[1].last[0], half[1].last[1]));
-      const int every_first = max(max(half[0].first[0], half[0].first[1]), max(half[1].first[0], half[1].first[1]));
+      const int every_first = a.window > 0 ? max(max(half[0].last[0], half[0].last[1]), max(half[1].last[0], half[1].last[1])) -
+                                                 a.window + 1
+                                           : 0;
       const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's quarter of the lanes
       const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + 256 + m * 128;
       bool ok = true;
@@ -449,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         const uint4 flag = *reinterpret_cast<const uint4*>(flags + 4 * s);
         const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < every_first ||
                                                        j0 + kTokens - 1 > every_last);
+        // Blocks of 16 rows x 64 columns.
 #pragma unroll 1
         for (int part = 0; part < 2; ++part) {
           const float* const my_meta = meta + s * 3 * kMetaFloats + part * (4 * kMetaPitch) + (lane & 3) * kMetaPitch;
@@ -456,38 +471,39 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t half_lanes = static_cast<uint32_t>(h) << 20;  // 16 lanes on
-            float x[32], most[2];
+            float f[32], most[2];
+            tmem_ld16x64(s_at + half_lanes + 64 * part, f);
             float2 add[2];
             uint32_t p[16];
-            tmem_ld16x64(s_at + half_lanes + 64 * part, x);
-            if (masked) probabilities<true>(x, my_meta, my_j0, half[h], p, add, most);
-            else probabilities<false>(x, my_meta, my_j0, half[h], p, add, most);
+            if (masked) probabilities<true>(f, my_meta, my_j0, half[h], p, add, most);
+            else probabilities<false>(f, my_meta, my_j0, half[h], p, add, most);
             // A row without a reference yet, or one whose reference has become too low (an infinite p among it).
             const bool low = top[h][0] == -INFINITY || top[h][1] == -INFINITY || most[0] > kMostP || most[1] > kMostP;
             if (__any_sync(0xFFFFFFFFu, low)) {
               tmem_wait_st();  // what was written before is read below
               float best[2];
-              references(x, my_meta, my_j0, half[h], best);
-              float2 fade[2];
+              tmem_ld16x64(s_at + half_lanes + 64 * part, f);
+              references(f, my_meta, my_j0, half[h], best);
+              float fade[2];
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 1));
                 best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 2));
-                const float next = fmaxf(top[h][k], best[k]), f = fade_to(top[h][k], next);
-                fade[k] = make_float2(f, f);
+                const float next = fmaxf(top[h][k], best[k]);
+                fade[k] = fade_to(top[h][k], next);
                 top[h][k] = next;
                 const float ref = next == -INFINITY ? 0.0F : kLift - next;
                 half[h].ref[k] = make_float2(ref, ref);
-                half[h].sum[k] = __fmul2_rn(half[h].sum[k], fade[k]);
+                half[h].sum[k] = __fmul2_rn(half[h].sum[k], make_float2(fade[k], fade[k]));
               }
+              probabilities<true>(f, my_meta, my_j0, half[h], p, add, most);
               if (i > 0) {  // the sums of the tiles before
 #pragma unroll 1
                 for (int d = 0; d < kDim; d += 64) {
-                  float o[32];
-                  tmem_ld16x64(o_at + half_lanes + d, o);
+                  tmem_ld16x64(o_at + half_lanes + d, f);
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) o[k] *= fade[(k >> 1) & 1].x;
-                  tmem_st16x64(o_at + half_lanes + d, o);
+                  for (int k = 0; k < 32; ++k) f[k] *= fade[(k >> 1) & 1];
+                  tmem_st16x64(o_at + half_lanes + d, f);
                 }
               }
               if (part > 0) {  // and the probabilities of the columns before
@@ -495,13 +511,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
                 tmem_ld16x32(s_at + half_lanes, w);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                  const __half2 v = *reinterpret_cast<const __half2*>(&w[k]);
-                  const float2 f = __half22float2(v);
-                  w[k] = pack_half2(f.x * fade[k & 1].x, f.y * fade[k & 1].x);
+                  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+                  w[k] = pack_half2(v.x * fade[k & 1], v.y * fade[k & 1]);
                 }
                 tmem_st16x32(s_at + half_lanes, w);
               }
-              probabilities<true>(x, my_meta, my_j0, half[h], p, add, most);
             }
             half[h].sum[0] = __fadd2_rn(half[h].sum[0], add[0]);
             half[h].sum[1] = __fadd2_rn(half[h].sum[1], add[1]);
@@ -536,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       if (ok && tiles > 0) ok = mbar_wait(o_full, 0, abort_flag);
       ok = __all_sync(0xFFFFFFFFu, ok) && !*abort_flag;
       tc_fence_after();
+      // Rows go out through the query tile's shared memory, 16 bytes a lane of a row.
 #pragma unroll
       for (int part = 0; part < kDim / 32; ++part) {
         float x[32];
@@ -543,19 +558,39 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         __align__(16) T e[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) e[k] = from_f32<T>(!ok ? NAN : l == 0.0F ? 0.0F : x[k] * inv);
-        if (live) {
-          T* out = static_cast<T*>(a.out) + out_row * kDim + 32 * part;
-          if ((reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) reinterpret_cast<uint4*>(out)[k] = reinterpret_cast<const uint4*>(e)[k];
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) out[k] = e[k];
-          }
+        for (int k = 0; k < 4; ++k) {
+          const uint4 v = reinterpret_cast<const uint4*>(e)[k];
+          const int piece = 4 * part + k;
+          store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled((warp & 3) * 32 + lane, piece & 7),
+                  v.x, v.y, v.z, v.w);
         }
       }
-      if (a.lse && live)
-        a.lse[out_row] = !ok ? NAN : l == 0.0F ? -INFINITY : ((reference == -INFINITY ? 0.0F : reference - kLift) + __log2f(l)) * 0.693147181F;
+      __syncwarp();
+      const bool out_aligned = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+#pragma unroll 4
+      for (int k = 0; k < kLoads; ++k) {
+        const int in_warp = k * kRowsAtOnce + lane / kRowLanes, r = m * kRowsTile + (warp & 3) * 32 + in_warp;
+        const int piece = lane % kRowLanes;
+        if (r >= row_count) continue;
+        const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
+        const int64_t out_row = (q.row0 + token) * a.heads + head * shared + in_group;
+        const uint4 v = *reinterpret_cast<const uint4*>(smem + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) +
+                                                        swizzled((warp & 3) * 32 + in_warp, piece & 7));
+        T* const out = static_cast<T*>(a.out) + out_row * kDim + piece * 8;
+        if (out_aligned) {
+          *reinterpret_cast<uint4*>(out) = v;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) out[i] = reinterpret_cast<const T*>(&v)[i];
+        }
+      }
+      const int mine = m * kRowsTile + (warp & 3) * 32 + lane;
+      if (a.lse && mine < row_count) {
+        const uint32_t token = (block_row0 + mine) / shared, in_group = block_row0 + mine - token * shared;
+        a.lse[(q.row0 + token) * a.heads + head * shared + in_group] =
+            !ok ? NAN : l == 0.0F ? -INFINITY : ((reference == -INFINITY ? 0.0F : reference - kLift) + __log2f(l)) * 0.693147181F;
+      }
     }
   } else if (warp < kMmaWarp) {
     // =================== unpacking ===================

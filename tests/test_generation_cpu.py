@@ -62,7 +62,7 @@ def test_append_and_read_arguments():
                                      (dict(rows=3), "rows must equal batch"), (dict(type=_lib.TYPE_F32), "fp16 or bf16"),
                                      (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
                                      (dict(window=-1), "window"), (dict(window=4, causal=0), "window needs causal"),
-                                     (dict(max_pages=1 << 28), "max_pages"), (dict(query=None), "NULL"),
+                                     (dict(max_pages=1 << 28), "max_pages"), (dict(rows=1 << 30, batch=1 << 30), "rows \\* heads"), (dict(query=None), "NULL"),
                                      (dict(lengths=None), "NULL"), (dict(out=None), "NULL"),
                                      (dict(page_table=None), "NULL")])
 def test_attend_arguments(kw, text):
