@@ -27,16 +27,17 @@ namespace {
 constexpr int kTokens = 128;         // of a tile
 constexpr int kRowsTile = 128;       // rows of one accumulator
 constexpr int kBlockRows = 256;
-constexpr int kSoftWarps = 8;        // warps 0-3: first row tile, 4-7: second
-constexpr int kUnpackWarp0 = 8;      // warps 8-11: keys, the tiles' scales, values
-constexpr int kMmaWarp = 12;
-constexpr int kThreads = 13 * 32;
+constexpr int kSoftWarps = 16;       // eight to a row tile: warp w has 16 rows, half (w / 4) % 2 of lane quarter w % 4
+constexpr int kUnpackWarp0 = 16;     // warps 16-19: keys, the tiles' scales, values
+constexpr int kMmaWarp = 20;
+constexpr int kThreads = 21 * 32;
 constexpr int kStages = 2;
 constexpr float kExponents = 110.0F;
 constexpr float kLift = 2.0F;        // a reference is set 2^2 below the largest p vs seen
 constexpr float kMostP = 60000.0F;   // and kept while p vs stays in fp16
-constexpr int kMetaPitch = 20;       // floats of the 16 columns (of 64) that one lane in four reads
-constexpr int kMetaFloats = 2 * 4 * kMetaPitch;
+constexpr int kCols = 32;            // columns of a softmax block
+constexpr int kMetaPitch = 12;       // floats between the columns of a block that neighbouring lanes read (8 each)
+constexpr int kMetaFloats = kTokens / kCols * 4 * kMetaPitch;
 constexpr uint64_t kTimeoutNs = 4000000000ull;
 
 template <int kDim>
@@ -48,8 +49,8 @@ struct Layout {
   static constexpr int off_v = off_k + kStages * kTileBytes;
   static constexpr int off_meta = off_v + kStages * kTileBytes;  // [stage][3]: key scales, value scales, their log2
   static constexpr int off_flags = off_meta + kStages * 3 * kMetaFloats * 4;  // [stage][4]: some token is not seen
-  static constexpr int off_rows = off_flags + kStages * 16;      // [256] factors, then references; [256] sums
-  static constexpr int off_bars = off_rows + 2 * kBlockRows * 4;
+  static constexpr int off_rows = off_flags + kStages * 16;      // [256] the rows' factors
+  static constexpr int off_bars = off_rows + kBlockRows * 4;
   static constexpr int kUsed = off_bars + 24 * 8 + 1024;        // and room to align to 1024
   // A block takes all of an SM's tensor memory: more than half of its shared memory keeps a second one away.
   static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
@@ -128,73 +129,37 @@ __device__ __forceinline__ uint32_t elect() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&f)[32]) {
-  uint32_t r[32];
+// A block of 16 lanes x 32 columns: thread t has, for j = 0..3, columns 8j + 2 (t % 4) + {0, 1} of lane t / 4 in f[4j],
+// f[4j + 1] and of lane t / 4 + 8 in f[4j + 2], f[4j + 3]; as fp16 pairs, 16 columns, r[2j] and r[2j + 1].
+__device__ __forceinline__ void tmem_ld_block(uint32_t taddr, float (&f)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
-}
-// 16 lanes x 64 columns: thread t receives, for j = 0..7, columns 8j + 2 (t % 4) + {0, 1} of lane t / 4 in f[4j],
-// f[4j + 1] and of lane t / 4 + 8 in f[4j + 2], f[4j + 3] - when tmem_arrived has returned.
-__device__ __forceinline__ void tmem_ask16x64(uint32_t taddr, float (&f)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]),
-        "=f"(f[8]), "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]),
-        "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]), "=f"(f[21]), "=f"(f[22]), "=f"(f[23]),
-        "=f"(f[24]), "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]), "=f"(f[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_arrived(float (&f)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-      : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]),
-        "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]), "+f"(f[12]), "+f"(f[13]), "+f"(f[14]), "+f"(f[15]),
-        "+f"(f[16]), "+f"(f[17]), "+f"(f[18]), "+f"(f[19]), "+f"(f[20]), "+f"(f[21]), "+f"(f[22]), "+f"(f[23]),
-        "+f"(f[24]), "+f"(f[25]), "+f"(f[26]), "+f"(f[27]), "+f"(f[28]), "+f"(f[29])
-      :
-      : "memory");
-  asm volatile("" : "+f"(f[30]), "+f"(f[31])::"memory");
-}
-__device__ __forceinline__ void tmem_ld16x64(uint32_t taddr, float (&f)[32]) {
-  tmem_ask16x64(taddr, f);
-  tmem_arrived(f);
-}
-__device__ __forceinline__ void tmem_st16x64(uint32_t taddr, const float (&f)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(f[0]),
-      "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]), "f"(f[8]), "f"(f[9]), "f"(f[10]),
-      "f"(f[11]), "f"(f[12]), "f"(f[13]), "f"(f[14]), "f"(f[15]), "f"(f[16]), "f"(f[17]), "f"(f[18]), "f"(f[19]),
-      "f"(f[20]), "f"(f[21]), "f"(f[22]), "f"(f[23]), "f"(f[24]), "f"(f[25]), "f"(f[26]), "f"(f[27]), "f"(f[28]),
-      "f"(f[29]), "f"(f[30]), "f"(f[31]), "r"(taddr)
-      : "memory");
-}
-// 16 lanes x 32 columns: thread t holds, for j = 0..7, column 4j + t % 4 of lane t / 4 in r[2j], of t / 4 + 8 in r[2j + 1]:
-// the fp16 pairs of what tmem_ld16x64 gave.
-__device__ __forceinline__ void tmem_st16x32(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x128b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
       " tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]),
+        "=f"(f[8]), "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15])
       : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_block(uint32_t taddr, const float (&f)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+      :
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]),
+        "f"(f[8]), "f"(f[9]), "f"(f[10]), "f"(f[11]), "f"(f[12]), "f"(f[13]), "f"(f[14]), "f"(f[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_pairs(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+      :
+      : "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -236,28 +201,29 @@ __device__ __forceinline__ void store16(uint32_t addr, uint32_t a, uint32_t b, u
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// Where column `c` of a tile keeps its scale: the 16 of each 64 columns that one lane reads lie together.
+// Where column `c` of a tile keeps its scale: those of a block that one lane reads lie together.
 __device__ __forceinline__ int meta_at(int c) {
-  return (c >> 6) * (4 * kMetaPitch) + ((c >> 1) & 3) * kMetaPitch + ((c >> 3) & 7) * 2 + (c & 1);
+  return c / kCols * (4 * kMetaPitch) + ((c >> 1) & 3) * kMetaPitch + (c % kCols >> 3) * 2 + (c & 1);
 }
 
-// What a thread keeps of its two rows of a 16-lane half.
+// What a thread keeps of its two rows, lane / 4 and + 8 of its warp's 16.
 struct Rows {
   float2 factor[2];   // scale * log2(e) * the row's power of two, twice
   float2 ref[2];      // 2^-(reference), as an exponent, twice
   float2 sum[2];      // of p, the thread's columns
   int last[2];        // the last token seen
   int window;         // and how many up to it (INT_MAX: all)
+  float top[2];       // the reference, -inf before there is one
 };
 
-// Scores (f: two rows x 16 columns) to probabilities times value scales, fp16 pairs; the largest into `most`.
+// Scores (f: two rows x 8 columns) to probabilities times value scales, fp16 pairs; the largest into `most`.
 template <bool kMasked>
-__device__ __forceinline__ void probabilities(const float (&f)[32], const float* meta, int j0, const Rows& rows, uint32_t (&p)[16],
+__device__ __forceinline__ void probabilities(const float (&f)[16], const float* meta, int j0, const Rows& rows, uint32_t (&p)[8],
                                               float2 (&add)[2], float (&most)[2]) {
   add[0] = add[1] = make_float2(0.0F, 0.0F);
   most[0] = most[1] = 0.0F;
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
+  for (int j = 0; j < kCols / 8; j += 2) {
     const float4 ks4 = *reinterpret_cast<const float4*>(meta + 2 * j);
     const float4 vs4 = *reinterpret_cast<const float4*>(meta + kMetaFloats + 2 * j);
     float4 e4 = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
@@ -286,10 +252,10 @@ __device__ __forceinline__ void probabilities(const float (&f)[32], const float*
   }
 }
 // The largest s + log2(vs) of the thread's seen columns, per row; -inf where there are none (or nothing but NaN).
-__device__ __forceinline__ void references(const float (&f)[32], const float* meta, int j0, const Rows& rows, float (&best)[2]) {
+__device__ __forceinline__ void references(const float (&f)[16], const float* meta, int j0, const Rows& rows, float (&best)[2]) {
   best[0] = best[1] = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < kCols / 8; ++j)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float ks = meta[2 * j + k], e = meta[2 * kMetaFloats + 2 * j + k];
@@ -346,14 +312,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 4);
       mbar_init(&v_empty[s], 1);
-      mbar_init(&meta_empty[s], 4 * tiles_m);
+      mbar_init(&meta_empty[s], 8 * tiles_m);
     }
     for (int m = 0; m < 2; ++m) {
       mbar_init(&s_full[m], 1);
-      mbar_init(&p_full[m], 4);
+      mbar_init(&p_full[m], 8);
     }
     mbar_init(o_full, 1);
-    mbar_init(q_full, 4 * tiles_m);
+    mbar_init(q_full, 8 * tiles_m);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -378,19 +344,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   };
 
   if (warp < kSoftWarps) {
-    // =================== softmax: a thread owns a row ===================
-    const int m = warp >> 2;
+    // =================== softmax: a warp has 16 rows, a thread two of them and a quarter of their columns ===================
+    const int m = warp >> 3;
     if (m < tiles_m) {
-      float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + (warp & 3) * 32;
-      float* const row_sum = row_factor + kBlockRows;
-      // The warp's 32 rows of the query tile, 8 dimensions a lane: scaled by a power of two to a maximum in
-      // [2^10, 2^11), fp16, in the codes' order.
-      constexpr int kRowLanes = kDim / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 32 / kRowsAtOnce;
-      {
-        uint4 x[kLoads];
+      const int row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16;  // of the row tile, and its lane of tensor memory
+      float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + row0;
+      constexpr int kRowLanes = kDim / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 16 / kRowsAtOnce;
+      // The warp's rows of the query tile, 8 dimensions a lane: scaled by a power of two to a maximum in [2^10, 2^11),
+      // fp16, in the codes' order.  (In a loop: straight code would be fetched from memory and used once.)
+      constexpr int kBatch = 4;
+#pragma unroll 1
+      for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
+        uint4 x[kBatch];
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) {
-          const int r = m * kRowsTile + (warp & 3) * 32 + k * kRowsAtOnce + lane / kRowLanes;
+        for (int k = 0; k < kBatch; ++k) {
+          const int r = m * kRowsTile + row0 + (k0 + k) * kRowsAtOnce + lane / kRowLanes;
           x[k] = make_uint4(0, 0, 0, 0);
           if (r < row_count) {
             const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
@@ -407,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           }
         }
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) {
+        for (int k = 0; k < kBatch; ++k) {
           const T* const v = reinterpret_cast<const T*>(&x[k]);
           float top = 0.0F;
 #pragma unroll
@@ -416,111 +384,99 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           for (int d = 1; d < kRowLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
           const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
           const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
-          const int r = (warp & 3) * 32 + k * kRowsAtOnce + lane / kRowLanes, piece = lane % kRowLanes;
-          store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled(r, piece & 7),
+          const int r = (k0 + k) * kRowsAtOnce + lane / kRowLanes, piece = lane % kRowLanes;
+          store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled(row0 + r, piece & 7),
                   pack_half2(to_f32(v[0]) * down, to_f32(v[4]) * down), pack_half2(to_f32(v[1]) * down, to_f32(v[5]) * down),
                   pack_half2(to_f32(v[2]) * down, to_f32(v[6]) * down), pack_half2(to_f32(v[3]) * down, to_f32(v[7]) * down));
-          if (piece == 0)
-            row_factor[k * kRowsAtOnce + lane / kRowLanes] =
-                a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
+          if (piece == 0) row_factor[r] = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
       }
-      // From here to the output a thread works on two rows of each 16-lane half of its warp's 32: lane / 4 and + 8,
-      // 32 of a tile's columns, so that a column's scales serve four rows.
-      Rows half[2];
-      float top[2][2];
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+
+      Rows rows;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int mine = 16 * h + 8 * k + (lane >> 2), at = m * kRowsTile + (warp & 3) * 32 + mine;
-          // Rows past the last do as it does: what they compute is not written.
-          const int pos = q.length - q.rows + static_cast<int>((block_row0 + min(at, row_count - 1)) / shared);
-          half[h].factor[k] = make_float2(row_factor[mine], row_factor[mine]);
-          half[h].ref[k] = half[h].sum[k] = make_float2(0.0F, 0.0F);
-          half[h].last[k] = a.causal ? pos : q.length - 1;
-          half[h].window = a.window > 0 ? a.window : INT_MAX;
-          top[h][k] = -INFINITY;
-        }
-      const int every_last = min(min(half[0].last[0], half[0].last[1]), min(half[1].last[0], half[1].last[1]));
-      const int every_first = a.window > 0 ? max(max(half[0].last[0], half[0].last[1]), max(half[1].last[0], half[1].last[1])) -
-                                                 a.window + 1
-                                           : 0;
-      const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's quarter of the lanes
-      const uint32_t s_at = tmem + lanes + m * 128, o_at = tmem + lanes + 256 + m * 128;
+      for (int k = 0; k < 2; ++k) {
+        // Rows past the last do as it does: what they compute is not written.
+        const int mine = 8 * k + (lane >> 2), at = min(m * kRowsTile + row0 + mine, row_count - 1);
+        const int pos = q.length - q.rows + static_cast<int>((block_row0 + at) / shared);
+        rows.factor[k] = make_float2(row_factor[mine], row_factor[mine]);
+        rows.ref[k] = rows.sum[k] = make_float2(0.0F, 0.0F);
+        rows.last[k] = a.causal ? pos : q.length - 1;
+        rows.top[k] = -INFINITY;
+      }
+      rows.window = a.window > 0 ? a.window : INT_MAX;
+      const int every_last = min(rows.last[0], rows.last[1]);
+      const int every_first = a.window > 0 ? max(rows.last[0], rows.last[1]) - a.window + 1 : 0;
+      const uint32_t s_at = tmem + (static_cast<uint32_t>(row0) << 16) + m * 128, o_at = s_at + 256;
       bool ok = true;
-      for (int i = 0; i < tiles && ok; ++i) {
+      for (int i = 0; i < tiles; ++i) {
         const int s = i & 1, j0 = begin + i * kTokens;
         ok = mbar_wait(&k_full[s], (i >> 1) & 1, abort_flag) && mbar_wait(&s_full[m], i & 1, abort_flag);
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
-          ok = false;
-          break;
-        }
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
         tc_fence_after();
         const uint4 flag = *reinterpret_cast<const uint4*>(flags + 4 * s);
         const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < every_first ||
                                                        j0 + kTokens - 1 > every_last);
-        // Blocks of 16 rows x 64 columns.
+        const float* my_meta = meta + s * 3 * kMetaFloats + (lane & 3) * kMetaPitch;
+        int my_j0 = j0 + 2 * (lane & 3);
+        // Blocks of 32 columns in one short loop: its instructions stay near, the other three warps of a scheduler
+        // fill its waits.
 #pragma unroll 1
-        for (int part = 0; part < 2; ++part) {
-          const float* const my_meta = meta + s * 3 * kMetaFloats + part * (4 * kMetaPitch) + (lane & 3) * kMetaPitch;
-          const int my_j0 = j0 + 64 * part + 2 * (lane & 3);
+        for (int part = 0; part < kTokens / kCols; ++part) {
+          float f[16], most[2];
+          float2 add[2];
+          uint32_t p[8];
+          tmem_ld_block(s_at + kCols * part, f);
+          if (masked) probabilities<true>(f, my_meta, my_j0, rows, p, add, most);
+          else probabilities<false>(f, my_meta, my_j0, rows, p, add, most);
+          // A row without a reference yet, or one whose reference has become too low (an infinite p among it).
+          const bool low = fminf(rows.top[0], rows.top[1]) == -INFINITY || fmaxf(most[0], most[1]) > kMostP;
+          if (__any_sync(0xFFFFFFFFu, low)) {
+            tmem_wait_st();  // what was written before is read below
+            float best[2], fade[2];
+            tmem_ld_block(s_at + kCols * part, f);
+            references(f, my_meta, my_j0, rows, best);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t half_lanes = static_cast<uint32_t>(h) << 20;  // 16 lanes on
-            float f[32], most[2];
-            tmem_ld16x64(s_at + half_lanes + 64 * part, f);
-            float2 add[2];
-            uint32_t p[16];
-            if (masked) probabilities<true>(f, my_meta, my_j0, half[h], p, add, most);
-            else probabilities<false>(f, my_meta, my_j0, half[h], p, add, most);
-            // A row without a reference yet, or one whose reference has become too low (an infinite p among it).
-            const bool low = top[h][0] == -INFINITY || top[h][1] == -INFINITY || most[0] > kMostP || most[1] > kMostP;
-            if (__any_sync(0xFFFFFFFFu, low)) {
-              tmem_wait_st();  // what was written before is read below
-              float best[2];
-              tmem_ld16x64(s_at + half_lanes + 64 * part, f);
-              references(f, my_meta, my_j0, half[h], best);
-              float fade[2];
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 1));
-                best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 2));
-                const float next = fmaxf(top[h][k], best[k]);
-                fade[k] = fade_to(top[h][k], next);
-                top[h][k] = next;
-                const float ref = next == -INFINITY ? 0.0F : kLift - next;
-                half[h].ref[k] = make_float2(ref, ref);
-                half[h].sum[k] = __fmul2_rn(half[h].sum[k], make_float2(fade[k], fade[k]));
-              }
-              probabilities<true>(f, my_meta, my_j0, half[h], p, add, most);
-              if (i > 0) {  // the sums of the tiles before
+            for (int k = 0; k < 2; ++k) {
+              best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 1));
+              best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 2));
+              const float next = fmaxf(rows.top[k], best[k]);
+              fade[k] = fade_to(rows.top[k], next);
+              rows.top[k] = next;
+              const float ref = next == -INFINITY ? 0.0F : kLift - next;
+              rows.ref[k] = make_float2(ref, ref);
+              rows.sum[k] = __fmul2_rn(rows.sum[k], make_float2(fade[k], fade[k]));
+            }
+            probabilities<true>(f, my_meta, my_j0, rows, p, add, most);
+            if (i > 0) {  // the sums of the tiles before
 #pragma unroll 1
-                for (int d = 0; d < kDim; d += 64) {
-                  tmem_ld16x64(o_at + half_lanes + d, f);
+              for (int d = 0; d < kDim; d += kCols) {
+                tmem_ld_block(o_at + d, f);
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) f[k] *= fade[(k >> 1) & 1];
-                  tmem_st16x64(o_at + half_lanes + d, f);
-                }
-              }
-              if (part > 0) {  // and the probabilities of the columns before
-                uint32_t w[16];
-                tmem_ld16x32(s_at + half_lanes, w);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-                  w[k] = pack_half2(v.x * fade[k & 1], v.y * fade[k & 1]);
-                }
-                tmem_st16x32(s_at + half_lanes, w);
+                for (int k = 0; k < 16; ++k) f[k] *= fade[(k >> 1) & 1];
+                tmem_st_block(o_at + d, f);
               }
             }
-            half[h].sum[0] = __fadd2_rn(half[h].sum[0], add[0]);
-            half[h].sum[1] = __fadd2_rn(half[h].sum[1], add[1]);
-            tmem_st16x32(s_at + half_lanes + 32 * part, p);
+#pragma unroll 1
+            for (int d = 0; d < part; ++d) {  // and the probabilities of the columns before
+              uint32_t w[8];
+              tmem_ld_pairs(s_at + kCols / 2 * d, w);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+                w[k] = pack_half2(v.x * fade[k & 1], v.y * fade[k & 1]);
+              }
+              tmem_st_pairs(s_at + kCols / 2 * d, w);
+            }
           }
+          rows.sum[0] = __fadd2_rn(rows.sum[0], add[0]);
+          rows.sum[1] = __fadd2_rn(rows.sum[1], add[1]);
+          tmem_st_pairs(s_at + kCols / 2 * part, p);
+          my_meta += 4 * kMetaPitch;
+          my_j0 += kCols;
         }
         tmem_wait_st();
         tc_fence_before();
@@ -530,53 +486,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           mbar_arrive(&meta_empty[s]);
         }
       }
-      // Back to a row a thread.
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float l = half[h].sum[k].x + half[h].sum[k].y;
-          l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-          l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-          if ((lane & 3) == 0) {
-            row_sum[16 * h + 8 * k + (lane >> 2)] = l;
-            row_factor[16 * h + 8 * k + (lane >> 2)] = top[h][k];
-          }
-        }
-      __syncwarp();
-      const float l = row_sum[lane], reference = row_factor[lane];
-      // The row's output.
-      const float inv = l == 0.0F ? 0.0F : 1.0F / l;
+      // The rows' outputs, through the query tile's shared memory to 16 bytes a lane.
       if (ok && tiles > 0) ok = mbar_wait(o_full, 0, abort_flag);
       ok = __all_sync(0xFFFFFFFFu, ok) && !*abort_flag;
       tc_fence_after();
-      // Rows go out through the query tile's shared memory, 16 bytes a lane of a row.
+      float inv[2], sum[2];
 #pragma unroll
-      for (int part = 0; part < kDim / 32; ++part) {
-        float x[32];
-        if (ok && tiles > 0) tmem_ld32(o_at + 32 * part, x);
-        __align__(16) T e[32];
+      for (int k = 0; k < 2; ++k) {
+        float l = rows.sum[k].x + rows.sum[k].y;
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+        sum[k] = l;
+        inv[k] = l == 0.0F ? 0.0F : 1.0F / l;
+      }
+#pragma unroll 1
+      for (int d = 0; d < kDim; d += kCols) {
+        float f[16];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) e[k] = from_f32<T>(!ok ? NAN : l == 0.0F ? 0.0F : x[k] * inv);
+        for (int k = 0; k < 16; ++k) f[k] = 0.0F;
+        if (ok && tiles > 0) tmem_ld_block(o_at + d, f);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint4 v = reinterpret_cast<const uint4*>(e)[k];
-          const int piece = 4 * part + k;
-          store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled((warp & 3) * 32 + lane, piece & 7),
-                  v.x, v.y, v.z, v.w);
+        for (int k = 0; k < 8; ++k) {
+          const float scale = inv[k & 1];
+          T e[2];
+          e[0] = from_f32<T>(!ok ? NAN : sum[k & 1] == 0.0F ? 0.0F : f[2 * k] * scale);
+          e[1] = from_f32<T>(!ok ? NAN : sum[k & 1] == 0.0F ? 0.0F : f[2 * k + 1] * scale);
+          const int r = row0 + 8 * (k & 1) + (lane >> 2), piece = (d >> 3) + (k >> 1);
+          uint32_t v;
+          memcpy(&v, e, 4);
+          *reinterpret_cast<uint32_t*>(smem + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) +
+                                       swizzled(r, piece & 7) + 4 * (lane & 3)) = v;
         }
       }
       __syncwarp();
       const bool out_aligned = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
 #pragma unroll 4
       for (int k = 0; k < kLoads; ++k) {
-        const int in_warp = k * kRowsAtOnce + lane / kRowLanes, r = m * kRowsTile + (warp & 3) * 32 + in_warp;
-        const int piece = lane % kRowLanes;
+        const int in_warp = k * kRowsAtOnce + lane / kRowLanes, r = m * kRowsTile + row0 + in_warp, piece = lane % kRowLanes;
         if (r >= row_count) continue;
         const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
         const int64_t out_row = (q.row0 + token) * a.heads + head * shared + in_group;
         const uint4 v = *reinterpret_cast<const uint4*>(smem + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) +
-                                                        swizzled((warp & 3) * 32 + in_warp, piece & 7));
+                                                        swizzled(row0 + in_warp, piece & 7));
         T* const out = static_cast<T*>(a.out) + out_row * kDim + piece * 8;
         if (out_aligned) {
           *reinterpret_cast<uint4*>(out) = v;
@@ -585,11 +536,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           for (int i = 0; i < 8; ++i) out[i] = reinterpret_cast<const T*>(&v)[i];
         }
       }
-      const int mine = m * kRowsTile + (warp & 3) * 32 + lane;
-      if (a.lse && mine < row_count) {
-        const uint32_t token = (block_row0 + mine) / shared, in_group = block_row0 + mine - token * shared;
-        a.lse[(q.row0 + token) * a.heads + head * shared + in_group] =
-            !ok ? NAN : l == 0.0F ? -INFINITY : ((reference == -INFINITY ? 0.0F : reference - kLift) + __log2f(l)) * 0.693147181F;
+      if (a.lse && (lane & 3) == 0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int r = m * kRowsTile + row0 + 8 * k + (lane >> 2);
+          if (r >= row_count) continue;
+          const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
+          const float reference = rows.top[k] == -INFINITY ? 0.0F : rows.top[k] - kLift;
+          a.lse[(q.row0 + token) * a.heads + head * shared + in_group] =
+              !ok ? NAN : sum[k] == 0.0F ? -INFINITY : (reference + __log2f(sum[k])) * 0.693147181F;
+        }
       }
     }
   } else if (warp < kMmaWarp) {
