@@ -29,8 +29,8 @@ constexpr int kRowsTile = 128;       // rows of one accumulator
 constexpr int kBlockRows = 256;
 constexpr int kSoftWarps = 16;       // eight to a row tile: warp w has 16 rows, half (w / 4) % 2 of lane quarter w % 4
 constexpr int kUnpackWarp0 = 16;     // warps 16-19: keys, the tiles' scales, values
-constexpr int kMmaWarp = 20;
-constexpr int kThreads = 21 * 32;
+constexpr int kMmaWarp = 20;         // warps 20, 21: a row tile's products each
+constexpr int kThreads = 22 * 32;
 constexpr int kStages = 2;
 constexpr float kExponents = 110.0F;
 constexpr float kLift = 2.0F;        // a reference is set 2^2 below the largest p vs seen
@@ -309,16 +309,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 4);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], tiles_m);
       mbar_init(&v_full[s], 4);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], tiles_m);
       mbar_init(&meta_empty[s], 8 * tiles_m);
     }
     for (int m = 0; m < 2; ++m) {
       mbar_init(&s_full[m], 1);
       mbar_init(&p_full[m], 8);
     }
-    mbar_init(o_full, 1);
+    mbar_init(o_full, tiles_m);
     mbar_init(q_full, 8 * tiles_m);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
   // Tensor memory: scores of the row tiles at columns 0 and 128 (probabilities over them), sums at 256 and 384.
 
   const int32_t* const pages = a.page_table + b * a.table_stride;
@@ -666,26 +666,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       if (lane == 0) mbar_arrive(&v_full[s]);
       if (i + 1 < tiles) load_values(i + 1);
     }
-  } else if (tiles > 0) {
-    // =================== products: one lane issues ===================
+  } else if (warp - kMmaWarp < tiles_m && tiles > 0) {
+    // =================== products of a row tile: one lane issues ===================
+    const int m = warp - kMmaWarp;
     const uint32_t leader = elect();
     constexpr uint32_t kInstrS = (1u << 4) | (static_cast<uint32_t>(kTokens >> 3) << 17) | (8u << 24);
     constexpr uint32_t kInstrO = (1u << 4) | (static_cast<uint32_t>(kDim >> 3) << 17) | (8u << 24);
-    auto scores = [&](int m, int s) {
+    const uint32_t s_tmem = tmem + m * 128, o_tmem = s_tmem + 256;
+    const uint64_t q_desc = operand_desc(base + L::off_q + m * L::kQBytes), k_desc = operand_desc(base + L::off_k);
+    const uint64_t v_desc = operand_desc(base + L::off_v);
+    auto scores = [&](int s) {
 #pragma unroll
       for (int k = 0; k < kDim / 16; ++k) {  // 16 dimensions: 32 bytes of a 128-byte row
-        const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
-        mma_ss(leader, tmem + m * 128, operand_desc(base + L::off_q + m * L::kQBytes + at),
-               operand_desc(base + L::off_k + s * L::kTileBytes + at), kInstrS, k > 0);
+        const uint32_t at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+        mma_ss(leader, s_tmem, q_desc + at, k_desc + (s * L::kTileBytes >> 4) + at, kInstrS, k > 0);
       }
-    };
-    auto sums = [&](int m, int s, bool add) {
-#pragma unroll
-      for (int k = 0; k < kTokens / 16; ++k) {
-        const uint32_t at = (k >> 2) * (kDim * 128) + (k & 3) * 32;
-        mma_ts(leader, tmem + 256 + m * 128, tmem + m * 128 + 8 * k, operand_desc(base + L::off_v + s * L::kTileBytes + at), kInstrO,
-               add || k > 0);
-      }
+      mma_commit(leader, &s_full[m]);
+      mma_commit(leader, &k_empty[s]);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0;
@@ -693,36 +690,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
     bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
     if (ok) {
       tc_fence_after();
-      for (int m = 0; m < tiles_m; ++m) {
-        scores(m, 0);
-        mma_commit(leader, &s_full[m]);
-      }
-      mma_commit(leader, &k_empty[0]);
-      for (int i = 0; i < tiles && ok; ++i) {
-        const int s = i & 1, next = (i + 1) & 1;
-        ok = wait(&v_full[s], (i >> 1) & 1);
-        for (int m = 0; m < tiles_m && ok; ++m) {
-          ok = wait(&p_full[m], i & 1);
-          if (!ok) break;
-          tc_fence_after();
-          sums(m, s, i > 0);
-          if (m == tiles_m - 1) mma_commit(leader, &v_empty[s]);
-          if (i + 1 < tiles) {
-            if (m == 0) ok = wait(&k_full[next], ((i + 1) >> 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            scores(m, next);
-            mma_commit(leader, &s_full[m]);
-            if (m == tiles_m - 1) mma_commit(leader, &k_empty[next]);
-          }
-        }
-      }
-      if (ok) mma_commit(leader, o_full);
+      scores(0);
     }
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int s = i & 1;
+      ok = wait(&v_full[s], (i >> 1) & 1) && wait(&p_full[m], i & 1);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < kTokens / 16; ++k) {  // 16 tokens
+        const uint32_t at = ((k >> 2) * (kDim * 128) + (k & 3) * 32) >> 4;
+        mma_ts(leader, o_tmem, s_tmem + 8 * k, v_desc + (s * L::kTileBytes >> 4) + at, kInstrO, i > 0 || k > 0);
+      }
+      mma_commit(leader, &v_empty[s]);
+      if (i + 1 < tiles) {
+        ok = wait(&k_full[s ^ 1], ((i + 1) >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        scores(s ^ 1);
+      }
+    }
+    if (ok) mma_commit(leader, o_full);
   }
   __syncwarp();
   // After a wait was given up, products under way end by themselves: time for that before the tensor memory is freed.
-  if (warp == kMmaWarp && *abort_flag) {
+  if (warp >= kMmaWarp && *abort_flag) {
     const uint64_t t0 = global_ns();
     while (global_ns() - t0 < 2000000ull) {
     }
