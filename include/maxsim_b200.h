@@ -358,7 +358,8 @@ int msb_w4_packed_bytes(int64_t n, int64_t k, int32_t group, int64_t* code_bytes
 int msb_w4_pack_device(const uint8_t* codes, const void* scales, int64_t n, int64_t k, int32_t group,
                        void* packed_codes, void* packed_scales, void* stream);
 /* y [rows, n] = x [rows, k] W^T + bias: fp16 or bf16 in and out, summed in fp32
- * (strides of x and y rows in elements; bias [n] of the same type, or NULL). */
+ * (strides of x and y rows in elements; rows of x on 16-byte boundaries; bias
+ * [n] of the same type, or NULL). */
 int msb_w4_product_device(const void* packed_codes, const void* packed_scales, int64_t n, int64_t k, int32_t group,
                           const void* x, int64_t x_stride, int64_t rows, const void* bias, void* y, int64_t y_stride,
                           int32_t type, int32_t device, void* stream);

@@ -1641,6 +1641,9 @@ int msb_w4_product_device(const void* packed_codes, const void* packed_scales, i
     if (rows < 0) throw InvalidArgument("rows must not be negative");
     if (rows == 0) return;
     if (!packed_codes || !packed_scales || !x || !y) throw InvalidArgument("NULL argument");
+    if ((reinterpret_cast<uintptr_t>(x) | static_cast<uint64_t>(x_stride) * 2) & 15)
+      throw InvalidArgument("rows of x must start on 16-byte boundaries");
+    if (rows > (int64_t{1} << 31) - 64) throw InvalidArgument("rows must be below 2^31");
     W4View w{};
     w.codes = static_cast<const uint8_t*>(packed_codes);
     w.scales = static_cast<const uint16_t*>(packed_scales);

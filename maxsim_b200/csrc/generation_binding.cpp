@@ -282,6 +282,9 @@ PyObject* linear(PyObject* const* args, Py_ssize_t n) {
   if (l->bias_type >= 0 && l->bias_type != type) refuse("bias and x must have the same dtype");
   at::Tensor rows = x.dim() == 2 ? x : x.reshape({-1, l->k});
   if (rows.stride(1) != 1) rows = rows.contiguous();
+  // The kernel reads 16 bytes at a time: rows that do not start on 16 bytes are copied.
+  if ((reinterpret_cast<uintptr_t>(rows.const_data_ptr()) | static_cast<uint64_t>(rows.stride(0)) * 2) & 15)
+    rows = rows.clone(at::MemoryFormat::Contiguous);
   c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = l->n;
   at::Tensor out;

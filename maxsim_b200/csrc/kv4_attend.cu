@@ -747,18 +747,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(Kv4View c, Kv
   }
 }
 
-// Opts a kernel in to its dynamic shared memory, once per device.
-template <auto kernel>
-void allow_shared(int bytes) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  check(cudaGetDevice(&dev), "get device");
-  const uint64_t bit = uint64_t{1} << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory of the cache attention kernel");
-  done.fetch_or(bit, std::memory_order_relaxed);
-}
-
 struct Shape {
   int tiles;        // column tiles of 8 rows
   int64_t blocks;   // blocks of the main kernel
@@ -794,7 +782,7 @@ void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
   const Line line{c.heads, a.heads / c.heads, 8 * kTiles, c.page_shift, (starts & 15) == 0};
   constexpr int kShared = ring_bytes(kDim);
   static_assert(kShared >= static_cast<int>(sizeof(float)) * kWarps * 8 * kTiles * (kDim + 4), "sums fit the ring");
-  allow_shared<kv4_attend_kernel<T, kDim, kTiles>>(kShared);
+  allow_dynamic_shared<kv4_attend_kernel<T, kDim, kTiles>>(kShared, "shared memory of the cache attention kernel");
   kv4_attend_kernel<T, kDim, kTiles><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
   count_launch();
   check(cudaGetLastError(), "launch cache attention kernel");

@@ -16,7 +16,6 @@
 //   moved (and the sums rescaled) only when it is passed by 2^8, which fp16 holds.
 // Every wait is bounded; a block that gives up writes NaN rows.
 #include <algorithm>
-#include <atomic>
 #include <climits>
 
 #include "quant4.cuh"
@@ -725,17 +724,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <auto kernel>
-void allow_shared(int bytes) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  check(cudaGetDevice(&dev), "get device");
-  const uint64_t bit = uint64_t{1} << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory of the chunk attention kernel");
-  done.fetch_or(bit, std::memory_order_relaxed);
-}
-
 template <class T, int kDim>
 void launch_dim(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
   const int shared = a.heads / c.heads;
@@ -744,7 +732,7 @@ void launch_dim(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
   if (blocks > INT_MAX) throw InvalidArgument("batch * heads * query rows are too many for one call");
   const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
-  allow_shared<kv4_chunk_kernel<T, kDim>>(Layout<kDim>::kBytes);
+  allow_dynamic_shared<kv4_chunk_kernel<T, kDim>>(Layout<kDim>::kBytes, "shared memory of the chunk attention kernel");
   kv4_chunk_kernel<T, kDim><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
       c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
   count_launch();

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace msb {
@@ -97,6 +99,18 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page
     s.rows = static_cast<int>(max(static_cast<int64_t>(0), min(hi - lo, static_cast<int64_t>(a.max_rows))));
   }
   return s;
+}
+
+// Opts a kernel in to its dynamic shared memory, once per device.
+template <auto kernel>
+void allow_dynamic_shared(int bytes, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  check(cudaGetDevice(&dev), "get device");
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+  done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 struct W4View {

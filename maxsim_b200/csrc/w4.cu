@@ -45,7 +45,7 @@ __global__ void w4_pack_kernel(const uint8_t* __restrict__ codes, const uint16_t
   }
 }
 
-constexpr int kWarps = 8;
+constexpr int kMaxWarps = 8;
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -77,157 +77,199 @@ __device__ __forceinline__ void unpack(uint32_t (&a)[4], uint32_t w, __nv_bfloat
   }
 }
 
-// kCols column tiles of 8 input rows, kRowTiles tiles of 16 weight rows to a warp, kFine: groups of 32.
+// 16 bytes (4 bytes) to shared memory, zeros where not `valid`.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// One input tile of a warp: codes of its row tiles, its inputs (rows of 128 bytes, 16-byte pieces), scales.
+template <int kCols, int kRowTiles, bool kFine>
+struct Stage {
+  static constexpr int kParts = kFine ? 2 : 1;   // scales of a 64-input tile
+  static constexpr int off_x = kRowTiles * 512;
+  static constexpr int off_scales = off_x + kCols * 1024;
+  static constexpr int kBytes = off_scales + kRowTiles * kParts * 32;
+  // Tiles on their way: enough bytes in flight with 16 warps to an SM (8 with 32 input rows).
+  static constexpr int kStages = kCols == 1 ? 8 / kRowTiles : 4;
+};
+
+// kCols column tiles of 8 input rows, kRowTiles tiles of 16 weight rows to a block, kFine: groups of 32.  The block's
+// warps share the inputs out.
 template <class T, int kCols, int kRowTiles, bool kFine>
-__global__ void __launch_bounds__(kWarps * 32) w4_product_kernel(W4View w, W4Product p, int split, bool aligned) {
-  constexpr int kParts = kFine ? 2 : 1;   // scales of a 64-input tile
-  constexpr int kAhead = kCols * kRowTiles >= 8 ? 1 : kCols * kRowTiles >= 4 ? 2 : 4;  // input tiles loaded together
-  constexpr int kPitch = 8 * kCols + 1;
-  __shared__ float sums[kWarps][kRowTiles * 16 * kPitch];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+__global__ void __launch_bounds__(kMaxWarps * 32, kCols < 4 ? 2 : 1) w4_product_kernel(W4View w, W4Product p) {
+  using S = Stage<kCols, kRowTiles, kFine>;
+  constexpr int kRows = 16 * kRowTiles, kPitch = 8 * kCols + 1;
+  extern __shared__ __align__(128) unsigned char ring[];
+  float(*sums)[kRows * kPitch] = reinterpret_cast<float(*)[kRows * kPitch]>(ring);  // after the last tile
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, warps = blockDim.x >> 5;
   const int tiles_n = static_cast<int>((w.n + 15) / 16), tiles_k = static_cast<int>((w.k + 63) / 64);
   const int groups = static_cast<int>((w.k + w.group - 1) / w.group), group_shift = w.group == 128 ? 1 : 0;
-  const int slice = warp % split;  // of the inputs
-  const int tile0 = (static_cast<int>(blockIdx.x) * (kWarps / split) + warp / split) * kRowTiles;
+  const int tile0 = static_cast<int>(blockIdx.x) * kRowTiles;
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * (8 * kCols);
-  const int k_begin = static_cast<int>(static_cast<int64_t>(tiles_k) * slice / split);
-  const int k_end = tile0 < tiles_n ? static_cast<int>(static_cast<int64_t>(tiles_k) * (slice + 1) / split) : k_begin;
+  const int k_begin = static_cast<int>(static_cast<int64_t>(tiles_k) * warp / warps);
+  const int k_end = static_cast<int>(static_cast<int64_t>(tiles_k) * (warp + 1) / warps);
 
   const uint4* codes[kRowTiles];
-  const uint32_t* scales[kRowTiles];  // bfloat16 of rows g and g + 8
+  const uint32_t* scales[kRowTiles];  // bfloat16 of rows g and g + 8: copied by the lanes with t = 0
 #pragma unroll
   for (int r = 0; r < kRowTiles; ++r) {
     const int64_t tile = min(tile0 + r, tiles_n - 1);
-    codes[r] = reinterpret_cast<const uint4*>(w.codes) + tile * tiles_k * 32 + lane;
+    codes[r] = reinterpret_cast<const uint4*>(w.codes) + (tile * tiles_k + k_begin) * 32 + lane;
     scales[r] = reinterpret_cast<const uint32_t*>(w.scales) + tile * groups * 8 + g;
   }
-  const T* x[kCols];
-  bool live[kCols];
+  // Copies of inputs: lane l takes piece l % 8 of rows l / 8 and on, by fours; `limit`: the inputs past its piece.
+  const int piece = lane & 7;
+  const T* x[2 * kCols];
+  int limit[2 * kCols];
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    live[c] = row0 + c * 8 + g < p.rows;
-    x[c] = static_cast<const T*>(p.x) + (live[c] ? row0 + c * 8 + g : 0) * p.x_stride + 8 * t;
+  for (int c = 0; c < 2 * kCols; ++c) {
+    const int64_t row = row0 + 4 * c + (lane >> 3);
+    x[c] = static_cast<const T*>(p.x) + (row < p.rows ? row : 0) * p.x_stride + 8 * piece;
+    limit[c] = row < p.rows ? static_cast<int>(w.k) - 8 * piece : 0;
   }
-
-  float acc[kRowTiles][kCols][4];
-#pragma unroll
-  for (int r = 0; r < kRowTiles; ++r)
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[r][c][i] = 0.0F;
-
-  for (int k0 = k_begin; k0 < k_end; k0 += kAhead) {
-    uint4 word[kAhead][kRowTiles], in[kAhead][kCols][2];
-    uint32_t scale[kAhead][kRowTiles][kParts];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int kt = min(k0 + u, k_end - 1);
+  unsigned char* const stages = ring + warp * (S::kStages * S::kBytes);
+  const uint32_t stage_at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
+  // Pieces of odd rows lie four on (of eight): the eight lanes that read together then meet no bank twice.
+  const uint32_t x_dst = static_cast<uint32_t>(S::off_x + (lane >> 3) * 128 + ((piece ^ ((lane >> 3) & 1) << 2) << 4));
+  auto copy_tile = [&](int kt, int stage) {
+    if (kt < k_end) {
+      const uint32_t dst = stage_at + stage * S::kBytes;
 #pragma unroll
       for (int r = 0; r < kRowTiles; ++r) {
-        word[u][r] = __ldcs(codes[r] + static_cast<int64_t>(kt) * 32);
+        copy16(dst + r * 512 + lane * 16, codes[r], true);
+        codes[r] += 32;
+        if (t == 0) {
 #pragma unroll
-        for (int h = 0; h < kParts; ++h) {
-          const int at = kFine ? 2 * kt + h : kt >> group_shift;
-          scale[u][r][h] = __ldg(scales[r] + min(at, groups - 1) * 8);
+          for (int h = 0; h < S::kParts; ++h)
+            copy4(dst + S::off_scales + (r * S::kParts + h) * 32 + g * 4,
+                  scales[r] + (kFine ? min(2 * kt + h, groups - 1) : kt >> group_shift) * 8);
         }
       }
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          in[u][c][h] = make_uint4(0, 0, 0, 0);
-          const int64_t k = static_cast<int64_t>(kt) * 64 + 32 * h;
-          if (live[c] && k + 8 * t < w.k) {
-            if (aligned) {
-              in[u][c][h] = __ldg(reinterpret_cast<const uint4*>(x[c] + k));
-            } else {
-              __align__(16) T e[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) e[i] = x[c][k + i];
-              in[u][c][h] = *reinterpret_cast<const uint4*>(e);
-            }
-          }
-        }
+      for (int c = 0; c < 2 * kCols; ++c) {
+        const bool valid = kt * 64 < limit[c];
+        copy16(dst + x_dst + c * 512, valid ? x[c] + kt * 64 : x[c], valid);
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  float2 acc[kRowTiles][kCols][2];  // rows g and g + 8, two columns each
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (k0 + u >= k_end) break;
+  for (int r = 0; r < kRowTiles; ++r)
 #pragma unroll
-      for (int r = 0; r < kRowTiles; ++r) {
-        const uint32_t words[4] = {word[u][r].x, word[u][r].y, word[u][r].z, word[u][r].w};
-        float part[kCols][4];
+    for (int c = 0; c < kCols; ++c) acc[r][c][0] = acc[r][c][1] = make_float2(0.0F, 0.0F);
+
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i == 0 || (kFine && i == 2)) {
+  for (int i = 0; i < S::kStages - 1; ++i) copy_tile(k_begin + i, i);
+  int stage = 0;
+  for (int kt = k_begin; kt < k_end; ++kt) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+    __syncwarp();
+    // Every lane has left the stage of the tile before: the next copies go there.
+    copy_tile(kt + S::kStages - 1, stage == 0 ? S::kStages - 1 : stage - 1);
+    const unsigned char* const here = stages + stage * S::kBytes;
+    stage = stage == S::kStages - 1 ? 0 : stage + 1;
+    uint4 in[kCols][2];
 #pragma unroll
-            for (int c = 0; c < kCols; ++c)
+    for (int c = 0; c < kCols; ++c)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) part[c][j] = 0.0F;
-          }
-          uint32_t a[4];
-          unpack(a, words[i], T());
+      for (int h = 0; h < 2; ++h)
+        in[c][h] = *reinterpret_cast<const uint4*>(here + S::off_x + (8 * c + g) * 128 + (((4 * h + t) ^ ((g & 1) << 2)) << 4));
+#pragma unroll
+    for (int r = 0; r < kRowTiles; ++r) {
+      const uint4 word = *reinterpret_cast<const uint4*>(here + r * 512 + lane * 16);
+      const uint32_t words[4] = {word.x, word.y, word.z, word.w};
+      float part[kCols][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i == 0 || (kFine && i == 2)) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) part[c][j] = 0.0F;
+        }
+        uint32_t a[4];
+        unpack(a, words[i], T());
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const uint4 v = in[c][i >> 1];
+          mma(part[c], a, i & 1 ? v.z : v.x, i & 1 ? v.w : v.y, T());
+        }
+        if (i == 3 || (kFine && i == 1)) {
+          const uint32_t sc = *reinterpret_cast<const uint32_t*>(here + S::off_scales + (r * S::kParts + (kFine ? i >> 1 : 0)) * 32 + g * 4);
+          const float lo = __uint_as_float(sc << 16), hi = __uint_as_float(sc & 0xFFFF0000u);
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
-            const uint4 v = in[u][c][i >> 1];
-            mma(part[c], a, i & 1 ? v.z : v.x, i & 1 ? v.w : v.y, T());
-          }
-          if (i == 3 || (kFine && i == 1)) {
-            const uint32_t sc = scale[u][r][kFine ? i >> 1 : 0];
-            const float lo = __uint_as_float(sc << 16), hi = __uint_as_float(sc & 0xFFFF0000u);
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              acc[r][c][0] = fmaf(part[c][0], lo, acc[r][c][0]);
-              acc[r][c][1] = fmaf(part[c][1], lo, acc[r][c][1]);
-              acc[r][c][2] = fmaf(part[c][2], hi, acc[r][c][2]);
-              acc[r][c][3] = fmaf(part[c][3], hi, acc[r][c][3]);
-            }
+            acc[r][c][0] = __ffma2_rn(make_float2(part[c][0], part[c][1]), make_float2(lo, lo), acc[r][c][0]);
+            acc[r][c][1] = __ffma2_rn(make_float2(part[c][2], part[c][3]), make_float2(hi, hi), acc[r][c][1]);
           }
         }
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
 
-  // The slices' sums, in their order, then the bias and the one rounding.
+  // The warps' sums, in their order, then the bias and the one rounding.
 #pragma unroll
   for (int r = 0; r < kRowTiles; ++r)
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sums[warp][(r * 16 + g + 8 * (i >> 1)) * kPitch + c * 8 + 2 * t + (i & 1)] = acc[r][c][i];
+      for (int h = 0; h < 2; ++h) {
+        float* to = &sums[warp][(r * 16 + g + 8 * h) * kPitch + c * 8 + 2 * t];
+        to[0] = acc[r][c][h].x;
+        to[1] = acc[r][c][h].y;
+      }
   __syncthreads();
-  constexpr int kOutputs = kRowTiles * 16 * 8 * kCols;
-  for (int i = threadIdx.x; i < kOutputs * (kWarps / split); i += kWarps * 32) {
-    const int unit = i / kOutputs, n = i % (kRowTiles * 16), m = (i % kOutputs) / (kRowTiles * 16);
-    const int64_t out_n = (static_cast<int64_t>(blockIdx.x) * (kWarps / split) + unit) * kRowTiles * 16 + n;
+  for (int i = threadIdx.x; i < kRows * 8 * kCols; i += blockDim.x) {
+    const int n = i % kRows, m = i / kRows;
+    const int64_t out_n = static_cast<int64_t>(blockIdx.x) * kRows + n;
     if (out_n >= w.n || row0 + m >= p.rows) continue;
     float y = 0.0F;
-    for (int k = 0; k < split; ++k) y += sums[unit * split + k][n * kPitch + m];
+    for (int k = 0; k < warps; ++k) y += sums[k][n * kPitch + m];
     if (p.bias) y += to_f32(static_cast<const T*>(p.bias)[out_n]);
     static_cast<T*>(p.y)[(row0 + m) * p.y_stride + out_n] = from_f32<T>(y);
   }
 }
 
+template <class T, int kCols, int kRowTiles, bool kFine>
+void launch_stages(const W4View& w, const W4Product& p, dim3 grid, int warps, cudaStream_t stream) {
+  using S = Stage<kCols, kRowTiles, kFine>;
+  constexpr int kPerWarp = S::kStages * S::kBytes;
+  static_assert(kPerWarp >= 16 * kRowTiles * (8 * kCols + 1) * static_cast<int>(sizeof(float)), "sums fit the ring");
+  allow_dynamic_shared<w4_product_kernel<T, kCols, kRowTiles, kFine>>(kMaxWarps * kPerWarp, "shared memory of the 4-bit weight product kernel");
+  w4_product_kernel<T, kCols, kRowTiles, kFine><<<grid, warps * 32, warps * kPerWarp, stream>>>(w, p);
+}
+
 template <class T, int kCols, int kRowTiles>
 void launch_cols(const W4View& w, const W4Product& p, cudaStream_t stream) {
-  const int64_t units = (w.n + 16 * kRowTiles - 1) / (16 * kRowTiles);
-  const int64_t tiles_k = (w.k + 63) / 64;
-  int split = kWarps;
-  while (split > 1 && split > tiles_k) split >>= 1;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | static_cast<uint64_t>(p.x_stride) * sizeof(T)) & 15) == 0;
-  const int per_block = kWarps / split;
-  const dim3 grid(static_cast<unsigned>((units + per_block - 1) / per_block),
-                  static_cast<unsigned>((p.rows + 8 * kCols - 1) / (8 * kCols)));
-  if (w.group == 32) w4_product_kernel<T, kCols, kRowTiles, true><<<grid, kWarps * 32, 0, stream>>>(w, p, split, aligned);
-  else w4_product_kernel<T, kCols, kRowTiles, false><<<grid, kWarps * 32, 0, stream>>>(w, p, split, aligned);
+  const int64_t units = (w.n + 16 * kRowTiles - 1) / (16 * kRowTiles), tiles_k = (w.k + 63) / 64;
+  // Few blocks: eight warps each, so that a block's inputs are through sooner; more than two to an SM: four, so that
+  // they are resident together.
+  int warps = units <= 2 * 148 ? 8 : 4;
+  while (warps > 1 && warps > tiles_k) warps >>= 1;
+  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>((p.rows + 8 * kCols - 1) / (8 * kCols)));
+  if (w.group == 32) launch_stages<T, kCols, kRowTiles, true>(w, p, grid, warps, stream);
+  else launch_stages<T, kCols, kRowTiles, false>(w, p, grid, warps, stream);
 }
 
 template <class T>
 void launch_typed(const W4View& w, const W4Product& p, cudaStream_t stream) {
-  if (p.rows <= 8) launch_cols<T, 1, 1>(w, p, stream);
-  else if (p.rows <= 16) launch_cols<T, 2, 2>(w, p, stream);
-  else launch_cols<T, 4, 2>(w, p, stream);
+  // Two row tiles to a block share its inputs' loads, where that leaves a block for every SM.
+  const bool wide = w.n >= 2 * 16 * 148;
+  if (p.rows <= 8) {
+    if (wide) launch_cols<T, 1, 2>(w, p, stream);
+    else launch_cols<T, 1, 1>(w, p, stream);
+  } else if (p.rows <= 16) {
+    launch_cols<T, 2, 2>(w, p, stream);
+  } else {
+    launch_cols<T, 4, 2>(w, p, stream);
+  }
 }
 
 }  // namespace

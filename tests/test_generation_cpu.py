@@ -88,6 +88,9 @@ def test_weights():
         check(lib.msb_w4_product_device(_PTR, None, 16, 64, 32, _PTR, 64, 1, None, _PTR, 16, _lib.TYPE_F16, 0, None))
     with pytest.raises(ValueError, match="fp16 or bf16"):
         check(lib.msb_w4_product_device(_PTR, _PTR, 16, 64, 32, _PTR, 64, 1, None, _PTR, 16, _lib.TYPE_F32, 0, None))
+    for x, stride in ((_PTR + 2, 64), (_PTR, 68)):
+        with pytest.raises(ValueError, match="16-byte"):
+            check(lib.msb_w4_product_device(_PTR, _PTR, 16, 64, 32, x, stride, 1, None, _PTR, 16, _lib.TYPE_F16, 0, None))
     check(lib.msb_w4_product_device(None, None, 16, 64, 32, None, 64, 0, None, None, 16, _lib.TYPE_F16, 0, None))
 
 
