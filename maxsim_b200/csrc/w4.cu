@@ -97,7 +97,7 @@ struct Stage {
 };
 
 // kCols column tiles of 8 input rows, kRowTiles tiles of 16 weight rows to a block, kFine: groups of 32.  The block's
-// warps share the inputs out.
+// warps take the input tiles in turn, so that together they read consecutive bytes.
 template <class T, int kCols, int kRowTiles, bool kFine>
 __global__ void __launch_bounds__(kMaxWarps * 32, kCols < 4 ? 2 : 1) w4_product_kernel(W4View w, W4Product p) {
   using S = Stage<kCols, kRowTiles, kFine>;
@@ -109,15 +109,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, kCols < 4 ? 2 : 1) w4_product_
   const int groups = static_cast<int>((w.k + w.group - 1) / w.group), group_shift = w.group == 128 ? 1 : 0;
   const int tile0 = static_cast<int>(blockIdx.x) * kRowTiles;
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * (8 * kCols);
-  const int k_begin = static_cast<int>(static_cast<int64_t>(tiles_k) * warp / warps);
-  const int k_end = static_cast<int>(static_cast<int64_t>(tiles_k) * (warp + 1) / warps);
 
   const uint4* codes[kRowTiles];
   const uint32_t* scales[kRowTiles];  // bfloat16 of rows g and g + 8: copied by the lanes with t = 0
 #pragma unroll
   for (int r = 0; r < kRowTiles; ++r) {
     const int64_t tile = min(tile0 + r, tiles_n - 1);
-    codes[r] = reinterpret_cast<const uint4*>(w.codes) + (tile * tiles_k + k_begin) * 32 + lane;
+    codes[r] = reinterpret_cast<const uint4*>(w.codes) + (tile * tiles_k + warp) * 32 + lane;
     scales[r] = reinterpret_cast<const uint32_t*>(w.scales) + tile * groups * 8 + g;
   }
   // Copies of inputs: lane l takes piece l % 8 of rows l / 8 and on, by fours; `limit`: the inputs past its piece.
@@ -135,12 +133,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, kCols < 4 ? 2 : 1) w4_product_
   // Pieces of odd rows lie four on (of eight): the eight lanes that read together then meet no bank twice.
   const uint32_t x_dst = static_cast<uint32_t>(S::off_x + (lane >> 3) * 128 + ((piece ^ ((lane >> 3) & 1) << 2) << 4));
   auto copy_tile = [&](int kt, int stage) {
-    if (kt < k_end) {
+    if (kt < tiles_k) {
       const uint32_t dst = stage_at + stage * S::kBytes;
 #pragma unroll
       for (int r = 0; r < kRowTiles; ++r) {
         copy16(dst + r * 512 + lane * 16, codes[r], true);
-        codes[r] += 32;
+        codes[r] += warps * 32;
         if (t == 0) {
 #pragma unroll
           for (int h = 0; h < S::kParts; ++h)
@@ -164,13 +162,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, kCols < 4 ? 2 : 1) w4_product_
     for (int c = 0; c < kCols; ++c) acc[r][c][0] = acc[r][c][1] = make_float2(0.0F, 0.0F);
 
 #pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) copy_tile(k_begin + i, i);
+  for (int i = 0; i < S::kStages - 1; ++i) copy_tile(warp + i * warps, i);
   int stage = 0;
-  for (int kt = k_begin; kt < k_end; ++kt) {
+  for (int kt = warp; kt < tiles_k; kt += warps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
     __syncwarp();
     // Every lane has left the stage of the tile before: the next copies go there.
-    copy_tile(kt + S::kStages - 1, stage == 0 ? S::kStages - 1 : stage - 1);
+    copy_tile(kt + (S::kStages - 1) * warps, stage == 0 ? S::kStages - 1 : stage - 1);
     const unsigned char* const here = stages + stage * S::kBytes;
     stage = stage == S::kStages - 1 ? 0 : stage + 1;
     uint4 in[kCols][2];
