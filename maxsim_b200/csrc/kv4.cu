@@ -6,9 +6,9 @@
 // units in the last place of the corpus packer's quotient.  A vector with an element that is not finite
 // stores scale NaN and codes 0: it reads back, and is attended to, as NaN, and nothing else changes.
 //
-// Both kernels are bound by memory.  A thread has 8 dimensions (one word of codes, 16 bytes of 16-bit
-// elements) of a token's key and value, D / 8 neighbouring threads a vector: loads and stores are whole
-// 32-byte sectors in one pass, and a thread's two vectors are two independent loads.
+// Both kernels are bound by memory.  Writing, a thread has 8 dimensions (one word of codes, 16 bytes of 16-bit
+// elements) of a token's key and value, D / 8 neighbouring threads a vector; reading, 16 bytes of output.  A thread
+// asks for several vectors before it works on the first: whole sectors, and enough of them on their way.
 #include <algorithm>
 
 #include "quant4.cuh"
@@ -25,9 +25,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // Eight consecutive elements as fp32.
-template <class T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p, bool aligned) {
-  if (aligned) {
+template <bool kAligned, class T>
+__device__ __forceinline__ void load8(float (&x)[8], const T* p) {
+  if constexpr (kAligned) {
     constexpr int kLoads = 8 * sizeof(T) / 16;
     uint4 v[kLoads];
 #pragma unroll
@@ -42,9 +42,10 @@ __device__ __forceinline__ void load8(float (&x)[8], const T* p, bool aligned) {
 }
 
 // rint(fl(x / s)) of eight elements with |x / s| <= 7.1, as a word of codes.
-// For s of ordinary size the quotients share one reciprocal: with r = RN(1 / s), two steps of
-// q += r (x - q s), each remainder exact in an FMA, give RN(x / s) (P. Markstein, "Computation of elementary
-// functions on the IBM RISC System/6000 processor", 1990); elsewhere the division itself.  Adding 1.5 * 2^23 + 8
+// For s of ordinary size the quotients share one reciprocal: with r = RN(1 / s) and q = RN(x r), one step
+// q + r (x - q s), the remainder exact in an FMA, gives RN(x / s) (P. Markstein, "Computation of elementary
+// functions on the IBM RISC System/6000 processor", 1990; checked for every significand of s at the seven x
+// around each half-integer quotient); elsewhere the division itself.  Adding 1.5 * 2^23 + 8
 // rounds to the nearest integer, ties to even, and leaves code + 8 in the last bits; the words' sum by
 // powers of 16 has the nibbles in place, the flip of each fourth bit makes them two's complement.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
@@ -55,7 +56,6 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
 #pragma unroll
     for (int i = 7; i >= 0; --i) {
       float q = __fmul_rn(x[i], r);
-      q = __fmaf_rn(__fmaf_rn(-q, s, x[i]), r, q);
       q = __fmaf_rn(__fmaf_rn(-q, s, x[i]), r, q);
       word = word * 16u + __float_as_uint(__fadd_rn(q, kRound));
     }
@@ -71,85 +71,116 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
   return word ^ 0x88888888u;
 }
 
-template <class T, int kDim>
-__global__ void __launch_bounds__(kThreads) kv4_append_kernel(Kv4View c, Kv4Append a, bool aligned) {
-  constexpr int kLanes = kDim / 8;  // threads of a vector
-  const uint32_t vec = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const int lane = threadIdx.x % kLanes;
-  const bool inside = vec < static_cast<uint32_t>(a.tokens) * c.heads;  // below 2^31
-  const uint32_t token = inside ? vec / c.heads : 0, head = inside ? vec - token * c.heads : 0;
-  const int64_t slot = inside ? __ldg(a.slots + token) : -1;
-  const bool held = slot >= 0 && slot < (c.num_pages << c.page_shift);
-  float x[2][8], m[2];
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[w][i] = 0.0F;
-    if (held)
-      load8(x[w], static_cast<const T*>(a.x[w]) + token * a.token_stride[w] + head * a.head_stride[w] + lane * 8, aligned);
-  }
-  // The maximum keeps a NaN, and is infinite where an element is: both mark a vector that is not finite.
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    m[w] = 0.0F;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m[w] = max_nan(m[w], fabsf(x[w][i]));
-#pragma unroll
-    for (int d = 1; d < kLanes; d <<= 1) m[w] = max_nan(m[w], __shfl_xor_sync(0xFFFFFFFFu, m[w], d));
-  }
-  if (!held) return;
-  const int64_t at = c.vector(slot >> c.page_shift, head, static_cast<int>(slot & ((1 << c.page_shift) - 1)));
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const bool finite = m[w] < INFINITY;
-    float s = __fmul_rn(m[w], 1.0F / 7.0F);
-    if (s == 0.0F) s = 1.0F;
-    const uint32_t word = finite ? codes_of(x[w], s) : 0u;
-    *reinterpret_cast<uint32_t*>(c.codes[w] + at * (kDim / 2) + lane * 4) = word;
-    if (lane == 0) c.scales[w][at] = finite ? s : __int_as_float(0x7FC00000);
-  }
-}
+// A block has one head: its vectors are neighbours in the cache, and a vector's place needs no division.
+constexpr int kWrites = 2;  // tokens of a thread, loaded together
 
-template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  __align__(16) T e[8];
+template <class T, int kDim, bool kAligned>
+__global__ void __launch_bounds__(kThreads) kv4_append_kernel(Kv4View c, Kv4Append a) {
+  constexpr int kLanes = kDim / 8, kStep = kThreads / kLanes;  // threads of a vector, vectors at a time
+  const int head = blockIdx.y, lane = threadIdx.x % kLanes;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kStep * kWrites) + threadIdx.x / kLanes;
+  float x[kWrites][2][8];
+  int64_t slot[kWrites];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i)
-    __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<const uint4*>(e)[i]);
-}
-
-template <class T, int kDim>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4View c, Kv4Read a) {
-  constexpr int kLanes = kDim / 8;
-  const uint32_t vec = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const int lane = threadIdx.x % kLanes;
-  if (vec >= static_cast<uint32_t>(a.tokens) * c.heads) return;
-  const uint32_t token = vec / c.heads, head = vec - token * c.heads;
-  const int64_t slot = __ldg(a.slots + token);
-  const bool held = slot >= 0 && slot < (c.num_pages << c.page_shift);
-  uint32_t word[2] = {0, 0};
-  float s[2] = {0.0F, 0.0F};
-  if (held) {
-    const int64_t at = c.vector(slot >> c.page_shift, head, static_cast<int>(slot & ((1 << c.page_shift) - 1)));
+  for (int k = 0; k < kWrites; ++k) {
+    const int64_t token = first + k * kStep;
+    const bool inside = token < a.tokens;
+    slot[k] = inside ? __ldg(a.slots + token) : -1;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      word[w] = __ldg(reinterpret_cast<const uint32_t*>(c.codes[w] + at * (kDim / 2) + lane * 4));
-      s[w] = __ldg(c.scales[w] + at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[k][w][i] = 0.0F;
+      if (inside) load8<kAligned>(x[k][w], static_cast<const T*>(a.x[w]) + token * a.token_stride[w] + head * a.head_stride[w] + lane * 8);
     }
   }
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    float x[8];
+  for (int k = 0; k < kWrites; ++k) {
+    // The maximum keeps a NaN, and is infinite where an element is: both mark a vector that is not finite.
+    float m[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // 2^23 + (code + 8) as float bits, less 2^23 + 8
-      const float u = __uint_as_float((((word[w] >> (4 * i)) & 15u) ^ 8u) | 0x4B000000u);
-      x[i] = __fmul_rn(__fsub_rn(u, 8388616.0F), s[w]);
+    for (int w = 0; w < 2; ++w) {
+      m[w] = 0.0F;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m[w] = max_nan(m[w], fabsf(x[k][w][i]));
+#pragma unroll
+      for (int d = 1; d < kLanes; d <<= 1) m[w] = max_nan(m[w], __shfl_xor_sync(0xFFFFFFFFu, m[w], d));
     }
-    store8(static_cast<T*>(a.out[w]) + static_cast<int64_t>(vec) * kDim + lane * 8, x);
+    if (slot[k] < 0 || slot[k] >= (c.num_pages << c.page_shift)) continue;
+    const int64_t at = c.vector(slot[k] >> c.page_shift, head, static_cast<int>(slot[k] & ((1 << c.page_shift) - 1)));
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const bool finite = m[w] < INFINITY;
+      float s = __fmul_rn(m[w], 1.0F / 7.0F);
+      if (s == 0.0F) s = 1.0F;
+      const uint32_t word = finite ? codes_of(x[k][w], s) : 0u;
+      *reinterpret_cast<uint32_t*>(c.codes[w] + at * (kDim / 2) + lane * 4) = word;
+      if (lane == 0) c.scales[w][at] = finite ? s : __int_as_float(0x7FC00000);
+    }
   }
+}
+
+// Vectors of a thread: their slots, then their codes, are asked for together.
+constexpr int kReads = 4;
+
+// A thread writes 16 bytes: 8 dimensions of a 16-bit type, 4 of fp32.
+template <class T, int kDim>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4View c, Kv4Read a) {
+  constexpr int kPer = 16 / sizeof(T), kLanes = kDim / kPer, kStep = kThreads / kLanes;
+  const uint32_t first = blockIdx.x * (kStep * kReads) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const uint32_t vectors = static_cast<uint32_t>(a.tokens) * c.heads;  // below 2^31
+  const int64_t slots = c.num_pages << c.page_shift;
+  int64_t slot[kReads];
+  uint32_t head[kReads];
+#pragma unroll
+  for (int k = 0; k < kReads; ++k) {
+    const uint32_t vec = first + k * kStep, token = vec / c.heads;
+    head[k] = vec - token * c.heads;
+    slot[k] = vec < vectors ? __ldg(a.slots + token) : -1;
+  }
+  uint32_t word[kReads][2];
+  float s[kReads][2];
+#pragma unroll
+  for (int k = 0; k < kReads; ++k) {
+    const bool held = slot[k] >= 0 && slot[k] < slots;
+    const int64_t at = held ? c.vector(slot[k] >> c.page_shift, head[k], static_cast<int>(slot[k] & ((1 << c.page_shift) - 1))) : 0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const uint8_t* codes = c.codes[w] + at * (kDim / 2) + lane * (kPer / 2);
+      word[k][w] = 0;
+      s[k][w] = 0.0F;
+      if (held) {
+        word[k][w] = kPer == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes)) : __ldg(reinterpret_cast<const uint16_t*>(codes));
+        s[k][w] = __ldg(c.scales[w] + at);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kReads; ++k) {
+    const uint32_t vec = first + k * kStep;
+    if (vec >= vectors) return;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      __align__(16) T e[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        // 2^23 + (code + 8) as float bits, less 2^23 + 8
+        const float u = __uint_as_float((((word[k][w] >> (4 * i)) & 15u) ^ 8u) | 0x4B000000u);
+        e[i] = from_f32<T>(__fmul_rn(__fsub_rn(u, 8388616.0F), s[k][w]));
+      }
+      __stcs(reinterpret_cast<uint4*>(static_cast<T*>(a.out[w]) + static_cast<int64_t>(vec) * kDim + lane * kPer),
+             *reinterpret_cast<const uint4*>(e));
+    }
+  }
+}
+
+template <class T, bool kAligned>
+void append_aligned(const Kv4View& c, const Kv4Append& a, cudaStream_t stream) {
+  const int64_t per_block = kThreads / (c.dim / 8) * kWrites;
+  const dim3 blocks(static_cast<unsigned>((a.tokens + per_block - 1) / per_block), static_cast<unsigned>(c.heads));
+  if (c.dim == 64) kv4_append_kernel<T, 64, kAligned><<<blocks, kThreads, 0, stream>>>(c, a);
+  else if (c.dim == 128) kv4_append_kernel<T, 128, kAligned><<<blocks, kThreads, 0, stream>>>(c, a);
+  else kv4_append_kernel<T, 256, kAligned><<<blocks, kThreads, 0, stream>>>(c, a);
 }
 
 template <class T>
@@ -159,17 +190,13 @@ void append_typed(const Kv4View& c, const Kv4Append& a, cudaStream_t stream) {
   for (int w = 0; w < 2; ++w)
     starts |= reinterpret_cast<uintptr_t>(a.x[w]) | static_cast<uint64_t>(a.token_stride[w]) * sizeof(T) |
               static_cast<uint64_t>(a.head_stride[w]) * sizeof(T);
-  const bool aligned = (starts & 15) == 0;
-  const int64_t vectors = a.tokens * c.heads, per_block = kThreads / (c.dim / 8);
-  const unsigned blocks = static_cast<unsigned>((vectors + per_block - 1) / per_block);
-  if (c.dim == 64) kv4_append_kernel<T, 64><<<blocks, kThreads, 0, stream>>>(c, a, aligned);
-  else if (c.dim == 128) kv4_append_kernel<T, 128><<<blocks, kThreads, 0, stream>>>(c, a, aligned);
-  else kv4_append_kernel<T, 256><<<blocks, kThreads, 0, stream>>>(c, a, aligned);
+  if ((starts & 15) == 0) append_aligned<T, true>(c, a, stream);
+  else append_aligned<T, false>(c, a, stream);
 }
 
 template <class T>
 void read_typed(const Kv4View& c, const Kv4Read& a, cudaStream_t stream) {
-  const int64_t vectors = a.tokens * c.heads, per_block = kThreads / (c.dim / 8);
+  const int64_t vectors = a.tokens * c.heads, per_block = kThreads / (c.dim * static_cast<int>(sizeof(T)) / 16) * kReads;
   const unsigned blocks = static_cast<unsigned>((vectors + per_block - 1) / per_block);
   if (c.dim == 64) kv4_read_kernel<T, 64><<<blocks, kThreads, 0, stream>>>(c, a);
   else if (c.dim == 128) kv4_read_kernel<T, 128><<<blocks, kThreads, 0, stream>>>(c, a);
