@@ -24,20 +24,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// Eight consecutive elements as fp32.
+// Eight consecutive elements as they lie.
+template <class T>
+struct Eight {
+  uint4 raw[8 * sizeof(T) / 16];
+  __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(raw)[i]); }
+};
 template <bool kAligned, class T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p) {
+__device__ __forceinline__ void load8(Eight<T>& x, const T* p) {
   if constexpr (kAligned) {
-    constexpr int kLoads = 8 * sizeof(T) / 16;
-    uint4 v[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-    const T* e = reinterpret_cast<const T*>(v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+    for (int i = 0; i < static_cast<int>(8 * sizeof(T) / 16); ++i) x.raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(x.raw)[i] = p[i];
   }
 }
 
@@ -48,23 +48,22 @@ __device__ __forceinline__ void load8(float (&x)[8], const T* p) {
 // around each half-integer quotient); elsewhere the division itself.  Adding 1.5 * 2^23 + 8
 // rounds to the nearest integer, ties to even, and leaves code + 8 in the last bits; the words' sum by
 // powers of 16 has the nibbles in place, the flip of each fourth bit makes them two's complement.
-__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
+template <bool kShared, class T>
+__device__ __forceinline__ uint32_t codes_of(const Eight<T>& x, float s) {
   constexpr float kRound = 12582912.0F + 8.0F;
+  const float r = kShared ? __frcp_rn(s) : 0.0F;
   uint32_t word = 0;
-  if (s > 0x1p-100F && s < 0x1p100F) {
-    const float r = __frcp_rn(s);
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-      float q = __fmul_rn(x[i], r);
-      q = __fmaf_rn(__fmaf_rn(-q, s, x[i]), r, q);
-      word = word * 16u + __float_as_uint(__fadd_rn(q, kRound));
+  for (int i = 7; i >= 0; --i) {
+    const float v = x.get(i);
+    float q;
+    if (kShared) {
+      q = __fmul_rn(v, r);
+      q = __fmaf_rn(__fmaf_rn(-q, s, v), r, q);
+    } else {
+      q = fminf(fmaxf(__fdiv_rn(v, s), -7.0F), 7.0F);
     }
-  } else {
-#pragma unroll
-    for (int i = 7; i >= 0; --i) {
-      const float q = fminf(fmaxf(__fdiv_rn(x[i], s), -7.0F), 7.0F);
-      word = word * 16u + __float_as_uint(__fadd_rn(q, kRound));
-    }
+    word = word * 16u + __float_as_uint(__fadd_rn(q, kRound));
   }
   // The bits of 1.5 * 2^23, 0x4B400000, came along with every power of 16.
   word -= 0x4B400000u * 0x11111111u;
@@ -73,48 +72,54 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
 
 // A block has one head: its vectors are neighbours in the cache, and a vector's place needs no division.
 constexpr int kWrites = 2;  // tokens of a thread, loaded together
-
 template <class T, int kDim, bool kAligned>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(Kv4View c, Kv4Append a) {
   constexpr int kLanes = kDim / 8, kStep = kThreads / kLanes;  // threads of a vector, vectors at a time
   const int head = blockIdx.y, lane = threadIdx.x % kLanes;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kStep * kWrites) + threadIdx.x / kLanes;
-  float x[kWrites][2][8];
+  Eight<T> x[kWrites][2];
   int64_t slot[kWrites];
 #pragma unroll
   for (int k = 0; k < kWrites; ++k) {
-    const int64_t token = first + k * kStep;
-    const bool inside = token < a.tokens;
-    slot[k] = inside ? __ldg(a.slots + token) : -1;
+    const int64_t token = first + k * kStep, here = min(token, a.tokens - 1);
+    slot[k] = token < a.tokens ? __ldg(a.slots + token) : -1;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[k][w][i] = 0.0F;
-      if (inside) load8<kAligned>(x[k][w], static_cast<const T*>(a.x[w]) + token * a.token_stride[w] + head * a.head_stride[w] + lane * 8);
-    }
+    for (int w = 0; w < 2; ++w)
+      load8<kAligned>(x[k][w], static_cast<const T*>(a.x[w]) + here * a.token_stride[w] + head * a.head_stride[w] + lane * 8);
   }
 #pragma unroll
   for (int k = 0; k < kWrites; ++k) {
     // The maximum keeps a NaN, and is infinite where an element is: both mark a vector that is not finite.
-    float m[2];
+    float m[2], s[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      m[w] = 0.0F;
+      m[w] = fabsf(x[k][w].get(0));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m[w] = max_nan(m[w], fabsf(x[k][w][i]));
+      for (int i = 1; i < 8; ++i) m[w] = max_nan(m[w], fabsf(x[k][w].get(i)));
 #pragma unroll
       for (int d = 1; d < kLanes; d <<= 1) m[w] = max_nan(m[w], __shfl_xor_sync(0xFFFFFFFFu, m[w], d));
+      s[w] = __fmul_rn(m[w], 1.0F / 7.0F);
     }
     if (slot[k] < 0 || slot[k] >= (c.num_pages << c.page_shift)) continue;
     const int64_t at = c.vector(slot[k] >> c.page_shift, head, static_cast<int>(slot[k] & ((1 << c.page_shift) - 1)));
+    uint32_t word[2];
+    // (False for a NaN.)
+    if (fminf(s[0], s[1]) > 0x1p-100F && max_nan(s[0], s[1]) < 0x1p100F) {
+      word[0] = codes_of<true>(x[k][0], s[0]);
+      word[1] = codes_of<true>(x[k][1], s[1]);
+    } else {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        if (s[w] == 0.0F) s[w] = 1.0F;
+        const bool finite = m[w] < INFINITY;
+        word[w] = finite ? codes_of<false>(x[k][w], s[w]) : 0u;
+        if (!finite) s[w] = __int_as_float(0x7FC00000);
+      }
+    }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const bool finite = m[w] < INFINITY;
-      float s = __fmul_rn(m[w], 1.0F / 7.0F);
-      if (s == 0.0F) s = 1.0F;
-      const uint32_t word = finite ? codes_of(x[k][w], s) : 0u;
-      *reinterpret_cast<uint32_t*>(c.codes[w] + at * (kDim / 2) + lane * 4) = word;
-      if (lane == 0) c.scales[w][at] = finite ? s : __int_as_float(0x7FC00000);
+      *reinterpret_cast<uint32_t*>(c.codes[w] + at * (kDim / 2) + lane * 4) = word[w];
+      if (lane == 0) c.scales[w][at] = s[w];
     }
   }
 }
