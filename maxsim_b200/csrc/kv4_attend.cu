@@ -96,21 +96,11 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// kN consecutive elements as fp32.
-template <int kN, class T>
-__device__ __forceinline__ void load_row(float (&x)[kN], const T* p, bool aligned) {
-  if (aligned) {
+// Consecutive elements from anywhere.
+template <int kRaw, class T>
+__device__ __noinline__ void load_scattered(uint4 (&raw)[kRaw], const T* p) {
 #pragma unroll
-    for (int d = 0; d < kN; d += 8) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + d);
-      const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[d + i] = to_f32(e[i]);
-    }
-  } else {
-#pragma unroll
-    for (int d = 0; d < kN; ++d) x[d] = to_f32(p[d]);
-  }
+  for (int i = 0; i < static_cast<int>(kRaw * 16 / sizeof(T)); ++i) reinterpret_cast<T*>(raw)[i] = p[i];
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -189,9 +179,31 @@ struct Place {
   int64_t before;
   int sequence;
 };
+// For 32 sequences and fewer each warp finds them by itself: units up to and of sequence `lane`.
+constexpr int kWarpBatch = 32;
+__device__ __forceinline__ void warp_line(const Kv4Attend& a, const Line& l, int64_t& before, int64_t& mine, int64_t& total) {
+  const int lane = threadIdx.x & 31;
+  mine = lane < a.batch ? sequence_work(a, l, lane).units(l) : 0;
+  int64_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  before = upto - mine;
+  total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+}
 template <class F>
 __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, F first, int64_t* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (a.batch <= kWarpBatch) {
+    int64_t before, mine, total;
+    warp_line(a, l, before, mine, total);
+    const int64_t target = first(total);
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, target >= before && target < before + mine);
+    const int at = hit ? __ffs(hit) - 1 : 0;
+    return Place{total, __shfl_sync(0xFFFFFFFFu, before, at), hit ? at : a.batch};
+  }
   constexpr int kBlock = kWarps * 32;
   int64_t mine = 0, total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kBlock) {
@@ -308,43 +320,26 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     const int head = static_cast<int>(segment / w.blocks), row0 = static_cast<int>(segment % w.blocks) * kRows;
     const int all_rows = w.q.rows * line.shared;
 
-    // Queries: lane (g, t) holds row g of each column tile, dimensions t * kDim / 4 and on.
-    uint32_t q[kTiles][2 * kKeyWords][2];
-    float2 lift[kTiles];     // what columns 2t, 2t + 1 start at (codes_key)
-    float2 factor[kTiles];   // scale * log2(e) * the row's power of two
+    // Rows: which tokens they see; lane (g, t) loads row g of each column tile, dimensions t * kDim / 4 and on.
+    constexpr int kRaw = kKeyWords * 8 * sizeof(T) / 16;
+    uint4 raw[kTiles][kRaw];
     int last[kTiles][2], first[kTiles][2];  // tokens that columns 2t, 2t + 1 see: first <= j <= last
     int every_last = INT_MAX, every_first = 0, any_last = -1, any_first = INT_MAX;
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int r = row0 + nt * 8 + g;
-      float x[kKeyWords * 8], top = 0.0F;
 #pragma unroll
-      for (int d = 0; d < kKeyWords * 8; ++d) x[d] = 0.0F;
+      for (int i = 0; i < kRaw; ++i) raw[nt][i] = make_uint4(0, 0, 0, 0);
       if (r < all_rows) {
         const T* p = static_cast<const T*>(a.query) + (w.q.row0 + r / line.shared) * a.q_row_stride +
                      static_cast<int64_t>(head * line.shared + r % line.shared) * a.q_head_stride + t * (kDim / 4);
-        load_row<kKeyWords * 8>(x, p, line.aligned);
+        if (line.aligned) {
+#pragma unroll
+          for (int i = 0; i < kRaw; ++i) raw[nt][i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+          load_scattered(raw[nt], p);
+        }
       }
-#pragma unroll
-      for (int d = 0; d < kKeyWords * 8; ++d) top = fmaxf(top, fabsf(x[d]));
-      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
-      const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
-      float sum[4] = {0.0F, 0.0F, 0.0F, 0.0F};
-#pragma unroll
-      for (int word = 0; word < kKeyWords; ++word) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          q[nt][2 * word + (i >> 1)][i & 1] = pack_half2(x[8 * word + i] * down, x[8 * word + 4 + i] * down);
-        // -72 (0xD480) times the queries of odd nibbles, summed where the scores will be
-        mma(sum, 0u, 0u, 0xD480D480u, 0xD480D480u, q[nt][2 * word][0], q[nt][2 * word][1]);
-        mma(sum, 0u, 0u, 0xD480D480u, 0xD480D480u, q[nt][2 * word + 1][0], q[nt][2 * word + 1][1]);
-      }
-      const float up = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
-      // from the lanes that hold rows 2t, 2t + 1 to the columns' lanes
-      lift[nt] = make_float2(sum[0], sum[1]);
-      factor[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, up, 8 * t), __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4));
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int rr = row0 + nt * 8 + 2 * t + k;
@@ -367,19 +362,6 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       every_first = max(every_first, __shfl_xor_sync(0xFFFFFFFFu, every_first, d));
       any_last = max(any_last, __shfl_xor_sync(0xFFFFFFFFu, any_last, d));
       any_first = min(any_first, __shfl_xor_sync(0xFFFFFFFFu, any_first, d));
-    }
-
-    float o[kOut][kTiles][4];
-    float top[kTiles][2];
-    float2 sum[kTiles];
-#pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int i = 0; i < kOut; ++i) o[i][nt][k] = 0.0F;
-      top[nt][0] = top[nt][1] = -INFINITY;
-      sum[nt] = make_float2(0.0F, 0.0F);
     }
 
     // This warp's steps of 32 tokens, those that some row sees.
@@ -438,6 +420,49 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       copy_step(j0 + i * kTile, i, i);
       ask_pages(j0 + (i + 1) * kTile);
     }
+    // Queries, while the first copies are on their way.
+    uint32_t q[kTiles][2 * kKeyWords][2];
+    float2 lift[kTiles];     // what columns 2t, 2t + 1 start at (codes_key)
+    float2 factor[kTiles];   // scale * log2(e) * the row's power of two
+#pragma unroll
+    for (int nt = 0; nt < kTiles; ++nt) {
+      const T* const x = reinterpret_cast<const T*>(raw[nt]);
+      float top = 0.0F;
+#pragma unroll
+      for (int d = 0; d < kKeyWords * 8; ++d) top = fmaxf(top, fabsf(to_f32(x[d])));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
+      float sum[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+#pragma unroll
+      for (int word = 0; word < kKeyWords; ++word) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[nt][2 * word + (i >> 1)][i & 1] = pack_half2(to_f32(x[8 * word + i]) * down, to_f32(x[8 * word + 4 + i]) * down);
+        // -72 (0xD480) times the queries of odd nibbles, summed where the scores will be
+        mma(sum, 0u, 0u, 0xD480D480u, 0xD480D480u, q[nt][2 * word][0], q[nt][2 * word][1]);
+        mma(sum, 0u, 0u, 0xD480D480u, 0xD480D480u, q[nt][2 * word + 1][0], q[nt][2 * word + 1][1]);
+      }
+      const float up = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
+      lift[nt] = make_float2(sum[0], sum[1]);
+      // from the lanes that hold rows 2t, 2t + 1 to the columns' lanes
+      factor[nt] = make_float2(__shfl_sync(0xFFFFFFFFu, up, 8 * t), __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4));
+    }
+
+    float o[kOut][kTiles][4];
+    float top[kTiles][2];
+    float2 sum[kTiles];
+#pragma unroll
+    for (int nt = 0; nt < kTiles; ++nt) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) o[i][nt][k] = 0.0F;
+      top[nt][0] = top[nt][1] = -INFINITY;
+      sum[nt] = make_float2(0.0F, 0.0F);
+    }
+
     int stage = 0;
     for (; j0 < upto; j0 += kTile) {
       copies_wait<kStages - 2>();
@@ -656,11 +681,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(Kv4View c, Kv
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x;
   const SequenceWork w = sequence_work(a, line, b);
+  int64_t before = 0, total = 0;
+  if (a.batch <= kWarpBatch) {
+    int64_t mine;
+    warp_line(a, line, before, mine, total);
+    before = __shfl_sync(0xFFFFFFFFu, before, b);
+  }
 #if __CUDA_ARCH__ >= 900
   cudaGridDependencySynchronize();
 #endif
-  const int64_t* line_starts = reinterpret_cast<const int64_t*>(a.workspace);
-  const int64_t before = line_starts[b], total = line_starts[a.batch], n = ranges(total, blocks);
+  if (a.batch > kWarpBatch) {
+    const int64_t* line_starts = reinterpret_cast<const int64_t*>(a.workspace);
+    before = line_starts[b];
+    total = line_starts[a.batch];
+  }
+  const int64_t n = ranges(total, blocks);
   const float* base = line_parts(a);
   const int rows_per_block = kJoinWarps / warps_per_row, group = warp % warps_per_row;
   const int64_t rows = static_cast<int64_t>(w.q.rows) * a.heads;
