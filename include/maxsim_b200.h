@@ -118,7 +118,10 @@ int64_t msb_launch_count(void);
  * made it slower.  "tc_row_replicas": 1 (default) copies a pass's query rows
  * (int8, at most 64) over the tensor memory's lane quarters.  "tc_fused_topk":
  * 1 selects the full-scan top-k inside the int8-query scan (bit-identical, 0 by
- * default: measured slower).  Unknown names return MSB_ERR_INVALID_ARGUMENT. */
+ * default: measured slower).  "kv4_engine": attention over the 4-bit cache, 0
+ * (default) chooses by size, 1 always runs the kernel for few query rows, 2
+ * that for many where it can (head_dim 64 and 128).  Unknown names return
+ * MSB_ERR_INVALID_ARGUMENT. */
 int msb_set_option(const char* name, int64_t value);
 int msb_get_option(const char* name, int64_t* value);
 

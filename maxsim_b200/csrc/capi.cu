@@ -66,6 +66,7 @@ static std::atomic<int> g_tc_f16_cache{0};   // keep an f16 copy instead (per-to
 // bit-identical to the unfused path, but measured slower (the list insertions serialise the epilogue's
 // document flush, and the unfused selection of a [B, D] score matrix costs well under 1 % of a scan).
 static std::atomic<int> g_tc_fused_topk{0};
+static std::atomic<int> g_kv4_engine{0};     // cache attention: 0 by size, 1 the kernel for few rows, 2 that for many
 static std::atomic<uint64_t> g_corpus_serial{0};
 }  // namespace msb
 
@@ -781,6 +782,11 @@ int msb_set_option(const char* name, int64_t value) {
       set_tc_row_replicas(static_cast<int>(value));
       return;
     }
+    if (std::strcmp(name, "kv4_engine") == 0) {
+      if (value < 0 || value > 2) throw InvalidArgument("kv4_engine must be 0 (auto), 1 (few rows) or 2 (many rows)");
+      g_kv4_engine.store(static_cast<int>(value));
+      return;
+    }
     throw InvalidArgument(std::string("unknown option: ") + name);
   });
 }
@@ -794,6 +800,10 @@ int msb_get_option(const char* name, int64_t* value) {
     }
     if (std::strcmp(name, "tc_int8_cache") == 0) {
       *value = g_tc_int8_cache.load();
+      return;
+    }
+    if (std::strcmp(name, "kv4_engine") == 0) {
+      *value = g_kv4_engine.load();
       return;
     }
     if (std::strcmp(name, "tc_f16_cache") == 0) {
@@ -1533,6 +1543,7 @@ Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   r.window = a->window;
   r.out = a->out;
   r.lse = a->lse;
+  r.engine = g_kv4_engine.load();
   r.workspace = a->workspace;
   r.workspace_bytes = a->workspace_bytes > 0 ? static_cast<size_t>(a->workspace_bytes) : 0;
   return r;

@@ -959,9 +959,17 @@ void launch_typed(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
   }
 }
 
-constexpr int kManyRows = 64;
+// Which kernel: this file's takes a time in proportion to the row blocks of 16, kv4_chunk.cu's to the waves of blocks
+// of 256 rows over the SMs, whatever fills them.  Measured per 128 tokens: 6.6 ns a row block over the whole device,
+// 2.9 us a wave (2.3 us with 128 rows or fewer).  (4 sequences of 4,096 tokens, 8 heads: 63 and 87 us at 128 rows a
+// head, 109 and 111 at 256; 32 of 2,000: 71 and 93 at 32, 121 and 95 at 64.)
 bool many_rows(const Kv4View& c, const Kv4Attend& a) {
-  return kv4_chunk_supported(c) && static_cast<int64_t>(a.max_rows) * (a.heads / c.heads) >= kManyRows;
+  if (!kv4_chunk_supported(c) || a.engine == 1) return false;
+  if (a.engine == 2) return true;
+  const int64_t rows = static_cast<int64_t>(a.max_rows) * (a.heads / c.heads);
+  const int64_t heads = static_cast<int64_t>(a.batch) * c.heads, sms = sm_count();
+  const int64_t waves = (heads * ((rows + 255) / 256) + sms - 1) / sms;
+  return heads * ((rows + 15) / 16) >= waves * (rows > 128 ? 440 : 350);
 }
 
 }  // namespace

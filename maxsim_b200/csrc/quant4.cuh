@@ -76,6 +76,7 @@ struct Kv4Attend {
   void* workspace;
   size_t workspace_bytes;
   int type;
+  int engine;                 // 0 by size, 1 the kernel for few rows, 2 that for many
 };
 
 // One sequence of an attention call, with what the device arrays say held to what the call can read:

@@ -94,6 +94,18 @@ def test_weights():
     check(lib.msb_w4_product_device(None, None, 16, 64, 32, None, 64, 0, None, None, 16, _lib.TYPE_F16, 0, None))
 
 
+def test_engine_option():
+    assert _lib.get_option("kv4_engine") == 0
+    try:
+        for v in (1, 2, 0):
+            _lib.set_option("kv4_engine", v)
+            assert _lib.get_option("kv4_engine") == v
+        with pytest.raises(ValueError, match="kv4_engine must be"):
+            _lib.set_option("kv4_engine", 3)
+    finally:
+        _lib.set_option("kv4_engine", 0)
+
+
 def test_package_refuses_host_tensors():
     torch = pytest.importorskip("torch")
     import maxsim_b200 as m
