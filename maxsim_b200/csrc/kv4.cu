@@ -9,6 +9,9 @@
 // Both kernels are bound by memory.  Writing, a thread has 8 dimensions (one word of codes, 16 bytes of 16-bit
 // elements) of a token's key and value, D / 8 neighbouring threads a vector; reading, 16 bytes of output.  A thread
 // asks for several vectors before it works on the first: whole sectors, and enough of them on their way.
+// Measured on the device, keys and values, 8 heads, D = 128: writing 32,768 tokens from bf16 38.3 us (4.4 TB/s; issue,
+// the conversions and quotients), from fp32 46.2 us (6.6 TB/s); reading them to bf16 28.3 us (6.0 TB/s), to fp32
+// 47.5 us (6.4 TB/s); either of 64 tokens 2.5 to 2.8 us.
 #include <algorithm>
 
 #include "quant4.cuh"

@@ -6,27 +6,36 @@
 // that sees nothing writes zeros and a log-sum-exp of -inf.
 //
 // kv4_attend_kernel: few rows a sequence (decode, drafted tokens).
-//   Bound: the codes' bytes, D + 8 per token and head, then the integer pipe that unpacks them.
+//   Bound: the codes' bytes, D + 8 per token and head, then instruction issue, above all the integer pipe that unpacks.
 //   Products.  m16n8k16 fp16 products with the tokens as the 16-row operand: S^T = K Q^T, O^T = V^T P^T, so
 //   8 query rows (the heads that share a key/value head, times the query tokens) fill a column tile instead
 //   of half a row tile.  tcgen05 wants 128 rows of queries, which decode has not.
-//   Operands straight from global memory: the order of the summed index is free, so lane (g, t) = (lane / 4,
-//   lane % 4) takes D / 4 consecutive dimensions of key tokens g and g + 8 (a 16-byte load each at D = 128),
-//   and D / 8 consecutive dimensions of value tokens 2t, 2t + 1, 2t + 8, 2t + 9; nothing passes through shared
-//   memory.  A 16-token tile lies in one page (pages are powers of two >= 16), so a tile has one page lookup.
-//   Unpacking.  Nibble n of a code is code & 15; (w & 0x00f000f0) ^ 0x54805480 is the fp16 pair 72 + code in
-//   one logic operation.  Keys keep the 72: accumulators start at -72 sum(q).  Values subtract it (their sum
-//   over tokens would lose digits to it): both are exact.
-//   Queries are fp16 after a power of two per row that puts their maximum in [1, 2): exact for fp16 inputs and
-//   for bf16 ones down to 2^-24 of the row's maximum.  Probabilities are fp16 (11 bits): they enter one sum
+//   Loads.  A warp takes steps of 32 tokens through a ring of its own in shared memory, three steps deep, filled by
+//   asynchronous copies: no barrier between warps, and the bytes on their way hold no registers.  A 16-token tile lies
+//   in one page (pages are powers of two >= 16), so a tile has one page lookup.
+//   Operands.  The order of the summed index is free, so lane (g, t) = (lane / 4, lane % 4) reads D / 4 consecutive
+//   dimensions of key tokens g and g + 8 (16 bytes at D = 128), and D / 8 consecutive dimensions of value tokens 2t,
+//   2t + 1, 2t + 8, 2t + 9; probabilities become operands by an 8 x 8 transpose in registers.
+//   Unpacking.  Nibbles i and i + 4 of a word are an fp16 pair in one logic operation: 1032 + code where they lie in
+//   a half's last bits, 72 + code where four above; a subtraction makes them exact codes.  Keys keep the 72:
+//   accumulators start at -72 sum(q) of those dimensions, exact products that cancel in fp32.  Values subtract
+//   both (their sum over all tokens would lose digits to them).  (As fp16 subnormals codes would need neither, but the
+//   products then lost 6 to 10 bits.)
+//   Queries are fp16 after a power of two per row that puts their maximum in [2^10, 2^11): exact for fp16 inputs
+//   down to 2^-34 of the row's maximum, and so for bf16 ones.  Probabilities are fp16 (11 bits): they enter one sum
 //   that is rounded to the output's type, of as many bits or fewer.
 //   Reference.  Probabilities carry the values' scales, p_j vs_j, so the running reference is the maximum of
-//   s_j + e_j with vs_j in 2^(e_j + [0, 1)): p_j vs_j stays in fp16's range whatever the scales are.  e_j is
-//   held to +-110, so the fp32 sum of the p_j stays finite.
-//   Work split.  The 128-token tiles of all (sequence, head, row block) segments form one line, cut into equal
+//   s_j + log2 vs_j less 8: p_j vs_j stays in fp16's normal range whatever the scales are.  The logarithm is held to
+//   +-110, so the fp32 sum of the p_j stays finite.
+//   Work split.  The 128-token units of all (sequence, head, row block) segments form one line, cut into equal
 //   ranges, one per resident block, from the lengths on the device: no plan, no host copy, no imbalance.
 //   A segment cut by a range's end leaves partial sums in the workspace (at most two per block), which
 //   kv4_join_kernel adds in a fixed order; it is launched early (programmatic dependent launch).
+//   Short contexts (launch_attend has the rule) take a cluster of 2 to 8 blocks a segment instead, whose parts are
+//   joined over distributed shared memory: one launch.
+//   Measured on the device, D = 128, 8 heads, 4 query heads each: 64 sequences of 4,096 tokens 75 us (3.8 TB/s of
+//   codes, 58% of a copy's rate), 2 of 115,000 65 us (3.9 TB/s), 1 of 16,384 17 us, 1 of 1,030 6.7 us.  At the first
+//   57% of the issue slots and of the integer pipe are used; 4 to 5 us are the join and both launches' ends.
 #include <cooperative_groups.h>
 
 #include <algorithm>
