@@ -8,10 +8,15 @@
 // [row tile][input tile]; scales are [row tile][group][rows 0, 8, 1, 9, .. 7, 15].  Rows and inputs past the matrix hold the
 // code 0 (stored 8), rows past it the scale 0.
 //
-// w4_product_kernel.  Bound: the weights' bytes; the integer pipe that unpacks them comes next (7 operations for 8
-// bf16 codes, 5 for fp16).  A warp takes 16-row tiles over a slice of the inputs, its block's warps the slices;
-// a group's sum of x * code is exact products in an fp32 accumulator, scaled once, added in fp32.  Inputs go to the
-// 8-column operand straight from global memory, 8 consecutive elements a load.
+// w4_product_kernel.  Bound: the weights' bytes, then instruction issue: unpacking takes 7 operations for 8 bf16 codes,
+// 5 for fp16 ones.  A block has 16 weight rows (or 32, below) and all inputs, which its warps take in turn, 64 at a
+// time, each through a ring of its own in shared memory that asynchronous copies fill with codes, scales and inputs: no
+// barrier before the last tile, and the weights on their way hold no registers.  A group's sum of x * code is exact
+// products in an fp32 accumulator, scaled once, added in fp32; the warps' sums are added in their order.  tcgen05 would
+// want 128 weight rows a tile and unpacked codes in shared memory: at 32 rows and fewer the products are not the bound.
+// Measured on the device, bf16, groups of 128: 16,384 x 8,192 1 row 20.9 us (3.3 TB/s of weights), 16 rows 27.4 us, 32
+// rows 42 us; 4,096 x 4,096 1 row 5.2 us, 32 rows 8.6 us; 4,096 x 14,336 1 row 11.8 us.  At 1 row the issue slots bound
+// it where blocks are many, and at 16,384 weight rows 512 blocks on 296 places leave some SMs idle at the end.
 #include <algorithm>
 
 #include "quant4.cuh"
@@ -247,9 +252,10 @@ void launch_stages(const W4View& w, const W4Product& p, dim3 grid, int warps, cu
 template <class T, int kCols, int kRowTiles>
 void launch_cols(const W4View& w, const W4Product& p, cudaStream_t stream) {
   const int64_t units = (w.n + 16 * kRowTiles - 1) / (16 * kRowTiles), tiles_k = (w.k + 63) / 64;
-  // Few blocks: eight warps each, so that a block's inputs are through sooner; more than two to an SM: four, so that
-  // they are resident together.
-  int warps = units <= 2 * 148 ? 8 : 4;
+  // Eight warps to a block are through its inputs soonest; where blocks outnumber the SMs and the inputs' columns are
+  // several, more blocks of fewer warps wait less.  (us with 2, 4 and 8 warps, bf16: 4,096 x 4,096, 16 rows 11.4, 7.3 and 6.3;
+  // 16,384 x 8,192, 8 rows 23.3, 21.9 and 21.3, 16 rows 28.1, 27.4 and 28.0, 32 rows 42.0, 43.3 and 47.2.)
+  int warps = kCols == 1 || units <= 148 ? 8 : kCols == 4 && units > 2 * 148 ? 2 : 4;
   while (warps > 1 && warps > tiles_k) warps >>= 1;
   const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>((p.rows + 8 * kCols - 1) / (8 * kCols)));
   if (w.group == 32) launch_stages<T, kCols, kRowTiles, true>(w, p, grid, warps, stream);
@@ -258,15 +264,18 @@ void launch_cols(const W4View& w, const W4Product& p, cudaStream_t stream) {
 
 template <class T>
 void launch_typed(const W4View& w, const W4Product& p, cudaStream_t stream) {
-  // Two row tiles to a block share its inputs' loads, where that leaves a block for every SM.
-  const bool wide = w.n >= 2 * 16 * 148;
+  // Two row tiles to a block share its inputs' loads, where that leaves blocks for three quarters of the SMs.  (us with one and
+  // two, 8 warps: 4,096 x 4,096, 1 row 5.6 and 5.2, 32 rows 11.5 and 8.6; 2,048 x 4,096 4.0 and 4.7, 6.3 and 8.4.)
+  const bool wide = 4 * w.n >= 3 * 148 * 32;
   if (p.rows <= 8) {
     if (wide) launch_cols<T, 1, 2>(w, p, stream);
     else launch_cols<T, 1, 1>(w, p, stream);
   } else if (p.rows <= 16) {
-    launch_cols<T, 2, 2>(w, p, stream);
+    if (wide) launch_cols<T, 2, 2>(w, p, stream);
+    else launch_cols<T, 2, 1>(w, p, stream);
   } else {
-    launch_cols<T, 4, 2>(w, p, stream);
+    if (wide) launch_cols<T, 4, 2>(w, p, stream);
+    else launch_cols<T, 4, 1>(w, p, stream);
   }
 }
 

@@ -15,6 +15,7 @@ torch = pytest.importorskip("torch")
 sys.path.insert(0, str(Path(__file__).resolve().parent))
 
 import test_gpu_kv4 as kv4  # noqa: E402
+import test_gpu_w4 as w4  # noqa: E402
 from test_gpu_kv4 import _check, _normal, _plain, _random_cache, _tables  # noqa: E402
 
 
@@ -203,3 +204,13 @@ def test_calls_on_two_streams_at_once():
                 got.append(cache.attend(q, table, length))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,k", [(3552, 200), (3551, 72), (5001, 328), (9600, 136)])
+@pytest.mark.parametrize("rows", [2, 8, 11, 16, 20, 32])
+def test_product_of_many_weight_rows(dtype, group, n, k, rows):
+    packed, scales, w = w4._codes(n, k, group, seed=n + k)
+    x = _normal((rows, k), rows, kv4.DTYPES[dtype])
+    w4._check(m.Int4Linear(packed, scales, group_size=group)(x), x, w, None, group)
