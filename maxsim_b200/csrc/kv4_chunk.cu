@@ -305,12 +305,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   uint64_t* const v_full = bars + 4;
   uint64_t* const v_empty = bars + 6;
   uint64_t* const meta_empty = bars + 8;   // [stage] scales read by every softmax warp
-  uint64_t* const s_full = bars + 10;      // [row tile] scores ready (and the sums of the tile before)
+  uint64_t* const s_full = bars + 10;      // [row tile] all scores ready (and the sums of the tile before)
   uint64_t* const p_full = bars + 12;      // [row tile] probabilities written
   uint64_t* const o_full = bars + 14;      // all sums done
   uint64_t* const q_full = bars + 15;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
-  volatile int* const abort_flag = reinterpret_cast<volatile int*>(bars + 17);
+  uint64_t* const s_half = bars + 16;      // [row tile] scores of the half that comes first ready
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(bars + 19);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 4);
@@ -320,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       mbar_init(&meta_empty[s], 8 * tiles_m);
     }
     for (int m = 0; m < 2; ++m) {
+      mbar_init(&s_half[m], 1);
       mbar_init(&s_full[m], 1);
       mbar_init(&p_full[m], 8);
     }
@@ -337,6 +339,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
   // Tensor memory: scores of the row tiles at columns 0 and 128 (probabilities over them), sums at 256 and 384.
+  // Half h of a tile's scores, 64 tokens, is in columns 64 h and on.  Of tile i the half i % 2 comes first and the
+  // probabilities of both go to its columns, so that the other half's are free for the half of tile i + 1 that
+  // comes first: its product does not wait for this tile's sums, nor its softmax.
 
   const int32_t* const pages = a.page_table + b * a.table_stride;
   const int page_mask = (1 << c.page_shift) - 1;
@@ -418,31 +423,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
         const int s = i & 1, j0 = begin + i * kTokens;
-        ok = mbar_wait(&k_full[s], (i >> 1) & 1, abort_flag) && mbar_wait(&s_full[m], i & 1, abort_flag);
+        ok = mbar_wait(&k_full[s], (i >> 1) & 1, abort_flag) && mbar_wait(&s_half[m], i & 1, abort_flag);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         tc_fence_after();
         const uint4 flag = *reinterpret_cast<const uint4*>(flags + 4 * s);
         const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < every_first ||
                                                        j0 + kTokens - 1 > every_last);
-        const float* my_meta = meta + s * 3 * kMetaFloats + (lane & 3) * kMetaPitch;
-        int my_j0 = j0 + 2 * (lane & 3);
+        const uint32_t p_at = s_at + s * (kTokens / 2);
         // Blocks of 32 columns in one short loop: its instructions stay near, the other three warps of a scheduler
         // fill its waits.
 #pragma unroll 1
         for (int part = 0; part < kTokens / kCols; ++part) {
+          const int piece = part ^ (2 * s);  // the block of columns
+          const float* const my_meta = meta + s * 3 * kMetaFloats + (4 * piece + (lane & 3)) * kMetaPitch;
+          const int my_j0 = j0 + kCols * piece + 2 * (lane & 3);
+          if (part == kTokens / kCols / 2) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], i & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+          }
           float f[16], most[2];
           float2 add[2];
           uint32_t p[8];
-          tmem_ld_block(s_at + kCols * part, f);
+          tmem_ld_block(s_at + kCols * piece, f);
           if (masked) probabilities<true>(f, my_meta, my_j0, rows, p, add, most);
           else probabilities<false>(f, my_meta, my_j0, rows, p, add, most);
           // A row without a reference yet, or one whose reference has become too low (an infinite p among it).
           const bool low = fminf(rows.top[0], rows.top[1]) == -INFINITY || fmaxf(most[0], most[1]) > kMostP;
           if (__any_sync(0xFFFFFFFFu, low)) {
-            tmem_wait_st();  // what was written before is read below
+            tmem_wait_st();  // what was written before is read below, the sums of the tiles before too
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], i & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
             float best[2], fade[2];
-            tmem_ld_block(s_at + kCols * part, f);
+            tmem_ld_block(s_at + kCols * piece, f);
             references(f, my_meta, my_j0, rows, best);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -468,21 +483,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
 #pragma unroll 1
             for (int d = 0; d < part; ++d) {  // and the probabilities of the columns before
               uint32_t w[8];
-              tmem_ld_pairs(s_at + kCols / 2 * d, w);
+              tmem_ld_pairs(p_at + kCols / 2 * d, w);
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
                 w[k] = pack_half2(v.x * fade[k & 1], v.y * fade[k & 1]);
               }
-              tmem_st_pairs(s_at + kCols / 2 * d, w);
+              tmem_st_pairs(p_at + kCols / 2 * d, w);
             }
           }
           rows.sum[0] = __fadd2_rn(rows.sum[0], add[0]);
           rows.sum[1] = __fadd2_rn(rows.sum[1], add[1]);
-          tmem_st_pairs(s_at + kCols / 2 * part, p);
-          my_meta += 4 * kMetaPitch;
-          my_j0 += kCols;
+          tmem_st_pairs(p_at + kCols / 2 * part, p);
         }
+        if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -675,17 +689,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
     // =================== products of a row tile: one lane issues ===================
     const int m = warp - kMmaWarp;
     const uint32_t leader = elect();
-    constexpr uint32_t kInstrS = (1u << 4) | (static_cast<uint32_t>(kTokens >> 3) << 17) | (8u << 24);
+    constexpr uint32_t kInstrS = (1u << 4) | (static_cast<uint32_t>(kTokens / 2 >> 3) << 17) | (8u << 24);
     constexpr uint32_t kInstrO = (1u << 4) | (static_cast<uint32_t>(kDim >> 3) << 17) | (8u << 24);
     const uint32_t s_tmem = tmem + m * 128, o_tmem = s_tmem + 256;
     const uint64_t q_desc = operand_desc(base + L::off_q + m * L::kQBytes), k_desc = operand_desc(base + L::off_k);
     const uint64_t v_desc = operand_desc(base + L::off_v);
-    auto scores = [&](int s) {
+    auto scores = [&](int s, int half) {
 #pragma unroll
       for (int k = 0; k < kDim / 16; ++k) {  // 16 dimensions: 32 bytes of a 128-byte row
         const uint32_t at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-        mma_ss(leader, s_tmem, q_desc + at, k_desc + (s * L::kTileBytes >> 4) + at, kInstrS, k > 0);
+        const uint32_t rows = half * (kTokens / 2 * 128) >> 4;
+        mma_ss(leader, s_tmem + half * (kTokens / 2), q_desc + at, k_desc + (s * L::kTileBytes >> 4) + rows + at, kInstrS, k > 0);
       }
+    };
+    auto first_half = [&](int s) {
+      scores(s, s);
+      mma_commit(leader, &s_half[m]);
+    };
+    auto other_half = [&](int s) {
+      scores(s, s ^ 1);
       mma_commit(leader, &s_full[m]);
       mma_commit(leader, &k_empty[s]);
     };
@@ -695,25 +717,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
     bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
     if (ok) {
       tc_fence_after();
-      scores(0);
+      first_half(0);
+      other_half(0);
     }
     for (int i = 0; i < tiles && ok; ++i) {
       const int s = i & 1;
-      ok = wait(&v_full[s], (i >> 1) & 1) && wait(&p_full[m], i & 1);
+      const bool more = i + 1 < tiles;
+      // Operands first, which are early: nothing but the products is then between probabilities and scores.
+      ok = wait(&v_full[s], (i >> 1) & 1) && (!more || wait(&k_full[s ^ 1], ((i + 1) >> 1) & 1)) && wait(&p_full[m], i & 1);
       if (!ok) break;
       tc_fence_after();
+      if (more) first_half(s ^ 1);
+      const uint32_t p_tmem = s_tmem + s * (kTokens / 2);
 #pragma unroll
       for (int k = 0; k < kTokens / 16; ++k) {  // 16 tokens
         const uint32_t at = ((k >> 2) * (kDim * 128) + (k & 3) * 32) >> 4;
-        mma_ts(leader, o_tmem, s_tmem + 8 * k, v_desc + (s * L::kTileBytes >> 4) + at, kInstrO, i > 0 || k > 0);
+        mma_ts(leader, o_tmem, p_tmem + 8 * (k ^ (4 * s)), v_desc + (s * L::kTileBytes >> 4) + at, kInstrO, i > 0 || k > 0);
       }
       mma_commit(leader, &v_empty[s]);
-      if (i + 1 < tiles) {
-        ok = wait(&k_full[s ^ 1], ((i + 1) >> 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        scores(s ^ 1);
-      }
+      if (more) other_half(s ^ 1);
     }
     if (ok) mma_commit(leader, o_full);
   }
