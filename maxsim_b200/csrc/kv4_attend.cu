@@ -970,8 +970,9 @@ void launch_typed(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
 
 // Which kernel: this file's takes a time in proportion to the row blocks of 16, kv4_chunk.cu's to the waves of blocks
 // of 256 rows over the SMs, whatever fills them.  Measured per 128 tokens: 6.6 ns a row block over the whole device,
-// 2.9 us a wave (2.3 us with 128 rows or fewer).  (4 sequences of 4,096 tokens, 8 heads: 63 and 87 us at 128 rows a
-// head, 109 and 111 at 256; 32 of 2,000: 71 and 93 at 32, 121 and 95 at 64.)
+// 2.8 us a wave (2.2 us with 128 rows or fewer) and 20 us, which the factors of 440 and 350 spread over contexts of some
+// thousand tokens.  (4 sequences of 4,096 tokens, 8 heads: 63 and 87 us at 128 rows a head, 109 and 111 at 256; 32 of
+// 2,000: 71 and 93 at 32, 121 and 95 at 64.)
 bool many_rows(const Kv4View& c, const Kv4Attend& a) {
   if (!kv4_chunk_supported(c) || a.engine == 1) return false;
   if (a.engine == 2) return true;

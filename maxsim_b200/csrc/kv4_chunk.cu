@@ -12,14 +12,16 @@
 //   pairs, queries alike), values as [dimension][token] - their nibbles are paired by tokens (byte permutes of two
 //   tokens' words), so nothing is transposed.  Codes are loaded a tile ahead into registers.
 //   Softmax.  Sixteen warps, eight to a row tile: a warp has 16 rows, a thread two of them and a quarter of their
-//   columns, in blocks of 32 columns.  (With half the warps, a row to a thread: 206 us where this takes 184.)
+//   columns, in blocks of 32 columns.  (With half the warps, a row to a thread: 206 us where this took 184.)
 //   Scales of keys and values are fp32 factors of scores and probabilities (they would lose digits in fp16 operands);
 //   the reference is the running maximum of s_j + log2(vs_j) as in kv4_attend.cu, set 2^2 below it and moved (and
 //   the sums rescaled) only when some p vs would pass 60,000, which fp16 just holds.
 //   Two further warps issue the products, one for each row tile.
 //   Measured: 4 sequences of 1,500 to 4,096 tokens, the last 512 of each as rows, 32 heads (8 of the cache), D = 128:
-//   184 us with the host's call.  A tile of 256 rows takes 4,600 to 5,000 cycles: the softmax of a row tile 2,400 to
-//   3,000, the exponentials alone 2,048 for both; its products 1,200.
+//   171 us with the host's call (183 before the scores were formed in halves, below).  A tile of 256 rows takes about
+//   5,000 cycles, of which the exponentials need 2,048 and the products as much: what bounds it is the softmax warps'
+//   chain of loads, conversions and stores, 1,000 cycles and more for 32 columns whatever waits beside it.  Half of the
+//   issue slots are used.  Reading the queries takes 8,000 cycles of a block and writing the rows 5,000.
 // Every wait is bounded; a block that gives up writes NaN rows.
 #include <algorithm>
 #include <climits>
