@@ -342,7 +342,7 @@ typedef struct msb_kv4_attend_args {
   void* workspace;              /* msb_kv4_attend_workspace_bytes, 16-byte aligned; one call at a time */
   int64_t workspace_bytes;
   int32_t batch;
-  int32_t max_pages;
+  int32_t max_pages;            /* times page_size at most 2^31 - 65536 */
   int32_t max_query_rows;
   int32_t heads;
   int32_t type;

@@ -1518,8 +1518,9 @@ Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   if (a->rows > (int64_t{1} << 31) - 1) throw InvalidArgument("rows must be below 2^31");
   if (a->heads > 0 && a->rows > ((int64_t{1} << 31) - 1) / a->heads) throw InvalidArgument("rows * heads must be below 2^31");
   if (a->heads < 1 || a->heads % c.heads) throw InvalidArgument("heads must be a positive multiple of kv_heads");
-  if ((static_cast<int64_t>(a->max_pages) << c.page_shift) > (int64_t{1} << 31) - 1)
-    throw InvalidArgument("max_pages * page_size must be below 2^31");
+  // The kernels look some tiles past a sequence's end, in 32 bits.
+  if ((static_cast<int64_t>(a->max_pages) << c.page_shift) > (int64_t{1} << 31) - 65536)
+    throw InvalidArgument("max_pages * page_size must be at most 2^31 - 65536");
   if (!a->query_offsets && a->rows != a->batch) throw InvalidArgument("without query_offsets rows must equal batch");
   if (!(a->scale > 0.0F) || !std::isfinite(a->scale)) throw InvalidArgument("scale must be finite and > 0");
   if (a->window < 0) throw InvalidArgument("window must not be negative");
@@ -1537,7 +1538,7 @@ Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   r.lengths = a->lengths;
   r.offsets = a->query_offsets;
   r.batch = a->batch;
-  r.max_rows = a->query_offsets ? a->max_query_rows : 1;
+  r.max_rows = a->query_offsets ? static_cast<int>(std::min<int64_t>(a->max_query_rows, a->rows)) : 1;
   r.scale = a->scale;
   r.causal = a->causal != 0;
   r.window = a->window;

@@ -70,6 +70,14 @@ def test_attend_arguments(kw, text):
         check(lib.msb_kv4_attend_device(ctypes.byref(_cache()), ctypes.byref(_args(**kw)), None))
 
 
+def test_tokens_of_a_table_leave_room_past_the_end():
+    """Kernels ask for pages some tiles past a sequence's end: positions must not pass 2^31 there."""
+    for size in (16, 1024):
+        c, a = _cache(page_size=size), _args(max_pages=((1 << 31) - 65536) // size + 1)
+        with pytest.raises(ValueError, match="max_pages"):
+            check(lib.msb_kv4_attend_device(ctypes.byref(c), ctypes.byref(a), None))
+
+
 def test_attend_with_nothing_to_do():
     check(lib.msb_kv4_attend_device(ctypes.byref(_cache()), ctypes.byref(_args(rows=0, batch=0, query=None, out=None)), None))
 

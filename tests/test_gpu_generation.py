@@ -75,6 +75,10 @@ def test_other_cases_of_the_cache(engine):
     kv4.test_nothing_to_do()
 
 
+def test_offsets_past_32_bits(engine):
+    kv4.test_offsets_past_32_bits()
+
+
 @pytest.mark.parametrize("batch,heads,rows,length", [(2, 16, 70, 300), (40, 8, 33, 150), (3, 8, 260, 900)])
 def test_sizes_that_choose_the_kernel_for_many_rows(batch, heads, rows, length):
     kv4._run(128, heads, 4, 32, "bf16", [length - 3 * b for b in range(batch)], rows=[max(1, rows - b) for b in range(batch)])
@@ -204,6 +208,17 @@ def test_calls_on_two_streams_at_once():
                 got.append(cache.attend(q, table, length))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
+def test_more_query_tokens_announced_than_there_are(engine):
+    cache = _random_cache(22, 16, 2, 128, seed=3)
+    table = torch.arange(22, dtype=torch.int32, device="cuda").flip(0).expand(2, -1)
+    query = _normal((7, 8, 128), 5, torch.bfloat16)
+    lengths = torch.tensor([300, 41], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, 5, 7], dtype=torch.int32, device="cuda")
+    want = cache.attend(query, table, lengths, query_offsets=offsets, max_query_tokens=7)
+    got = cache.attend(query, table, lengths, query_offsets=offsets, max_query_tokens=(1 << 31) - 1)
+    assert torch.equal(got, want)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
