@@ -187,7 +187,8 @@ __device__ __forceinline__ float* line_parts(const Kv4Attend& a) {
 }
 
 // Units of all sequences, the sequence that holds unit `first(total)` and the units before it, by all threads of
-// the block, as many sequences at a time as it has threads.  The first block writes the sequences' starts.
+// the block, as many sequences at a time as it has threads.  The first block writes the sequences' starts where a
+// join follows (else there is no workspace to write to).
 struct Place {
   int64_t total;
   int64_t before;
@@ -907,8 +908,14 @@ Shape shape_of(const Kv4View& c, const Kv4Attend& a) {
   return s;
 }
 
+// Whether the line may cut a segment: one of a single unit never is.
+bool needs_join(const Kv4View& c, const Kv4Attend& a) { return (static_cast<int64_t>(a.max_pages) << c.page_shift) > kTile; }
+
 template <class T, int kDim, int kTiles>
-void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStream_t stream) {
+void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cudaStream_t stream) {
+  Kv4Attend a = given;
+  // What the call did not ask for (kv4_attend_workspace_bytes) is not its to write, whatever the caller passed.
+  if (!needs_join(c, a)) a.workspace = nullptr;
   const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
   const Line line{c.heads, a.heads / c.heads, 8 * kTiles, c.page_shift, (starts & 15) == 0, s.row_blocks};
@@ -935,7 +942,7 @@ void launch_shape(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
   kv4_attend_kernel<T, kDim, kTiles, false><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
   count_launch();
   check(cudaGetLastError(), "launch cache attention kernel");
-  if ((static_cast<int64_t>(a.max_pages) << c.page_shift) <= kTile) return;  // no segment can be cut
+  if (!needs_join(c, a)) return;
   const int64_t rows = static_cast<int64_t>(a.max_rows) * a.heads;
   const int64_t segments = c.heads * ((static_cast<int64_t>(a.max_rows) * line.shared + line.block_rows - 1) / line.block_rows);
   // Eight warps a row where a segment has 16 parts or more on average, each adding two or more.
@@ -985,8 +992,7 @@ bool many_rows(const Kv4View& c, const Kv4Attend& a) {
 }  // namespace
 
 size_t kv4_attend_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
-  if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0 || many_rows(c, a)) return 0;
-  if ((static_cast<int64_t>(a.max_pages) << c.page_shift) <= kTile) return 0;
+  if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0 || many_rows(c, a) || !needs_join(c, a)) return 0;
   const Shape s = shape_of(c, a);
   if (s.cluster > 0) return 0;
   return starts_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(s.blocks) * partial_floats(8 * s.tiles, c.dim);

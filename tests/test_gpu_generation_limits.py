@@ -1,0 +1,70 @@
+"""The cache attention and the weight products where their arguments or their data reach a limit."""
+
+import ctypes
+import sys
+from pathlib import Path
+
+import pytest
+
+import maxsim_b200 as m
+from maxsim_b200 import _lib
+from maxsim_b200._lib import check, lib
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+sys.path.insert(0, str(Path(__file__).resolve().parent))
+
+from test_gpu_kv4 import _check, _normal, _plain, _random_cache, _tables  # noqa: E402
+
+
+@pytest.fixture(params=[0, 1, 2], ids=["auto", "few", "many"])
+def engine(request):
+    """The attention kernel: by size, that for few rows, that for many."""
+    _lib.set_option("kv4_engine", request.param)
+    yield request.param
+    _lib.set_option("kv4_engine", 0)
+
+
+def _ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# --------------------------------------------------------------------------- the C entry's workspace
+
+def _c_attend(cache, query, table, lengths, workspace, workspace_bytes, out):
+    """One row a sequence through the C entry, with the caller's workspace."""
+    c = _lib.Kv4Cache(cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(), cache.v_scales.data_ptr(),
+                      cache.num_pages, cache.page_size, cache.num_kv_heads, cache.head_dim, 0)
+    a = _lib.Kv4AttendArgs(query=query.data_ptr(), query_row_stride=query.stride(0), query_head_stride=query.stride(1),
+                           rows=query.shape[0], page_table=table.data_ptr(), page_table_stride=table.stride(0),
+                           lengths=lengths.data_ptr(), out=out.data_ptr(), workspace=workspace, workspace_bytes=workspace_bytes,
+                           batch=table.shape[0], max_pages=table.shape[1], max_query_rows=1, heads=query.shape[1],
+                           type=_lib.TYPE_F16, causal=1, scale=query.shape[2] ** -0.5)
+    need = ctypes.c_int64()
+    check(lib.msb_kv4_attend_workspace_bytes(ctypes.byref(c), ctypes.byref(a), ctypes.byref(need)))
+    if workspace is not None:
+        if workspace_bytes is None:
+            a.workspace_bytes = need.value
+        check(lib.msb_kv4_attend_device(ctypes.byref(c), ctypes.byref(a), torch.cuda.current_stream().cuda_stream))
+    return need.value
+
+
+@pytest.mark.parametrize("batch", [1, 32, 33, 40, 300])
+@pytest.mark.parametrize("pages_each", [1, 8, 9, 70])
+def test_the_workspace_that_was_asked_for_is_all_that_is_written(batch, pages_each):
+    """Memory past what msb_kv4_attend_workspace_bytes names keeps what it held; where it names nothing, all of it."""
+    page, dim = 16, 64
+    cache = _random_cache(pages_each * 2, page, 2, dim, seed=1)
+    lengths = _ints(*[(7 * b) % (pages_each * page + 1) for b in range(batch)])
+    table = torch.arange(pages_each, dtype=torch.int32, device="cuda").expand(batch, -1).contiguous()
+    query = _normal((batch, 4, dim), 2, torch.float16)
+    out = torch.zeros_like(query)
+    need = _c_attend(cache, query, table, lengths, None, 0, out)
+    room = torch.full((need + 8192,), 0x5A, dtype=torch.uint8, device="cuda")
+    assert _c_attend(cache, query, table, lengths, room.data_ptr(), need, out) == need
+    assert (room[need:] == 0x5A).all()
+    if pages_each * page <= 128:
+        assert need == 0
+    assert torch.equal(out, cache.attend(query, table, lengths))
