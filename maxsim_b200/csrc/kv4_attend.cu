@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
         if (rr < all_rows) {
           const int pos = w.q.length - w.q.rows + rr / line.shared;
           last[nt][k] = a.causal ? pos : w.q.length - 1;
-          first[nt][k] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+          first[nt][k] = a.window > 0 ? max(0, max(0, pos) - a.window + 1) : 0;
           every_last = min(every_last, last[nt][k]);
           every_first = max(every_first, first[nt][k]);
           any_last = max(any_last, last[nt][k]);

@@ -293,7 +293,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   const int pos0 = q.length - q.rows + static_cast<int>(block_row0 / shared);
   const int pos1 = q.length - q.rows + static_cast<int>((block_row0 + row_count - 1) / shared);
   const int any_last = a.causal ? pos1 : q.length - 1;
-  const int any_first = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+  // (Rows before the sequence's first token have negative positions; less a window these would pass 32 bits.)
+  const int any_first = a.window > 0 ? max(0, max(0, pos0) - a.window + 1) : 0;
   const int begin = any_first & ~15;
   const int tiles = any_last >= any_first ? (any_last - begin) / kTokens + 1 : 0;
 
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       }
       rows.window = a.window > 0 ? a.window : INT_MAX;
       const int every_last = min(rows.last[0], rows.last[1]);
-      const int every_first = a.window > 0 ? max(rows.last[0], rows.last[1]) - a.window + 1 : 0;
+      const int every_first = a.window > 0 ? max(0, max(rows.last[0], rows.last[1])) - a.window + 1 : 0;
       const uint32_t s_at = tmem + (static_cast<uint32_t>(row0) << 16) + m * 128, o_at = s_at + 256;
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {

@@ -68,3 +68,25 @@ def test_the_workspace_that_was_asked_for_is_all_that_is_written(batch, pages_ea
     if pages_each * page <= 128:
         assert need == 0
     assert torch.equal(out, cache.attend(query, table, lengths))
+
+
+# --------------------------------------------------------------------------- windows
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 2, (1 << 31) - 100, 1 << 31, 1 << 62])
+@pytest.mark.parametrize("wide", [0, 200])
+def test_windows_of_any_size_where_rows_outnumber_tokens(engine, dim, window, wide):
+    """A window as large as a number can be hides nothing: the bits of the call without one, in blocks of rows that all
+    lie before the sequence's first token, that lie on both sides of it, and after."""
+    lengths, rows, page = [200, 1, 0, 40, 70], [600, 290, 5, 43, 1], 16
+    cache = _random_cache(24, page, 2, dim, seed=dim)
+    table = _tables(lengths, page, 24, extra=1 + wide)
+    starts = [0]
+    for n in rows:
+        starts.append(starts[-1] + n)
+    query = _normal((starts[-1], 6, dim), 3, torch.bfloat16)
+    kw = dict(query_offsets=_ints(*starts), max_query_tokens=max(rows), return_lse=True)
+    want, want_lse = cache.attend(query, table, _ints(*lengths), **kw)
+    _check(want, _plain(query, cache, table, lengths, starts, dim**-0.5), want_lse)
+    got, lse = cache.attend(query, table, _ints(*lengths), window=window, **kw)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
