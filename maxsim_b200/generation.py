@@ -130,9 +130,17 @@ class Int4KVCache:
         return _native.read(self._address, slots, dtype, out)
 
     def slots(self, page_table, sequences, positions):
-        """int64 slots of ``positions`` of ``sequences`` (tensors of one shape) under ``page_table``."""
-        positions = positions.long()
-        return page_table[sequences.long(), positions // self.page_size].long() * self.page_size + positions % self.page_size
+        """int64 slots of ``positions`` of ``sequences`` (tensors of one shape) under ``page_table``; -1, which `append`
+        skips, where the table has no such sequence or position (a negative one is padding) or names no page."""
+        sequences, positions = sequences.long(), positions.long()
+        batch, width = page_table.shape
+        if page_table.numel() == 0:
+            return positions.new_full(positions.shape, -1)
+        column = positions // self.page_size
+        row_held, column_held = sequences.clamp(0, batch - 1), column.clamp(0, width - 1)
+        known = (sequences == row_held) & (column == column_held)
+        slot = (positions % self.page_size).add(page_table[row_held, column_held].long(), alpha=self.page_size)
+        return slot.clamp(min=-1).where(known, -1)
 
     def attend(self, query, page_table, lengths, *, query_offsets=None, max_query_tokens=None, scale=None, causal=True,
                window=None, return_lse=False, out=None):
