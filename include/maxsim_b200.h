@@ -280,7 +280,7 @@ int msb_docs_topk_device_noalloc(msb_docs* docs, const float* query, int32_t bat
  * code format of the int4 corpora (no counterpart in the reference).  All
  * pointers are device pointers on `device`, work is enqueued on `stream`
  * without synchronising, nothing is allocated, and calls can be captured into
- * a graph.  Sizes are checked on the host; what device arrays hold (slots,
+ * a graph.  Sizes and alignment are checked on the host; what device arrays hold (slots,
  * page ids, lengths, offsets) is bounds-checked by the kernels. */
 #define MSB_TYPE_F32 0
 #define MSB_TYPE_F16 1
@@ -356,7 +356,8 @@ int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args*
 /* Weights [n, k] as int4 codes [n, k / 2] with one bfloat16 scale per row and
  * `group` (32, 64 or 128) inputs, [n, ceil(k / group)]; k a multiple of 8.
  * msb_w4_pack_device lays them out once for the product kernel, into buffers
- * of the sizes msb_w4_packed_bytes names. */
+ * of the sizes msb_w4_packed_bytes names (codes 16-byte aligned, scales 4), on
+ * the current device. */
 int msb_w4_packed_bytes(int64_t n, int64_t k, int32_t group, int64_t* code_bytes, int64_t* scale_bytes);
 int msb_w4_pack_device(const uint8_t* codes, const void* scales, int64_t n, int64_t k, int32_t group,
                        void* packed_codes, void* packed_scales, void* stream);

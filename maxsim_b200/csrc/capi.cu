@@ -1499,6 +1499,12 @@ Kv4View kv4_view(const msb_kv4_cache* c) {
   return v;
 }
 
+// The kernels read and write whole elements (or `bytes` at a time): an address off that would fault on the device.
+void check_address(const void* p, uintptr_t bytes, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % bytes)
+    throw InvalidArgument(std::string(what) + " must be " + std::to_string(bytes) + "-byte aligned");
+}
+
 int element_type(int32_t type, bool f32) {
   if (type == MSB_TYPE_F16) return kElemF16;
   if (type == MSB_TYPE_BF16) return kElemBF16;
@@ -1570,6 +1576,9 @@ int msb_kv4_append_device(const msb_kv4_cache* cache, const void* keys, const vo
     check_tokens(tokens, v);
     if (tokens == 0) return;
     if (!keys || !values || !slots) throw InvalidArgument("NULL argument");
+    check_address(keys, type == MSB_TYPE_F32 ? 4 : 2, "keys");
+    check_address(values, type == MSB_TYPE_F32 ? 4 : 2, "values");
+    check_address(slots, 8, "slots");
     a.x[0] = keys;
     a.x[1] = values;
     a.token_stride[0] = key_token_stride;
@@ -1594,6 +1603,7 @@ int msb_kv4_read_device(const msb_kv4_cache* cache, const int64_t* slots, int64_
     if (!keys || !values || !slots) throw InvalidArgument("NULL argument");
     if ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15)
       throw InvalidArgument("keys and values must be 16-byte aligned");
+    check_address(slots, 8, "slots");
     a.out[0] = keys;
     a.out[1] = values;
     a.slots = slots;
@@ -1618,6 +1628,14 @@ int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args*
     const Kv4Attend a = kv4_attend(v, args);
     if (a.rows == 0 || a.batch == 0) return;
     if (!a.query || !a.lengths || !a.out || (a.max_pages > 0 && !a.page_table)) throw InvalidArgument("NULL argument");
+    check_address(a.query, 2, "query");
+    check_address(a.out, 2, "out");
+    check_address(a.page_table, 4, "page_table");
+    check_address(a.lengths, 4, "lengths");
+    check_address(a.offsets, 4, "query_offsets");
+    check_address(a.lse, 4, "lse");
+    check_address(a.workspace, 16, "workspace");
+    if (!a.workspace && a.workspace_bytes > 0) throw InvalidArgument("workspace is NULL");
     DeviceGuard g(cache->device);
     if (a.workspace_bytes < kv4_attend_workspace_bytes(v, a)) throw InvalidArgument("workspace is too small");
     launch_kv4_attend(v, a, static_cast<cudaStream_t>(stream));
@@ -1638,6 +1656,9 @@ int msb_w4_pack_device(const uint8_t* codes, const void* scales, int64_t n, int6
   return guarded([&] {
     check_w4(n, k, group);
     if (!codes || !scales || !packed_codes || !packed_scales) throw InvalidArgument("NULL argument");
+    check_address(scales, 2, "scales");
+    check_address(packed_codes, 16, "packed_codes");
+    check_address(packed_scales, 4, "packed_scales");
     launch_w4_pack(codes, static_cast<const uint16_t*>(scales), n, k, group, static_cast<uint8_t*>(packed_codes),
                    static_cast<uint16_t*>(packed_scales), static_cast<cudaStream_t>(stream));
   });
@@ -1653,6 +1674,10 @@ int msb_w4_product_device(const void* packed_codes, const void* packed_scales, i
     if (rows < 0) throw InvalidArgument("rows must not be negative");
     if (rows == 0) return;
     if (!packed_codes || !packed_scales || !x || !y) throw InvalidArgument("NULL argument");
+    check_address(packed_codes, 16, "packed_codes");
+    check_address(packed_scales, 4, "packed_scales");
+    check_address(bias, 2, "bias");
+    check_address(y, 2, "y");
     if ((reinterpret_cast<uintptr_t>(x) | static_cast<uint64_t>(x_stride) * 2) & 15)
       throw InvalidArgument("rows of x must start on 16-byte boundaries");
     if (rows > (int64_t{1} << 31) - 64) throw InvalidArgument("rows must be below 2^31");

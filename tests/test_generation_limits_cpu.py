@@ -1,10 +1,15 @@
 """The cache's and the weights' host side where its arguments reach a limit: no device needed."""
 
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import maxsim_b200 as m  # noqa: E402
+from maxsim_b200 import _lib  # noqa: E402
+from maxsim_b200._lib import check, lib  # noqa: E402
+from test_generation_cpu import _PTR, _append, _args, _cache as _c_cache  # noqa: E402
 
 
 def _cache(page_size):
@@ -36,3 +41,38 @@ def test_slots_of_an_empty_table(shape):
     table = torch.zeros(shape, dtype=torch.int32)
     assert _cache(64).slots(table, torch.tensor([0, 1]), torch.tensor([0, 7])).tolist() == [-1, -1]
     assert _cache(64).slots(table, torch.zeros(0, dtype=torch.int64), torch.zeros(0, dtype=torch.int64)).tolist() == []
+
+
+@pytest.mark.parametrize("kw,text", [(dict(workspace=_PTR + 8, workspace_bytes=1 << 30), "workspace must be 16-byte"),
+                                     (dict(workspace=None, workspace_bytes=1 << 30), "workspace is NULL"),
+                                     (dict(query=_PTR + 1), "query must be 2-byte"), (dict(out=_PTR + 1), "out must be 2-byte"),
+                                     (dict(page_table=_PTR + 2), "page_table must be 4-byte"),
+                                     (dict(lengths=_PTR + 1), "lengths must be 4-byte"),
+                                     (dict(query_offsets=_PTR + 2), "query_offsets must be 4-byte"),
+                                     (dict(lse=_PTR + 2), "lse must be 4-byte")])
+def test_attention_refuses_addresses_its_kernels_cannot_use(kw, text):
+    with pytest.raises(ValueError, match=text):
+        check(lib.msb_kv4_attend_device(ctypes.byref(_c_cache()), ctypes.byref(_args(**kw)), None))
+
+
+def test_the_other_entries_refuse_addresses_their_kernels_cannot_use():
+    for kw, text in ((dict(keys=_PTR + 2), "keys must be 4-byte"), (dict(values=_PTR + 1, type=_lib.TYPE_BF16), "values must be 2-byte"),
+                     (dict(slots=_PTR + 4), "slots must be 8-byte")):
+        with pytest.raises(ValueError, match=text):
+            check(_append(_c_cache(), **kw))
+    with pytest.raises(ValueError, match="slots must be 8-byte"):
+        check(lib.msb_kv4_read_device(ctypes.byref(_c_cache()), _PTR + 4, 1, _lib.TYPE_BF16, _PTR, _PTR, None))
+
+    def pack(codes=_PTR, scales=_PTR, to_codes=_PTR, to_scales=_PTR):
+        check(lib.msb_w4_pack_device(codes, scales, 16, 64, 32, to_codes, to_scales, None))
+
+    def product(codes=_PTR, scales=_PTR, bias=None, y=_PTR):
+        check(lib.msb_w4_product_device(codes, scales, 16, 64, 32, _PTR, 64, 1, bias, y, 16, _lib.TYPE_F16, 0, None))
+
+    for call, kw, text in ((pack, dict(scales=_PTR + 1), "scales must be 2-byte"), (pack, dict(to_codes=_PTR + 4), "packed_codes must be 16-byte"),
+                           (pack, dict(to_scales=_PTR + 2), "packed_scales must be 4-byte"),
+                           (product, dict(codes=_PTR + 8), "packed_codes must be 16-byte"),
+                           (product, dict(scales=_PTR + 2), "packed_scales must be 4-byte"),
+                           (product, dict(bias=_PTR + 1), "bias must be 2-byte"), (product, dict(y=_PTR + 1), "y must be 2-byte")):
+        with pytest.raises(ValueError, match=text):
+            call(**kw)
