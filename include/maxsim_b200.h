@@ -326,8 +326,8 @@ int msb_kv4_read_device(const msb_kv4_cache* cache, const int64_t* slots, int64_
  * the last `window` of these.  Query heads share key/value heads in groups of
  * heads / kv_heads.  A row that sees nothing gives zeros (lse -inf).  A token
  * on a page outside the cache is not seen.  Rows that no sequence owns, or
- * past max_query_rows of one, are not written.  fp16 or bf16; softmax
- * statistics and sums in fp32. */
+ * past max_query_rows of one, are not written (they count in n all the same).
+ * fp16 or bf16; softmax statistics and sums in fp32. */
 typedef struct msb_kv4_attend_args {
   const void* query;            /* [rows, heads, head_dim], strides in elements */
   int64_t query_row_stride;
@@ -343,7 +343,7 @@ typedef struct msb_kv4_attend_args {
   int64_t workspace_bytes;
   int32_t batch;
   int32_t max_pages;            /* times page_size at most 2^31 - 65536 */
-  int32_t max_query_rows;
+  int32_t max_query_rows;       /* positive where there are rows and offsets */
   int32_t heads;
   int32_t type;
   int32_t causal;

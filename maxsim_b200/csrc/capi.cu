@@ -1527,6 +1527,8 @@ Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   // The kernels look some tiles past a sequence's end, in 32 bits.
   if ((static_cast<int64_t>(a->max_pages) << c.page_shift) > (int64_t{1} << 31) - 65536)
     throw InvalidArgument("max_pages * page_size must be at most 2^31 - 65536");
+  if (a->query_offsets && a->rows > 0 && a->max_query_rows == 0)
+    throw InvalidArgument("max_query_rows must be positive where there are rows");
   if (!a->query_offsets && a->rows != a->batch) throw InvalidArgument("without query_offsets rows must equal batch");
   if (!(a->scale > 0.0F) || !std::isfinite(a->scale)) throw InvalidArgument("scale must be finite and > 0");
   if (a->window < 0) throw InvalidArgument("window must not be negative");

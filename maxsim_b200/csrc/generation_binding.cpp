@@ -196,6 +196,7 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
     offsets = o.contiguous();
     most = args[5] == Py_None ? rows : integer(args[5]);
     if (most < 0) refuse("max_query_tokens must not be negative");
+    if (most == 0 && rows > 0) refuse("max_query_tokens must be positive where there are rows");
     most = std::min(most, rows);  // a sequence has no more rows than there are
   }
   const int causal = PyObject_IsTrue(args[7]), return_lse = PyObject_IsTrue(args[9]);

@@ -170,7 +170,7 @@ __device__ __forceinline__ SequenceWork sequence_work(const Kv4Attend& a, const 
   SequenceWork w;
   w.q = kv4_sequence(a, l.page_shift, b);
   w.begin = 0;
-  if (a.window > 0) w.begin = max(0, max(0, w.q.length - w.q.rows) - a.window + 1) & ~(kStep - 1);
+  if (a.window > 0) w.begin = max(0, max(0, w.q.pos0) - a.window + 1) & ~(kStep - 1);
   // A sequence of no tokens keeps one empty unit: its rows are written as zeros.
   w.tiles = max(1, (w.q.length - w.begin + kTile - 1) / kTile);
   w.blocks = (w.q.rows * l.shared + l.block_rows - 1) / l.block_rows;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
         first[nt][k] = 0;
         last[nt][k] = INT_MAX;  // rows past the block are not written: no reason to mask for them
         if (rr < all_rows) {
-          const int pos = w.q.length - w.q.rows + rr / line.shared;
+          const int pos = w.q.pos0 + rr / line.shared;
           last[nt][k] = a.causal ? pos : w.q.length - 1;
           first[nt][k] = a.window > 0 ? max(0, max(0, pos) - a.window + 1) : 0;
           every_last = min(every_last, last[nt][k]);

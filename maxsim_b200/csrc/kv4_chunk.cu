@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   const int row_count = static_cast<int>(min(static_cast<uint32_t>(kBlockRows), all_rows - block_row0));
   const int tiles_m = row_count > kRowsTile ? 2 : 1;
   // Tokens that some row of the block sees, and the tiles over them.
-  const int pos0 = q.length - q.rows + static_cast<int>(block_row0 / shared);
-  const int pos1 = q.length - q.rows + static_cast<int>((block_row0 + row_count - 1) / shared);
+  const int pos0 = q.pos0 + static_cast<int>(block_row0 / shared);
+  const int pos1 = q.pos0 + static_cast<int>((block_row0 + row_count - 1) / shared);
   const int any_last = a.causal ? pos1 : q.length - 1;
   // (Rows before the sequence's first token have negative positions; less a window these would pass 32 bits.)
   const int any_first = a.window > 0 ? max(0, max(0, pos0) - a.window + 1) : 0;
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       for (int k = 0; k < 2; ++k) {
         // Rows past the last do as it does: what they compute is not written.
         const int mine = 8 * k + (lane >> 2), at = min(m * kRowsTile + row0 + mine, row_count - 1);
-        const int pos = q.length - q.rows + static_cast<int>((block_row0 + at) / shared);
+        const int pos = q.pos0 + static_cast<int>((block_row0 + at) / shared);
         rows.factor[k] = make_float2(row_factor[mine], row_factor[mine]);
         rows.ref[k] = rows.sum[k] = make_float2(0.0F, 0.0F);
         rows.last[k] = a.causal ? pos : q.length - 1;

@@ -80,11 +80,13 @@ struct Kv4Attend {
 };
 
 // One sequence of an attention call, with what the device arrays say held to what the call can read:
-// lengths to the table's pages, rows to the query's rows and the announced maximum.
+// lengths to the table's pages, rows to the query's rows.  Of these the announced maximum is worked on; positions count
+// from all of them.
 struct Kv4Sequence {
   int64_t row0;
   int rows;
   int length;
+  int pos0;   // position of row 0, negative where rows outnumber tokens
 };
 __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page_shift, int b) {
   Kv4Sequence s;
@@ -93,11 +95,14 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page
   if (a.offsets == nullptr) {
     s.row0 = b;
     s.rows = 1;
+    s.pos0 = s.length - 1;
   } else {
     const int64_t lo = max(0, a.offsets[b]);
     const int64_t hi = min(static_cast<int64_t>(a.offsets[b + 1]), a.rows);
     s.row0 = lo;
-    s.rows = static_cast<int>(max(static_cast<int64_t>(0), min(hi - lo, static_cast<int64_t>(a.max_rows))));
+    const int all = static_cast<int>(max(static_cast<int64_t>(0), hi - lo));  // at most a.rows
+    s.rows = min(all, a.max_rows);
+    s.pos0 = s.length - all;
   }
   return s;
 }

@@ -150,7 +150,8 @@ class Int4KVCache:
         ``page_table`` ``[batch, max_pages]`` names their pages.  Sequence ``b`` owns rows ``query_offsets[b] ..
         query_offsets[b + 1]`` (int32 ``[batch + 1]``, at most ``max_query_tokens`` each), which are its last
         positions; without ``query_offsets`` each sequence has one row.  Every row must belong to a sequence:
-        others are not written.
+        others are not written, nor are a sequence's rows past ``max_query_tokens`` (its first rows keep their
+        positions all the same).
 
         A row at position ``p`` sees tokens up to ``p`` (``causal``; otherwise all of its sequence), the last
         ``window`` of them where a window is given.  ``heads`` is a multiple of the cache's heads, consecutive

@@ -90,3 +90,36 @@ def test_windows_of_any_size_where_rows_outnumber_tokens(engine, dim, window, wi
     _check(want, _plain(query, cache, table, lengths, starts, dim**-0.5), want_lse)
     got, lse = cache.attend(query, table, _ints(*lengths), window=window, **kw)
     assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
+# --------------------------------------------------------------------------- announced rows
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("most", [1, 3, 20])
+@pytest.mark.parametrize("wide", [0, 200])
+@pytest.mark.parametrize("window", [None, 30])
+def test_fewer_query_tokens_announced_than_there_are(engine, dim, most, wide, window):
+    """Rows up to the announced number are those of the whole call, at their own positions; rows past it keep what the
+    caller's output held."""
+    lengths, starts, page = [40, 90, 25, 3], [0, 3, 33, 35, 45], 16
+    cache = _random_cache(14, page, 2, dim, seed=dim)
+    table = _tables(lengths, page, 14, extra=1 + wide)
+    query = _normal((starts[-1], 6, dim), 3, torch.bfloat16)
+    out = torch.full_like(query, 7.0)
+    got, lse = cache.attend(query, table, _ints(*lengths), query_offsets=_ints(*starts), max_query_tokens=most, window=window,
+                            return_lse=True, out=out)
+    want = _plain(query, cache, table, lengths, starts, dim**-0.5, window=window)
+    kept = torch.zeros(starts[-1], dtype=torch.bool, device="cuda")
+    for lo, hi in zip(starts, starts[1:]):
+        kept[lo : min(hi, lo + most)] = True
+    _check(got[kept], [t[kept] for t in want], lse[kept])
+    assert (out[~kept] == 7.0).all()
+
+
+def test_no_query_tokens_announced_where_there_are_some():
+    cache = _random_cache(4, 16, 2, 64, seed=1)
+    q = _normal((3, 4, 64), 1, torch.float16)
+    table, lengths = _ints(0, 1, 2, 3).view(2, 2), _ints(20, 30)
+    with pytest.raises(ValueError, match="max_query"):
+        cache.attend(q, table, lengths, query_offsets=_ints(0, 1, 3), max_query_tokens=0)
+    assert cache.attend(q[:0], table, lengths, query_offsets=_ints(0, 0, 0), max_query_tokens=0).shape == (0, 4, 64)
