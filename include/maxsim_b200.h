@@ -352,6 +352,10 @@ typedef struct msb_kv4_attend_args {
 } msb_kv4_attend_args;
 int msb_kv4_attend_workspace_bytes(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, int64_t* bytes);
 int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream);
+/* The same into an output that holds nothing yet: rows that no sequence owns
+ * (before the first offset, past the last) become zeros with lse -inf, rows
+ * past max_query_rows of their sequence NaN (where batch is positive). */
+int msb_kv4_attend_fill_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream);
 
 /* Weights [n, k] as int4 codes [n, k / 2] with one bfloat16 scale per row and
  * `group` (32, 64 or 128) inputs, [n, ceil(k / group)]; k a multiple of 8.

@@ -156,6 +156,7 @@ SIGNATURES = {
     "msb_kv4_attend_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs),
                                                       ctypes.POINTER(_i64)]),
     "msb_kv4_attend_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs), _vp]),
+    "msb_kv4_attend_fill_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs), _vp]),
     "msb_w4_packed_bytes": (ctypes.c_int, [_i64, _i64, _i32, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
     "msb_w4_pack_device": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "msb_w4_product_device": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32,

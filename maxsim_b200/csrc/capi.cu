@@ -1558,6 +1558,27 @@ Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   return r;
 }
 
+int attend(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, bool fill, void* stream) {
+  return guarded([&] {
+    const Kv4View v = kv4_view(cache);
+    Kv4Attend a = kv4_attend(v, args);
+    a.fill = fill;
+    if (a.rows == 0 || a.batch == 0) return;
+    if (!a.query || !a.lengths || !a.out || (a.max_pages > 0 && !a.page_table)) throw InvalidArgument("NULL argument");
+    check_address(a.query, 2, "query");
+    check_address(a.out, 2, "out");
+    check_address(a.page_table, 4, "page_table");
+    check_address(a.lengths, 4, "lengths");
+    check_address(a.offsets, 4, "query_offsets");
+    check_address(a.lse, 4, "lse");
+    check_address(a.workspace, 16, "workspace");
+    if (!a.workspace && a.workspace_bytes > 0) throw InvalidArgument("workspace is NULL");
+    DeviceGuard g(cache->device);
+    if (a.workspace_bytes < kv4_attend_workspace_bytes(v, a)) throw InvalidArgument("workspace is too small");
+    launch_kv4_attend(v, a, static_cast<cudaStream_t>(stream));
+  });
+}
+
 void check_w4(int64_t n, int64_t k, int32_t group) {
   if (n < 1 || k < 8 || k % 8) throw InvalidArgument("n must be positive and k a positive multiple of 8");
   if (group != 32 && group != 64 && group != 128) throw InvalidArgument("group must be 32, 64 or 128");
@@ -1625,23 +1646,11 @@ int msb_kv4_attend_workspace_bytes(const msb_kv4_cache* cache, const msb_kv4_att
 }
 
 int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream) {
-  return guarded([&] {
-    const Kv4View v = kv4_view(cache);
-    const Kv4Attend a = kv4_attend(v, args);
-    if (a.rows == 0 || a.batch == 0) return;
-    if (!a.query || !a.lengths || !a.out || (a.max_pages > 0 && !a.page_table)) throw InvalidArgument("NULL argument");
-    check_address(a.query, 2, "query");
-    check_address(a.out, 2, "out");
-    check_address(a.page_table, 4, "page_table");
-    check_address(a.lengths, 4, "lengths");
-    check_address(a.offsets, 4, "query_offsets");
-    check_address(a.lse, 4, "lse");
-    check_address(a.workspace, 16, "workspace");
-    if (!a.workspace && a.workspace_bytes > 0) throw InvalidArgument("workspace is NULL");
-    DeviceGuard g(cache->device);
-    if (a.workspace_bytes < kv4_attend_workspace_bytes(v, a)) throw InvalidArgument("workspace is too small");
-    launch_kv4_attend(v, a, static_cast<cudaStream_t>(stream));
-  });
+  return attend(cache, args, false, stream);
+}
+
+int msb_kv4_attend_fill_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream) {
+  return attend(cache, args, true, stream);
 }
 
 int msb_w4_packed_bytes(int64_t n, int64_t k, int32_t group, int64_t* code_bytes, int64_t* scale_bytes) {

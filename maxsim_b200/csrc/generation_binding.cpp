@@ -249,7 +249,11 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
     a.workspace = workspace.mutable_data_ptr();
     a.workspace_bytes = need;
   }
-  check_status(msb_kv4_attend_device(c, &a, stream_of(device)));
+  // Outputs made here are fresh memory: rows that the call does not work on are filled, by the kernel where both are.
+  const bool fresh = args[10] == Py_None;
+  if (fresh && batch == 0) out.zero_();
+  if (return_lse && a.query_offsets && (!fresh || batch == 0)) lse.fill_(-INFINITY);
+  check_status((fresh ? msb_kv4_attend_fill_device : msb_kv4_attend_device)(c, &a, stream_of(device)));
   if (!return_lse) return THPVariable_Wrap(std::move(out));
   PyObject* pair = PyTuple_New(2);
   if (!pair) throw PythonError{};

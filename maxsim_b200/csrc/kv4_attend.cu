@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     b = here / (line.heads * line.most_blocks);
     cluster_segment = here - b * (line.heads * line.most_blocks);
     w = sequence_work(a, line, b);
-    if (static_cast<int>(cluster_segment % line.most_blocks) >= w.blocks) return;  // the whole cluster
+    if (static_cast<int>(cluster_segment % line.most_blocks) >= w.blocks) unit_end = 0;  // nothing for the whole cluster
   } else {
     const Place place = find_place(
         a, line, [&](int64_t total) { return range_start(total, block, ranges(total, gridDim.x)); }, scratch);
@@ -331,9 +331,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
 #if __CUDA_ARCH__ >= 900
     cudaTriggerProgrammaticLaunchCompletion();
 #endif
-    if (block >= n) return;
-    unit = range_start(place.total, block, n);
-    unit_end = range_start(place.total, block + 1, n);
+    unit = block < n ? range_start(place.total, block, n) : 0;
+    unit_end = block < n ? range_start(place.total, block + 1, n) : 0;
     before = place.before;
     b = place.sequence;
     if (unit < unit_end) w = sequence_work(a, line, b);
@@ -751,6 +750,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       unit += tile1 - tile0;
     }
   }
+  kv4_fill_rows<T>(a, kDim);
 }
 
 // Adds the partial sums of the segments that were cut.  A warp adds the parts of one output row, or, where

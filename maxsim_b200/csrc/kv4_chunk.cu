@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   const int b = static_cast<int>(blockIdx.x % per_block / c.heads), head = static_cast<int>(blockIdx.x % c.heads);
   const Kv4Sequence q = kv4_sequence(a, c.page_shift, b);
   const uint32_t all_rows = static_cast<uint32_t>(q.rows) * shared, block_row0 = static_cast<uint32_t>(block) * kBlockRows;  // below 2^31
+  kv4_fill_rows<T>(a, kDim);
   if (block_row0 >= all_rows) return;
   const int row_count = static_cast<int>(min(static_cast<uint32_t>(kBlockRows), all_rows - block_row0));
   const int tiles_m = row_count > kRowsTile ? 2 : 1;

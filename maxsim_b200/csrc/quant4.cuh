@@ -77,6 +77,7 @@ struct Kv4Attend {
   size_t workspace_bytes;
   int type;
   int engine;                 // 0 by size, 1 the kernel for few rows, 2 that for many
+  int fill;                   // rows that are not worked on are written too (kv4_fill_rows)
 };
 
 // One sequence of an attention call, with what the device arrays say held to what the call can read:
@@ -105,6 +106,31 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page
     s.pos0 = s.length - all;
   }
   return s;
+}
+
+// Where the caller's output is fresh memory, the rows that no block works on are written here, by all blocks of a kernel:
+// zeros and a log-sum-exp of -inf where no sequence owns the row, NaN past a sequence's announced number of rows (that
+// number was wrong, and it shows).
+template <class T>
+__device__ __forceinline__ void kv4_fill_rows(const Kv4Attend& a, int dim) {
+  if (!a.fill || a.offsets == nullptr) return;
+  auto fill = [&](int64_t lo, int64_t hi, int64_t thread, int64_t threads, float value, float lse) {
+    const int64_t width = static_cast<int64_t>(a.heads) * dim;
+    for (int64_t i = lo * width + thread; i < hi * width; i += threads) static_cast<T*>(a.out)[i] = from_f32<T>(value);
+    if (a.lse)
+      for (int64_t i = lo * a.heads + thread; i < hi * a.heads; i += threads) a.lse[i] = lse;
+  };
+  const int64_t first = max(static_cast<int64_t>(0), min(static_cast<int64_t>(a.offsets[0]), a.rows));
+  const int64_t last = max(first, min(static_cast<int64_t>(a.offsets[a.batch]), a.rows));
+  const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  fill(0, first, thread, threads, 0.0F, -INFINITY);
+  fill(last, a.rows, thread, threads, 0.0F, -INFINITY);
+  if (a.max_rows >= a.rows) return;
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    const int64_t lo = max(0, a.offsets[b]), hi = min(static_cast<int64_t>(a.offsets[b + 1]), a.rows);
+    if (hi - lo > a.max_rows) fill(lo + a.max_rows, hi, threadIdx.x, blockDim.x, NAN, NAN);
+  }
 }
 
 // Opts a kernel in to its dynamic shared memory, once per device.

@@ -149,9 +149,9 @@ class Int4KVCache:
         ``lengths`` int32 ``[batch]`` counts each sequence's cached tokens, the rows' own among them; int32
         ``page_table`` ``[batch, max_pages]`` names their pages.  Sequence ``b`` owns rows ``query_offsets[b] ..
         query_offsets[b + 1]`` (int32 ``[batch + 1]``, at most ``max_query_tokens`` each), which are its last
-        positions; without ``query_offsets`` each sequence has one row.  Every row must belong to a sequence:
-        others are not written, nor are a sequence's rows past ``max_query_tokens`` (its first rows keep their
-        positions all the same).
+        positions; without ``query_offsets`` each sequence has one row.  Rows before the first offset and past the last
+        (padding) are zeros, rows past their sequence's ``max_query_tokens`` NaN; a given ``out`` keeps what it holds
+        in both (and their log-sum-exp is -inf).
 
         A row at position ``p`` sees tokens up to ``p`` (``causal``; otherwise all of its sequence), the last
         ``window`` of them where a window is given.  ``heads`` is a multiple of the cache's heads, consecutive

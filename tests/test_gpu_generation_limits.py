@@ -123,3 +123,49 @@ def test_no_query_tokens_announced_where_there_are_some():
     with pytest.raises(ValueError, match="max_query"):
         cache.attend(q, table, lengths, query_offsets=_ints(0, 1, 3), max_query_tokens=0)
     assert cache.attend(q[:0], table, lengths, query_offsets=_ints(0, 0, 0), max_query_tokens=0).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("batch,wide", [(3, 0), (3, 300), (40, 0), (40, 300), (140, 300)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rows_without_a_sequence_are_zero(engine, dim, batch, wide, dtype):
+    """In an output of the call's own, rows before the first offset and after the last are zeros with a log-sum-exp of
+    -inf, rows past the announced number NaN; a caller's output keeps what it held there."""
+    page, most = 16, 2
+    lengths = [(29 * b) % 60 for b in range(batch)]
+    starts = [5]
+    for b in range(batch):
+        starts.append(starts[-1] + b % 4)
+    rows = starts[-1] + 37
+    pages = sum(-(-n // page) for n in lengths) + 1
+    cache = _random_cache(pages, page, 2, dim, seed=batch)
+    table = _tables(lengths, page, pages, extra=1 + wide)
+    query = _normal((rows, 6, dim), 3, dtype)
+    past = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    kept = past.clone()
+    for lo, hi in zip(starts, starts[1:]):
+        kept[lo : min(hi, lo + most)] = True
+        past[min(hi, lo + most) : hi] = True
+    nobody = ~(kept | past)
+    args = (query, table, _ints(*lengths))
+    kw = dict(query_offsets=_ints(*starts), max_query_tokens=most)
+    for _ in range(3):
+        held = torch.full((rows, 6, dim), 7.0, dtype=dtype, device="cuda"), torch.full((rows, 6), 7.0, device="cuda")
+        del held  # memory of these sizes is the allocator's next answer, and not zero
+        got, lse = cache.attend(*args, return_lse=True, **kw)
+        assert not got[nobody].any() and (lse[nobody] == -torch.inf).all()
+        assert torch.isnan(got[past]).all() and torch.isnan(lse[past]).all()
+    out = torch.full_like(query, 7.0)
+    _, lse = cache.attend(*args, out=out, return_lse=True, **kw)
+    assert (out[~kept] == 7.0).all() and torch.equal(out[kept], got[kept])
+    assert (lse[~kept] == -torch.inf).all()
+
+
+def test_no_sequence_has_rows(engine):
+    cache = _random_cache(4, 16, 2, 64, seed=1)
+    for batch, offsets in ((2, _ints(0, 0, 0)), (2, _ints(9, 9, 9)), (0, _ints(0))):
+        q = _normal((9, 4, 64), 1, torch.float16)
+        torch.full_like(q, 7.0)
+        got, lse = cache.attend(q, _ints(0, 1, 2, 3).view(2, 2)[:batch], _ints(20, 30)[:batch], query_offsets=offsets,
+                                return_lse=True)
+        assert not got.any() and (lse == -torch.inf).all()
