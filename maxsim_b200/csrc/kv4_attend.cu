@@ -25,8 +25,8 @@
 //   down to 2^-34 of the row's maximum, and so for bf16 ones.  Probabilities are fp16 (11 bits): they enter one sum
 //   that is rounded to the output's type, of as many bits or fewer.
 //   Reference.  Probabilities carry the values' scales, p_j vs_j, so the running reference is the maximum of
-//   s_j + log2 vs_j less 8: p_j vs_j stays in fp16's normal range whatever the scales are.  The logarithm is held to
-//   +-110, so the fp32 sum of the p_j stays finite.
+//   s_j + log2 vs_j less 8: the largest p_j vs_j is about 2^8 whatever the scales are, and those 2^-22 of it are
+//   normal in fp16.  keep_sums_finite has what holds the fp32 sum of the p_j.
 //   Work split.  The 128-token units of all (sequence, head, row block) segments form one line, cut into equal
 //   ranges, one per resident block, from the lengths on the device: no plan, no host copy, no imbalance.
 //   A segment cut by a range's end leaves partial sums in the workspace (at most two per block), which
@@ -53,7 +53,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStep = 32;              // tokens a warp takes at a time
 constexpr int kTile = kWarps * kStep;  // tokens of one unit of the work line
-constexpr float kExponents = 110.0F;   // powers of two that scales and queries are brought back from
 constexpr int kStages = 3;             // steps in a warp's ring: one worked on, two on their way
 constexpr float kLift = 8.0F;          // references lie 2^8 below the maximum: probabilities of 2^-22 are normal in fp16
 
@@ -119,32 +118,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-// What sums with reference `from` are multiplied by to have reference `to` >= from.  Sums with reference -inf
-// are 0, or NaN where a score was: they stay so.
-__device__ __forceinline__ float fade_to(float from, float to) { return from == to ? 1.0F : exp2_fast(from - to); }
 __device__ __forceinline__ float log_sum(float m, float l) {
   return l == 0.0F ? -INFINITY : (m - kLift + __log2f(l)) * 0.693147181F;
-}
-// About log2 of a scale, held to +-110 (and so a number where the scale is 0, NaN or infinite).
-__device__ __forceinline__ float scale_exponent(float s) {
-  float r;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-  return fminf(fmaxf(r, -kExponents), kExponents);
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 // The work line: units of kTile tokens of every (sequence, key/value head, row block).
@@ -568,7 +543,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float e = scale_exponent(vs[i][k].x);
+          const float e = scale_exponent(vs[i][k].x, a.least_exponent);
           raise[i][k] = make_float2(e, e);
         }
       bool moved = false;
@@ -916,6 +891,7 @@ void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cuda
   Kv4Attend a = given;
   // What the call did not ask for (kv4_attend_workspace_bytes) is not its to write, whatever the caller passed.
   if (!needs_join(c, a)) a.workspace = nullptr;
+  keep_sums_finite(a, c.page_shift, kLift);
   const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
   const Line line{c.heads, a.heads / c.heads, 8 * kTiles, c.page_shift, (starts & 15) == 0, s.row_blocks};

@@ -15,7 +15,9 @@
 //   columns, in blocks of 32 columns.  (With half the warps, a row to a thread: 206 us where this took 184.)
 //   Scales of keys and values are fp32 factors of scores and probabilities (they would lose digits in fp16 operands);
 //   the reference is the running maximum of s_j + log2(vs_j) as in kv4_attend.cu, set 2^2 below it and moved (and
-//   the sums rescaled) only when some p vs would pass 60,000, which fp16 just holds.
+//   the sums rescaled) only when some p vs would pass 60,000, which fp16 just holds, or p what keep_sums_finite allows.
+//   2^2 leaves the maximum 2^14 to grow before sums are read and rescaled; p vs below 2^-16 of the maximum are
+//   subnormal in fp16 then, each off by at most 2^-27 of the maximum.
 //   Two further warps issue the products, one for each row tile.
 //   Measured: 4 sequences of 1,500 to 4,096 tokens, the last 512 of each as rows, 32 heads (8 of the cache), D = 128:
 //   171 us with the host's call (183 before the scores were formed in halves, below).  A tile of 256 rows takes about
@@ -39,7 +41,6 @@ constexpr int kUnpackWarp0 = 16;     // warps 16-19: keys, the tiles' scales, va
 constexpr int kMmaWarp = 20;         // warps 20, 21: a row tile's products each
 constexpr int kThreads = 22 * 32;
 constexpr int kStages = 2;
-constexpr float kExponents = 110.0F;
 constexpr float kLift = 2.0F;        // a reference is set 2^2 below the largest p vs seen
 constexpr float kMostP = 60000.0F;   // and kept while p vs stays in fp16
 constexpr int kCols = 32;            // columns of a softmax block
@@ -171,27 +172,6 @@ __device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float scale_exponent(float s) {
-  float r;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-  return fminf(fmaxf(r, -kExponents), kExponents);
-}
-__device__ __forceinline__ float fade_to(float from, float to) { return from == to ? 1.0F : exp2_fast(from - to); }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 // Nibbles kI and kI + 4 of a word as an exact fp16 pair (kv4_attend.cu).
 template <int kI>
 __device__ __forceinline__ uint32_t codes_exact(uint32_t w) {
@@ -453,8 +433,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           tmem_ld_block(s_at + kCols * piece, f);
           if (masked) probabilities<true>(f, my_meta, my_j0, rows, p, add, most);
           else probabilities<false>(f, my_meta, my_j0, rows, p, add, most);
-          // A row without a reference yet, or one whose reference has become too low (an infinite p among it).
-          const bool low = fminf(rows.top[0], rows.top[1]) == -INFINITY || fmaxf(most[0], most[1]) > kMostP;
+          // A row without a reference yet, or one whose reference has become too low: for p vs, or for p, which value
+          // scales near zero let grow unseen by p vs (an infinite p among either).
+          const float weights = fmax3(fmaxf(add[0].x, add[0].y), add[1].x, add[1].y);
+          const bool low = fminf(rows.top[0], rows.top[1]) == -INFINITY || fmaxf(most[0], most[1]) > kMostP || weights > a.most_weight;
           if (__any_sync(0xFFFFFFFFu, low)) {
             tmem_wait_st();  // what was written before is read below, the sums of the tiles before too
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], i & 1, abort_flag));
@@ -652,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       float* const ms = meta + s * 3 * kMetaFloats + meta_at(32 * uw + lane);
       ms[0] = seen ? ks : 0.0F;
       ms[kMetaFloats] = seen ? vs : 0.0F;
-      ms[2 * kMetaFloats] = seen ? scale_exponent(vs) : -INFINITY;
+      ms[2 * kMetaFloats] = seen ? scale_exponent(vs, a.least_exponent) : -INFINITY;
       const uint32_t all = __ballot_sync(0xFFFFFFFFu, seen);
       if (lane == 0) flags[4 * s + uw] = ~all;
       fence_proxy_async();
@@ -757,7 +739,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
 }
 
 template <class T, int kDim>
-void launch_dim(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
+void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
+  Kv4Attend a = given;
+  keep_sums_finite(a, c.page_shift, kLift);
   const int shared = a.heads / c.heads;
   const int64_t row_blocks = (static_cast<int64_t>(a.max_rows) * shared + kBlockRows - 1) / kBlockRows;
   const int64_t blocks = row_blocks * a.batch * c.heads;

@@ -5,7 +5,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "common.cuh"
 
@@ -71,6 +73,10 @@ struct Kv4Attend {
   float scale;
   int causal;
   int window;                 // 0: none
+  // What keeps sums of weights finite (set by the launch, see keep_sums_finite): the least log2 of a value scale that
+  // references count, and the weight that none may pass.
+  float least_exponent;
+  float most_weight;
   void* out;                  // [rows, heads, dim], contiguous
   float* lse;                 // [rows, heads] or nullptr
   void* workspace;
@@ -131,6 +137,42 @@ __device__ __forceinline__ void kv4_fill_rows(const Kv4Attend& a, int dim) {
     const int64_t lo = max(0, a.offsets[b]), hi = min(static_cast<int64_t>(a.offsets[b + 1]), a.rows);
     if (hi - lo > a.max_rows) fill(lo + a.max_rows, hi, threadIdx.x, blockDim.x, NAN, NAN);
   }
+}
+
+// A weight p = 2^(s - reference) is as large as 1 / vs where the value scale vs is small, since references are maxima of
+// s + log2(vs), less `lift`.  With log2(vs) held to -h and up, p stays at or below 2^(lift + h); h leaves as many of
+// these as the table has tokens below 2^127.  Upwards the logarithm is held to 110: p vs keeps 16 powers above the
+// smallest p.  Scales below 2^-h lose digits in p vs, where that sinks below fp16's normal numbers.
+constexpr float kExponents = 110.0F;
+inline void keep_sums_finite(Kv4Attend& a, int page_shift, float lift) {
+  int bits = 0;
+  while ((int64_t{1} << bits) < (static_cast<int64_t>(a.max_pages) << page_shift)) ++bits;
+  a.least_exponent = -std::min(kExponents, 127.0F - static_cast<float>(bits) - lift);
+  a.most_weight = std::ldexp(1.0F, 127 - bits);
+}
+// About log2 of a value scale, held to [least, 110] (and so a number where the scale is 0, NaN or infinite).
+__device__ __forceinline__ float scale_exponent(float s, float least) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fminf(fmaxf(r, least), kExponents);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// What sums with reference `from` are multiplied by to have reference `to` >= from.  Sums with reference -inf
+// are 0, or NaN where a score was: they stay so.
+__device__ __forceinline__ float fade_to(float from, float to) { return from == to ? 1.0F : exp2_fast(from - to); }
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 // Opts a kernel in to its dynamic shared memory, once per device.

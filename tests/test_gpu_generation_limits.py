@@ -169,3 +169,44 @@ def test_no_sequence_has_rows(engine):
         got, lse = cache.attend(q, _ints(0, 1, 2, 3).view(2, 2)[:batch], _ints(20, 30)[:batch], query_offsets=offsets,
                                 return_lse=True)
         assert not got.any() and (lse == -torch.inf).all()
+
+
+# --------------------------------------------------------------------------- sizes of values
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("exponent", [-112, -120, None])
+@pytest.mark.parametrize("tokens", [4096, 20000])
+def test_values_so_small_that_weights_grow(engine, dim, rows, exponent, tokens):
+    """Thousands of like tokens whose value scales are 2^-112 or less (or zero): sums of weights stay finite.
+
+    Outputs: the bound of `_check` without its absolute part.  Log-sum-exp: fp32 sums of at most 20,000 terms in parts,
+    1e-5."""
+    page = 64
+    pages = -(-tokens // page)
+    cache = _random_cache(pages, page, 1, dim, seed=2)
+    cache.v_scales.fill_(0.0 if exponent is None else 2.0**exponent)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, -1)
+    q = _normal((rows, 4, dim), 3, torch.bfloat16, 0.1)
+    got, lse = cache.attend(q, table, _ints(tokens), query_offsets=_ints(0, rows), max_query_tokens=rows, return_lse=True)
+    out, want_lse, bound, slack = _plain(q, cache, table, [tokens], [0, rows], dim**-0.5)
+    assert ((lse.double() - want_lse).abs() <= slack + 1e-5 + 1e-6 * want_lse.abs()).all()
+    assert ((got.double() - out).abs() <= 2.0**-8 * out.abs() + (2.0**-10 + 2 * slack.unsqueeze(-1)) * bound).all()
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_zero_scales_and_scores_that_rise(engine, rows):
+    """Value scales of zero never raise a reference by their products: scores that rise by hundreds of powers of two
+    along the sequence must not overflow their weights."""
+    n, page = 640, 16
+    cache = m.Int4KVCache(40, page, 1, 128)
+    direction = _normal((1, 1, 128), 4)
+    cache.append(direction * torch.linspace(-30, 30, n, device="cuda").view(-1, 1, 1), _normal((n, 1, 128), 6),
+                 torch.arange(n, device="cuda"))
+    cache.v_scales.zero_()
+    cache.v_scales[0, 0, 3] = 1.0
+    table = torch.arange(40, dtype=torch.int32, device="cuda").view(1, 40)
+    q = (direction * 2).expand(rows, 4, 128).to(torch.bfloat16)
+    got, lse = cache.attend(q, table, _ints(n), query_offsets=_ints(0, rows), max_query_tokens=rows, return_lse=True)
+    want = _plain(q, cache, table, [n], [0, rows], 128**-0.5)
+    _check(got, want, lse)
