@@ -26,7 +26,8 @@
 //   that is rounded to the output's type, of as many bits or fewer.
 //   Reference.  Probabilities carry the values' scales, p_j vs_j, so the running reference is the maximum of
 //   s_j + log2 vs_j less 8: the largest p_j vs_j is about 2^8 whatever the scales are, and those 2^-22 of it are
-//   normal in fp16.  keep_sums_finite has what holds the fp32 sum of the p_j.
+//   normal in fp16.  Vectors of zeros are left out of it (zero_codes); keep_sums_finite has what holds the fp32 sum of
+//   the p_j.
 //   Work split.  The 128-token units of all (sequence, head, row block) segments form one line, cut into equal
 //   ranges, one per resident block, from the lengths on the device: no plan, no host copy, no imbalance.
 //   A segment cut by a range's end leaves partial sums in the workspace (at most two per block), which
@@ -524,8 +525,15 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
             s[i][nt][k] = __fmul2_rn(make_float2(d[nt][2 * k], d[nt][2 * k + 1]), __fmul2_rn(factor[nt], make_float2(ks, ks)));
         }
       }
-      const bool masked = seen != 3u || j0 < every_first || j0 + kStep - 1 > every_last;
+      const bool one = vs[0][0].x == 1.0F || vs[0][1].x == 1.0F || vs[1][0].x == 1.0F || vs[1][1].x == 1.0F;
+      const bool masked = seen != 3u || j0 < every_first || j0 + kStep - 1 > every_last || one;
       if (masked) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (vs[i][k].x == 1.0F && zero_codes<kDim>(here + kCodeBytes + (16 * i + g + 8 * k) * (kDim / 2)))
+              vs[i][k] = make_float2(0.0F, 0.0F);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll

@@ -14,8 +14,8 @@
 //   Softmax.  Sixteen warps, eight to a row tile: a warp has 16 rows, a thread two of them and a quarter of their
 //   columns, in blocks of 32 columns.  (With half the warps, a row to a thread: 206 us where this took 184.)
 //   Scales of keys and values are fp32 factors of scores and probabilities (they would lose digits in fp16 operands);
-//   the reference is the running maximum of s_j + log2(vs_j) as in kv4_attend.cu, set 2^2 below it and moved (and
-//   the sums rescaled) only when some p vs would pass 60,000, which fp16 just holds, or p what keep_sums_finite allows.
+//   the reference is the running maximum of s_j + log2(vs_j) (without vectors of zeros) as in kv4_attend.cu, set 2^2
+//   below it and moved (and the sums rescaled) only when some p vs would pass 60,000, which fp16 just holds, or p what keep_sums_finite allows.
 //   2^2 leaves the maximum 2^14 to grow before sums are read and rescaled; p vs below 2^-16 of the maximum are
 //   subnormal in fp16 then, each off by at most 2^-27 of the maximum.
 //   Two further warps issue the products, one for each row tile.
@@ -252,6 +252,13 @@ __device__ __forceinline__ void references(const float (&f)[16], const float* me
         if (e != -INFINITY && c <= rows.last[r] && rows.last[r] - c < rows.window)
           best[r] = fmaxf(best[r], f[4 * j + 2 * r + k] * ks * rows.factor[r].x + e);
     }
+}
+
+// Whether token j's value is a vector of zeros.  Out of line: in the unpacking warps' loop it cost 5 us of 170.
+template <int kDim>
+__device__ __noinline__ bool zero_value(const uint8_t* codes, const int32_t* pages, int heads, int head, int page_shift, int j) {
+  const int64_t page = __ldg(pages + (j >> page_shift));
+  return zero_codes<kDim>(codes + (((page * heads + head) << page_shift) + (j & ((1 << page_shift) - 1))) * (kDim / 2));
 }
 
 template <class T, int kDim>
@@ -632,6 +639,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         }
       }
       float* const ms = meta + s * 3 * kMetaFloats + meta_at(32 * uw + lane);
+      if (seen && vs == 1.0F &&
+          zero_value<kDim>(c.codes[1], pages, c.heads, head, c.page_shift, begin + i * kTokens + 32 * uw + lane))
+        vs = 0.0F;
       ms[0] = seen ? ks : 0.0F;
       ms[kMetaFloats] = seen ? vs : 0.0F;
       ms[2 * kMetaFloats] = seen ? scale_exponent(vs, a.least_exponent) : -INFINITY;

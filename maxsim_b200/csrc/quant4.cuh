@@ -156,6 +156,15 @@ __device__ __forceinline__ float scale_exponent(float s, float least) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   return fminf(fmaxf(r, least), kExponents);
 }
+// Whether a vector's codes are all 0.  Such a vector is stored with scale 1 (append), which says nothing of its
+// neighbours' size: it counts in the sum of weights, with a value scale of 0, but not in references.
+template <int kDim>
+__device__ __forceinline__ bool zero_codes(const uint8_t* codes) {
+  uint32_t any = 0;
+#pragma unroll 1  // seldom run, among kernels whose registers are all in use
+  for (int i = 0; i < kDim / 8; ++i) any |= reinterpret_cast<const uint32_t*>(codes)[i];
+  return any == 0;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -76,7 +76,8 @@ class Int4KVCache:
 
     @classmethod
     def from_tensors(cls, k_codes, k_scales, v_codes, v_scales):
-        """A cache over arrays the caller owns (shapes above, contiguous)."""
+        """A cache over arrays the caller owns (shapes above, contiguous).  Codes are those of `append`: a vector's largest
+        is 7 or near it, a vector of zeros has scale 1 (or 0)."""
         self = cls.__new__(cls)
         self._bind(k_codes, k_scales, v_codes, v_scales)
         return self

@@ -210,3 +210,34 @@ def test_zero_scales_and_scores_that_rise(engine, rows):
     got, lse = cache.attend(q, table, _ints(n), query_offsets=_ints(0, rows), max_query_tokens=rows, return_lse=True)
     want = _plain(q, cache, table, [n], [0, rows], 128**-0.5)
     _check(got, want, lse)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("size", [1e-5, 1e-6, 1e-8, 1e-9, 1e-20])
+@pytest.mark.parametrize("every", [2, 3, 40])
+def test_zero_vectors_among_small_values(engine, dim, rows, size, every):
+    """A vector of zeros is stored with scale 1, whatever its neighbours' sizes: it must not decide how the others'
+    weights are held.  Bound: that of `_check` without its absolute part."""
+    n, page = 300, 16
+    cache = m.Int4KVCache(19, page, 1, dim)
+    v = _normal((n, 1, dim), 5) * size
+    v[1::every] = 0
+    cache.append(_normal((n, 1, dim), 3), v, torch.arange(n, device="cuda"))
+    table = torch.arange(19, dtype=torch.int32, device="cuda").view(1, -1)
+    q = _normal((rows, 4, dim), 4, torch.bfloat16)
+    got, lse = cache.attend(q, table, _ints(n), query_offsets=_ints(0, rows), max_query_tokens=rows, return_lse=True)
+    out, want_lse, bound, slack = _plain(q, cache, table, [n], [0, rows], dim**-0.5)
+    assert ((lse.double() - want_lse).abs() <= slack + 1e-5 + 1e-6 * want_lse.abs()).all()
+    off, limit = (got.double() - out).abs(), 2.0**-8 * out.abs() + (2.0**-10 + 2 * slack.unsqueeze(-1)) * bound
+    assert (off <= limit).all(), f"worst {(off / limit).max().item():.3g} of the bound"
+
+
+def test_scales_of_one_that_are_not_zero_vectors(engine):
+    """Ordinary vectors with a scale of exactly 1 keep their part."""
+    cache = _random_cache(10, 16, 2, 128, seed=8)
+    cache.v_scales[:, :, ::2] = 1.0
+    table = _ints(*range(10)).view(1, 10)
+    q = _normal((70, 8, 128), 4, torch.bfloat16)
+    got, lse = cache.attend(q, table, _ints(150), query_offsets=_ints(0, 70), max_query_tokens=70, return_lse=True)
+    _check(got, _plain(q, cache, table, [150], [0, 70], 128**-0.5), lse)
