@@ -1562,7 +1562,7 @@ int attend(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, bool fil
   return guarded([&] {
     const Kv4View v = kv4_view(cache);
     Kv4Attend a = kv4_attend(v, args);
-    a.fill = fill;
+    a.fill = fill && a.offsets;  // without offsets every row is a sequence's
     if (a.rows == 0 || a.batch == 0) return;
     if (!a.query || !a.lengths || !a.out || (a.max_pages > 0 && !a.page_table)) throw InvalidArgument("NULL argument");
     check_address(a.query, 2, "query");

@@ -299,7 +299,10 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     b = here / (line.heads * line.most_blocks);
     cluster_segment = here - b * (line.heads * line.most_blocks);
     w = sequence_work(a, line, b);
-    if (static_cast<int>(cluster_segment % line.most_blocks) >= w.blocks) unit_end = 0;  // nothing for the whole cluster
+    if (a.fill)
+      kv4_fill_rows<T>(a, kDim, b, w.q, cluster_segment * cluster_size + cluster_rank, line.heads * line.most_blocks * cluster_size,
+                       threadIdx.x, kWarps * 32);
+    if (static_cast<int>(cluster_segment % line.most_blocks) >= w.blocks) return;  // the whole cluster
   } else {
     const Place place = find_place(
         a, line, [&](int64_t total) { return range_start(total, block, ranges(total, gridDim.x)); }, scratch);
@@ -307,8 +310,14 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
 #if __CUDA_ARCH__ >= 900
     cudaTriggerProgrammaticLaunchCompletion();
 #endif
-    unit = block < n ? range_start(place.total, block, n) : 0;
-    unit_end = block < n ? range_start(place.total, block + 1, n) : 0;
+    // Without a join, which has time for it, the rows left over are filled here.
+    if (a.fill && a.workspace == nullptr) {
+      for (int s = blockIdx.x; s < a.batch; s += gridDim.x)
+        kv4_fill_rows<T>(a, kDim, s, kv4_sequence(a, c.page_shift, s), 0, 1, threadIdx.x, kWarps * 32);
+    }
+    if (block >= n) return;
+    unit = range_start(place.total, block, n);
+    unit_end = range_start(place.total, block + 1, n);
     before = place.before;
     b = place.sequence;
     if (unit < unit_end) w = sequence_work(a, line, b);
@@ -733,7 +742,6 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       unit += tile1 - tile0;
     }
   }
-  kv4_fill_rows<T>(a, kDim);
 }
 
 // Adds the partial sums of the segments that were cut.  A warp adds the parts of one output row, or, where
@@ -754,6 +762,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(Kv4View c, Kv
     warp_line(a, line, before, mine, total);
     before = __shfl_sync(0xFFFFFFFFu, before, b);
   }
+  if (a.fill) kv4_fill_rows<T>(a, kDim, b, w.q, blockIdx.y, gridDim.y, threadIdx.x, kJoinWarps * 32);
 #if __CUDA_ARCH__ >= 900
   cudaGridDependencySynchronize();
 #endif

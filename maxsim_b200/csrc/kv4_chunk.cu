@@ -273,8 +273,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   const int b = static_cast<int>(blockIdx.x % per_block / c.heads), head = static_cast<int>(blockIdx.x % c.heads);
   const Kv4Sequence q = kv4_sequence(a, c.page_shift, b);
   const uint32_t all_rows = static_cast<uint32_t>(q.rows) * shared, block_row0 = static_cast<uint32_t>(block) * kBlockRows;  // below 2^31
-  kv4_fill_rows<T>(a, kDim);
-  if (block_row0 >= all_rows) return;
+  const int share = block * c.heads + head, shares = row_blocks * c.heads;  // of the sequence's blocks
+  if (block_row0 >= all_rows) {
+    if (a.fill) kv4_fill_rows<T>(a, kDim, b, q, share, shares, threadIdx.x, kThreads);
+    return;
+  }
   const int row_count = static_cast<int>(min(static_cast<uint32_t>(kBlockRows), all_rows - block_row0));
   const int tiles_m = row_count > kRowsTile ? 2 : 1;
   // Tokens that some row of the block sees, and the tiles over them.
@@ -681,6 +684,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       if (lane == 0) mbar_arrive(&v_full[s]);
       if (i + 1 < tiles) load_values(i + 1);
     }
+    // These warps are done first.
+    if (a.fill)
+      kv4_fill_rows<T>(a, kDim, b, kv4_sequence(a, c.page_shift, b), share, shares, threadIdx.x - kUnpackWarp0 * 32,
+                       (kMmaWarp - kUnpackWarp0) * 32);
   } else if (warp - kMmaWarp < tiles_m && tiles > 0) {
     // =================== products of a row tile: one lane issues ===================
     const int m = warp - kMmaWarp;

@@ -94,6 +94,7 @@ struct Kv4Sequence {
   int rows;
   int length;
   int pos0;   // position of row 0, negative where rows outnumber tokens
+  int left;   // rows past the announced maximum
 };
 __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page_shift, int b) {
   Kv4Sequence s;
@@ -103,6 +104,7 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page
     s.row0 = b;
     s.rows = 1;
     s.pos0 = s.length - 1;
+    s.left = 0;
   } else {
     const int64_t lo = max(0, a.offsets[b]);
     const int64_t hi = min(static_cast<int64_t>(a.offsets[b + 1]), a.rows);
@@ -110,32 +112,38 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page
     const int all = static_cast<int>(max(static_cast<int64_t>(0), hi - lo));  // at most a.rows
     s.rows = min(all, a.max_rows);
     s.pos0 = s.length - all;
+    s.left = all - s.rows;
   }
   return s;
 }
 
-// Where the caller's output is fresh memory, the rows that no block works on are written here, by all blocks of a kernel:
-// zeros and a log-sum-exp of -inf where no sequence owns the row, NaN past a sequence's announced number of rows (that
-// number was wrong, and it shows).
+// A block's `share` of `shares` of rows lo .. hi of an output (`width` elements a row) and of their log-sum-exp (`heads` a row)
+// to one value each.  (Out of line, as seldom run: the kernels' own code then lies together.)
 template <class T>
-__device__ __forceinline__ void kv4_fill_rows(const Kv4Attend& a, int dim) {
-  if (!a.fill || a.offsets == nullptr) return;
-  auto fill = [&](int64_t lo, int64_t hi, int64_t thread, int64_t threads, float value, float lse) {
-    const int64_t width = static_cast<int64_t>(a.heads) * dim;
-    for (int64_t i = lo * width + thread; i < hi * width; i += threads) static_cast<T*>(a.out)[i] = from_f32<T>(value);
-    if (a.lse)
-      for (int64_t i = lo * a.heads + thread; i < hi * a.heads; i += threads) a.lse[i] = lse;
-  };
-  const int64_t first = max(static_cast<int64_t>(0), min(static_cast<int64_t>(a.offsets[0]), a.rows));
-  const int64_t last = max(first, min(static_cast<int64_t>(a.offsets[a.batch]), a.rows));
-  const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  fill(0, first, thread, threads, 0.0F, -INFINITY);
-  fill(last, a.rows, thread, threads, 0.0F, -INFINITY);
-  if (a.max_rows >= a.rows) return;
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    const int64_t lo = max(0, a.offsets[b]), hi = min(static_cast<int64_t>(a.offsets[b + 1]), a.rows);
-    if (hi - lo > a.max_rows) fill(lo + a.max_rows, hi, threadIdx.x, blockDim.x, NAN, NAN);
+__device__ __noinline__ void set_rows(T* out, float* lse, int64_t width, int heads, int64_t lo, int64_t hi, float value,
+                                      float lse_value, int share, int shares, int thread, int threads) {
+  const int64_t first = lo + (hi - lo) * share / shares, last = lo + (hi - lo) * (share + 1) / shares;
+#pragma unroll 1
+  for (int64_t i = first * width + thread; i < last * width; i += threads) out[i] = from_f32<T>(value);
+  if (lse == nullptr) return;
+#pragma unroll 1
+  for (int64_t i = first * heads + thread; i < last * heads; i += threads) lse[i] = lse_value;
+}
+// Where the caller's output is fresh memory, the rows that no block works on are written by the blocks that have sequence
+// b (this one is `share` of `shares`): zeros and a log-sum-exp of -inf in the rows before the first sequence's and after
+// the last's, NaN past a sequence's announced number of rows (that number was wrong, and it shows).
+template <class T>
+__device__ __forceinline__ void kv4_fill_rows(const Kv4Attend& a, int dim, int b, const Kv4Sequence& q, int share, int shares,
+                                              int thread, int threads) {
+  const int64_t end = q.row0 + q.rows + q.left;
+  const bool before = b == 0 && q.row0 > 0, after = b == a.batch - 1 && end < a.rows;
+  if (!before && !after && q.left == 0) return;
+#pragma unroll 1
+  for (int part = 0; part < 3; ++part) {  // one call in the code
+    const int64_t lo = part == 0 ? 0 : part == 1 ? end - q.left : end;
+    const int64_t hi = part == 0 ? (b == 0 ? min(q.row0, a.rows) : 0) : part == 1 ? end : b == a.batch - 1 ? a.rows : end;
+    set_rows(static_cast<T*>(a.out), a.lse, static_cast<int64_t>(a.heads) * dim, a.heads, lo, max(lo, hi), part == 1 ? NAN : 0.0F,
+             part == 1 ? NAN : -INFINITY, share, shares, thread, threads);
   }
 }
 
