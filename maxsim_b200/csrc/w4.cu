@@ -290,11 +290,18 @@ void launch_w4_pack(const uint8_t* codes, const uint16_t* scales, int64_t n, int
 }
 
 void launch_w4_product(const W4View& w, const W4Product& p, cudaStream_t stream) {
-  if (p.rows <= 0) return;
-  if (p.type == kElemF16) launch_typed<__half>(w, p, stream);
-  else launch_typed<__nv_bfloat16>(w, p, stream);
-  count_launch();
-  check(cudaGetLastError(), "launch 4-bit weight product kernel");
+  // Row blocks (of 32 rows where rows are many) are a grid's second dimension, which ends at 65,535.
+  constexpr int64_t kMostRows = int64_t{65535} * 32;
+  for (int64_t row = 0; row < p.rows; row += kMostRows) {
+    W4Product part = p;
+    part.x = static_cast<const uint16_t*>(p.x) + row * p.x_stride;
+    part.y = static_cast<uint16_t*>(p.y) + row * p.y_stride;
+    part.rows = std::min(kMostRows, p.rows - row);
+    if (p.type == kElemF16) launch_typed<__half>(w, part, stream);
+    else launch_typed<__nv_bfloat16>(w, part, stream);
+    count_launch();
+    check(cudaGetLastError(), "launch 4-bit weight product kernel");
+  }
 }
 
 }  // namespace msb

@@ -241,3 +241,17 @@ def test_scales_of_one_that_are_not_zero_vectors(engine):
     q = _normal((70, 8, 128), 4, torch.bfloat16)
     got, lse = cache.attend(q, table, _ints(150), query_offsets=_ints(0, 70), max_query_tokens=70, return_lse=True)
     _check(got, _plain(q, cache, table, [150], [0, 70], 128**-0.5), lse)
+
+
+# --------------------------------------------------------------------------- products
+
+@pytest.mark.parametrize("rows", [65535 * 32, 65535 * 32 + 1, 65536 * 32 + 33])
+def test_products_of_millions_of_rows(rows):
+    """More row blocks than a grid's second dimension has: every row is the product that it is alone."""
+    w = _normal((16, 64), 1, scale=0.1)
+    linear = m.Int4Linear.from_weight(w, group_size=64)
+    x = _normal((rows, 64), 2, torch.bfloat16)
+    got = linear(x)
+    for at in (0, 1 << 20, 65535 * 32 - 64, rows - 100):
+        at = min(at, rows - 64)
+        assert torch.equal(got[at : at + 64], linear(x[at : at + 64].clone()))
