@@ -70,6 +70,29 @@ at::Tensor empty(c10::IntArrayRef sizes, c10::ScalarType type, c10::Device devic
 }
 void* stream_of(c10::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
 
+// Refuses an output (contiguous) that shares memory with what the kernel reads: other blocks may still be reading there.
+// `in` is [rows, heads, dim] with any strides but the last; the very same rows in the same places are let through where
+// a block writes only what it alone has read (`same_is_fine`).
+void no_overlap(const at::Tensor& out, const char* name, const at::Tensor& in, const char* in_name, bool same_is_fine) {
+  if (out.numel() == 0 || in.numel() == 0) return;
+  const char* const o0 = static_cast<const char*>(out.const_data_ptr());
+  const char* const o1 = o0 + out.numel() * out.element_size();
+  const char* const i0 = static_cast<const char*>(in.const_data_ptr());
+  int64_t last = 0;
+  for (int64_t d = 0; d < in.dim(); ++d) last += (in.size(d) - 1) * in.stride(d);
+  const int64_t size = in.element_size();
+  if (o1 <= i0 || i0 + (last + 1) * size <= o0) return;
+  if (same_is_fine && o0 == i0 && in.is_contiguous() && in.numel() == out.numel()) return;
+  // The spans meet; the rows may still lie beside the output.
+  const int64_t rows = in.size(0), row = in.stride(0) * size, heads = in.dim() == 3 ? in.size(1) : 1;
+  const int64_t head = in.dim() == 3 ? in.stride(1) * size : 0, width = in.size(-1) * size;
+  for (int64_t r = 0; r < rows; ++r)
+    for (int64_t h = 0; h < heads; ++h) {
+      const char* const p = i0 + r * row + h * head;
+      if (o0 < p + width && p < o1) refuse(std::string(name) + " must not overlap " + in_name);
+    }
+}
+
 const msb_kv4_cache* cache_of(PyObject* o) {
   void* p = PyLong_AsVoidPtr(o);
   if (PyErr_Occurred()) throw PythonError{};
@@ -149,6 +172,7 @@ PyObject* read(PyObject* const* args, Py_ssize_t n) {
       if (!out[i].sizes().equals(shape) || !out[i].is_contiguous())
         refuse(std::string(names[i]) + " must be contiguous with shape " + text(shape));
     }
+    no_overlap(out[0], names[0], out[1].view({shape[0], shape[1] * shape[2]}), names[1], false);
   }
   check_status(msb_kv4_read_device(c, slots.const_data_ptr<int64_t>(), shape[0], type_id(type, true),
                                    out[0].mutable_data_ptr(), out[1].mutable_data_ptr(), stream_of(device)));
@@ -221,6 +245,7 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
     out = tensor(args[10], "out", device);
     want_dtype(out, "out", query.scalar_type());
     if (!out.sizes().equals(shape) || !out.is_contiguous()) refuse("out must be contiguous with shape " + text(shape));
+    no_overlap(out, "out", query, "query", true);
   }
   at::Tensor lse;
   if (return_lse) lse = empty({rows, heads}, c10::kFloat, device);
@@ -299,6 +324,7 @@ PyObject* linear(PyObject* const* args, Py_ssize_t n) {
     out = tensor(args[2], "out", device);
     want_dtype(out, "out", x.scalar_type());
     if (!out.sizes().equals(shape) || !out.is_contiguous()) refuse("out must be contiguous with shape " + text(shape));
+    no_overlap(out, "out", rows, "x", false);
   }
   check_status(msb_w4_product_device(l->codes, l->scales, l->n, l->k, l->group, rows.const_data_ptr(), rows.stride(0),
                                      rows.size(0), l->bias, out.mutable_data_ptr(), l->n, type, l->device,

@@ -159,7 +159,7 @@ class Int4KVCache:
         query heads share one.  ``scale`` defaults to ``head_dim ** -0.5``.  A row that sees nothing is zero.
         Returns ``[rows, heads, head_dim]`` in the query's dtype, with ``return_lse`` also the fp32 natural
         log-sum-exp ``[rows, heads]`` (-inf where nothing is seen), with which results over parts of a context
-        can be joined."""
+        can be joined.  ``out`` may be the (contiguous) query itself, but not overlap it otherwise."""
         return _native.attend(self._address, query, page_table, lengths, query_offsets, max_query_tokens, scale, causal,
                               window, return_lse, out)
 
@@ -253,5 +253,6 @@ class Int4Linear:
         return self._codes.numel() + self._scales.numel()
 
     def __call__(self, x, *, out=None):
-        """``x`` ``[..., in]`` (fp16 or bf16) to ``[..., out]``; sums are fp32, rounded once."""
+        """``x`` ``[..., in]`` (fp16 or bf16) to ``[..., out]``; sums are fp32, rounded once.  ``out`` must not overlap
+        ``x``."""
         return _native.linear(self._address, x, out)

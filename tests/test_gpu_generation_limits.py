@@ -255,3 +255,58 @@ def test_products_of_millions_of_rows(rows):
     for at in (0, 1 << 20, 65535 * 32 - 64, rows - 100):
         at = min(at, rows - 64)
         assert torch.equal(got[at : at + 64], linear(x[at : at + 64].clone()))
+
+
+# --------------------------------------------------------------------------- outputs over inputs
+
+def test_outputs_that_overlap_what_is_read_are_refused():
+    """Blocks write while others read: a product into its own input, rows or heads of it, or a shifted view of it."""
+    linear = m.Int4Linear.from_weight(_normal((64, 64), 1, scale=0.1), group_size=64)
+    room = _normal((40, 64), 2, torch.bfloat16)
+    x = room[:16]
+    want = linear(x)
+    for out in (x, room[8:24], room[15:31]):
+        with pytest.raises(ValueError, match="overlap"):
+            linear(x, out=out)
+    assert torch.equal(linear(x, out=room[16:32]), want)  # the rows after
+    wide = _normal((16, 128), 3, torch.bfloat16)
+    want = linear(wide[1:2, 64:])
+    assert torch.equal(linear(wide[1:2, 64:], out=wide[1:2, :64]), want)  # the other half of the row
+    with pytest.raises(ValueError, match="overlap"):
+        linear(wide[:, 64:], out=wide.flatten()[: 16 * 64].view(16, 64))
+    odd = _normal((3 * 64 + 1,), 4, torch.bfloat16)[1:].view(3, 64)  # off 16 bytes: copied first, nothing to overlap
+    want = linear(odd)
+    assert torch.equal(linear(odd, out=odd), want)
+
+    cache = _random_cache(8, 16, 2, 64, seed=1)
+    rows = torch.zeros((20, 4, 64), dtype=torch.float16, device="cuda")
+    rows.copy_(_normal((20, 4, 64), 5, torch.float16))
+    table, lengths = _ints(*range(8)).view(1, 8), _ints(120)
+    kw = dict(query_offsets=_ints(0, 10), max_query_tokens=10)
+    for out in (rows[5:15], rows[9:19]):
+        with pytest.raises(ValueError, match="overlap"):
+            cache.attend(rows[:10], table, lengths, out=out, **kw)
+    want = cache.attend(rows[:10], table, lengths, **kw)
+    assert torch.equal(cache.attend(rows[:10], table, lengths, out=rows[10:], **kw), want)
+    slots = torch.arange(4, device="cuda")
+    pair = torch.zeros((6, 2, 64), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        cache.read(slots, out=(pair[:4], pair[2:]))
+    both = torch.zeros((8, 2, 64), dtype=torch.float16, device="cuda")
+    keys, values = cache.read(slots, out=(both[:4], both[4:]))
+    assert torch.equal(keys, cache.read(slots, dtype=torch.float16)[0]) and torch.equal(values, cache.read(slots, dtype=torch.float16)[1])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,length", [(1, 100), (5, 120), (3, 3000), (90, 3000)])
+def test_attention_in_place_of_its_query(engine, dim, rows, length):
+    """The output in the query's own memory: every block reads its rows before it writes them."""
+    page = 16
+    pages = -(-length // page)
+    cache = _random_cache(pages, page, 2, dim, seed=dim)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(2, -1)
+    query = _normal((2 * rows, 6, dim), 5, torch.bfloat16)
+    kw = dict(query_offsets=_ints(0, rows, 2 * rows), max_query_tokens=rows)
+    lengths = _ints(length, length - 1)
+    want = cache.attend(query, table, lengths, **kw)
+    assert torch.equal(cache.attend(query, table, lengths, out=query, **kw), want)
