@@ -8,6 +8,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -58,6 +59,12 @@ void want_dtype(const at::Tensor& t, const char* name, c10::ScalarType type) {
 void want_dim(const at::Tensor& t, const char* name, int64_t dim) {
   if (t.dim() != dim)
     refuse(std::string(name) + " must have " + std::to_string(dim) + " dimensions, got " + std::to_string(t.dim()));
+}
+// The operators have no backward pass: a result without a history must not pass for one with it.
+void no_gradient(const at::Tensor& t, const char* name) {
+  if (c10::GradMode::is_enabled() && t.requires_grad())
+    refuse(std::string(name) + " requires a gradient, which this operator does not have: call it under torch.no_grad() or on " +
+           name + ".detach()");
 }
 int32_t type_id(c10::ScalarType type, bool f32) {
   if (type == c10::kHalf) return MSB_TYPE_F16;
@@ -169,6 +176,7 @@ PyObject* read(PyObject* const* args, Py_ssize_t n) {
     type_id(type, true);
     for (int i = 0; i < 2; ++i) {
       want_dtype(out[i], names[i], type);
+      no_gradient(out[i], names[i]);
       if (!out[i].sizes().equals(shape) || !out[i].is_contiguous())
         refuse(std::string(names[i]) + " must be contiguous with shape " + text(shape));
     }
@@ -190,6 +198,7 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
   msb_kv4_attend_args a{};
   const at::Tensor& given = tensor(args[1], "query", device);
   want_dim(given, "query", 3);
+  no_gradient(given, "query");
   a.type = type_id(given.scalar_type(), false);
   const int64_t rows = given.size(0), heads = given.size(1), dim = given.size(2);
   if (dim != c->head_dim || heads == 0 || heads % c->kv_heads)
@@ -245,6 +254,7 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
     out = tensor(args[10], "out", device);
     want_dtype(out, "out", query.scalar_type());
     if (!out.sizes().equals(shape) || !out.is_contiguous()) refuse("out must be contiguous with shape " + text(shape));
+    no_gradient(out, "out");
     no_overlap(out, "out", query, "query", true);
   }
   at::Tensor lse;
@@ -307,6 +317,7 @@ PyObject* linear(PyObject* const* args, Py_ssize_t n) {
   const c10::Device device = device_of(l->device);
   const at::Tensor& x = tensor(args[1], "x", device);
   const int32_t type = type_id(x.scalar_type(), false);
+  no_gradient(x, "x");
   if (x.dim() < 1 || x.size(-1) != l->k)
     refuse("x must have shape [..., " + std::to_string(l->k) + "], got " + text(x.sizes()));
   if (l->bias_type >= 0 && l->bias_type != type) refuse("bias and x must have the same dtype");
@@ -324,6 +335,7 @@ PyObject* linear(PyObject* const* args, Py_ssize_t n) {
     out = tensor(args[2], "out", device);
     want_dtype(out, "out", x.scalar_type());
     if (!out.sizes().equals(shape) || !out.is_contiguous()) refuse("out must be contiguous with shape " + text(shape));
+    no_gradient(out, "out");
     no_overlap(out, "out", rows, "x", false);
   }
   check_status(msb_w4_product_device(l->codes, l->scales, l->n, l->k, l->group, rows.const_data_ptr(), rows.stride(0),

@@ -6,7 +6,8 @@ and attended to where they lie.  ``Int4Linear`` multiplies a few rows
 with 4-bit weights.  Both take and return CUDA tensors, run on torch's current stream without synchronising,
 allocate through torch only, and can be captured into a CUDA graph.
 
-There is no backward pass: codes have no gradient, and these are the operators of serving.
+There is no backward pass: these are the operators of serving.  A query or rows that require a gradient are refused
+while gradients are enabled; codes, scales and a bias are constants, and keys and values are quantised without one.
 """
 
 from __future__ import annotations
@@ -212,7 +213,7 @@ class Int4Linear:
             _type_id(bias.dtype, "fp16 or bf16")
             if bias.shape[0] != self.out_features:
                 raise ValueError(f"bias must have shape [{self.out_features}]")
-            bias = bias.contiguous()
+            bias = bias.detach().contiguous()
         self.bias = bias
         codes, scales = codes.contiguous(), scales.contiguous()
         with torch.cuda.device(self.device):

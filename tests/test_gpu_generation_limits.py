@@ -310,3 +310,30 @@ def test_attention_in_place_of_its_query(engine, dim, rows, length):
     lengths = _ints(length, length - 1)
     want = cache.attend(query, table, lengths, **kw)
     assert torch.equal(cache.attend(query, table, lengths, out=query, **kw), want)
+
+
+# --------------------------------------------------------------------------- gradients
+
+def test_inputs_that_require_a_gradient_are_refused():
+    """There is no backward pass: a result without a history must not pass for one with it."""
+    linear = m.Int4Linear.from_weight(_normal((16, 64), 1), group_size=64)
+    x = _normal((2, 64), 2, torch.bfloat16).requires_grad_()
+    cache = _random_cache(4, 16, 2, 64, seed=1)
+    table, lengths = _ints(0, 1, 2, 3).view(2, 2), _ints(20, 30)
+    q = _normal((2, 4, 64), 3, torch.float16).requires_grad_()
+    for call in (lambda: linear(x), lambda: cache.attend(q, table, lengths)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            want = call()
+        with torch.inference_mode():
+            assert torch.equal(call(), want)
+    assert torch.equal(linear(x.detach()), linear(x.detach() * 1))
+    bias = torch.nn.Parameter(_normal((16,), 4, torch.bfloat16))
+    m.Int4Linear.from_weight(_normal((16, 64), 1), group_size=64, bias=bias)(x.detach())  # held as a constant
+    out = torch.zeros((2, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    pair = [torch.zeros((1, 2, 64), dtype=torch.float16, device="cuda", requires_grad=True) for _ in range(2)]
+    for call in (lambda: linear(x.detach(), out=out), lambda: cache.attend(q.detach(), table, lengths, out=q),
+                 lambda: cache.read(torch.zeros(1, dtype=torch.int64, device="cuda"), out=pair)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
