@@ -105,16 +105,22 @@ class Int4KVCache:
             raise ValueError("num_pages and num_kv_heads must be positive")
         if any(t.data_ptr() % 16 for t in (k_codes, k_scales, v_codes, v_scales)):
             raise ValueError("cache arrays must be 16-byte aligned")
-        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self._arrays = (k_codes, k_scales, v_codes, v_scales)
         self.device = device
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = pages, heads, size, 2 * half
         self._c = _lib.Kv4Cache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), pages,
                                 size, heads, 2 * half, device.index)
         self._address = ctypes.addressof(self._c)
 
+    # Read-only: the kernels use the addresses of the arrays that the cache was made with.
+    k_codes = property(lambda self: self._arrays[0])
+    k_scales = property(lambda self: self._arrays[1])
+    v_codes = property(lambda self: self._arrays[2])
+    v_scales = property(lambda self: self._arrays[3])
+
     @property
     def resident_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales))
+        return sum(t.numel() * t.element_size() for t in self._arrays)
 
     def append(self, keys, values, slots) -> None:
         """Quantise ``keys`` and ``values`` ``[tokens, kv_heads, head_dim]`` (fp32, fp16 or bf16, any token and
@@ -214,7 +220,7 @@ class Int4Linear:
             if bias.shape[0] != self.out_features:
                 raise ValueError(f"bias must have shape [{self.out_features}]")
             bias = bias.detach().contiguous()
-        self.bias = bias
+        self._bias = bias
         codes, scales = codes.contiguous(), scales.contiguous()
         with torch.cuda.device(self.device):
             self._codes = torch.empty(code_bytes.value, dtype=torch.uint8, device=self.device)
@@ -248,6 +254,8 @@ class Int4Linear:
         codes = torch.round(w / scales.float().unsqueeze(2)).clamp_(-7, 7).to(torch.int16).view(n, -1)[:, :k]
         packed = ((codes[:, 0::2] & 15) | ((codes[:, 1::2] & 15) << 4)).to(torch.uint8)
         return cls(packed, scales, group_size=group_size, bias=bias)
+
+    bias = property(lambda self: self._bias)  # read-only, as its address is held
 
     @property
     def resident_bytes(self) -> int:

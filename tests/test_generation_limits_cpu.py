@@ -76,3 +76,14 @@ def test_the_other_entries_refuse_addresses_their_kernels_cannot_use():
                            (product, dict(bias=_PTR + 1), "bias must be 2-byte"), (product, dict(y=_PTR + 1), "y must be 2-byte")):
         with pytest.raises(ValueError, match=text):
             call(**kw)
+
+
+def test_arrays_whose_addresses_are_held_cannot_be_exchanged():
+    """The kernels read the arrays that an object was made with: assigning another would leave them reading freed memory."""
+    cache, linear = m.Int4KVCache.__new__(m.Int4KVCache), m.Int4Linear.__new__(m.Int4Linear)
+    for thing, names in ((cache, ("k_codes", "k_scales", "v_codes", "v_scales")), (linear, ("bias",))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(thing, name, torch.zeros(1))
+            with pytest.raises(AttributeError):
+                delattr(thing, name)
