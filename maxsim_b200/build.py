@@ -7,15 +7,20 @@ Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` into
 depend on which libcudart torch bundles).  nvcc cross-compiles without a GPU.
 ``csrc/generation_binding.cpp`` becomes ``maxsim_b200/_generation.so``, the
 Python module between torch and the library's cache and weight operators
-(g++, torch's own headers and libraries).
+(g++, torch's own headers and libraries).  Where torch is not installed only
+the library is built; another torch than the module was built for makes the
+module stale.
 """
 
 from __future__ import annotations
 
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -39,17 +44,56 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
+def torch_build() -> str | None:
+    """What the Python module depends on of torch and Python (without importing torch), None without torch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        version = "unknown"
+    return f"{version} {spec.origin} {sysconfig.get_config_var('SOABI')}"
+
+
+def _older(target: Path, deps: list[Path]) -> bool:
+    return not target.exists() or any(p.stat().st_mtime > target.stat().st_mtime for p in deps if p.exists())
+
+
+def _header() -> Path:
+    return PKG.parent / "include" / "maxsim_b200.h"
+
+
+def _stamp() -> Path:
+    return PKG / "_build" / "generation.torch"
+
+
+def library_stale() -> bool:
+    return _older(LIB, sources() + sorted(CSRC.glob("*.cuh")) + [_header()])
+
+
+def binding_stale() -> bool:
+    torch = torch_build()
+    if torch is None:
+        return False
+    return _older(BINDING, [BINDING_SRC, _header()]) or not _stamp().exists() or _stamp().read_text() != torch
+
+
 def needs_build() -> bool:
-    if not LIB.exists() or not BINDING.exists():
-        return True
-    mtime = min(LIB.stat().st_mtime, BINDING.stat().st_mtime)
-    deps = sources() + [BINDING_SRC] + sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "maxsim_b200.h"]
-    return any(p.stat().st_mtime > mtime for p in deps if p.exists())
+    return library_stale() or binding_stale()
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not needs_build():
-        return LIB
+    if force or library_stale():
+        build_library(verbose)
+    if torch_build() is None:
+        sys.stderr.write("torch is not installed: _generation.so (Int4KVCache, Int4Linear) is not built\n")
+    elif force or binding_stale():
+        build_binding()
+    return LIB
+
+
+def build_library(verbose: bool = False) -> Path:
     nvcc = nvcc_path()
     objdir = PKG / "_build"
     objdir.mkdir(exist_ok=True)
@@ -75,13 +119,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objs), "-cudart", "static"]
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
-    build_binding()
     return LIB
 
 
 def build_binding() -> Path:
-    import sysconfig
-
     import torch
 
     base = Path(torch.__file__).resolve().parent
@@ -94,6 +135,8 @@ def build_binding() -> Path:
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING)
+    _stamp().parent.mkdir(exist_ok=True)
+    _stamp().write_text(torch_build())
     return BINDING
 
 
