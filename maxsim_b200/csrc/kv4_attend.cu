@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       for (int d = 0; d < kKeyWords * 8; ++d) top = fmaxf(top, fabsf(to_f32(x[d])));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      const int e = max(-110, min(127, static_cast<int>(__float_as_uint(top) >> 23) - 127));
       const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
       float sum[4] = {0.0F, 0.0F, 0.0F, 0.0F};
 #pragma unroll

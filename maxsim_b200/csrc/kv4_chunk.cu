@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_f32(v[i])));
 #pragma unroll
           for (int d = 1; d < kRowLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-          const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+          const int e = max(-110, min(127, static_cast<int>(__float_as_uint(top) >> 23) - 127));
           const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
           const int r = (k0 + k) * kRowsAtOnce + lane / kRowLanes, piece = lane % kRowLanes;
           store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled(row0 + r, piece & 7),

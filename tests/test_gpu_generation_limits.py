@@ -243,6 +243,20 @@ def test_scales_of_one_that_are_not_zero_vectors(engine):
     _check(got, _plain(q, cache, table, [150], [0, 70], 128**-0.5), lse)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("size", [1e-37, 1e-35, 1e33, 1e35, 1e37])
+def test_the_largest_and_smallest_queries(engine, dim, rows, size):
+    """Queries near both ends of bf16 over keys near the other end: their scores are ordinary numbers."""
+    n, page = 150, 16
+    cache = m.Int4KVCache(10, page, 1, dim)
+    cache.append(_normal((n, 1, dim), 3) / size, _normal((n, 1, dim), 5), torch.arange(n, device="cuda"))
+    table = _ints(*range(10)).view(1, 10)
+    q = (_normal((rows, 4, dim), 4) * size).to(torch.bfloat16)
+    got, lse = cache.attend(q, table, _ints(n), query_offsets=_ints(0, rows), max_query_tokens=rows, return_lse=True)
+    _check(got, _plain(q, cache, table, [n], [0, rows], dim**-0.5), lse)
+
+
 # --------------------------------------------------------------------------- products
 
 @pytest.mark.parametrize("rows", [65535 * 32, 65535 * 32 + 1, 65536 * 32 + 33])
