@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float e = scale_exponent(vs[i][k].x, a.least_exponent);
+          const float e = scale_exponent(vs[i][k].x, a.least_exponent, most_exponent(kLift));
           raise[i][k] = make_float2(e, e);
         }
       bool moved = false;

@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         vs = 0.0F;
       ms[0] = seen ? ks : 0.0F;
       ms[kMetaFloats] = seen ? vs : 0.0F;
-      ms[2 * kMetaFloats] = seen ? scale_exponent(vs, a.least_exponent) : -INFINITY;
+      ms[2 * kMetaFloats] = seen ? scale_exponent(vs, a.least_exponent, most_exponent(kLift)) : -INFINITY;
       const uint32_t all = __ballot_sync(0xFFFFFFFFu, seen);
       if (lane == 0) flags[4 * s + uw] = ~all;
       fence_proxy_async();

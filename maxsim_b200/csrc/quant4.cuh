@@ -149,20 +149,22 @@ __device__ __forceinline__ void kv4_fill_rows(const Kv4Attend& a, int dim, int b
 
 // A weight p = 2^(s - reference) is as large as 1 / vs where the value scale vs is small, since references are maxima of
 // s + log2(vs), less `lift`.  With log2(vs) held to -h and up, p stays at or below 2^(lift + h); h leaves as many of
-// these as the table has tokens below 2^127.  Upwards the logarithm is held to 110: p vs keeps 16 powers above the
-// smallest p.  Scales below 2^-h lose digits in p vs, where that sinks below fp16's normal numbers.
-constexpr float kExponents = 110.0F;
+// these as the table has tokens below 2^127.  Upwards the logarithm is held to lift + 109.5 (most_exponent): p vs of the
+// largest scales, 2^125.2, stays at 2^15.7, which fp16 holds; p of these is 2^-109.5, and weights 2^-16 of it are the last
+// that fp32 holds.  Scales below 2^-h lose digits in p vs, where that sinks below fp16's normal numbers.
+constexpr float kExponents = 110.0F;  // h at most
+constexpr float most_exponent(float lift) { return lift + 109.5F; }
 inline void keep_sums_finite(Kv4Attend& a, int page_shift, float lift) {
   int bits = 0;
   while ((int64_t{1} << bits) < (static_cast<int64_t>(a.max_pages) << page_shift)) ++bits;
   a.least_exponent = -std::min(kExponents, 127.0F - static_cast<float>(bits) - lift);
   a.most_weight = std::ldexp(1.0F, 127 - bits);
 }
-// About log2 of a value scale, held to [least, 110] (and so a number where the scale is 0, NaN or infinite).
-__device__ __forceinline__ float scale_exponent(float s, float least) {
+// About log2 of a value scale, held to [least, most] (and so a number where the scale is 0, NaN or infinite).
+__device__ __forceinline__ float scale_exponent(float s, float least, float most) {
   float r;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-  return fminf(fmaxf(r, least), kExponents);
+  return fminf(fmaxf(r, least), most);
 }
 // Whether a vector's codes are all 0.  Such a vector is stored with scale 1 (append), which says nothing of its
 // neighbours' size: it counts in the sum of weights, with a value scale of 0, but not in references.

@@ -257,6 +257,27 @@ def test_the_largest_and_smallest_queries(engine, dim, rows, size):
     _check(got, _plain(q, cache, table, [n], [0, rows], dim**-0.5), lse)
 
 
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("size", [1e33, 1e35, 1e37, 1e38])
+def test_the_largest_finite_values(engine, dim, rows, size):
+    """Values up to fp32's and bf16's largest numbers: outputs are finite where their averages are.  Scores lie close
+    together, so no weight is far from the largest; bound: that of `_check` without its absolute part."""
+    n, page = 150, 16
+    cache = m.Int4KVCache(10, page, 1, dim)
+    v = (_normal((n, 1, dim), 5) * size).clamp(-3e38, 3e38)
+    cache.append(_normal((n, 1, dim), 3), v, torch.arange(n, device="cuda"))
+    assert torch.isfinite(cache.v_scales[:9]).all()
+    table = _ints(*range(10)).view(1, 10)
+    q = _normal((rows, 4, dim), 4, torch.bfloat16, 0.1)
+    got, lse = cache.attend(q, table, _ints(n), query_offsets=_ints(0, rows), max_query_tokens=rows, return_lse=True)
+    out, want_lse, bound, slack = _plain(q, cache, table, [n], [0, rows], dim**-0.5)
+    assert ((lse.double() - want_lse).abs() <= slack + 1e-5 + 1e-6 * want_lse.abs()).all()
+    off, limit = (got.double() - out).abs(), 2.0**-8 * out.abs() + (2.0**-10 + 2 * slack.unsqueeze(-1)) * bound
+    assert (off <= limit).all(), f"worst {(off / limit).max().item():.3g} of the bound"
+
+
 # --------------------------------------------------------------------------- products
 
 @pytest.mark.parametrize("rows", [65535 * 32, 65535 * 32 + 1, 65536 * 32 + 33])
