@@ -299,10 +299,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     b = here / (line.heads * line.most_blocks);
     cluster_segment = here - b * (line.heads * line.most_blocks);
     w = sequence_work(a, line, b);
-    if (a.fill)
-      kv4_fill_rows<T>(a, kDim, b, w.q, cluster_segment * cluster_size + cluster_rank, line.heads * line.most_blocks * cluster_size,
-                       threadIdx.x, kWarps * 32);
-    if (static_cast<int>(cluster_segment % line.most_blocks) >= w.blocks) return;  // the whole cluster
+    if (static_cast<int>(cluster_segment % line.most_blocks) >= w.blocks) unit_end = 0;  // nothing for the whole cluster
   } else {
     const Place place = find_place(
         a, line, [&](int64_t total) { return range_start(total, block, ranges(total, gridDim.x)); }, scratch);
@@ -741,6 +738,12 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       __syncthreads();
       unit += tile1 - tile0;
     }
+  }
+  if constexpr (kCluster) {
+    // Last: ahead of the first loads it costs 0.1 us of 6.9.
+    if (a.fill)
+      kv4_fill_rows<T>(a, kDim, b, w.q, cluster_segment * cluster_size + cluster_rank, line.heads * line.most_blocks * cluster_size,
+                       threadIdx.x, kWarps * 32);
   }
 }
 
