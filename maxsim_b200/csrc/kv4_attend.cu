@@ -6,7 +6,8 @@
 // that sees nothing writes zeros and a log-sum-exp of -inf.
 //
 // kv4_attend_kernel: few rows a sequence (decode, drafted tokens).
-//   Bound: the codes' bytes, D + 8 per token and head, then instruction issue, above all the integer pipe that unpacks.
+//   Bound: the codes' bytes, D + 8 per token and head; then latency, a warp's chain a step (unpacking, products, maximum,
+//   vote, exponentials, products): of 16 warps an SM it leaves 57% of the issue slots and of the memory's rate used.
 //   Products.  m16n8k16 fp16 products with the tokens as the 16-row operand: S^T = K Q^T, O^T = V^T P^T, so
 //   8 query rows (the heads that share a key/value head, times the query tokens) fill a column tile instead
 //   of half a row tile.  tcgen05 wants 128 rows of queries, which decode has not.
@@ -22,7 +23,7 @@
 //   both (their sum over all tokens would lose digits to them).  (As fp16 subnormals codes would need neither, but the
 //   products then lost 6 to 10 bits.)
 //   Queries are fp16 after a power of two per row that puts their maximum in [2^10, 2^11): exact for fp16 inputs
-//   down to 2^-34 of the row's maximum, and so for bf16 ones.  Probabilities are fp16 (11 bits): they enter one sum
+//   down to 2^-34 of the row's maximum, and so for bf16 ones, up to their largest.  Probabilities are fp16 (11 bits): they enter one sum
 //   that is rounded to the output's type, of as many bits or fewer.
 //   Reference.  Probabilities carry the values' scales, p_j vs_j, so the running reference is the maximum of
 //   s_j + log2 vs_j less 8: the largest p_j vs_j is about 2^8 whatever the scales are, and those 2^-22 of it are
@@ -32,11 +33,11 @@
 //   ranges, one per resident block, from the lengths on the device: no plan, no host copy, no imbalance.
 //   A segment cut by a range's end leaves partial sums in the workspace (at most two per block), which
 //   kv4_join_kernel adds in a fixed order; it is launched early (programmatic dependent launch).
-//   Short contexts (launch_attend has the rule) take a cluster of 2 to 8 blocks a segment instead, whose parts are
+//   Short contexts (shape_of has the rule) take a cluster of 2 to 8 blocks a segment instead, whose parts are
 //   joined over distributed shared memory: one launch.
-//   Measured on the device, D = 128, 8 heads, 4 query heads each: 64 sequences of 4,096 tokens 75 us (3.8 TB/s of
-//   codes, 58% of a copy's rate), 2 of 115,000 65 us (3.9 TB/s), 1 of 16,384 17 us, 1 of 1,030 6.7 us.  At the first
-//   57% of the issue slots and of the integer pipe are used; 4 to 5 us are the join and both launches' ends.
+//   Measured on the device, D = 128, 8 heads, 4 query heads each: 64 sequences of 4,096 tokens 77 us (3.7 TB/s of
+//   codes, 57% of a copy's rate), 2 of 115,000 66 us (3.8 TB/s), 1 of 16,384 17 us, 1 of 1,030 6.9 us; of the first 4 to
+//   5 us are the join and both launches' ends.  D = 256: the first 134 us (4.1 TB/s).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -890,8 +891,8 @@ Shape shape_of(const Kv4View& c, const Kv4Attend& a) {
   const int64_t slots = sm_count() * resident_blocks(c.dim, s.tiles);
   s.blocks = std::max<int64_t>(1, std::min<int64_t>(slots, units));
   // Short contexts and few segments: a cluster to a segment, joined without a second kernel, where every block is
-  // resident at once and walks four tiles at most.  (One sequence of 1,030 tokens, 8 heads: 9.6 us on the line, 6.7 us so; eight of
-  // 2,048: 18.0 and 11.6 us.)
+  // resident at once and walks four tiles at most.  (One sequence of 1,030 tokens, 8 heads: 9.6 us on the line, 6.9 us so; eight of
+  // 2,048: 18.0 and 11.9 us.)
   const int64_t row_blocks = (rows + 8 * s.tiles - 1) / (8 * s.tiles), segments = row_blocks * a.batch * c.heads;
   int64_t seen = most;  // tokens of a segment, at most
   if (a.window > 0) seen = std::min<int64_t>(seen, static_cast<int64_t>(a.window) + a.max_rows + kStep);
@@ -974,8 +975,9 @@ void launch_typed(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStre
 // Which kernel: this file's takes a time in proportion to the row blocks of 16, kv4_chunk.cu's to the waves of blocks
 // of 256 rows over the SMs, whatever fills them.  Measured per 128 tokens: 6.6 ns a row block over the whole device,
 // 2.8 us a wave (2.2 us with 128 rows or fewer) and 20 us, which the factors of 440 and 350 spread over contexts of some
-// thousand tokens.  (4 sequences of 4,096 tokens, 8 heads: 63 and 87 us at 128 rows a head, 109 and 111 at 256; 32 of
-// 2,000: 71 and 93 at 32, 121 and 95 at 64.)
+// thousand tokens.  (4 sequences of 4,096 tokens, 8 heads: 63 and 81 us at 128 rows a head, 111 and 100 at 256; 32 of
+// 2,000: 73 and 93 at 32, 125 and 93 at 64.)  Rows are those announced, for every sequence: what the device arrays hold
+// is not known here, and a call that announces far more than there are gets the kernel for many.
 bool many_rows(const Kv4View& c, const Kv4Attend& a) {
   if (!kv4_chunk_supported(c) || a.engine == 1) return false;
   if (a.engine == 2) return true;

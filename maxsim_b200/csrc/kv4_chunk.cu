@@ -15,15 +15,18 @@
 //   columns, in blocks of 32 columns.  (With half the warps, a row to a thread: 206 us where this took 184.)
 //   Scales of keys and values are fp32 factors of scores and probabilities (they would lose digits in fp16 operands);
 //   the reference is the running maximum of s_j + log2(vs_j) (without vectors of zeros) as in kv4_attend.cu, set 2^2
-//   below it and moved (and the sums rescaled) only when some p vs would pass 60,000, which fp16 just holds, or p what keep_sums_finite allows.
+//   below it and moved (and the sums rescaled) only when some p vs would pass 60,000, which fp16 just holds, or p what
+//   keep_sums_finite allows (a test of the block's sums that costs 4 us of the 172 below: it waits for the exponentials).
 //   2^2 leaves the maximum 2^14 to grow before sums are read and rescaled; p vs below 2^-16 of the maximum are
 //   subnormal in fp16 then, each off by at most 2^-27 of the maximum.
 //   Two further warps issue the products, one for each row tile.
 //   Measured: 4 sequences of 1,500 to 4,096 tokens, the last 512 of each as rows, 32 heads (8 of the cache), D = 128:
-//   171 us with the host's call (183 before the scores were formed in halves, below).  A tile of 256 rows takes about
-//   5,000 cycles, of which the exponentials need 2,048 and the products as much: what bounds it is the softmax warps'
-//   chain of loads, conversions and stores, 1,000 cycles and more for 32 columns whatever waits beside it.  Half of the
-//   issue slots are used.  Reading the queries takes 8,000 cycles of a block and writing the rows 5,000.
+//   172 us on the device, 174 to 176 with the host's call (12 us more before the scores were formed in halves, below).  A
+//   tile of 256 rows takes about 5,000 cycles, of which the exponentials need 2,048 and the products as much: what bounds
+//   it is the softmax warps' chain of loads, conversions and stores, 1,000 cycles and more for 32 columns whatever waits
+//   beside it.  Half of the issue slots are used.  Reading the queries takes 8,000 cycles of a block and writing the rows
+//   5,000.  And the blocks' order: 256 of them start by row block, then by sequence, whatever their length.  Replayed on
+//   148 SMs from these cycles that ends after 153 to 156 us; longest first would end after 116, evenly spread after 105.
 // Every wait is bounded; a block that gives up writes NaN rows.
 #include <algorithm>
 #include <climits>

@@ -159,7 +159,8 @@ class Int4KVCache:
         query_offsets[b + 1]`` (int32 ``[batch + 1]``, at most ``max_query_tokens`` each), which are its last
         positions; without ``query_offsets`` each sequence has one row.  Rows before the first offset and past the last
         (padding) are zeros, rows past their sequence's ``max_query_tokens`` NaN; a given ``out`` keeps what it holds
-        in both (and their log-sum-exp is -inf).
+        in both (and their log-sum-exp is -inf).  ``max_query_tokens`` defaults to all rows, and the kernel is chosen for
+        as many in every sequence: give it where sequences share the rows.
 
         A row at position ``p`` sees tokens up to ``p`` (``causal``; otherwise all of its sequence), the last
         ``window`` of them where a window is given.  ``heads`` is a multiple of the cache's heads, consecutive
