@@ -440,7 +440,7 @@ def _plain_extend(state):
     fits = (want <= columns) & (end <= rows)
     grow = torch.where(fits, want - have, 0)
     upto = torch.cumsum(grow, 0)
-    served = fits & (upto <= count)
+    served = fits & ((grow == 0) | (upto <= count))  # one that lacks no page gets its rows all the same
     column = torch.arange(columns, device=device).unsqueeze(0)
     entered = served.unsqueeze(1) & (column >= have.unsqueeze(1)) & (column < want.unsqueeze(1))
     place = count.long() - 1 - ((upto - grow - have).unsqueeze(1) + column)
