@@ -357,6 +357,97 @@ int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args*
  * past max_query_rows of their sequence NaN (where batch is positive). */
 int msb_kv4_attend_fill_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream);
 
+/* What rows see beside their window, or in its place.
+ * sinks > 0 (needs a window): tokens below `sinks` stay visible, up to the row's own position.
+ * ancestors (needs causal and query_offsets): the sequence's rows are nodes of a tree of drafted tokens, cached as its
+ * last tokens in the rows' order.  Bit k % 64 of word k / 64 of a row: it sees row k of its sequence (itself among
+ * them; bits of rows that are not there count nothing).  Of what is cached before the sequence's rows it sees all, or,
+ * with a window, the last window - n tokens, n its bits, and the sinks. */
+typedef struct msb_kv4_attend_mask {
+  const int64_t* ancestors;   /* [rows, ancestor_words], rows ancestors_stride elements apart, or NULL */
+  int64_t ancestors_stride;
+  int32_t ancestor_words;
+  int32_t sinks;
+} msb_kv4_attend_mask;
+/* Attention with such a mask (NULL: none); `fill`: as msb_kv4_attend_fill_device. */
+int msb_kv4_attend_masked_workspace_bytes(const msb_kv4_cache* cache, const msb_kv4_attend_args* args,
+                                          const msb_kv4_attend_mask* mask, int64_t* bytes);
+int msb_kv4_attend_masked_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args,
+                                 const msb_kv4_attend_mask* mask, int32_t fill, void* stream);
+/* Masks and depths of the nodes of drafted trees: parents[i] of row i is a row of the same sequence with a lower place
+ * (counted from its first row); any other number: the context's last token.  ancestors [rows, words], words at least
+ * ceil(max_query_rows / 64): the row's path up, itself among it; depths [rows]: nodes above it.  max_query_rows at most
+ * 1024; rows past it of their sequence, and rows that no sequence owns, get 0. */
+int msb_draft_ancestors_device(const int32_t* parents, int64_t rows, const int32_t* query_offsets, int32_t batch,
+                               int32_t max_query_rows, int32_t words, int64_t* ancestors, int32_t* depths,
+                               int32_t device, void* stream);
+
+/* Copies cached vectors of source[i] to target[i], keys and values, codes and scales: as if every source were read
+ * before any target is written.  A pair with either slot outside the cache does nothing; a target given twice holds
+ * one of the two, possibly mixed.  Workspace: msb_kv4_move_workspace_bytes (0 up to 1,024 tokens), 16-byte aligned. */
+int msb_kv4_move_workspace_bytes(const msb_kv4_cache* cache, int64_t tokens, int64_t* bytes);
+int msb_kv4_move_device(const msb_kv4_cache* cache, const int64_t* source, const int64_t* target, int64_t tokens,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The pages of a batch of sequences: page_table [sequences, max_pages], lengths [sequences], a stack of free pages
+ * [num_pages] and the number of entries it has [1], all int32 on `device`, changed by the calls below. */
+typedef struct msb_page_table {
+  int32_t* page_table;
+  int32_t* lengths;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int64_t num_pages;
+  int32_t sequences;
+  int32_t max_pages;            /* times page_size at most 2^31 - 65536 */
+  int32_t page_size;            /* a power of two, 16 to 1024 */
+  int32_t device;
+} msb_page_table;
+/* For both calls; `rows` of the extend call (0: truncate).  16-byte aligned. */
+int msb_pages_workspace_bytes(const msb_page_table* table, int64_t rows, int64_t* bytes);
+/* Gives every sequence tokens[b] more tokens (a negative number: none): pages from the stack's top, in the sequences'
+ * order, entered in the table; lengths grow.  The rows of the step, `rows` of them, lie in the sequences' order:
+ * query_offsets [sequences + 1] their starts (held to `rows`), slots and positions [rows] where each is cached and its
+ * place in the sequence.  A sequence whose pages do not fit its table row, whose rows pass `rows`, or that lacks pages
+ * where those before it have taken what there is, is refused: it keeps its length, its rows, and those past the last,
+ * get -1. */
+int msb_pages_extend_device(const msb_page_table* table, const int32_t* tokens, int64_t rows, int32_t* query_offsets,
+                            int64_t* slots, int32_t* positions, void* workspace, int64_t workspace_bytes, void* stream);
+/* Shortens every sequence to lengths[b] (a longer one changes nothing, a negative one counts as 0): its pages past that
+ * go back to the stack, the first sequence's first one on top, and their entries become -1. */
+int msb_pages_truncate_device(const msb_page_table* table, const int32_t* lengths, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/* Rotary positions.  Of each vector of query [tokens, query_heads, head_dim] and keys the first 2 * pairs dimensions
+ * turn, the rest is copied: pair i by positions[axes[i]][token] * turns[i] * 2^-64 whole turns, (a, b) to
+ * (a cos - b sin, a sin + b cos), `inverse` the other way; its dimensions are i and pairs + i, or, `neighbours`, 2i and
+ * 2i + 1.  In place where an output is its input; no output may overlap an input otherwise. */
+typedef struct msb_rotary {
+  const uint64_t* turns;        /* [pairs], device */
+  const uint8_t* axes;          /* [pairs], device, each below the positions' axes */
+  int32_t pairs;                /* 2 * pairs at most head_dim */
+  int32_t head_dim;             /* at most 1024 */
+  int32_t neighbours;
+  int32_t device;
+} msb_rotary;
+typedef struct msb_rotate_args {
+  const void* x[2];             /* query, keys (NULL where it has no heads) */
+  void* y[2];
+  int64_t x_token_stride[2];    /* strides in elements, dimensions contiguous */
+  int64_t x_head_stride[2];
+  int64_t y_token_stride[2];
+  int64_t y_head_stride[2];
+  const void* positions;        /* [axes, tokens], int32 or int64 */
+  int64_t position_axis_stride;
+  int64_t position_token_stride;
+  int64_t tokens;
+  int32_t heads[2];
+  int32_t wide_positions;       /* int64 */
+  int32_t inverse;
+  int32_t type;
+  int32_t reserved;
+} msb_rotate_args;
+int msb_rotate_device(const msb_rotary* rotary, const msb_rotate_args* args, void* stream);
+
 /* Weights [n, k] as int4 codes [n, k / 2] with one bfloat16 scale per row and
  * `group` (32, 64 or 128) inputs, [n, ceil(k / group)]; k a multiple of 8.
  * msb_w4_pack_device lays them out once for the product kernel, into buffers

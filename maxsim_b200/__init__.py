@@ -5,7 +5,8 @@ Drop-in for the reference ``maxsim`` package's GPU path: the same public names
 ``to_device``, ``score``, ``maxsim``, ``topk_maxsim``, the residual cascade
 API) over ``libmaxsim_b200.so``; beside it, for a reader model that answers
 from what was retrieved, a key/value cache in the same 4-bit codes
-(``Int4KVCache``) and products with 4-bit weights (``Int4Linear``).
+(``Int4KVCache``, ``PageTable``, ``draft_ancestors``), rotary positions
+(``Rotary``) and products with 4-bit weights (``Int4Linear``).
 ``maxsim_b200._maxsim_cuda`` reproduces the reference's native extension module
 and can be installed as ``maxsim._maxsim_cuda``.
 
@@ -45,7 +46,7 @@ from maxsim_b200.experimental import (
 )
 from maxsim_b200.sdk import MODE_PRESETS, Corpus, CorpusMemoryReport, Index, Reranker, SearchResult
 from maxsim_b200.loader import load_reranker, load_resident_corpus
-from maxsim_b200.generation import Int4KVCache, Int4Linear
+from maxsim_b200.generation import Int4KVCache, Int4Linear, PageTable, Rotary, draft_ancestors
 
 __all__ = [
     "PackedDocs",
@@ -89,4 +90,7 @@ __all__ = [
     "binary_cascade_topk",
     "Int4KVCache",
     "Int4Linear",
+    "PageTable",
+    "Rotary",
+    "draft_ancestors",
 ]

@@ -109,6 +109,60 @@ class Kv4AttendArgs(ctypes.Structure):
     ]
 
 
+class Kv4AttendMask(ctypes.Structure):
+    _fields_ = [
+        ("ancestors", ctypes.c_void_p),
+        ("ancestors_stride", ctypes.c_int64),
+        ("ancestor_words", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+    ]
+
+
+class PageTableArrays(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("sequences", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+    ]
+
+
+class RotaryTable(ctypes.Structure):
+    _fields_ = [
+        ("turns", ctypes.c_void_p),
+        ("axes", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("neighbours", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+    ]
+
+
+class RotateArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p * 2),
+        ("y", ctypes.c_void_p * 2),
+        ("x_token_stride", ctypes.c_int64 * 2),
+        ("x_head_stride", ctypes.c_int64 * 2),
+        ("y_token_stride", ctypes.c_int64 * 2),
+        ("y_head_stride", ctypes.c_int64 * 2),
+        ("positions", ctypes.c_void_p),
+        ("position_axis_stride", ctypes.c_int64),
+        ("position_token_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int32 * 2),
+        ("wide_positions", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
@@ -157,6 +211,17 @@ SIGNATURES = {
                                                       ctypes.POINTER(_i64)]),
     "msb_kv4_attend_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs), _vp]),
     "msb_kv4_attend_fill_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs), _vp]),
+    "msb_kv4_attend_masked_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs),
+                                                             ctypes.POINTER(Kv4AttendMask), ctypes.POINTER(_i64)]),
+    "msb_kv4_attend_masked_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttendArgs),
+                                                    ctypes.POINTER(Kv4AttendMask), _i32, _vp]),
+    "msb_draft_ancestors_device": (ctypes.c_int, [_vp, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "msb_kv4_move_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), _i64, ctypes.POINTER(_i64)]),
+    "msb_kv4_move_device": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), _vp, _vp, _i64, _vp, _i64, _vp]),
+    "msb_pages_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(PageTableArrays), _i64, ctypes.POINTER(_i64)]),
+    "msb_pages_extend_device": (ctypes.c_int, [ctypes.POINTER(PageTableArrays), _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "msb_pages_truncate_device": (ctypes.c_int, [ctypes.POINTER(PageTableArrays), _vp, _vp, _i64, _vp]),
+    "msb_rotate_device": (ctypes.c_int, [ctypes.POINTER(RotaryTable), ctypes.POINTER(RotateArgs), _vp]),
     "msb_w4_packed_bytes": (ctypes.c_int, [_i64, _i64, _i32, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
     "msb_w4_pack_device": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "msb_w4_product_device": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32,

@@ -14,7 +14,9 @@
 
 #include "../../include/maxsim_b200.h"
 #include "common.cuh"
+#include "pages.cuh"
 #include "quant4.cuh"
+#include "rotary.cuh"
 
 namespace msb {
 void launch_simt_scan(const DocsView&, const QueryView&, const ReduceView&, const TargetsView&, bool, float*,
@@ -50,6 +52,13 @@ void launch_expand_codes16(const uint8_t* codes, int64_t num_tokens, uint16_t* o
 void launch_kv4_append(const Kv4View&, const Kv4Append&, cudaStream_t);
 void launch_kv4_read(const Kv4View&, const Kv4Read&, cudaStream_t);
 size_t kv4_attend_workspace_bytes(const Kv4View&, const Kv4Attend&);
+size_t kv4_move_workspace_bytes(const Kv4View&, int64_t);
+void launch_kv4_move(const Kv4View&, const Kv4Move&, cudaStream_t);
+size_t pages_workspace_bytes(const Pages&, int64_t);
+void launch_pages_extend(const Pages&, const PagesExtend&, cudaStream_t);
+void launch_pages_truncate(const Pages&, const int32_t*, void*, cudaStream_t);
+void launch_draft_ancestors(const DraftTrees&, cudaStream_t);
+void launch_rotate(const Rotate&, cudaStream_t);
 void launch_kv4_attend(const Kv4View&, const Kv4Attend&, cudaStream_t);
 void launch_w4_pack(const uint8_t*, const uint16_t*, int64_t, int64_t, int, uint8_t*, uint16_t*, cudaStream_t);
 void launch_w4_product(const W4View&, const W4Product&, cudaStream_t);
@@ -1517,7 +1526,7 @@ void check_tokens(int64_t tokens, const Kv4View& v) {
   if (tokens > ((int64_t{1} << 31) - 1) / v.heads) throw InvalidArgument("tokens * kv_heads must be below 2^31");
 }
 
-Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
+Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a, const msb_kv4_attend_mask* mask = nullptr) {
   if (!a) throw InvalidArgument("arguments are NULL");
   if (a->rows < 0 || a->batch < 0 || a->max_pages < 0 || a->max_query_rows < 0)
     throw InvalidArgument("sizes must not be negative");
@@ -1555,13 +1564,31 @@ Kv4Attend kv4_attend(const Kv4View& c, const msb_kv4_attend_args* a) {
   r.engine = g_kv4_engine.load();
   r.workspace = a->workspace;
   r.workspace_bytes = a->workspace_bytes > 0 ? static_cast<size_t>(a->workspace_bytes) : 0;
+  if (mask) {
+    if (mask->sinks < 0) throw InvalidArgument("sinks must not be negative");
+    if (mask->sinks > 0 && a->window == 0) throw InvalidArgument("sinks need a window");
+    r.sinks = std::min(mask->sinks, 1 << 30);  // the kernels round it up, in 32 bits
+    if (static_cast<int64_t>(r.sinks) >= static_cast<int64_t>(a->max_pages) << c.page_shift)  // no more than there are
+      r.sinks = static_cast<int>(static_cast<int64_t>(a->max_pages) << c.page_shift);
+    if (mask->ancestors) {
+      if (!a->causal || !a->query_offsets) throw InvalidArgument("ancestors need causal and query_offsets");
+      if (mask->ancestor_words < 1) throw InvalidArgument("ancestor_words must be positive");
+      if (mask->ancestor_words > 1 << 24) throw InvalidArgument("ancestor_words must be at most 2^24");
+      if (a->rows > (int64_t{1} << 31) - 65536) throw InvalidArgument("rows must be at most 2^31 - 65536 with ancestors");
+      check_address(mask->ancestors, 8, "ancestors");
+      r.ancestors = mask->ancestors;
+      r.ancestors_stride = mask->ancestors_stride;
+      r.words = mask->ancestor_words;
+    }
+  }
   return r;
 }
 
-int attend(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, bool fill, void* stream) {
+int attend(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, const msb_kv4_attend_mask* mask, bool fill,
+           void* stream) {
   return guarded([&] {
     const Kv4View v = kv4_view(cache);
-    Kv4Attend a = kv4_attend(v, args);
+    Kv4Attend a = kv4_attend(v, args, mask);
     a.fill = fill && a.offsets;  // without offsets every row is a sequence's
     if (a.rows == 0 || a.batch == 0) return;
     if (!a.query || !a.lengths || !a.out || (a.max_pages > 0 && !a.page_table)) throw InvalidArgument("NULL argument");
@@ -1577,6 +1604,29 @@ int attend(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, bool fil
     if (a.workspace_bytes < kv4_attend_workspace_bytes(v, a)) throw InvalidArgument("workspace is too small");
     launch_kv4_attend(v, a, static_cast<cudaStream_t>(stream));
   });
+}
+
+Pages pages_of(const msb_page_table* t) {
+  if (!t) throw InvalidArgument("page table is NULL");
+  if (!t->page_table || !t->lengths || !t->free_pages || !t->free_count) throw InvalidArgument("a page table array is NULL");
+  check_address(t->page_table, 4, "page_table");
+  check_address(t->lengths, 4, "lengths");
+  check_address(t->free_pages, 4, "free_pages");
+  check_address(t->free_count, 4, "free_count");
+  if (t->num_pages < 1 || t->num_pages > (int64_t{1} << 31) - 1) throw InvalidArgument("num_pages must be from 1 to 2^31 - 1");
+  if (t->sequences < 1 || t->max_pages < 1) throw InvalidArgument("sequences and max_pages must be positive");
+  if (t->page_size < 16 || t->page_size > 1024 || (t->page_size & (t->page_size - 1)))
+    throw InvalidArgument("page_size must be a power of two from 16 to 1024");
+  Pages p{t->page_table, t->lengths, t->free_pages, t->free_count, t->num_pages, t->sequences, t->max_pages, 4};
+  while ((1 << p.page_shift) < t->page_size) ++p.page_shift;
+  if ((static_cast<int64_t>(p.max_pages) << p.page_shift) > (int64_t{1} << 31) - 65536)
+    throw InvalidArgument("max_pages * page_size must be at most 2^31 - 65536");
+  return p;
+}
+void check_pages_workspace(const Pages& p, int64_t rows, const void* workspace, int64_t bytes) {
+  check_address(workspace, 16, "workspace");
+  if (!workspace && bytes > 0) throw InvalidArgument("workspace is NULL");
+  if (bytes < static_cast<int64_t>(pages_workspace_bytes(p, rows))) throw InvalidArgument("workspace is too small");
 }
 
 void check_w4(int64_t n, int64_t k, int32_t group) {
@@ -1646,11 +1696,156 @@ int msb_kv4_attend_workspace_bytes(const msb_kv4_cache* cache, const msb_kv4_att
 }
 
 int msb_kv4_attend_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream) {
-  return attend(cache, args, false, stream);
+  return attend(cache, args, nullptr, false, stream);
 }
 
 int msb_kv4_attend_fill_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args, void* stream) {
-  return attend(cache, args, true, stream);
+  return attend(cache, args, nullptr, true, stream);
+}
+
+int msb_kv4_attend_masked_workspace_bytes(const msb_kv4_cache* cache, const msb_kv4_attend_args* args,
+                                          const msb_kv4_attend_mask* mask, int64_t* bytes) {
+  return guarded([&] {
+    if (!bytes) throw InvalidArgument("NULL argument");
+    const Kv4View v = kv4_view(cache);
+    DeviceGuard g(cache->device);
+    *bytes = static_cast<int64_t>(kv4_attend_workspace_bytes(v, kv4_attend(v, args, mask)));
+  });
+}
+
+int msb_kv4_attend_masked_device(const msb_kv4_cache* cache, const msb_kv4_attend_args* args,
+                                 const msb_kv4_attend_mask* mask, int32_t fill, void* stream) {
+  return attend(cache, args, mask, fill != 0, stream);
+}
+
+int msb_draft_ancestors_device(const int32_t* parents, int64_t rows, const int32_t* query_offsets, int32_t batch,
+                               int32_t max_query_rows, int32_t words, int64_t* ancestors, int32_t* depths,
+                               int32_t device, void* stream) {
+  return guarded([&] {
+    if (rows < 0 || batch < 0 || max_query_rows < 0) throw InvalidArgument("sizes must not be negative");
+    if (rows > (int64_t{1} << 31) - 1) throw InvalidArgument("rows must be below 2^31");
+    if (max_query_rows > kMostTreeRows) throw InvalidArgument("max_query_rows must be at most 1024");
+    if (words < 1 || words < (max_query_rows + 63) / 64) throw InvalidArgument("words must be at least ceil(max_query_rows / 64)");
+    if (words > 1 << 24) throw InvalidArgument("words must be at most 2^24");
+    if (rows == 0 || batch == 0) return;
+    if (!parents || !query_offsets || !ancestors || !depths) throw InvalidArgument("NULL argument");
+    check_address(parents, 4, "parents");
+    check_address(query_offsets, 4, "query_offsets");
+    check_address(ancestors, 8, "ancestors");
+    check_address(depths, 4, "depths");
+    DraftTrees t{parents, query_offsets, rows, ancestors, depths, batch, max_query_rows, words};
+    DeviceGuard g(device);
+    launch_draft_ancestors(t, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_kv4_move_workspace_bytes(const msb_kv4_cache* cache, int64_t tokens, int64_t* bytes) {
+  return guarded([&] {
+    if (!bytes) throw InvalidArgument("NULL argument");
+    const Kv4View v = kv4_view(cache);
+    check_tokens(tokens, v);
+    *bytes = static_cast<int64_t>(kv4_move_workspace_bytes(v, tokens));
+  });
+}
+
+int msb_kv4_move_device(const msb_kv4_cache* cache, const int64_t* source, const int64_t* target, int64_t tokens,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const Kv4View v = kv4_view(cache);
+    check_tokens(tokens, v);
+    if (tokens == 0) return;
+    if (!source || !target) throw InvalidArgument("NULL argument");
+    check_address(source, 8, "source");
+    check_address(target, 8, "target");
+    check_address(workspace, 16, "workspace");
+    if (!workspace && workspace_bytes > 0) throw InvalidArgument("workspace is NULL");
+    if (workspace_bytes < static_cast<int64_t>(kv4_move_workspace_bytes(v, tokens))) throw InvalidArgument("workspace is too small");
+    DeviceGuard g(cache->device);
+    launch_kv4_move(v, Kv4Move{source, target, tokens, workspace}, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_pages_workspace_bytes(const msb_page_table* table, int64_t rows, int64_t* bytes) {
+  return guarded([&] {
+    if (!bytes) throw InvalidArgument("NULL argument");
+    *bytes = static_cast<int64_t>(pages_workspace_bytes(pages_of(table), rows));
+  });
+}
+
+int msb_pages_extend_device(const msb_page_table* table, const int32_t* tokens, int64_t rows, int32_t* query_offsets,
+                            int64_t* slots, int32_t* positions, void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const Pages p = pages_of(table);
+    if (rows < 0 || rows > (int64_t{1} << 31) - 1) throw InvalidArgument("rows must be from 0 to 2^31 - 1");
+    if (!tokens || !query_offsets || (rows > 0 && (!slots || !positions))) throw InvalidArgument("NULL argument");
+    check_address(tokens, 4, "tokens");
+    check_address(query_offsets, 4, "query_offsets");
+    check_address(slots, 8, "slots");
+    check_address(positions, 4, "positions");
+    check_pages_workspace(p, rows, workspace, workspace_bytes);
+    DeviceGuard g(table->device);
+    launch_pages_extend(p, PagesExtend{tokens, rows, query_offsets, slots, positions, workspace},
+                        static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_pages_truncate_device(const msb_page_table* table, const int32_t* lengths, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const Pages p = pages_of(table);
+    if (!lengths) throw InvalidArgument("NULL argument");
+    check_address(lengths, 4, "lengths");
+    check_pages_workspace(p, 0, workspace, workspace_bytes);
+    DeviceGuard g(table->device);
+    launch_pages_truncate(p, lengths, workspace, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int msb_rotate_device(const msb_rotary* rotary, const msb_rotate_args* args, void* stream) {
+  return guarded([&] {
+    if (!rotary || !args) throw InvalidArgument("NULL argument");
+    if (rotary->head_dim < 1 || rotary->head_dim > 1024) throw InvalidArgument("head_dim must be from 1 to 1024");
+    if (rotary->pairs < 1 || rotary->pairs > rotary->head_dim / 2)
+      throw InvalidArgument("pairs must be positive, and 2 * pairs at most head_dim");
+    if (!rotary->turns || !rotary->axes) throw InvalidArgument("NULL argument");
+    check_address(rotary->turns, 8, "turns");
+    Rotate r{};
+    r.type = element_type(args->type, true);
+    const uintptr_t bytes = r.type == kElemF32 ? 4 : 2;
+    if (args->tokens < 0) throw InvalidArgument("tokens must not be negative");
+    if (args->tokens > (int64_t{1} << 31) - 1) throw InvalidArgument("tokens must be below 2^31");
+    for (int w = 0; w < 2; ++w) {
+      if (args->heads[w] < 0 || args->heads[w] > 65535) throw InvalidArgument("heads must be from 0 to 65535");
+      r.heads[w] = args->heads[w];
+      r.x[w] = args->x[w];
+      r.y[w] = args->y[w];
+      r.x_token[w] = args->x_token_stride[w];
+      r.x_head[w] = args->x_head_stride[w];
+      r.y_token[w] = args->y_token_stride[w];
+      r.y_head[w] = args->y_head_stride[w];
+    }
+    if (args->tokens == 0 || r.heads[0] + r.heads[1] == 0) return;
+    for (int w = 0; w < 2; ++w) {
+      if (r.heads[w] > 0 && (!r.x[w] || !r.y[w])) throw InvalidArgument("NULL argument");
+      check_address(r.x[w], bytes, "query and keys");
+      check_address(r.y[w], bytes, "outputs");
+    }
+    if (!args->positions) throw InvalidArgument("NULL argument");
+    check_address(args->positions, args->wide_positions ? 8 : 4, "positions");
+    r.dim = rotary->head_dim;
+    r.half = rotary->pairs;
+    r.turns = rotary->turns;
+    r.axis = rotary->axes;
+    r.positions = args->positions;
+    r.position_axis = args->position_axis_stride;
+    r.position_token = args->position_token_stride;
+    r.wide = args->wide_positions != 0;
+    r.tokens = args->tokens;
+    r.neighbours = rotary->neighbours != 0;
+    r.inverse = args->inverse != 0;
+    DeviceGuard g(rotary->device);
+    launch_rotate(r, static_cast<cudaStream_t>(stream));
+  });
 }
 
 int msb_w4_packed_bytes(int64_t n, int64_t k, int32_t group, int64_t* code_bytes, int64_t* scale_bytes) {

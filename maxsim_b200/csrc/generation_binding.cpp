@@ -1,4 +1,4 @@
-// Python entry of the 4-bit cache's and the 4-bit weights' operators (maxsim_b200/generation.py): checks tensors,
+// Python entry of the operators of a reader model (maxsim_b200/generation.py): checks tensors,
 // allocates outputs and workspaces through torch, calls the C ABI on torch's current stream.
 //
 // A decode step calls these a few times per layer with kernels of 3 to 10 us, so the host's part decides: reading
@@ -100,6 +100,14 @@ void no_overlap(const at::Tensor& out, const char* name, const at::Tensor& in, c
     }
 }
 
+PyObject* pair_of(at::Tensor first, at::Tensor second) {
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) throw PythonError{};
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(first)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(second)));
+  return pair;
+}
+
 const msb_kv4_cache* cache_of(PyObject* o) {
   void* p = PyLong_AsVoidPtr(o);
   if (PyErr_Occurred()) throw PythonError{};
@@ -112,10 +120,10 @@ int64_t integer(PyObject* o) {
   return v;
 }
 
-at::Tensor slots_of(PyObject* o, c10::Device device) {
-  const at::Tensor& t = tensor(o, "slots", device);
-  want_dtype(t, "slots", c10::kLong);
-  want_dim(t, "slots", 1);
+at::Tensor slots_of(PyObject* o, c10::Device device, const char* name = "slots") {
+  const at::Tensor& t = tensor(o, name, device);
+  want_dtype(t, name, c10::kLong);
+  want_dim(t, name, 1);
   return t.contiguous();
 }
 at::Tensor vectors_of(PyObject* o, const char* name, const msb_kv4_cache* c, c10::Device device, int64_t tokens) {
@@ -184,15 +192,29 @@ PyObject* read(PyObject* const* args, Py_ssize_t n) {
   }
   check_status(msb_kv4_read_device(c, slots.const_data_ptr<int64_t>(), shape[0], type_id(type, true),
                                    out[0].mutable_data_ptr(), out[1].mutable_data_ptr(), stream_of(device)));
-  PyObject* pair = PyTuple_New(2);
-  if (!pair) throw PythonError{};
-  for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(std::move(out[i])));
-  return pair;
+  return pair_of(std::move(out[0]), std::move(out[1]));
 }
 
-// attend(cache, query, page_table, lengths, query_offsets, max_query_tokens, scale, causal, window, return_lse, out)
+// move(cache, source, target)
+PyObject* move(PyObject* const* args, Py_ssize_t n) {
+  if (n != 3) throw TypeError{"move takes 3 arguments"};
+  const msb_kv4_cache* c = cache_of(args[0]);
+  const c10::Device device = device_of(c->device);
+  const at::Tensor source = slots_of(args[1], device, "source"), target = slots_of(args[2], device, "target");
+  if (source.size(0) != target.size(0)) refuse("source and target must have the same number of tokens");
+  int64_t need = 0;
+  check_status(msb_kv4_move_workspace_bytes(c, source.size(0), &need));
+  at::Tensor workspace;
+  if (need > 0) workspace = empty({need}, c10::kByte, device);
+  check_status(msb_kv4_move_device(c, source.const_data_ptr<int64_t>(), target.const_data_ptr<int64_t>(), source.size(0),
+                                   need > 0 ? workspace.mutable_data_ptr() : nullptr, need, stream_of(device)));
+  Py_RETURN_NONE;
+}
+
+// attend(cache, query, page_table, lengths, query_offsets, max_query_tokens, scale, causal, window, sinks, ancestors,
+//        return_lse, out)
 PyObject* attend(PyObject* const* args, Py_ssize_t n) {
-  if (n != 11) throw TypeError{"attend takes 11 arguments"};
+  if (n != 13) throw TypeError{"attend takes 13 arguments"};
   const msb_kv4_cache* c = cache_of(args[0]);
   const c10::Device device = device_of(c->device);
   msb_kv4_attend_args a{};
@@ -232,7 +254,7 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
     if (most == 0 && rows > 0) refuse("max_query_tokens must be positive where there are rows");
     most = std::min(most, rows);  // a sequence has no more rows than there are
   }
-  const int causal = PyObject_IsTrue(args[7]), return_lse = PyObject_IsTrue(args[9]);
+  const int causal = PyObject_IsTrue(args[7]), return_lse = PyObject_IsTrue(args[11]);
   if (causal < 0 || return_lse < 0) throw PythonError{};
   int64_t window = 0;
   if (args[8] != Py_None) {
@@ -240,6 +262,26 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
     if (window < 1 || !causal) refuse("window must be at least 1 and needs causal");
     window = std::min<int64_t>(window, INT32_MAX);
   }
+  msb_kv4_attend_mask mask{};
+  const int64_t sinks = integer(args[9]);
+  if (sinks < 0) refuse("sinks must not be negative");
+  if (sinks > 0 && window == 0) refuse("sinks need a window");
+  mask.sinks = static_cast<int32_t>(std::min<int64_t>(sinks, INT32_MAX));
+  at::Tensor ancestors;
+  if (args[10] != Py_None) {
+    const at::Tensor& t = tensor(args[10], "ancestors", device);
+    want_dtype(t, "ancestors", c10::kLong);
+    want_dim(t, "ancestors", 2);
+    if (t.size(0) != rows || t.size(1) < 1)
+      refuse("ancestors must have shape [" + std::to_string(rows) + ", words], got " + text(t.sizes()));
+    if (t.size(1) > (1 << 24)) refuse("ancestors must have at most 2^24 words");
+    if (!causal || args[4] == Py_None) refuse("ancestors need causal and query_offsets");
+    ancestors = t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t;
+    mask.ancestors = ancestors.const_data_ptr<int64_t>();
+    mask.ancestors_stride = ancestors.stride(0);
+    mask.ancestor_words = static_cast<int32_t>(ancestors.size(1));
+  }
+  const bool masked = mask.sinks > 0 || ancestors.defined();
   double scale = 1.0 / std::sqrt(static_cast<double>(dim));
   if (args[6] != Py_None) {
     scale = PyFloat_AsDouble(args[6]);
@@ -248,14 +290,15 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
   if (!(static_cast<float>(scale) > 0.0F) || !std::isfinite(static_cast<float>(scale))) refuse("scale must be finite and > 0");
   at::Tensor out;
   const int64_t shape[3] = {rows, heads, dim};
-  if (args[10] == Py_None) {
+  if (args[12] == Py_None) {
     out = empty(shape, query.scalar_type(), device);
   } else {
-    out = tensor(args[10], "out", device);
+    out = tensor(args[12], "out", device);
     want_dtype(out, "out", query.scalar_type());
     if (!out.sizes().equals(shape) || !out.is_contiguous()) refuse("out must be contiguous with shape " + text(shape));
     no_gradient(out, "out");
     no_overlap(out, "out", query, "query", true);
+    if (ancestors.defined()) no_overlap(out, "out", ancestors, "ancestors", false);
   }
   at::Tensor lse;
   if (return_lse) lse = empty({rows, heads}, c10::kFloat, device);
@@ -277,7 +320,7 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
   a.window = static_cast<int32_t>(window);
   a.scale = static_cast<float>(scale);
   int64_t need = 0;
-  check_status(msb_kv4_attend_workspace_bytes(c, &a, &need));
+  check_status(masked ? msb_kv4_attend_masked_workspace_bytes(c, &a, &mask, &need) : msb_kv4_attend_workspace_bytes(c, &a, &need));
   at::Tensor workspace;
   if (need > 0) {
     workspace = empty({need}, c10::kByte, device);
@@ -285,15 +328,250 @@ PyObject* attend(PyObject* const* args, Py_ssize_t n) {
     a.workspace_bytes = need;
   }
   // Outputs made here are fresh memory: rows that the call does not work on are filled, by the kernel where both are.
-  const bool fresh = args[10] == Py_None;
+  const bool fresh = args[12] == Py_None;
   if (fresh && batch == 0) out.zero_();
   if (return_lse && a.query_offsets && (!fresh || batch == 0)) lse.fill_(-INFINITY);
-  check_status((fresh ? msb_kv4_attend_fill_device : msb_kv4_attend_device)(c, &a, stream_of(device)));
+  check_status(masked ? msb_kv4_attend_masked_device(c, &a, &mask, fresh, stream_of(device))
+                      : (fresh ? msb_kv4_attend_fill_device : msb_kv4_attend_device)(c, &a, stream_of(device)));
   if (!return_lse) return THPVariable_Wrap(std::move(out));
+  return pair_of(std::move(out), std::move(lse));
+}
+
+// draft_ancestors(parents, query_offsets, max_query_tokens or None) -> (ancestors, depths)
+PyObject* draft_ancestors(PyObject* const* args, Py_ssize_t n) {
+  if (n != 3) throw TypeError{"draft_ancestors takes 3 arguments"};
+  if (!THPVariable_Check(args[0])) throw TypeError{"parents must be a torch tensor"};
+  const at::Tensor& given = THPVariable_Unpack(args[0]);
+  const c10::Device device = given.device();
+  if (device.type() != c10::kCUDA) refuse("parents must be on a CUDA device, got " + device.str());
+  want_dtype(given, "parents", c10::kInt);
+  want_dim(given, "parents", 1);
+  const at::Tensor& starts = tensor(args[1], "query_offsets", device);
+  want_dtype(starts, "query_offsets", c10::kInt);
+  want_dim(starts, "query_offsets", 1);
+  if (starts.size(0) < 1) refuse("query_offsets must have shape [batch + 1]");
+  const int64_t rows = given.size(0), batch = starts.size(0) - 1;
+  if (batch > INT32_MAX) refuse("sizes must be below 2^31");
+  int64_t most = args[2] == Py_None ? rows : integer(args[2]);
+  if (most < 0) refuse("max_query_tokens must not be negative");
+  most = std::min(most, rows);
+  if (most > 1024) refuse("a sequence's tree has at most 1024 rows: give max_query_tokens where sequences share the rows");
+  const int64_t words = std::max<int64_t>(1, (most + 63) / 64);
+  const at::Tensor parents = given.contiguous(), offsets = starts.contiguous();
+  at::Tensor ancestors = empty({rows, words}, c10::kLong, device), depths = empty({rows}, c10::kInt, device);
+  if (batch == 0) {
+    ancestors.zero_();
+    depths.zero_();
+  }
+  check_status(msb_draft_ancestors_device(parents.const_data_ptr<int32_t>(), rows, offsets.const_data_ptr<int32_t>(),
+                                          static_cast<int32_t>(batch), static_cast<int32_t>(most),
+                                          static_cast<int32_t>(words), ancestors.mutable_data_ptr<int64_t>(),
+                                          depths.mutable_data_ptr<int32_t>(), device.index(), stream_of(device)));
+  return pair_of(std::move(ancestors), std::move(depths));
+}
+
+const msb_page_table* pages_of(PyObject* o) {
+  void* p = PyLong_AsVoidPtr(o);
+  if (PyErr_Occurred()) throw PythonError{};
+  return static_cast<const msb_page_table*>(p);
+}
+// int32 [sequences], apart from what the call writes (its own lengths themselves are fine: each is read first).
+at::Tensor per_sequence(PyObject* o, const char* name, const msb_page_table* t, c10::Device device) {
+  const at::Tensor& x = tensor(o, name, device);
+  want_dtype(x, name, c10::kInt);
+  if (x.dim() != 1 || x.size(0) != t->sequences)
+    refuse(std::string(name) + " must have shape [" + std::to_string(t->sequences) + "], got " + text(x.sizes()));
+  const at::Tensor r = x.contiguous();
+  const char* const p = static_cast<const char*>(r.const_data_ptr());
+  const auto meets = [&](const int32_t* q, int64_t count) {
+    const char* const c = reinterpret_cast<const char*>(q);
+    return p < c + 4 * count && c < p + 4 * static_cast<int64_t>(t->sequences);
+  };
+  if (meets(t->page_table, static_cast<int64_t>(t->sequences) * t->max_pages) || meets(t->free_pages, t->num_pages) ||
+      meets(t->free_count, 1) || (r.const_data_ptr() != t->lengths && meets(t->lengths, t->sequences)))
+    refuse(std::string(name) + " must not overlap the page table's arrays");
+  return r;
+}
+at::Tensor pages_workspace(const msb_page_table* t, int64_t rows, c10::Device device, int64_t& need) {
+  check_status(msb_pages_workspace_bytes(t, rows, &need));
+  at::Tensor workspace;
+  if (need > 0) workspace = empty({need}, c10::kByte, device);
+  return workspace;
+}
+
+// extend(table, tokens, rows) -> (query_offsets, slots, positions)
+PyObject* extend(PyObject* const* args, Py_ssize_t n) {
+  if (n != 3) throw TypeError{"extend takes 3 arguments"};
+  const msb_page_table* t = pages_of(args[0]);
+  const c10::Device device = device_of(t->device);
+  const at::Tensor tokens = per_sequence(args[1], "tokens", t, device);
+  const int64_t rows = integer(args[2]);
+  if (rows < 0 || rows > INT32_MAX) refuse("rows must be from 0 to 2^31 - 1");
+  at::Tensor offsets = empty({static_cast<int64_t>(t->sequences) + 1}, c10::kInt, device);
+  at::Tensor slots = empty({rows}, c10::kLong, device), positions = empty({rows}, c10::kInt, device);
+  int64_t need = 0;
+  at::Tensor workspace = pages_workspace(t, rows, device, need);
+  check_status(msb_pages_extend_device(t, tokens.const_data_ptr<int32_t>(), rows, offsets.mutable_data_ptr<int32_t>(),
+                                       slots.mutable_data_ptr<int64_t>(), positions.mutable_data_ptr<int32_t>(),
+                                       need > 0 ? workspace.mutable_data_ptr() : nullptr, need, stream_of(device)));
+  PyObject* triple = PyTuple_New(3);
+  if (!triple) throw PythonError{};
+  PyTuple_SET_ITEM(triple, 0, THPVariable_Wrap(std::move(offsets)));
+  PyTuple_SET_ITEM(triple, 1, THPVariable_Wrap(std::move(slots)));
+  PyTuple_SET_ITEM(triple, 2, THPVariable_Wrap(std::move(positions)));
+  return triple;
+}
+
+// truncate(table, lengths)
+PyObject* truncate(PyObject* const* args, Py_ssize_t n) {
+  if (n != 2) throw TypeError{"truncate takes 2 arguments"};
+  const msb_page_table* t = pages_of(args[0]);
+  const c10::Device device = device_of(t->device);
+  const at::Tensor lengths = per_sequence(args[1], "lengths", t, device);
+  int64_t need = 0;
+  at::Tensor workspace = pages_workspace(t, 0, device, need);
+  check_status(msb_pages_truncate_device(t, lengths.const_data_ptr<int32_t>(),
+                                         need > 0 ? workspace.mutable_data_ptr() : nullptr, need, stream_of(device)));
+  Py_RETURN_NONE;
+}
+
+// What Rotary keeps (mirrored in generation.py).
+struct RotaryHandle {
+  msb_rotary table;
+  int32_t axes;
+};
+// Vectors of a rotary call: [tokens, heads, dim] with the last dimension contiguous, in bytes.
+struct Vectors {
+  const char* at;
+  int64_t tokens, heads, token, head, width;
+};
+Vectors vectors(const at::Tensor& t) {
+  const int64_t size = t.element_size();
+  return {static_cast<const char*>(t.const_data_ptr()), t.size(0), t.size(1), t.size(0) > 1 ? t.stride(0) * size : 0,
+          t.size(1) > 1 ? t.stride(1) * size : 0, t.size(2) * size};
+}
+int64_t span(const Vectors& v) { return (v.tokens - 1) * v.token + (v.heads - 1) * v.head + v.width; }
+// Whether [a, a + na) and [b, b + nb), repeated every `period` bytes, stay apart.
+bool apart_every(int64_t period, int64_t from_a_to_b, int64_t na, int64_t nb) {
+  if (period <= 0) return false;
+  const int64_t d = ((from_a_to_b % period) + period) % period;
+  return d >= na && d + nb <= period;
+}
+// Whether two sets of vectors are seen to lie apart: by their spans, or as parts of rows (or of heads) of one array.
+bool apart(const Vectors& a, const Vectors& b) {
+  if (a.at + span(a) <= b.at || b.at + span(b) <= a.at) return true;
+  const int64_t d = b.at - a.at;
+  const auto inner = [](const Vectors& v, bool tokens) {
+    return tokens ? (v.heads - 1) * v.head + v.width : (v.tokens - 1) * v.token + v.width;
+  };
+  if (a.token == b.token && apart_every(a.token, d, inner(a, true), inner(b, true))) return true;
+  if (a.head == b.head && apart_every(a.head, d, inner(a, false), inner(b, false))) return true;
+  // Both strides alike, one a multiple of the other: parts of the same vectors.
+  const int64_t lo = std::min(a.token, a.head), hi = std::max(a.token, a.head);
+  return a.token == b.token && a.head == b.head && lo > 0 && hi % lo == 0 && apart_every(lo, d, a.width, b.width);
+}
+bool written_once(const Vectors& v) {
+  const bool tokens_in = v.token < v.head;
+  const int64_t in = tokens_in ? v.token : v.head, n = tokens_in ? v.tokens : v.heads;
+  const int64_t out = tokens_in ? v.head : v.token, m = tokens_in ? v.heads : v.tokens;
+  return (n <= 1 || in >= v.width) && (m <= 1 || out >= (n - 1) * in + v.width);
+}
+bool same(const Vectors& a, const Vectors& b) { return a.at == b.at && a.token == b.token && a.head == b.head; }
+
+// rotate(handle, query, keys or None, positions, inverse, out or None) -> (query, keys or None)
+PyObject* rotate(PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) throw TypeError{"rotate takes 6 arguments"};
+  const RotaryHandle* handle = static_cast<const RotaryHandle*>(PyLong_AsVoidPtr(args[0]));
+  if (PyErr_Occurred()) throw PythonError{};
+  const msb_rotary& table = handle->table;
+  const c10::Device device = device_of(table.device);
+  static const char* const names[2] = {"query", "keys"};
+  static const char* const out_names[2] = {"out[0]", "out[1]"};
+  msb_rotate_args a{};
+  at::Tensor x[2], y[2];
+  int count = 0;
+  for (int w = 0; w < 2; ++w) {
+    if (w == 1 && args[2] == Py_None) continue;
+    const at::Tensor& t = tensor(args[1 + w], names[w], device);
+    want_dim(t, names[w], 3);
+    no_gradient(t, names[w]);
+    if (t.size(2) != table.head_dim)
+      refuse(std::string(names[w]) + " must have shape [tokens, heads, " + std::to_string(table.head_dim) + "], got " + text(t.sizes()));
+    if (w == 1 && t.scalar_type() != x[0].scalar_type()) refuse("query and keys must have the same dtype");
+    if (w == 1 && t.size(0) != x[0].size(0)) refuse("query and keys must have the same number of tokens");
+    if (t.size(1) > 65535) refuse("heads must be at most 65535");
+    x[w] = t;
+    ++count;
+  }
+  const int64_t tokens = x[0].size(0);
+  a.type = type_id(x[0].scalar_type(), true);
+  const at::Tensor& given = tensor(args[3], "positions", device);
+  if (given.scalar_type() != c10::kLong && given.scalar_type() != c10::kInt)
+    refuse(std::string("positions must have dtype Int or Long, got ") + c10::toString(given.scalar_type()));
+  const bool flat = given.dim() == 1 && handle->axes == 1;
+  if (!flat && (given.dim() != 2 || given.size(0) != handle->axes))
+    refuse("positions must have shape [" + std::to_string(handle->axes) + ", tokens], got " + text(given.sizes()));
+  if (given.size(flat ? 0 : 1) != tokens) refuse("positions and query must have the same number of tokens");
+  const int inverse = PyObject_IsTrue(args[4]);
+  if (inverse < 0) throw PythonError{};
+  if (args[5] == Py_None) {
+    for (int w = 0; w < count; ++w) y[w] = empty(x[w].sizes(), x[w].scalar_type(), device);
+  } else {
+    if (!PySequence_Check(args[5]) || PySequence_Size(args[5]) != 2) throw TypeError{"out must be a pair of tensors"};
+    for (int w = 0; w < 2; ++w) {
+      PyObject* item = PySequence_GetItem(args[5], w);
+      if (!item) throw PythonError{};
+      const bool none = item == Py_None, is_tensor = THPVariable_Check(item);
+      if (is_tensor) y[w] = THPVariable_Unpack(item);
+      Py_DECREF(item);
+      if (w == 1 && count == 1) {
+        if (!none) refuse("out[1] must be None where keys are");
+        continue;
+      }
+      if (!is_tensor) throw TypeError{std::string(out_names[w]) + " must be a torch tensor"};
+      if (y[w].device() != device) refuse(std::string(out_names[w]) + " must be on " + device.str());
+      want_dtype(y[w], out_names[w], x[w].scalar_type());
+      no_gradient(y[w], out_names[w]);
+      if (!y[w].sizes().equals(x[w].sizes()) || (y[w].stride(2) != 1 && y[w].size(2) > 1))
+        refuse(std::string(out_names[w]) + " must have shape " + text(x[w].sizes()) + " with contiguous dimensions");
+    }
+    for (int w = 0; w < count && tokens > 0; ++w) {
+      if (y[w].numel() == 0) continue;
+      const Vectors out = vectors(y[w]);
+      if (!written_once(out)) refuse(std::string(out_names[w]) + " must not overlap itself");
+      for (int i = 0; i < count; ++i) {
+        if (x[i].numel() == 0) continue;
+        const bool in_place = i == w && x[i].stride(2) == 1 && same(out, vectors(x[i]));
+        // (An input with other strides in its vectors is copied first, but its memory is written nonetheless.)
+        if (!in_place && x[i].stride(2) == 1 && !apart(out, vectors(x[i])))
+          refuse(std::string(out_names[w]) + " must be " + names[w] + " itself or lie apart from " + names[i]);
+        if (i > w && y[i].numel() > 0 && !apart(out, vectors(y[i]))) refuse("out[0] and out[1] must lie apart");
+      }
+    }
+  }
+  for (int w = 0; w < count; ++w) {
+    if (x[w].stride(2) != 1 && x[w].size(2) > 1) x[w] = x[w].contiguous();
+    a.x[w] = x[w].const_data_ptr();
+    a.y[w] = y[w].mutable_data_ptr();
+    // Strides of a single token or head are never used, and say nothing of alignment.
+    a.x_token_stride[w] = tokens > 1 ? x[w].stride(0) : 0;
+    a.y_token_stride[w] = tokens > 1 ? y[w].stride(0) : 0;
+    a.x_head_stride[w] = x[w].size(1) > 1 ? x[w].stride(1) : 0;
+    a.y_head_stride[w] = x[w].size(1) > 1 ? y[w].stride(1) : 0;
+    a.heads[w] = static_cast<int32_t>(x[w].size(1));
+  }
+  a.positions = given.const_data_ptr();
+  a.position_axis_stride = flat ? 0 : given.stride(0);
+  a.position_token_stride = given.stride(flat ? 0 : 1);
+  a.wide_positions = given.scalar_type() == c10::kLong;
+  a.tokens = tokens;
+  a.inverse = inverse;
+  check_status(msb_rotate_device(&table, &a, stream_of(device)));
   PyObject* pair = PyTuple_New(2);
   if (!pair) throw PythonError{};
-  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
-  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(y[0])));
+  if (count == 1) Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(pair, 1, count == 1 ? Py_None : THPVariable_Wrap(std::move(y[1])));
   return pair;
 }
 
@@ -373,7 +651,8 @@ PyMethodDef method(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<kCall>)), METH_FASTCALL, nullptr};
 }
 PyMethodDef methods[] = {method<append>("append"), method<read>("read"), method<attend>("attend"),
-                         method<linear>("linear"), {nullptr, nullptr, 0, nullptr}};
+                         method<linear>("linear"), method<move>("move"), method<draft_ancestors>("draft_ancestors"),
+                         method<extend>("extend"), method<truncate>("truncate"), method<rotate>("rotate"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_generation", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -182,6 +182,73 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4View c, Kv4Read a
   }
 }
 
+// Moving cached vectors: every source is read before a target is written, so that a token may be the one's target and
+// the other's source (the accepted path of a tree of drafted tokens takes the places after the context's last one).
+// Heads, and the parts of a vector, do not meet: where one block has all tokens of one part (32 bytes of codes, or the
+// scales) of one head, a barrier between its reads and its writes is enough.
+constexpr int kMoveThreads = 512;
+constexpr int kMoves = 2;                             // tokens of a thread
+constexpr int kMostMoved = kMoveThreads * kMoves;     // of one launch
+__device__ __forceinline__ int64_t moved_vector(const Kv4View& c, int64_t slot, int head) {
+  return c.vector(slot >> c.page_shift, head, static_cast<int>(slot & ((1 << c.page_shift) - 1)));
+}
+__global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Move a) {
+  const int parts = c.dim / 64 + 1, part = blockIdx.x % parts, which = blockIdx.x / parts, head = blockIdx.y;
+  const int64_t slots = c.num_pages << c.page_shift;
+  int64_t to[kMoves];
+  uint4 x[kMoves][2];
+#pragma unroll
+  for (int k = 0; k < kMoves; ++k) {
+    const int64_t i = threadIdx.x + k * kMoveThreads;
+    to[k] = -1;
+    if (i >= a.tokens) continue;
+    const int64_t source = __ldg(a.source + i), target = __ldg(a.target + i);
+    if (source < 0 || source >= slots || target < 0 || target >= slots) continue;
+    to[k] = moved_vector(c, target, head);
+    const int64_t from = moved_vector(c, source, head);
+    if (part == 0) {
+      x[k][0].x = __float_as_uint(c.scales[which][from]);
+    } else {
+      const uint4* p = reinterpret_cast<const uint4*>(c.codes[which] + from * (c.dim / 2) + (part - 1) * 32);
+      x[k][0] = p[0];
+      x[k][1] = p[1];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kMoves; ++k) {
+    if (to[k] < 0) continue;
+    if (part == 0) {
+      c.scales[which][to[k]] = __uint_as_float(x[k][0].x);
+    } else {
+      uint4* p = reinterpret_cast<uint4*>(c.codes[which] + to[k] * (c.dim / 2) + (part - 1) * 32);
+      p[0] = x[k][0];
+      p[1] = x[k][1];
+    }
+  }
+}
+// More tokens: out to a workspace, [key or value][head][token] codes, then scales alike, and back in a second launch.
+// A thread has 16 bytes of codes, the first of a vector its scale too.
+template <bool kOut>
+__global__ void __launch_bounds__(kThreads) kv4_move_many_kernel(Kv4View c, Kv4Move a) {
+  const int lanes = c.dim / 32, head = blockIdx.y, which = blockIdx.z;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
+  const int lane = threadIdx.x % lanes;
+  if (i >= a.tokens) return;
+  const int64_t slots = c.num_pages << c.page_shift, source = __ldg(a.source + i), target = __ldg(a.target + i);
+  if (source < 0 || source >= slots || target < 0 || target >= slots) return;
+  const int64_t here = moved_vector(c, kOut ? source : target, head);
+  const int64_t there = (static_cast<int64_t>(which) * c.heads + head) * a.tokens + i;
+  uint4* const codes = reinterpret_cast<uint4*>(c.codes[which] + here * (c.dim / 2)) + lane;
+  uint4* const kept = static_cast<uint4*>(a.workspace) + there * lanes + lane;
+  float* const kept_scales = reinterpret_cast<float*>(static_cast<uint4*>(a.workspace) + 2 * c.heads * a.tokens * lanes);
+  if (kOut) *kept = *codes;
+  else *codes = *kept;
+  if (lane != 0) return;
+  if (kOut) kept_scales[there] = c.scales[which][here];
+  else c.scales[which][here] = kept_scales[there];
+}
+
 template <class T, bool kAligned>
 void append_aligned(const Kv4View& c, const Kv4Append& a, cudaStream_t stream) {
   const int64_t per_block = kThreads / (c.dim / 8) * kWrites;
@@ -212,6 +279,25 @@ void read_typed(const Kv4View& c, const Kv4Read& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+size_t kv4_move_workspace_bytes(const Kv4View& c, int64_t tokens) {
+  return tokens > kMostMoved ? static_cast<size_t>(2) * c.heads * tokens * (c.dim / 2 + 4) : 0;
+}
+
+void launch_kv4_move(const Kv4View& c, const Kv4Move& a, cudaStream_t stream) {
+  if (a.tokens <= 0) return;
+  if (a.tokens <= kMostMoved) {
+    kv4_move_kernel<<<dim3(2 * (c.dim / 64 + 1), static_cast<unsigned>(c.heads)), kMoveThreads, 0, stream>>>(c, a);
+    count_launch();
+  } else {
+    const int64_t per_block = kThreads / (c.dim / 32);
+    const dim3 blocks(static_cast<unsigned>((a.tokens + per_block - 1) / per_block), static_cast<unsigned>(c.heads), 2);
+    kv4_move_many_kernel<true><<<blocks, kThreads, 0, stream>>>(c, a);
+    kv4_move_many_kernel<false><<<blocks, kThreads, 0, stream>>>(c, a);
+    count_launch(2);
+  }
+  check(cudaGetLastError(), "launch cache move kernel");
+}
 
 void launch_kv4_append(const Kv4View& c, const Kv4Append& a, cudaStream_t stream) {
   if (a.tokens <= 0) return;

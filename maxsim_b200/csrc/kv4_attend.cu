@@ -136,20 +136,28 @@ struct Line {
 constexpr int kMostCluster = 8;
 struct SequenceWork {
   Kv4Sequence q;
-  int begin;        // first token that a row may see, down to a multiple of kStep
+  int begin;        // first token that a row may see, down to a multiple of kStep (of sparse rows: past the front)
+  int front;        // of sparse rows: tokens 0 .. front are seen too
   int tiles;        // units of one segment
   int blocks;       // row blocks
   __device__ __forceinline__ int64_t units(const Line& l) const {
     return static_cast<int64_t>(l.heads) * blocks * tiles;
   }
 };
+template <bool kSparse>
 __device__ __forceinline__ SequenceWork sequence_work(const Kv4Attend& a, const Line& l, int b) {
   SequenceWork w;
   w.q = kv4_sequence(a, l.page_shift, b);
-  w.begin = 0;
-  if (a.window > 0) w.begin = max(0, max(0, w.q.pos0) - a.window + 1) & ~(kStep - 1);
+  w.begin = w.front = 0;
+  if constexpr (kSparse) {
+    const Kv4Runs runs = kv4_runs(a, w.q.pos0, kStep);
+    w.begin = runs.begin;
+    w.front = runs.front;
+  } else if (a.window > 0) {
+    w.begin = max(0, max(0, w.q.pos0) - a.window + 1) & ~(kStep - 1);
+  }
   // A sequence of no tokens keeps one empty unit: its rows are written as zeros.
-  w.tiles = max(1, (w.q.length - w.begin + kTile - 1) / kTile);
+  w.tiles = max(1, (w.q.length - w.begin + w.front + kTile - 1) / kTile);
   w.blocks = (w.q.rows * l.shared + l.block_rows - 1) / l.block_rows;
   return w;
 }
@@ -173,9 +181,10 @@ struct Place {
 };
 // For 32 sequences and fewer each warp finds them by itself: units up to and of sequence `lane`.
 constexpr int kWarpBatch = 32;
+template <bool kSparse>
 __device__ __forceinline__ void warp_line(const Kv4Attend& a, const Line& l, int64_t& before, int64_t& mine, int64_t& total) {
   const int lane = threadIdx.x & 31;
-  mine = lane < a.batch ? sequence_work(a, l, lane).units(l) : 0;
+  mine = lane < a.batch ? sequence_work<kSparse>(a, l, lane).units(l) : 0;
   int64_t upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -185,12 +194,12 @@ __device__ __forceinline__ void warp_line(const Kv4Attend& a, const Line& l, int
   before = upto - mine;
   total = __shfl_sync(0xFFFFFFFFu, upto, 31);
 }
-template <class F>
+template <bool kSparse, class F>
 __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, F first, int64_t* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (a.batch <= kWarpBatch) {
     int64_t before, mine, total;
-    warp_line(a, l, before, mine, total);
+    warp_line<kSparse>(a, l, before, mine, total);
     const int64_t target = first(total);
     const uint32_t hit = __ballot_sync(0xFFFFFFFFu, target >= before && target < before + mine);
     const int at = hit ? __ffs(hit) - 1 : 0;
@@ -199,7 +208,7 @@ __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, F
   constexpr int kBlock = kWarps * 32;
   int64_t mine = 0, total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kBlock) {
-    mine = b0 + threadIdx.x < a.batch ? sequence_work(a, l, b0 + threadIdx.x).units(l) : 0;
+    mine = b0 + threadIdx.x < a.batch ? sequence_work<kSparse>(a, l, b0 + threadIdx.x).units(l) : 0;
     total += mine;
   }
 #pragma unroll
@@ -216,7 +225,7 @@ __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, F
   if (writes && threadIdx.x == 0) starts[a.batch] = total;
   int64_t carry = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kBlock) {
-    if (a.batch > kBlock) mine = b0 + threadIdx.x < a.batch ? sequence_work(a, l, b0 + threadIdx.x).units(l) : 0;
+    if (a.batch > kBlock) mine = b0 + threadIdx.x < a.batch ? sequence_work<kSparse>(a, l, b0 + threadIdx.x).units(l) : 0;
     int64_t upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -270,8 +279,9 @@ __host__ __device__ constexpr int resident_blocks(int dim, int tiles) {
 __host__ __device__ constexpr int ring_bytes(int dim) { return kWarps * kStages * (kStep * dim + 2 * kStep * 4); }
 
 // kCluster: instead of the line, a cluster of blocks has each segment (sequence, head, row block) and adds its parts
-// over distributed shared memory.
-template <class T, int kDim, int kTiles, bool kCluster>
+// over distributed shared memory.  kSparse: rows that see sinks past their window, or a tree of drafted tokens: the line
+// counts the sequence's two runs of tokens (kv4_runs) as one.
+template <class T, int kDim, int kTiles, bool kCluster, bool kSparse>
 __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv4_attend_kernel(Kv4View c, Kv4Attend a, Line line) {
   constexpr int kRows = 8 * kTiles;      // rows of a row block
   constexpr int kKeyWords = kDim / 32;   // of one token, per lane
@@ -299,10 +309,10 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     const uint32_t here = blockIdx.x / cluster_size;
     b = here / (line.heads * line.most_blocks);
     cluster_segment = here - b * (line.heads * line.most_blocks);
-    w = sequence_work(a, line, b);
+    w = sequence_work<kSparse>(a, line, b);
     if (static_cast<int>(cluster_segment % line.most_blocks) >= w.blocks) unit_end = 0;  // nothing for the whole cluster
   } else {
-    const Place place = find_place(
+    const Place place = find_place<kSparse>(
         a, line, [&](int64_t total) { return range_start(total, block, ranges(total, gridDim.x)); }, scratch);
     const int64_t n = ranges(place.total, gridDim.x);
 #if __CUDA_ARCH__ >= 900
@@ -318,7 +328,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     unit_end = range_start(place.total, block + 1, n);
     before = place.before;
     b = place.sequence;
-    if (unit < unit_end) w = sequence_work(a, line, b);
+    if (unit < unit_end) w = sequence_work<kSparse>(a, line, b);
   }
 
   while (unit < unit_end) {
@@ -332,7 +342,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     } else {
       while (unit >= before + w.units(line)) {
         before += w.units(line);
-        w = sequence_work(a, line, ++b);
+        w = sequence_work<kSparse>(a, line, ++b);
       }
       const int64_t inside = unit - before;
       const int64_t segment = inside / w.tiles;
@@ -369,12 +379,18 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
         first[nt][k] = 0;
         last[nt][k] = INT_MAX;  // rows past the block are not written: no reason to mask for them
         if (rr < all_rows) {
-          const int pos = w.q.pos0 + rr / line.shared;
-          last[nt][k] = a.causal ? pos : w.q.length - 1;
-          first[nt][k] = a.window > 0 ? max(0, max(0, pos) - a.window + 1) : 0;
+          if constexpr (kSparse) {
+            const Kv4Seen seen = kv4_seen(a, w.q, rr / line.shared);
+            last[nt][k] = seen.last;
+            first[nt][k] = seen.first;
+          } else {
+            const int pos = w.q.pos0 + rr / line.shared;
+            last[nt][k] = a.causal ? pos : w.q.length - 1;
+            first[nt][k] = a.window > 0 ? max(0, max(0, pos) - a.window + 1) : 0;
+          }
           every_last = min(every_last, last[nt][k]);
           every_first = max(every_first, first[nt][k]);
-          any_last = max(any_last, last[nt][k]);
+          any_last = max(any_last, kSparse && a.ancestors ? w.q.length - 1 : last[nt][k]);
           any_first = min(any_first, first[nt][k]);
         }
       }
@@ -387,10 +403,13 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       any_first = min(any_first, __shfl_xor_sync(0xFFFFFFFFu, any_first, d));
     }
 
-    // This warp's steps of 32 tokens, those that some row sees.
-    const int upto = min(w.begin + tile1 * kTile, any_last + 1);
-    int j0 = w.begin + tile0 * kTile + warp * kStep;
-    if (any_first > j0) j0 += (any_first - j0) / kTile * kTile;
+    // This warp's steps of 32 tokens, those that some row sees.  (Sparse rows: j0 and upto count the front's tokens and
+    // those from begin on as one run; token_of has the token.)
+    const int gap = kSparse ? w.begin - w.front : 0, base = kSparse ? 0 : w.begin;
+    auto token_of = [&](int j) { return kSparse && j >= w.front ? j + gap : j; };
+    const int upto = min(base + tile1 * kTile, any_last + 1 - gap);
+    int j0 = base + tile0 * kTile + warp * kStep;
+    if (any_first > token_of(j0) && (!kSparse || j0 >= w.front)) j0 += (any_first - token_of(j0)) / kTile * kTile;
 
     const int32_t* pages = a.page_table + b * a.table_stride;
     const bool two_pages = c.page_shift == 4;  // else 32 aligned tokens lie in one
@@ -402,8 +421,9 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     int next_page[2];  // the pages of the next step to be copied, -1 past the last token seen
     uint32_t seen_queue = 0;  // two bits a step, the oldest lowest: its 16-token tiles lie on pages of the cache
     auto ask_pages = [&](int j) {
-      next_page[0] = j < upto ? __ldg(pages + (j >> c.page_shift)) : -1;
-      next_page[1] = !two_pages ? next_page[0] : j + 16 < upto ? __ldg(pages + ((j + 16) >> c.page_shift)) : -1;
+      const int at = token_of(j);
+      next_page[0] = j < upto ? __ldg(pages + (at >> c.page_shift)) : -1;
+      next_page[1] = !two_pages ? next_page[0] : j + 16 < upto ? __ldg(pages + ((at + 16) >> c.page_shift)) : -1;
     };
     // Copies the step at j into a stage; tiles without a page copy the cache's first vectors.
     auto copy_step = [&](int j, int stage, int slot) {
@@ -413,7 +433,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
           if (static_cast<uint32_t>(next_page[i]) >= static_cast<uint32_t>(c.num_pages)) return 0;
           seen_queue |= (!two_pages ? 3u : 1u << i) << (2 * slot);
           return (static_cast<int64_t>(static_cast<uint32_t>(next_page[i]) * c.heads + head) << c.page_shift) +
-                 ((j + 16 * i) & page_mask);
+                 ((token_of(j) + 16 * i) & page_mask);
         };
         const int64_t tile = tile_of(0);
         const uint8_t* src[2] = {lane_codes[0] + tile * (kDim / 2), lane_codes[1] + tile * (kDim / 2)};
@@ -533,7 +553,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
         }
       }
       const bool one = vs[0][0].x == 1.0F || vs[0][1].x == 1.0F || vs[1][0].x == 1.0F || vs[1][1].x == 1.0F;
-      const bool masked = seen != 3u || j0 < every_first || j0 + kStep - 1 > every_last || one;
+      const int token0 = token_of(j0);
+      const bool masked = seen != 3u || token0 < every_first || token0 + kStep - 1 > every_last || one;
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -541,16 +562,37 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
           for (int k = 0; k < 2; ++k)
             if (vs[i][k].x == 1.0F && zero_codes<kDim>(here + kCodeBytes + (16 * i + g + 8 * k) * (kDim / 2)))
               vs[i][k] = make_float2(0.0F, 0.0F);
+        uint32_t bits[kTiles][2];
+        if constexpr (kSparse) {
+#pragma unroll
+          for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int rr = row0 + nt * 8 + 2 * t + k;
+              bits[nt][k] = a.ancestors && rr < all_rows ? kv4_tree_bits(a, w.q, rr / line.shared, token0) : 0u;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int nt = 0; nt < kTiles; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const int j = j0 + 16 * i + g + 8 * k;
+              const int j = token0 + 16 * i + g + 8 * k;
               const bool off = !((seen >> i) & 1u);
-              if (off || j < first[nt][0] || j > last[nt][0]) s[i][nt][k].x = -INFINITY;
-              if (off || j < first[nt][1] || j > last[nt][1]) s[i][nt][k].y = -INFINITY;
+              bool off0 = j < first[nt][0], off1 = j < first[nt][1];
+              if constexpr (kSparse) {
+                off0 = off0 && j >= a.sinks;
+                off1 = off1 && j >= a.sinks;
+              }
+              off0 = off0 || j > last[nt][0];
+              off1 = off1 || j > last[nt][1];
+              if constexpr (kSparse) {
+                off0 = off0 && !((bits[nt][0] >> (16 * i + g + 8 * k)) & 1u);
+                off1 = off1 && !((bits[nt][1] >> (16 * i + g + 8 * k)) & 1u);
+              }
+              if (off || off0) s[i][nt][k].x = -INFINITY;
+              if (off || off1) s[i][nt][k].y = -INFINITY;
             }
       }
       float2 raise[2][2];
@@ -752,18 +794,18 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
 // segments have many parts, each of a block's kJoinWarps warps adds every kJoinWarps-th of one row's and the first
 // adds the warps' sums: in either case in an order that the cut alone decides.
 constexpr int kJoinWarps = 8;
-template <class T, int kDim, int kTiles>
+template <class T, int kDim, int kTiles, bool kSparse>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(Kv4View c, Kv4Attend a, Line line, int64_t blocks,
                                                                   int warps_per_row) {
   constexpr int kRows = 8 * kTiles, kPer = kDim / 32;
   __shared__ float sums[kJoinWarps][kDim + 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x;
-  const SequenceWork w = sequence_work(a, line, b);
+  const SequenceWork w = sequence_work<kSparse>(a, line, b);
   int64_t before = 0, total = 0;
   if (a.batch <= kWarpBatch) {
     int64_t mine;
-    warp_line(a, line, before, mine, total);
+    warp_line<kSparse>(a, line, before, mine, total);
     before = __shfl_sync(0xFFFFFFFFu, before, b);
   }
   if (a.fill) kv4_fill_rows<T>(a, kDim, b, w.q, blockIdx.y, gridDim.y, threadIdx.x, kJoinWarps * 32);
@@ -895,7 +937,7 @@ Shape shape_of(const Kv4View& c, const Kv4Attend& a) {
   // 2,048: 18.0 and 11.9 us.)
   const int64_t row_blocks = (rows + 8 * s.tiles - 1) / (8 * s.tiles), segments = row_blocks * a.batch * c.heads;
   int64_t seen = most;  // tokens of a segment, at most
-  if (a.window > 0) seen = std::min<int64_t>(seen, static_cast<int64_t>(a.window) + a.max_rows + kStep);
+  if (a.window > 0) seen = std::min<int64_t>(seen, static_cast<int64_t>(a.window) + a.sinks + a.max_rows + 2 * kStep);
   const int64_t tiles = (seen + kTile - 1) / kTile;
   s.cluster = 0;
   s.row_blocks = static_cast<int>(std::min<int64_t>(row_blocks, INT_MAX));
@@ -907,7 +949,7 @@ Shape shape_of(const Kv4View& c, const Kv4Attend& a) {
 // Whether the line may cut a segment: one of a single unit never is.
 bool needs_join(const Kv4View& c, const Kv4Attend& a) { return (static_cast<int64_t>(a.max_pages) << c.page_shift) > kTile; }
 
-template <class T, int kDim, int kTiles>
+template <class T, int kDim, int kTiles, bool kSparse>
 void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cudaStream_t stream) {
   Kv4Attend a = given;
   // What the call did not ask for (kv4_attend_workspace_bytes) is not its to write, whatever the caller passed.
@@ -919,7 +961,7 @@ void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cuda
   constexpr int kShared = ring_bytes(kDim);
   static_assert(kShared >= static_cast<int>(sizeof(float)) * kWarps * 8 * kTiles * (kDim + 4), "sums fit the ring");
   if (s.cluster > 0) {
-    allow_dynamic_shared<kv4_attend_kernel<T, kDim, kTiles, true>>(kShared, "shared memory of the cache attention kernel");
+    allow_dynamic_shared<kv4_attend_kernel<T, kDim, kTiles, true, kSparse>>(kShared, "shared memory of the cache attention kernel");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(s.row_blocks) * a.batch * c.heads * s.cluster));
     cfg.blockDim = dim3(kWarps * 32);
@@ -931,12 +973,12 @@ void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cuda
     size.val.clusterDim.y = size.val.clusterDim.z = 1;
     cfg.attrs = &size;
     cfg.numAttrs = 1;
-    check(cudaLaunchKernelEx(&cfg, kv4_attend_kernel<T, kDim, kTiles, true>, c, a, line), "launch cache attention kernel");
+    check(cudaLaunchKernelEx(&cfg, kv4_attend_kernel<T, kDim, kTiles, true, kSparse>, c, a, line), "launch cache attention kernel");
     count_launch();
     return;
   }
-  allow_dynamic_shared<kv4_attend_kernel<T, kDim, kTiles, false>>(kShared, "shared memory of the cache attention kernel");
-  kv4_attend_kernel<T, kDim, kTiles, false><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
+  allow_dynamic_shared<kv4_attend_kernel<T, kDim, kTiles, false, kSparse>>(kShared, "shared memory of the cache attention kernel");
+  kv4_attend_kernel<T, kDim, kTiles, false, kSparse><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
   count_launch();
   check(cudaGetLastError(), "launch cache attention kernel");
   if (!needs_join(c, a)) return;
@@ -954,21 +996,21 @@ void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cuda
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  check(cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, kDim, kTiles>, c, a, line, s.blocks, warps_per_row),
+  check(cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, kDim, kTiles, kSparse>, c, a, line, s.blocks, warps_per_row),
         "launch cache attention join kernel");
   count_launch();
 }
 
-template <class T>
+template <class T, bool kSparse>
 void launch_typed(const Kv4View& c, const Kv4Attend& a, const Shape& s, cudaStream_t stream) {
   if (c.dim == 64) {
-    if (s.tiles == 1) launch_shape<T, 64, 1>(c, a, s, stream);
-    else launch_shape<T, 64, 2>(c, a, s, stream);
+    if (s.tiles == 1) launch_shape<T, 64, 1, kSparse>(c, a, s, stream);
+    else launch_shape<T, 64, 2, kSparse>(c, a, s, stream);
   } else if (c.dim == 128) {
-    if (s.tiles == 1) launch_shape<T, 128, 1>(c, a, s, stream);
-    else launch_shape<T, 128, 2>(c, a, s, stream);
+    if (s.tiles == 1) launch_shape<T, 128, 1, kSparse>(c, a, s, stream);
+    else launch_shape<T, 128, 2, kSparse>(c, a, s, stream);
   } else {
-    launch_shape<T, 256, 1>(c, a, s, stream);
+    launch_shape<T, 256, 1, kSparse>(c, a, s, stream);
   }
 }
 
@@ -1003,8 +1045,10 @@ void launch_kv4_attend(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream
     return;
   }
   const Shape s = shape_of(c, a);
-  if (a.type == kElemF16) launch_typed<__half>(c, a, s, stream);
-  else launch_typed<__nv_bfloat16>(c, a, s, stream);
+  // Rows that see one run of tokens do without the masks (and their registers).
+  const bool sparse = a.sinks > 0 || a.ancestors;
+  if (a.type == kElemF16) sparse ? launch_typed<__half, true>(c, a, s, stream) : launch_typed<__half, false>(c, a, s, stream);
+  else sparse ? launch_typed<__nv_bfloat16, true>(c, a, s, stream) : launch_typed<__nv_bfloat16, false>(c, a, s, stream);
 }
 
 }  // namespace msb

@@ -203,11 +203,21 @@ struct Rows {
   float2 sum[2];      // of p, the thread's columns
   int last[2];        // the last token seen
   int window;         // and how many up to it (INT_MAX: all)
+  int first[2];       // of sparse rows: the first one,
+  int sinks;          // those before it that are seen too,
+  uint32_t bits[2];   // and of the 32 columns at hand those that the row sees whatever else (a tree of drafted tokens)
   float top[2];       // the reference, -inf before there is one
 };
 
+// Whether row r does not see token c, the j-th column of its lane's eight (of four lanes') of a block.
+template <bool kSparse>
+__device__ __forceinline__ bool not_seen(const Rows& rows, int r, int c, int column) {
+  if constexpr (!kSparse) return c > rows.last[r] || rows.last[r] - c >= rows.window;
+  const bool run = c <= rows.last[r] && (c >= rows.first[r] || c < rows.sinks);
+  return !run && !((rows.bits[r] >> column) & 1u);
+}
 // Scores (f: two rows x 8 columns) to probabilities times value scales, fp16 pairs; the largest into `most`.
-template <bool kMasked>
+template <bool kMasked, bool kSparse>
 __device__ __forceinline__ void probabilities(const float (&f)[16], const float* meta, int j0, const Rows& rows, uint32_t (&p)[8],
                                               float2 (&add)[2], float (&most)[2]) {
   add[0] = add[1] = make_float2(0.0F, 0.0F);
@@ -231,8 +241,9 @@ __device__ __forceinline__ void probabilities(const float (&f)[16], const float*
         float2 pv = __fmul2_rn(pr, vs);
         if (kMasked) {
           const int c = j0 + 8 * (j + h);
-          if (e.x == -INFINITY || c > rows.last[r] || rows.last[r] - c >= rows.window) pr.x = pv.x = 0.0F;
-          if (e.y == -INFINITY || c + 1 > rows.last[r] || rows.last[r] - c - 1 >= rows.window) pr.y = pv.y = 0.0F;
+          const int column = 8 * (j + h) + 2 * (threadIdx.x & 3);
+          if (e.x == -INFINITY || not_seen<kSparse>(rows, r, c, column)) pr.x = pv.x = 0.0F;
+          if (e.y == -INFINITY || not_seen<kSparse>(rows, r, c + 1, column + 1)) pr.y = pv.y = 0.0F;
         }
         add[r] = __fadd2_rn(add[r], pr);
         most[r] = fmax3(most[r], pv.x, pv.y);
@@ -242,6 +253,7 @@ __device__ __forceinline__ void probabilities(const float (&f)[16], const float*
   }
 }
 // The largest s + log2(vs) of the thread's seen columns, per row; -inf where there are none (or nothing but NaN).
+template <bool kSparse>
 __device__ __forceinline__ void references(const float (&f)[16], const float* meta, int j0, const Rows& rows, float (&best)[2]) {
   best[0] = best[1] = -INFINITY;
 #pragma unroll
@@ -252,7 +264,7 @@ __device__ __forceinline__ void references(const float (&f)[16], const float* me
       const int c = j0 + 8 * j + k;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        if (e != -INFINITY && c <= rows.last[r] && rows.last[r] - c < rows.window)
+        if (e != -INFINITY && !not_seen<kSparse>(rows, r, c, 8 * j + k + 2 * (threadIdx.x & 3)))
           best[r] = fmaxf(best[r], f[4 * j + 2 * r + k] * ks * rows.factor[r].x + e);
     }
 }
@@ -264,7 +276,8 @@ __device__ __noinline__ bool zero_value(const uint8_t* codes, const int32_t* pag
   return zero_codes<kDim>(codes + (((page * heads + head) << page_shift) + (j & ((1 << page_shift) - 1))) * (kDim / 2));
 }
 
-template <class T, int kDim>
+// kSparse: rows that see sinks past their window, or a tree of drafted tokens (kv4_seen): tiles over the sinks come first.
+template <class T, int kDim, bool kSparse>
 __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4Attend a, uint32_t shared, int row_blocks,
                                                                 bool aligned) {
   using L = Layout<kDim>;
@@ -286,11 +299,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   // Tokens that some row of the block sees, and the tiles over them.
   const int pos0 = q.pos0 + static_cast<int>(block_row0 / shared);
   const int pos1 = q.pos0 + static_cast<int>((block_row0 + row_count - 1) / shared);
-  const int any_last = a.causal ? pos1 : q.length - 1;
+  const bool tree = kSparse && a.ancestors != nullptr;
+  const int any_last = a.causal && !tree ? pos1 : q.length - 1;
   // (Rows before the sequence's first token have negative positions; less a window these would pass 32 bits.)
-  const int any_first = a.window > 0 ? max(0, max(0, pos0) - a.window + 1) : 0;
-  const int begin = any_first & ~15;
-  const int tiles = any_last >= any_first ? (any_last - begin) / kTokens + 1 : 0;
+  const int any_first = a.window > 0 ? max(0, max(0, tree ? q.pos0 - 1 : pos0) - a.window + 1) : 0;
+  int begin = any_first & ~15;
+  // The tiles over the sinks; where these reach the window, all is one run.
+  int front = 0;
+  if constexpr (kSparse) {
+    front = a.window > 0 ? (a.sinks + kTokens - 1) / kTokens : 0;
+    if (front * kTokens >= begin) front = begin = 0;
+  }
+  const int tiles = any_last >= any_first ? front + (any_last - begin) / kTokens + 1 : 0;
+  auto tile_start = [&](int i) { return kSparse && i < front ? i * kTokens : begin + (i - front) * kTokens; };
 
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
   const uint32_t base = smem_u32(smem);
@@ -412,14 +433,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         rows.ref[k] = rows.sum[k] = make_float2(0.0F, 0.0F);
         rows.last[k] = a.causal ? pos : q.length - 1;
         rows.top[k] = -INFINITY;
+        if constexpr (kSparse) {
+          const Kv4Seen seen = kv4_seen(a, q, pos - q.pos0);
+          rows.first[k] = seen.first;
+          rows.last[k] = seen.last;
+          rows.bits[k] = 0;
+        }
       }
+      rows.sinks = a.sinks;
       rows.window = a.window > 0 ? a.window : INT_MAX;
       const int every_last = min(rows.last[0], rows.last[1]);
-      const int every_first = a.window > 0 ? max(0, max(rows.last[0], rows.last[1])) - a.window + 1 : 0;
+      const int every_first = kSparse        ? max(rows.first[0], rows.first[1])
+                              : a.window > 0 ? max(0, max(rows.last[0], rows.last[1])) - a.window + 1
+                                             : 0;
       const uint32_t s_at = tmem + (static_cast<uint32_t>(row0) << 16) + m * 128, o_at = s_at + 256;
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
-        const int s = i & 1, j0 = begin + i * kTokens;
+        const int s = i & 1, j0 = tile_start(i);
         ok = mbar_wait(&k_full[s], (i >> 1) & 1, abort_flag) && mbar_wait(&s_half[m], i & 1, abort_flag);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
@@ -440,12 +470,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
             if (!ok) break;
             tc_fence_after();
           }
+          if (tree && masked) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int at = min(m * kRowsTile + row0 + 8 * k + (lane >> 2), row_count - 1);
+              rows.bits[k] = kv4_tree_bits(a, q, static_cast<int>((block_row0 + at) / shared), j0 + kCols * piece);
+            }
+          }
           float f[16], most[2];
           float2 add[2];
           uint32_t p[8];
           tmem_ld_block(s_at + kCols * piece, f);
-          if (masked) probabilities<true>(f, my_meta, my_j0, rows, p, add, most);
-          else probabilities<false>(f, my_meta, my_j0, rows, p, add, most);
+          if (masked) probabilities<true, kSparse>(f, my_meta, my_j0, rows, p, add, most);
+          else probabilities<false, kSparse>(f, my_meta, my_j0, rows, p, add, most);
           // A row without a reference yet, or one whose reference has become too low: for p vs, or for p, which value
           // scales near zero let grow unseen by p vs (an infinite p among either).
           const float weights = fmax3(fmaxf(add[0].x, add[0].y), add[1].x, add[1].y);
@@ -457,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
             tc_fence_after();
             float best[2], fade[2];
             tmem_ld_block(s_at + kCols * piece, f);
-            references(f, my_meta, my_j0, rows, best);
+            references<kSparse>(f, my_meta, my_j0, rows, best);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 1));
@@ -469,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
               rows.ref[k] = make_float2(ref, ref);
               rows.sum[k] = __fmul2_rn(rows.sum[k], make_float2(fade[k], fade[k]));
             }
-            probabilities<true>(f, my_meta, my_j0, rows, p, add, most);
+            probabilities<true, kSparse>(f, my_meta, my_j0, rows, p, add, most);
             if (i > 0) {  // the sums of the tiles before
 #pragma unroll 1
               for (int d = 0; d < kDim; d += kCols) {
@@ -574,9 +611,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
     uint32_t word[4][kWords];
     float ks = 0.0F, vs = 0.0F;
     bool seen = false;
-    int page[2] = {ask_page(begin + 32 * uw), ask_page(begin + 32 * uw + 16)};
+    int page[2] = {ask_page(tile_start(0) + 32 * uw), ask_page(tile_start(0) + 32 * uw + 16)};
     auto load_keys = [&](int i) {
-      const int j = begin + i * kTokens + 32 * uw;
+      const int j = tile_start(i) + 32 * uw;
       const int64_t v[2] = {vector_of(page[0], j), vector_of(page[1], j + 16)};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -592,20 +629,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       const int mine = j + lane;
       const int64_t at = (lane < 16 ? v[0] : v[1]) + (lane & 15);
       seen = static_cast<uint32_t>(lane < 16 ? page[0] : page[1]) < static_cast<uint32_t>(c.num_pages) &&
-             mine >= any_first && mine <= any_last;
+             (mine >= any_first || (kSparse && mine < a.sinks)) && mine <= any_last;
       ks = __ldg(c.scales[0] + at);
       vs = __ldg(c.scales[1] + at);
-      page[0] = ask_page(j + kTokens);
-      page[1] = ask_page(j + kTokens + 16);
+      const int next = kSparse ? tile_start(i + 1) + 32 * uw : j + kTokens;
+      page[0] = ask_page(next);
+      page[1] = ask_page(next + 16);
     };
     // Values: a lane takes 8 tokens and 8 or 16 dimensions.
     constexpr int kValueWords = kDim / 64;                  // 8-dimension words of a token, per lane
     const int group = (uw >> 1) * 8 + (lane & 7);           // its 8 tokens
     const int piece = (uw & 1) * 4 + (lane >> 3);           // its words: piece * kValueWords and on
     uint32_t value[8][kValueWords];
-    int value_page = ask_page(begin + (group >> 1) * 16);
+    int value_page = ask_page(tile_start(0) + (group >> 1) * 16);
     auto load_values = [&](int i) {
-      const int j = begin + i * kTokens + (group >> 1) * 16;
+      const int j = tile_start(i) + (group >> 1) * 16;
       const uint8_t* src = c.codes[1] + (vector_of(value_page, j) + 8 * (group & 1)) * (kDim / 2) + piece * (4 * kValueWords);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -616,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           value[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * (kDim / 2)));
         }
       }
-      value_page = ask_page(j + kTokens);
+      value_page = ask_page(kSparse ? tile_start(i + 1) + (group >> 1) * 16 : j + kTokens);
     };
     if (tiles > 0) {
       load_keys(0);
@@ -646,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       }
       float* const ms = meta + s * 3 * kMetaFloats + meta_at(32 * uw + lane);
       if (seen && vs == 1.0F &&
-          zero_value<kDim>(c.codes[1], pages, c.heads, head, c.page_shift, begin + i * kTokens + 32 * uw + lane))
+          zero_value<kDim>(c.codes[1], pages, c.heads, head, c.page_shift, tile_start(i) + 32 * uw + lane))
         vs = 0.0F;
       ms[0] = seen ? ks : 0.0F;
       ms[kMetaFloats] = seen ? vs : 0.0F;
@@ -758,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <class T, int kDim>
+template <class T, int kDim, bool kSparse>
 void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
   Kv4Attend a = given;
   keep_sums_finite(a, c.page_shift, kLift);
@@ -768,8 +806,8 @@ void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
   if (blocks > INT_MAX) throw InvalidArgument("batch * heads * query rows are too many for one call");
   const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
-  allow_dynamic_shared<kv4_chunk_kernel<T, kDim>>(Layout<kDim>::kBytes, "shared memory of the chunk attention kernel");
-  kv4_chunk_kernel<T, kDim><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
+  allow_dynamic_shared<kv4_chunk_kernel<T, kDim, kSparse>>(Layout<kDim>::kBytes, "shared memory of the chunk attention kernel");
+  kv4_chunk_kernel<T, kDim, kSparse><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
       c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
   count_launch();
   check(cudaGetLastError(), "launch chunk attention kernel");
@@ -777,8 +815,9 @@ void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
 
 template <class T>
 void launch_typed(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
-  if (c.dim == 64) launch_dim<T, 64>(c, a, stream);
-  else launch_dim<T, 128>(c, a, stream);
+  const bool sparse = a.sinks > 0 || a.ancestors;
+  if (c.dim == 64) sparse ? launch_dim<T, 64, true>(c, a, stream) : launch_dim<T, 64, false>(c, a, stream);
+  else sparse ? launch_dim<T, 128, true>(c, a, stream) : launch_dim<T, 128, false>(c, a, stream);
 }
 
 }  // namespace

@@ -58,6 +58,13 @@ struct Kv4Read {
   int type;
 };
 
+struct Kv4Move {
+  const int64_t* source;      // [tokens]; a pair with either outside the cache does nothing
+  const int64_t* target;
+  int64_t tokens;
+  void* workspace;
+};
+
 struct Kv4Attend {
   const void* query;          // [rows, heads, dim]
   int64_t q_row_stride, q_head_stride;
@@ -73,6 +80,10 @@ struct Kv4Attend {
   float scale;
   int causal;
   int window;                 // 0: none
+  int sinks;                  // first tokens that stay visible past the window (0 without one)
+  const int64_t* ancestors;   // [rows, words] masks over a sequence's own rows, or nullptr: those up to the row
+  int64_t ancestors_stride;
+  int words;
   // What keeps sums of weights finite (set by the launch, see keep_sums_finite): the least log2 of a value scale that
   // references count, and the weight that none may pass.
   float least_exponent;
@@ -115,6 +126,61 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page
     s.left = all - s.rows;
   }
   return s;
+}
+
+// What a row sees.  Without masks: tokens first .. last, and those below `sinks` up to last.  With masks (a tree of
+// drafted tokens), a row's bits are the sequence's rows that it sees, n of them; first .. last are the context, what is
+// cached before the sequence's rows, and of it the last window - n.
+struct Kv4Seen {
+  int first, last;
+};
+__device__ __forceinline__ Kv4Seen kv4_seen(const Kv4Attend& a, const Kv4Sequence& q, int row) {
+  Kv4Seen s;
+  if (a.ancestors == nullptr) {
+    const int pos = q.pos0 + row;
+    s.last = a.causal ? pos : q.length - 1;
+    s.first = a.window > 0 ? max(0, max(0, pos) - a.window + 1) : 0;
+    return s;
+  }
+  s.last = q.pos0 - 1;
+  s.first = 0;
+  if (a.window > 0) {
+    const int64_t* bits = a.ancestors + (q.row0 + row) * a.ancestors_stride;
+    const int all = q.rows + q.left;
+    int n = 0;
+    for (int w = 0; w < a.words && 64 * w < all; ++w) {
+      uint64_t word = static_cast<uint64_t>(__ldg(bits + w));
+      if (all - 64 * w < 64) word &= (uint64_t{1} << (all - 64 * w)) - 1;
+      n += __popcll(word);
+    }
+    s.first = max(0, max(0, q.pos0) - a.window + n);
+  }
+  return s;
+}
+// The bits of a row for 32 tokens from j0 on: bit k, it sees token j0 + k, one of the sequence's rows.
+__device__ __forceinline__ uint32_t kv4_tree_bits(const Kv4Attend& a, const Kv4Sequence& q, int row, int j0) {
+  const int at = j0 - q.pos0, all = q.rows + q.left;  // of its rows; may lie before the first
+  if (at <= -32 || at >= all) return 0;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(a.ancestors + (q.row0 + row) * a.ancestors_stride);
+  const int w = at >> 5;
+  const uint32_t lo = w >= 0 && w < 2 * a.words ? __ldg(words + w) : 0u;
+  const uint32_t hi = w + 1 < 2 * a.words ? __ldg(words + w + 1) : 0u;
+  const uint32_t bits = __funnelshift_r(lo, hi, at & 31);
+  return all - at < 32 ? bits & ((1u << (all - at)) - 1) : bits;
+}
+// Tokens of a sequence that its rows may see, as two runs: 0 .. front (sinks, rounded up to `step`), and begin .. its
+// end, `begin` down to a multiple of `step` (and at or past `front`); with nothing between them front is 0 or begin.
+struct Kv4Runs {
+  int front, begin;
+};
+__device__ __forceinline__ Kv4Runs kv4_runs(const Kv4Attend& a, int pos0, int step) {
+  Kv4Runs r{0, 0};
+  if (a.window > 0) {
+    // A row of a tree may see none of its sequence's rows, and the window's tokens before them.
+    r.begin = max(0, max(0, pos0) - a.window + (a.ancestors ? 0 : 1)) & ~(step - 1);
+    r.front = min((a.sinks + step - 1) & ~(step - 1), r.begin);
+  }
+  return r;
 }
 
 // A block's `share` of `shares` of rows lo .. hi of an output (`width` elements a row) and of their log-sum-exp (`heads` a row)

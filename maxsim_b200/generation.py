@@ -2,17 +2,20 @@
 
 ``Int4KVCache`` holds keys and values as symmetric 4-bit codes with one fp32 scale per vector (one token, one
 head), the layout of a corpus packed as ``int4_per_token``.  Tokens are written as they are produced, read back,
-and attended to where they lie.  ``Int4Linear`` multiplies a few rows
-with 4-bit weights.  Both take and return CUDA tensors, run on torch's current stream without synchronising,
-allocate through torch only, and can be captured into a CUDA graph.
+moved, and attended to where they lie, under a window with first tokens that stay visible and for trees of drafted
+tokens (``draft_ancestors``) too.  ``PageTable`` keeps which pages sequences own, ``Rotary`` turns queries and keys by
+their positions, ``Int4Linear`` multiplies a few rows with 4-bit weights.  All take and return CUDA tensors, run on
+torch's current stream without synchronising, allocate through torch only, and can be captured into a CUDA graph.
 
-There is no backward pass: these are the operators of serving.  A query or rows that require a gradient are refused
-while gradients are enabled; codes, scales and a bias are constants, and keys and values are quantised without one.
+There is no backward pass: these are the operators of serving.  A query, keys to rotate or rows that require a gradient
+are refused while gradients are enabled; codes, scales and a bias are constants, and keys and values are quantised
+without one.
 """
 
 from __future__ import annotations
 
 import ctypes
+from fractions import Fraction
 
 torch = _lib = lib = check = _native = None
 
@@ -150,8 +153,15 @@ class Int4KVCache:
         slot = (positions % self.page_size).add(page_table[row_held, column_held].long(), alpha=self.page_size)
         return slot.clamp(min=-1).where(known, -1)
 
+    def move(self, source, target) -> None:
+        """Copy the cached vectors of int64 slots ``source`` ``[tokens]`` to ``target`` ``[tokens]``, as if every source
+        were read before any target is written: an accepted path of drafted tokens takes the places after the context's
+        last token, a prefix is copied for another sequence.  A pair with either slot outside the cache (-1, say) is
+        skipped; a target must not be given twice in one call."""
+        _native.move(self._address, source, target)
+
     def attend(self, query, page_table, lengths, *, query_offsets=None, max_query_tokens=None, scale=None, causal=True,
-               window=None, return_lse=False, out=None):
+               window=None, sinks=0, ancestors=None, return_lse=False, out=None):
         """Attention of ``query`` ``[rows, heads, head_dim]`` (fp16 or bf16) over cached tokens.
 
         ``lengths`` int32 ``[batch]`` counts each sequence's cached tokens, the rows' own among them; int32
@@ -163,20 +173,204 @@ class Int4KVCache:
         as many in every sequence: give it where sequences share the rows.
 
         A row at position ``p`` sees tokens up to ``p`` (``causal``; otherwise all of its sequence), the last
-        ``window`` of them where a window is given.  ``heads`` is a multiple of the cache's heads, consecutive
+        ``window`` of them where a window is given, and, ``sinks`` given beside it, the first ``sinks`` ones.
+
+        ``ancestors`` int64 ``[rows, words]`` makes a sequence's rows the nodes of a tree of drafted tokens: a row sees
+        those of its sequence's rows whose bit it has (bit ``k % 64`` of word ``k // 64``, from `draft_ancestors`; its own
+        bit too), and all that is cached before them, or, with a window, the last ``window - n`` of it, ``n`` its bits, and
+        the sinks.
+
+        ``heads`` is a multiple of the cache's heads, consecutive
         query heads share one.  ``scale`` defaults to ``head_dim ** -0.5``.  A row that sees nothing is zero.
         Returns ``[rows, heads, head_dim]`` in the query's dtype, with ``return_lse`` also the fp32 natural
         log-sum-exp ``[rows, heads]`` (-inf where nothing is seen), with which results over parts of a context
         can be joined.  ``out`` may be the (contiguous) query itself, but not overlap it otherwise."""
         return _native.attend(self._address, query, page_table, lengths, query_offsets, max_query_tokens, scale, causal,
-                              window, return_lse, out)
+                              window, sinks, ancestors, return_lse, out)
 
 
 def _check_cache_sizes(page_size, head_dim):
     if head_dim not in (64, 128, 256):
         raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
+    _check_page_size(page_size)
+
+
+def draft_ancestors(parents, query_offsets, *, max_query_tokens=None):
+    """``(ancestors, depths)`` of the nodes of drafted trees, one tree a sequence.
+
+    ``parents`` int32 ``[rows]``: a node's parent as a row of its sequence, counted from the sequence's first and before
+    the node; -1 (any other number) for a node that follows the context's last token.  Sequence ``b`` owns rows
+    ``query_offsets[b] .. query_offsets[b + 1]`` (int32 ``[batch + 1]``, at most ``max_query_tokens`` each, which defaults
+    to all rows and is at most 1024).  ``ancestors`` int64 ``[rows, ceil(max_query_tokens / 64)]``: the nodes on the path
+    from the context to the row, itself among them, as `Int4KVCache.attend` takes them; ``depths`` int32 ``[rows]``: how
+    many are above it, so that its position is its sequence's context length plus that.  Rows that no sequence owns, and
+    those past their sequence's ``max_query_tokens``, get 0."""
+    _load()
+    return _native.draft_ancestors(parents, query_offsets, max_query_tokens)
+
+
+class PageTable:
+    """Which pages of a cache the sequences of a batch own, kept on the device.
+
+    ``max_sequences`` sequences of up to ``max_pages`` pages of ``page_size`` tokens (a power of two, 16 to 1024) share
+    ``num_pages`` pages.  ``page_table`` int32 ``[max_sequences, max_pages]`` (-1 where there is none) and ``lengths``
+    int32 ``[max_sequences]`` are what `Int4KVCache.attend` takes; pages that no sequence owns lie on a stack,
+    ``free_pages`` int32 ``[num_pages]`` of which the first ``free_count`` (int32 ``[1]``) are valid.  A page belongs to
+    one sequence.  All four change in place."""
+
+    def __init__(self, num_pages, page_size, max_sequences, max_pages, *, device="cuda"):
+        _load()
+        if min(int(num_pages), int(max_sequences), int(max_pages)) < 1:
+            raise ValueError("num_pages, max_sequences and max_pages must be positive")
+        _check_page_size(int(page_size))
+        if torch.device(device).type != "cuda":
+            raise ValueError(f"the page table must be on a CUDA device, got {device}")
+        self._bind(torch.full((int(max_sequences), int(max_pages)), -1, dtype=torch.int32, device=device),
+                   torch.zeros(int(max_sequences), dtype=torch.int32, device=device),
+                   torch.arange(int(num_pages) - 1, -1, -1, dtype=torch.int32, device=device),
+                   torch.full((1,), int(num_pages), dtype=torch.int32, device=device), int(page_size))
+
+    @classmethod
+    def from_tensors(cls, page_table, lengths, free_pages, free_count, *, page_size):
+        """A page table over arrays the caller owns (shapes above, contiguous)."""
+        self = cls.__new__(cls)
+        self._bind(page_table, lengths, free_pages, free_count, int(page_size))
+        return self
+
+    def _bind(self, page_table, lengths, free_pages, free_count, page_size):
+        _load()
+        if not hasattr(page_table, "data_ptr") or page_table.dim() != 2:
+            raise ValueError("page_table must have shape [max_sequences, max_pages]")
+        device = page_table.device
+        if device.type != "cuda":
+            raise ValueError(f"the page table must be on a CUDA device, got {device}")
+        for name, t, ndim in (("page_table", page_table, 2), ("lengths", lengths, 1), ("free_pages", free_pages, 1),
+                              ("free_count", free_count, 1)):
+            _on(t, name, device, torch.int32, ndim)
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+        sequences, columns = page_table.shape
+        if lengths.shape[0] != sequences or free_count.shape[0] != 1:
+            raise ValueError(f"lengths must have shape [{sequences}], free_count [1]")
+        if min(sequences, columns, free_pages.shape[0]) < 1:
+            raise ValueError("num_pages, max_sequences and max_pages must be positive")
+        _check_page_size(page_size)
+        if columns * page_size > 2**31 - 65536:
+            raise ValueError("max_pages * page_size must be at most 2^31 - 65536")
+        if max(sequences, free_pages.shape[0]) >= 2**31:
+            raise ValueError("num_pages and max_sequences must be below 2^31")
+        arrays = (page_table, lengths, free_pages, free_count)
+        spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in arrays)
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("the page table's arrays must not overlap")
+        self._arrays = arrays
+        self.device = device
+        self.num_pages, self.page_size = free_pages.shape[0], page_size
+        self.max_sequences, self.max_pages = sequences, columns
+        self._c = _lib.PageTableArrays(*(t.data_ptr() for t in arrays), self.num_pages, sequences, columns, page_size,
+                                       device.index)
+        self._address = ctypes.addressof(self._c)
+
+    # Read-only: the kernels use the addresses of the arrays that the table was made with.
+    page_table = property(lambda self: self._arrays[0])
+    lengths = property(lambda self: self._arrays[1])
+    free_pages = property(lambda self: self._arrays[2])
+    free_count = property(lambda self: self._arrays[3])
+
+    def extend(self, tokens, rows):
+        """Give sequence ``b`` ``tokens[b]`` more tokens (int32 ``[max_sequences]``, 0 or less: none) and the pages that
+        they need.  Returns ``(query_offsets, slots, positions)`` of the step's ``rows`` rows (a number that the host
+        knows, the tokens' sum or more), which lie in the sequences' order: int32 ``[max_sequences + 1]``, int64
+        ``[rows]`` (for `Int4KVCache.append`), int32 ``[rows]`` (places in the sequence).
+
+        Pages are taken from the stack's top in the sequences' order.  A sequence is refused whose tokens do not fit its
+        row of the table, whose rows pass ``rows``, or that lacks pages when the sequences before it have asked for all
+        there are; it keeps its length, and its rows, as those past the last, get slot and position -1."""
+        return _native.extend(self._address, tokens, rows)
+
+    def truncate(self, lengths) -> None:
+        """Shorten sequences to int32 ``lengths`` ``[max_sequences]`` (a longer one changes nothing; 0 or less ends the
+        sequence).  Pages past that go back to the stack, the first sequence's first one on top."""
+        _native.truncate(self._address, lengths)
+
+
+def _check_page_size(page_size):
     if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
         raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+
+
+class _RotaryHandle(ctypes.Structure):  # as csrc/generation_binding.cpp reads it
+    _fields_ = [
+        ("turns", ctypes.c_void_p),
+        ("axes", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("neighbours", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+        ("position_axes", ctypes.c_int32),
+    ]
+
+
+# 1 / (2 pi) to 50 digits.
+_PER_TURN = Fraction("0.15915494309189533576888376337251436203445964574046")
+
+
+class Rotary:
+    """Rotary positions with one or several axes (time, height and width of page images, say).
+
+    The first ``rotary_dim`` dimensions of a head (all of ``head_dim`` by default) are ``rotary_dim / 2`` pairs: ``i`` and
+    ``rotary_dim / 2 + i`` (``pairs="halves"``) or ``2i`` and ``2i + 1`` (``"neighbours"``).  Pair ``i`` turns by ``position *
+    theta ** (-2i / rotary_dim)``, or ``position * frequencies[i]`` where these are given (radians a position).
+    ``sections`` says how many pairs go by each axis, one axis by default: consecutive runs, or ``interleaved``, pair
+    ``i`` of ``n`` axes by axis ``i % n`` while ``i < n * sections[i % n]`` and by the first one from there.  Angles are
+    exact at any position: turns are held to 2^-64."""
+
+    def __init__(self, head_dim, *, sections=None, theta=10000.0, rotary_dim=None, interleaved=False, pairs="halves",
+                 frequencies=None, device="cuda"):
+        _load()
+        head_dim = int(head_dim)
+        rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+        if head_dim < 2 or head_dim > 1024:
+            raise ValueError(f"head_dim must be from 2 to 1024, got {head_dim}")
+        if rotary_dim < 2 or rotary_dim > head_dim or rotary_dim % 2:
+            raise ValueError(f"rotary_dim must be even, from 2 to head_dim, got {rotary_dim}")
+        if pairs not in ("halves", "neighbours"):
+            raise ValueError(f"pairs must be 'halves' or 'neighbours', got {pairs!r}")
+        half = rotary_dim // 2
+        sections = [half] if sections is None else [int(n) for n in sections]
+        if not sections or min(sections) < 0 or sum(sections) != half or len(sections) > 256:
+            raise ValueError(f"sections must be at most 256 numbers of pairs, {half} together, got {sections}")
+        n = len(sections)
+        if interleaved:
+            axes = [i % n if i < n * sections[i % n] else 0 for i in range(half)]
+            if [axes.count(a) for a in range(n)] != sections:
+                raise ValueError(f"sections {sections} cannot be interleaved over {half} pairs")
+        else:
+            axes = [a for a, count in enumerate(sections) for _ in range(count)]
+        if frequencies is None:
+            if not (0.0 < float(theta) < float("inf")):
+                raise ValueError("theta must be finite and > 0")
+            frequencies = [float(theta) ** (-i / half) for i in range(half)]
+        frequencies = [float(f) for f in frequencies]
+        if len(frequencies) != half or not all(abs(f) < float("inf") for f in frequencies):
+            raise ValueError(f"frequencies must be {half} finite numbers")
+        if torch.device(device).type != "cuda":
+            raise ValueError(f"Rotary must be on a CUDA device, got {device}")
+        turns = [round(Fraction(f) * _PER_TURN * 2**64) % 2**64 for f in frequencies]
+        self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64, device=device)
+        self._axes = torch.tensor(axes, dtype=torch.uint8, device=device)
+        self.device = self._turns.device
+        self.head_dim, self.rotary_dim, self.sections = head_dim, rotary_dim, tuple(sections)
+        self._c = _RotaryHandle(self._turns.data_ptr(), self._axes.data_ptr(), half, head_dim, pairs == "neighbours",
+                                self.device.index, n)
+        self._address = ctypes.addressof(self._c)
+
+    def __call__(self, query, keys, positions, *, inverse=False, out=None):
+        """``(query, keys)`` ``[tokens, heads, head_dim]`` (fp32, fp16 or bf16, any token and head strides; ``keys`` may
+        be None) turned by ``positions`` ``[axes, tokens]`` (int32 or int64; ``[tokens]`` with one axis), ``inverse`` turned
+        back.  Products are fp32, rounded once; dimensions past ``rotary_dim`` are copied.  ``out``: a pair of tensors of
+        any token and head strides, apart from the inputs, or the inputs themselves."""
+        return _native.rotate(self._address, query, keys, positions, inverse, out)
 
 
 class _Linear(ctypes.Structure):  # as csrc/generation_binding.cpp reads it
