@@ -48,6 +48,7 @@
 
 namespace msb {
 bool kv4_chunk_supported(const Kv4View&);
+size_t kv4_chunk_workspace_bytes(const Kv4View&, const Kv4Attend&);
 void launch_kv4_chunk(const Kv4View&, const Kv4Attend&, cudaStream_t);
 
 namespace {
@@ -162,15 +163,6 @@ __device__ __forceinline__ SequenceWork sequence_work(const Kv4Attend& a, const 
   return w;
 }
 
-// The workspace: where each sequence starts on the line ([batch + 1], the last is the line's end), then the blocks'
-// partial sums.
-__host__ __device__ __forceinline__ size_t starts_bytes(int64_t batch) {
-  return (static_cast<size_t>(batch + 1) * sizeof(int64_t) + 127) & ~static_cast<size_t>(127);
-}
-__device__ __forceinline__ float* line_parts(const Kv4Attend& a) {
-  return reinterpret_cast<float*>(static_cast<char*>(a.workspace) + starts_bytes(a.batch));
-}
-
 // Units of all sequences, the sequence that holds unit `first(total)` and the units before it, by all threads of
 // the block, as many sequences at a time as it has threads.  The first block writes the sequences' starts where a
 // join follows (else there is no workspace to write to).
@@ -259,17 +251,6 @@ __device__ __forceinline__ Place find_place(const Kv4Attend& a, const Line& l, F
   __syncthreads();
   return p;
 }
-// Of n = min(blocks, total) ranges, range c is [c total / n, (c + 1) total / n): none is empty.
-__device__ __forceinline__ int64_t ranges(int64_t total, int64_t blocks) {
-  return total < blocks ? (total > 0 ? total : 1) : blocks;
-}
-__device__ __forceinline__ int64_t range_start(int64_t total, int64_t c, int64_t n) { return c * total / n; }
-// The range that holds unit u.
-__device__ __forceinline__ int64_t range_of(int64_t total, int64_t u, int64_t n) { return ((u + 1) * n - 1) / total; }
-
-// Partial sums of one segment's row block: rows x dim unnormalised outputs, then (reference, sum) per row.
-__host__ __device__ constexpr int partial_floats(int rows, int dim) { return rows * dim + 2 * rows; }
-
 // Resident blocks per SM that the registers are held to (128 threads, 65,536 registers).
 __host__ __device__ constexpr int resident_blocks(int dim, int tiles) {
   return dim == 256 ? 2 : dim == 128 ? (tiles == 1 ? 4 : 3) : (tiles == 1 ? 5 : 4);
@@ -910,18 +891,6 @@ struct Shape {
   int cluster;      // blocks to a segment, 0: the work line
   int row_blocks;   // of the largest sequence
 };
-int sm_count() {
-  static std::atomic<int> known{0};
-  int n = known.load(std::memory_order_relaxed);
-  if (n == 0) {
-    int dev = 0;
-    check(cudaGetDevice(&dev), "get device");
-    check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "SM count");
-    known.store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 Shape shape_of(const Kv4View& c, const Kv4Attend& a) {
   const int shared = a.heads / c.heads;
   const int64_t rows = static_cast<int64_t>(a.max_rows) * shared;
@@ -1032,7 +1001,9 @@ bool many_rows(const Kv4View& c, const Kv4Attend& a) {
 }  // namespace
 
 size_t kv4_attend_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
-  if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0 || many_rows(c, a) || !needs_join(c, a)) return 0;
+  if (a.rows <= 0 || a.batch <= 0 || a.max_rows <= 0) return 0;
+  if (many_rows(c, a)) return kv4_chunk_workspace_bytes(c, a);
+  if (!needs_join(c, a)) return 0;
   const Shape s = shape_of(c, a);
   if (s.cluster > 0) return 0;
   return starts_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(s.blocks) * partial_floats(8 * s.tiles, c.dim);

@@ -30,6 +30,7 @@
 // Every wait is bounded; a block that gives up writes NaN rows.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "quant4.cuh"
 
@@ -43,6 +44,7 @@ constexpr int kSoftWarps = 16;       // eight to a row tile: warp w has 16 rows,
 constexpr int kUnpackWarp0 = 16;     // warps 16-19: keys, the tiles' scales, values
 constexpr int kMmaWarp = 20;         // warps 20, 21: a row tile's products each
 constexpr int kThreads = 22 * 32;
+constexpr int kLineThreads = 24 * 32;  // of a line's block: whole warpgroups, whose registers can be shared out
 constexpr int kStages = 2;
 constexpr float kLift = 2.0F;        // a reference is set 2^2 below the largest p vs seen
 constexpr float kMostP = 60000.0F;   // and kept while p vs stays in fp16
@@ -61,7 +63,8 @@ struct Layout {
   static constexpr int off_meta = off_v + kStages * kTileBytes;  // [stage][3]: key scales, value scales, their log2
   static constexpr int off_flags = off_meta + kStages * 3 * kMetaFloats * 4;  // [stage][4]: some token is not seen
   static constexpr int off_rows = off_flags + kStages * 16;      // [256] the rows' factors
-  static constexpr int off_bars = off_rows + kBlockRows * 4;
+  static constexpr int off_seen = off_rows + kBlockRows * 4;     // [256] what sparse rows see
+  static constexpr int off_bars = off_seen + kBlockRows * 8;
   static constexpr int kUsed = off_bars + 24 * 8 + 1024;        // and room to align to 1024
   // A block takes all of an SM's tensor memory: more than half of its shared memory keeps a second one away.
   static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
@@ -203,23 +206,14 @@ struct Rows {
   float2 sum[2];      // of p, the thread's columns
   int last[2];        // the last token seen
   int window;         // and how many up to it (INT_MAX: all)
-  int first[2];       // of sparse rows: the first one,
-  int sinks;          // those before it that are seen too,
-  uint32_t bits[2];   // and of the 32 columns at hand those that the row sees whatever else (a tree of drafted tokens)
   float top[2];       // the reference, -inf before there is one
 };
 
-// Whether row r does not see token c, the j-th column of its lane's eight (of four lanes') of a block.
-template <bool kSparse>
-__device__ __forceinline__ bool not_seen(const Rows& rows, int r, int c, int column) {
-  if constexpr (!kSparse) return c > rows.last[r] || rows.last[r] - c >= rows.window;
-  const bool run = c <= rows.last[r] && (c >= rows.first[r] || c < rows.sinks);
-  return !run && !((rows.bits[r] >> column) & 1u);
-}
-// Scores (f: two rows x 8 columns) to probabilities times value scales, fp16 pairs; the largest into `most`.
+// Scores (f: two rows x 8 columns) to probabilities times value scales, fp16 pairs; the largest into `most`.  Of sparse
+// rows, `seen` has what each sees of the block, shifted to the thread's first column.
 template <bool kMasked, bool kSparse>
-__device__ __forceinline__ void probabilities(const float (&f)[16], const float* meta, int j0, const Rows& rows, uint32_t (&p)[8],
-                                              float2 (&add)[2], float (&most)[2]) {
+__device__ __forceinline__ void probabilities(const float (&f)[16], const float* meta, int j0, const Rows& rows,
+                                              const uint32_t (&seen)[2], uint32_t (&p)[8], float2 (&add)[2], float (&most)[2]) {
   add[0] = add[1] = make_float2(0.0F, 0.0F);
   most[0] = most[1] = 0.0F;
 #pragma unroll
@@ -227,7 +221,7 @@ __device__ __forceinline__ void probabilities(const float (&f)[16], const float*
     const float4 ks4 = *reinterpret_cast<const float4*>(meta + 2 * j);
     const float4 vs4 = *reinterpret_cast<const float4*>(meta + kMetaFloats + 2 * j);
     float4 e4 = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-    if (kMasked) e4 = *reinterpret_cast<const float4*>(meta + 2 * kMetaFloats + 2 * j);
+    if (kMasked && !kSparse) e4 = *reinterpret_cast<const float4*>(meta + 2 * kMetaFloats + 2 * j);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float2 ks = h ? make_float2(ks4.z, ks4.w) : make_float2(ks4.x, ks4.y);
@@ -241,9 +235,11 @@ __device__ __forceinline__ void probabilities(const float (&f)[16], const float*
         float2 pv = __fmul2_rn(pr, vs);
         if (kMasked) {
           const int c = j0 + 8 * (j + h);
-          const int column = 8 * (j + h) + 2 * (threadIdx.x & 3);
-          if (e.x == -INFINITY || not_seen<kSparse>(rows, r, c, column)) pr.x = pv.x = 0.0F;
-          if (e.y == -INFINITY || not_seen<kSparse>(rows, r, c + 1, column + 1)) pr.y = pv.y = 0.0F;
+          if (kSparse ? !(seen[r] & (1u << (8 * (j + h)))) : e.x == -INFINITY || c > rows.last[r] || rows.last[r] - c >= rows.window)
+            pr.x = pv.x = 0.0F;
+          if (kSparse ? !(seen[r] & (2u << (8 * (j + h))))
+                      : e.y == -INFINITY || c + 1 > rows.last[r] || rows.last[r] - c - 1 >= rows.window)
+            pr.y = pv.y = 0.0F;
         }
         add[r] = __fadd2_rn(add[r], pr);
         most[r] = fmax3(most[r], pv.x, pv.y);
@@ -254,7 +250,8 @@ __device__ __forceinline__ void probabilities(const float (&f)[16], const float*
 }
 // The largest s + log2(vs) of the thread's seen columns, per row; -inf where there are none (or nothing but NaN).
 template <bool kSparse>
-__device__ __forceinline__ void references(const float (&f)[16], const float* meta, int j0, const Rows& rows, float (&best)[2]) {
+__device__ __forceinline__ void references(const float (&f)[16], const float* meta, int j0, const Rows& rows,
+                                           const uint32_t (&seen)[2], float (&best)[2]) {
   best[0] = best[1] = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kCols / 8; ++j)
@@ -264,7 +261,8 @@ __device__ __forceinline__ void references(const float (&f)[16], const float* me
       const int c = j0 + 8 * j + k;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        if (e != -INFINITY && !not_seen<kSparse>(rows, r, c, 8 * j + k + 2 * (threadIdx.x & 3)))
+        if (kSparse ? (seen[r] & (1u << (8 * j + k))) != 0u
+                    : e != -INFINITY && c <= rows.last[r] && rows.last[r] - c < rows.window)
           best[r] = fmaxf(best[r], f[4 * j + 2 * r + k] * ks * rows.factor[r].x + e);
     }
 }
@@ -276,42 +274,239 @@ __device__ __noinline__ bool zero_value(const uint8_t* codes, const int32_t* pag
   return zero_codes<kDim>(codes + (((page * heads + head) << page_shift) + (j & ((1 << page_shift) - 1))) * (kDim / 2));
 }
 
-// kSparse: rows that see sinks past their window, or a tree of drafted tokens (kv4_seen): tiles over the sinks come first.
+// What a block does of one segment (sequence, head, 256 rows).
+struct Work {
+  Kv4Sequence q;
+  int b, head;
+  uint32_t block_row0;
+  int row_count, tiles_m;
+  int any_first, any_last;  // tokens that some row sees
+  int begin, front;         // the tiles over them start at `begin`; sparse rows: `front` tiles over the sinks come first
+  int tile0, tiles;         // this block's tiles
+  bool whole;               // which are the segment's
+  // Of the block's segments before: tiles, those of either row tile, and segments with tiles (the phases of barriers).
+  int done, row_done[2], segments;
+  template <bool kSparse>
+  __device__ __forceinline__ int tile_start(int i) const {
+    if (!kSparse) return begin + i * kTokens;
+    return tile0 + i < front ? (tile0 + i) * kTokens : begin + (tile0 + i - front) * kTokens;
+  }
+};
+template <bool kSparse>
+__device__ __forceinline__ Work work_of(const Kv4Attend& a, uint32_t shared, const Kv4Sequence& q, int b, int head, int block) {
+  Work w;
+  w.q = q;
+  w.b = b;
+  w.head = head;
+  w.block_row0 = static_cast<uint32_t>(block) * kBlockRows;  // below 2^31
+  w.row_count = static_cast<int>(min(static_cast<uint32_t>(kBlockRows), static_cast<uint32_t>(q.rows) * shared - w.block_row0));
+  w.tiles_m = w.row_count > kRowsTile ? 2 : 1;
+  const int pos0 = q.pos0 + static_cast<int>(w.block_row0 / shared);
+  const int pos1 = q.pos0 + static_cast<int>((w.block_row0 + w.row_count - 1) / shared);
+  const bool tree = kSparse && a.ancestors != nullptr;
+  w.any_last = a.causal && !tree ? pos1 : q.length - 1;
+  // (Rows before the sequence's first token have negative positions; less a window these would pass 32 bits.)
+  w.any_first = a.window > 0 ? max(0, max(0, tree ? q.pos0 - 1 : pos0) - a.window + 1) : 0;
+  w.begin = w.any_first & ~15;
+  w.front = 0;
+  if constexpr (kSparse) {
+    w.front = a.window > 0 ? (a.sinks + kTokens - 1) / kTokens : 0;
+    if (w.front * kTokens >= w.begin) w.front = w.begin = 0;  // sinks that reach the window: one run
+  }
+  w.tile0 = 0;
+  w.tiles = w.any_last >= w.any_first ? w.front + (w.any_last - w.begin) / kTokens + 1 : 0;
+  w.whole = true;
+  return w;
+}
+
+// Sparse rows' segments lie on a line: units of one tile, of every (sequence, head, row block), cut into equal ranges, one a
+// block.  Every segment of a sequence has as many units as the largest could have tiles, and some for what a segment costs
+// beside its tiles (reading queries, the first tile's chain, writing rows: 12 to 15 us, a tile 3 to 3.5).
+constexpr int kSegmentUnits = 4;
+struct Line {
+  int units;   // of a segment
+  int blocks;  // row blocks
+  __device__ __forceinline__ int64_t all(int heads) const { return static_cast<int64_t>(heads) * blocks * units; }
+};
+__device__ __forceinline__ Line line_of(const Kv4Attend& a, const Kv4Sequence& q, uint32_t shared) {
+  Line l;
+  l.blocks = static_cast<int>((static_cast<uint32_t>(q.rows) * shared + kBlockRows - 1) / kBlockRows);
+  l.units = max(1, (q.length + kTokens - 1) / kTokens);
+  if (a.window > 0) {
+    // A block's rows are those of this many query tokens (of a tree: all see the same tiles); a window that starts up
+    // to 15 tokens early, and a tree's that starts one early.
+    const int64_t tokens = a.ancestors ? q.rows + q.left + 1 : min(static_cast<int64_t>(q.rows), static_cast<int64_t>((kBlockRows - 1) / shared + 2));
+    const int64_t seen = (a.sinks + kTokens - 1) / kTokens + (tokens - 1 + a.window + 14) / kTokens + 1;
+    l.units = static_cast<int>(min(static_cast<int64_t>(l.units), seen));
+  }
+  l.units += kSegmentUnits;
+  return l;
+}
+// Segment `segment` of a sequence.
+__device__ __forceinline__ Work segment_of(const Kv4Attend& a, uint32_t shared, const Kv4Sequence& q, const Line& l, int b, int64_t segment) {
+  return work_of<true>(a, shared, q, b, static_cast<int>(segment / l.blocks), static_cast<int>(segment % l.blocks));
+}
+// Where a block is on the line.
+struct Place {
+  int64_t unit, unit_end, before;  // before: units of the sequences before b
+  int b;
+};
+// The block's next segments, up to `most`, into a list; by one thread.  A part past a segment's tiles is nobody's.
+__device__ __forceinline__ int next_works(const Kv4View& c, const Kv4Attend& a, uint32_t shared, Place& p, Work* works, int most) {
+  int count = 0, done = 0, row_done[2] = {0, 0}, segments = 0;
+  const Work* const last_work = works + most - 1;
+  if (p.unit < p.unit_end && p.before >= 0) {
+    // (Counters go on from the list before, whose last entry is still there.)
+    if (most > 0 && last_work->segments >= 0) {
+      done = last_work->done + last_work->tiles;
+      segments = last_work->segments + (last_work->tiles > 0);
+      row_done[0] = last_work->row_done[0] + last_work->tiles;
+      row_done[1] = last_work->row_done[1] + (last_work->tiles_m > 1 ? last_work->tiles : 0);
+    }
+    Kv4Sequence q = kv4_sequence(a, c.page_shift, p.b);
+    Line l = line_of(a, q, shared);
+    while (p.unit < p.unit_end && count < most) {
+      while (p.unit >= p.before + l.all(c.heads)) {
+        p.before += l.all(c.heads);
+        q = kv4_sequence(a, c.page_shift, ++p.b);
+        l = line_of(a, q, shared);
+      }
+      const int64_t inside = p.unit - p.before, segment = inside / l.units;
+      const int first = static_cast<int>(inside - segment * l.units);
+      const int last = static_cast<int>(min(static_cast<int64_t>(l.units), first + (p.unit_end - p.unit)));
+      p.unit += last - first;
+      Work w = segment_of(a, shared, q, l, p.b, segment);
+      if (first >= max(1, w.tiles)) continue;
+      w.whole = first == 0 && last >= w.tiles;
+      w.tile0 = first;
+      w.tiles = max(0, min(last, w.tiles) - first);
+      w.done = done;
+      w.row_done[0] = row_done[0];
+      w.row_done[1] = row_done[1];
+      w.segments = segments;
+      done += w.tiles;
+      row_done[0] += w.tiles;
+      row_done[1] += w.tiles_m > 1 ? w.tiles : 0;
+      segments += w.tiles > 0;
+      works[count++] = w;
+    }
+  }
+  return count;
+}
+// The block's range, by all of its threads; the first block writes the sequences' starts for the join.
+__device__ __noinline__ Place find_place(const Kv4View& c, const Kv4Attend& a, uint32_t shared) {
+  __shared__ int64_t sums[kLineThreads / 32];
+  __shared__ int64_t found[2];
+  constexpr int kWarps = kLineThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto units_of = [&](int b) {
+    if (b >= a.batch) return int64_t{0};
+    return line_of(a, kv4_sequence(a, c.page_shift, b), shared).all(c.heads);
+  };
+  int64_t total = 0;
+  for (int b = threadIdx.x; b < a.batch; b += kLineThreads) total += units_of(b);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+  if (lane == 0) sums[warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int i = 0; i < kWarps; ++i) total += sums[i];
+  const int64_t n = ranges(total, gridDim.x), c0 = blockIdx.x;
+  Place p{0, 0, 0, 0};
+  if (c0 < n) {
+    p.unit = range_start(total, c0, n);
+    p.unit_end = min(range_start(total, c0 + 1, n), total);
+  }
+  int64_t* const starts = static_cast<int64_t*>(a.workspace);
+  int64_t carry = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kLineThreads) {
+    const int b = b0 + threadIdx.x;
+    const int64_t mine = units_of(b);
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+      if (lane >= d) upto += o;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int64_t base = carry;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) base += sums[i];
+      carry += sums[i];
+    }
+    const int64_t before = base + upto - mine;
+    if (blockIdx.x == 0 && b < a.batch) starts[b] = before;
+    if (p.unit >= before && p.unit < before + mine) {
+      found[0] = before;
+      found[1] = b;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) starts[a.batch] = total;
+  __syncthreads();
+  if (p.unit < p.unit_end) {
+    p.before = found[0];
+    p.b = static_cast<int>(found[1]);
+  }
+  return p;
+}
+
+template <int kCount>
+__device__ __forceinline__ void registers_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCount));
+}
+template <int kCount>
+__device__ __forceinline__ void registers_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCount));
+}
+// Bits 0 .. n - 1, of any n.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+// Which of the 32 tokens from j on a row sees, but for its tree's (kv4_tree_bits).
+__device__ __forceinline__ uint32_t run_bits(const Kv4Seen& run, int sinks, int j) {
+  return low_bits(run.last + 1 - j) & (~low_bits(run.first - j) | low_bits(sinks - j));
+}
+
+// kSparse: rows that see sinks past their window, or a tree of drafted tokens (kv4_seen), by ranges of the line: a block
+// has one segment after the other, of the first and the last perhaps a part, whose sums go to the workspace.  Its roles
+// pass from a segment to the next by themselves, as barriers' phases count on.
 template <class T, int kDim, bool kSparse>
-__global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4Attend a, uint32_t shared, int row_blocks,
+__global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chunk_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ Kv4Attend a, uint32_t shared, int row_blocks,
                                                                 bool aligned) {
   using L = Layout<kDim>;
   extern __shared__ unsigned char raw_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // Later row blocks see more tokens under a causal mask: they start first.
-  const int64_t per_block = static_cast<int64_t>(a.batch) * c.heads;
-  const int block = row_blocks - 1 - static_cast<int>(blockIdx.x / per_block);
-  const int b = static_cast<int>(blockIdx.x % per_block / c.heads), head = static_cast<int>(blockIdx.x % c.heads);
-  const Kv4Sequence q = kv4_sequence(a, c.page_shift, b);
-  const uint32_t all_rows = static_cast<uint32_t>(q.rows) * shared, block_row0 = static_cast<uint32_t>(block) * kBlockRows;  // below 2^31
-  const int share = block * c.heads + head, shares = row_blocks * c.heads;  // of the sequence's blocks
-  if (block_row0 >= all_rows) {
-    if (a.fill) kv4_fill_rows<T>(a, kDim, b, q, share, shares, threadIdx.x, kThreads);
-    return;
-  }
-  const int row_count = static_cast<int>(min(static_cast<uint32_t>(kBlockRows), all_rows - block_row0));
-  const int tiles_m = row_count > kRowsTile ? 2 : 1;
-  // Tokens that some row of the block sees, and the tiles over them.
-  const int pos0 = q.pos0 + static_cast<int>(block_row0 / shared);
-  const int pos1 = q.pos0 + static_cast<int>((block_row0 + row_count - 1) / shared);
-  const bool tree = kSparse && a.ancestors != nullptr;
-  const int any_last = a.causal && !tree ? pos1 : q.length - 1;
-  // (Rows before the sequence's first token have negative positions; less a window these would pass 32 bits.)
-  const int any_first = a.window > 0 ? max(0, max(0, tree ? q.pos0 - 1 : pos0) - a.window + 1) : 0;
-  int begin = any_first & ~15;
-  // The tiles over the sinks; where these reach the window, all is one run.
-  int front = 0;
+  // On a line: the block's next segments, and how many.  (In shared memory: read once a tile, in registers they would cost
+  // those of the loops.)
+  constexpr int kList = kSparse ? 32 : 1;
+  __shared__ Work works[kList];
+  __shared__ Place place;
+  __shared__ int work_count;
+  Work only{};
+  int share = 0, shares = 1;
   if constexpr (kSparse) {
-    front = a.window > 0 ? (a.sinks + kTokens - 1) / kTokens : 0;
-    if (front * kTokens >= begin) front = begin = 0;
+#if __CUDA_ARCH__ >= 900
+    cudaTriggerProgrammaticLaunchCompletion();
+#endif
+    const Place start = find_place(c, a, shared);
+    if (threadIdx.x == 0) {
+      place = start;
+      works[kList - 1].segments = -1;
+    }
+  } else {
+    // Later row blocks see more tokens under a causal mask: they start first.
+    const int64_t per_block = static_cast<int64_t>(a.batch) * c.heads;
+    const int block = row_blocks - 1 - static_cast<int>(blockIdx.x / per_block);
+    const int b = static_cast<int>(blockIdx.x % per_block / c.heads), head = static_cast<int>(blockIdx.x % c.heads);
+    const Kv4Sequence q = kv4_sequence(a, c.page_shift, b);
+    share = block * c.heads + head, shares = row_blocks * c.heads;  // of the sequence's blocks
+    if (static_cast<uint32_t>(block) * kBlockRows >= static_cast<uint32_t>(q.rows) * shared) {
+      if (a.fill) kv4_fill_rows<T>(a, kDim, b, q, share, shares, threadIdx.x, kThreads);
+      return;
+    }
+    only = work_of<false>(a, shared, q, b, head, block);
   }
-  const int tiles = any_last >= any_first ? front + (any_last - begin) / kTokens + 1 : 0;
-  auto tile_start = [&](int i) { return kSparse && i < front ? i * kTokens : begin + (i - front) * kTokens; };
+  const bool tree = kSparse && a.ancestors != nullptr;
 
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
   const uint32_t base = smem_u32(smem);
@@ -330,21 +525,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   uint64_t* const s_half = bars + 16;      // [row tile] scores of the half that comes first ready
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(bars + 19);
+  // Row tiles that arrive: on a line always two; where a segment has one, that one's warps arrive for both.
+  const int row_tiles = kSparse ? 2 : only.tiles_m;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 4);
-      mbar_init(&k_empty[s], tiles_m);
+      mbar_init(&k_empty[s], row_tiles);
       mbar_init(&v_full[s], 4);
-      mbar_init(&v_empty[s], tiles_m);
-      mbar_init(&meta_empty[s], 8 * tiles_m);
+      mbar_init(&v_empty[s], row_tiles);
+      mbar_init(&meta_empty[s], 8 * row_tiles);
     }
     for (int m = 0; m < 2; ++m) {
       mbar_init(&s_half[m], 1);
       mbar_init(&s_full[m], 1);
       mbar_init(&p_full[m], 8);
     }
-    mbar_init(o_full, tiles_m);
-    mbar_init(q_full, 8 * tiles_m);
+    mbar_init(o_full, row_tiles);
+    mbar_init(q_full, 8 * row_tiles);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -361,249 +558,331 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   // probabilities of both go to its columns, so that the other half's are free for the half of tile i + 1 that
   // comes first: its product does not wait for this tile's sums, nor its softmax.
 
-  const int32_t* const pages = a.page_table + b * a.table_stride;
   const int page_mask = (1 << c.page_shift) - 1;
   // Vector of token j's 16-token group on page p (-1: none), and whether the page is the cache's.
-  auto ask_page = [&](int j) { return j <= any_last ? __ldg(pages + (j >> c.page_shift)) : -1; };
-  auto vector_of = [&](int page, int j) {
+  auto ask_page = [&](const Work& w, int j) {
+    return j <= w.any_last ? __ldg(a.page_table + w.b * a.table_stride + (j >> c.page_shift)) : -1;
+  };
+  auto vector_of = [&](const Work& w, int page, int j) {
     return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages)
-               ? (static_cast<int64_t>(static_cast<uint32_t>(page) * c.heads + head) << c.page_shift) + (j & page_mask)
+               ? (static_cast<int64_t>(static_cast<uint32_t>(page) * c.heads + w.head) << c.page_shift) + (j & page_mask)
                : int64_t{0};
   };
 
+  auto work = [&](int k) -> const Work& {
+    if constexpr (kSparse) return works[k];
+    return only;
+  };
+  int count = 1;
+  if constexpr (kSparse) {
+    if (threadIdx.x == 0) work_count = next_works(c, a, shared, place, works, kList);
+    __syncthreads();
+    count = work_count;
+  }
+  // The next list, after a full one: every role comes here (with the loop over lists around the roles, what one of them
+  // needs would be formed before it and held through all).
+  auto next_list = [&](bool writes) {
+    if (!kSparse || count < kList) return false;
+    asm volatile("bar.sync 0;" ::: "memory");
+    if constexpr (kSparse)
+      if (writes && threadIdx.x == (kMmaWarp + 2) * 32) work_count = next_works(c, a, shared, place, works, kList);
+    asm volatile("bar.sync 0;" ::: "memory");
+    count = work_count;
+    return count > 0;
+  };
   if (warp < kSoftWarps) {
+    if constexpr (kSparse) registers_inc<88>();
     // =================== softmax: a warp has 16 rows, a thread two of them and a quarter of their columns ===================
     const int m = warp >> 3;
-    if (m < tiles_m) {
-      const int row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16;  // of the row tile, and its lane of tensor memory
-      float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + row0;
-      constexpr int kRowLanes = kDim / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 16 / kRowsAtOnce;
-      // The warp's rows of the query tile, 8 dimensions a lane: scaled by a power of two to a maximum in [2^10, 2^11),
-      // fp16, in the codes' order.  (In a loop: straight code would be fetched from memory and used once.)
-      constexpr int kBatch = 4;
-#pragma unroll 1
-      for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
-        uint4 x[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const int r = m * kRowsTile + row0 + (k0 + k) * kRowsAtOnce + lane / kRowLanes;
-          x[k] = make_uint4(0, 0, 0, 0);
-          if (r < row_count) {
-            const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
-            const T* src = static_cast<const T*>(a.query) + (q.row0 + token) * a.q_row_stride +
-                           static_cast<int64_t>(head * shared + in_group) * a.q_head_stride + (lane % kRowLanes) * 8;
-            if (aligned) {
-              x[k] = __ldg(reinterpret_cast<const uint4*>(src));
-            } else {
-              __align__(16) T e[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) e[i] = src[i];
-              x[k] = *reinterpret_cast<const uint4*>(e);
+    bool ok = true;
+    do {
+      for (int segment = 0; segment < count; ++segment) {
+        const Work& w = work(segment);
+        if (m >= w.tiles_m) {
+          if constexpr (kSparse) {  // the other row tile's segment: passed together, as a wait may not fall a phase behind
+            if (w.tiles > 0) {
+              if (lane == 0) mbar_arrive(q_full);
+              ok = ok && mbar_wait(o_full, w.segments & 1, abort_flag);
+              ok = __all_sync(0xFFFFFFFFu, ok);
             }
           }
+          continue;
         }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const T* const v = reinterpret_cast<const T*>(&x[k]);
-          float top = 0.0F;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_f32(v[i])));
-#pragma unroll
-          for (int d = 1; d < kRowLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-          const int e = max(-110, min(127, static_cast<int>(__float_as_uint(top) >> 23) - 127));
-          const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
-          const int r = (k0 + k) * kRowsAtOnce + lane / kRowLanes, piece = lane % kRowLanes;
-          store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled(row0 + r, piece & 7),
-                  pack_half2(to_f32(v[0]) * down, to_f32(v[4]) * down), pack_half2(to_f32(v[1]) * down, to_f32(v[5]) * down),
-                  pack_half2(to_f32(v[2]) * down, to_f32(v[6]) * down), pack_half2(to_f32(v[3]) * down, to_f32(v[7]) * down));
-          if (piece == 0) row_factor[r] = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
-        }
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-
-      Rows rows;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        // Rows past the last do as it does: what they compute is not written.
-        const int mine = 8 * k + (lane >> 2), at = min(m * kRowsTile + row0 + mine, row_count - 1);
-        const int pos = q.pos0 + static_cast<int>((block_row0 + at) / shared);
-        rows.factor[k] = make_float2(row_factor[mine], row_factor[mine]);
-        rows.ref[k] = rows.sum[k] = make_float2(0.0F, 0.0F);
-        rows.last[k] = a.causal ? pos : q.length - 1;
-        rows.top[k] = -INFINITY;
-        if constexpr (kSparse) {
-          const Kv4Seen seen = kv4_seen(a, q, pos - q.pos0);
-          rows.first[k] = seen.first;
-          rows.last[k] = seen.last;
-          rows.bits[k] = 0;
-        }
-      }
-      rows.sinks = a.sinks;
-      rows.window = a.window > 0 ? a.window : INT_MAX;
-      const int every_last = min(rows.last[0], rows.last[1]);
-      const int every_first = kSparse        ? max(rows.first[0], rows.first[1])
-                              : a.window > 0 ? max(0, max(rows.last[0], rows.last[1])) - a.window + 1
-                                             : 0;
-      const uint32_t s_at = tmem + (static_cast<uint32_t>(row0) << 16) + m * 128, o_at = s_at + 256;
-      bool ok = true;
-      for (int i = 0; i < tiles; ++i) {
-        const int s = i & 1, j0 = tile_start(i);
-        ok = mbar_wait(&k_full[s], (i >> 1) & 1, abort_flag) && mbar_wait(&s_half[m], i & 1, abort_flag);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint4 flag = *reinterpret_cast<const uint4*>(flags + 4 * s);
-        const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < every_first ||
-                                                       j0 + kTokens - 1 > every_last);
-        const uint32_t p_at = s_at + s * (kTokens / 2);
-        // Blocks of 32 columns in one short loop: its instructions stay near, the other three warps of a scheduler
-        // fill its waits.
+        const int row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16;  // of the row tile, and its lane of tensor memory
+        float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + row0;
+        constexpr int kRowLanes = kDim / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 16 / kRowsAtOnce;
+        // The warp's rows of the query tile, 8 dimensions a lane: scaled by a power of two to a maximum in [2^10, 2^11),
+        // fp16, in the codes' order.  (In a loop: straight code would be fetched from memory and used once.)
+        constexpr int kBatch = kSparse ? kLoads : 4;
 #pragma unroll 1
-        for (int part = 0; part < kTokens / kCols; ++part) {
-          const int piece = part ^ (2 * s);  // the block of columns
-          const float* const my_meta = meta + s * 3 * kMetaFloats + (4 * piece + (lane & 3)) * kMetaPitch;
-          const int my_j0 = j0 + kCols * piece + 2 * (lane & 3);
-          if (part == kTokens / kCols / 2) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], i & 1, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-          }
-          if (tree && masked) {
+        for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
+          uint4 x[kBatch];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int at = min(m * kRowsTile + row0 + 8 * k + (lane >> 2), row_count - 1);
-              rows.bits[k] = kv4_tree_bits(a, q, static_cast<int>((block_row0 + at) / shared), j0 + kCols * piece);
-            }
-          }
-          float f[16], most[2];
-          float2 add[2];
-          uint32_t p[8];
-          tmem_ld_block(s_at + kCols * piece, f);
-          if (masked) probabilities<true, kSparse>(f, my_meta, my_j0, rows, p, add, most);
-          else probabilities<false, kSparse>(f, my_meta, my_j0, rows, p, add, most);
-          // A row without a reference yet, or one whose reference has become too low: for p vs, or for p, which value
-          // scales near zero let grow unseen by p vs (an infinite p among either).
-          const float weights = fmax3(fmaxf(add[0].x, add[0].y), add[1].x, add[1].y);
-          const bool low = fminf(rows.top[0], rows.top[1]) == -INFINITY || fmaxf(most[0], most[1]) > kMostP || weights > a.most_weight;
-          if (__any_sync(0xFFFFFFFFu, low)) {
-            tmem_wait_st();  // what was written before is read below, the sums of the tiles before too
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], i & 1, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            float best[2], fade[2];
-            tmem_ld_block(s_at + kCols * piece, f);
-            references<kSparse>(f, my_meta, my_j0, rows, best);
+          for (int k = 0; k < kBatch; ++k) {
+            const int r = m * kRowsTile + row0 + (k0 + k) * kRowsAtOnce + lane / kRowLanes;
+            x[k] = make_uint4(0, 0, 0, 0);
+            if (r < w.row_count) {
+              const uint32_t token = (w.block_row0 + r) / shared, in_group = w.block_row0 + r - token * shared;
+              const T* src = static_cast<const T*>(a.query) + (w.q.row0 + token) * a.q_row_stride +
+                             static_cast<int64_t>(w.head * shared + in_group) * a.q_head_stride + (lane % kRowLanes) * 8;
+              if (aligned) {
+                x[k] = __ldg(reinterpret_cast<const uint4*>(src));
+              } else {
+                __align__(16) T e[8];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 1));
-              best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 2));
-              const float next = fmaxf(rows.top[k], best[k]);
-              fade[k] = fade_to(rows.top[k], next);
-              rows.top[k] = next;
-              const float ref = next == -INFINITY ? 0.0F : kLift - next;
-              rows.ref[k] = make_float2(ref, ref);
-              rows.sum[k] = __fmul2_rn(rows.sum[k], make_float2(fade[k], fade[k]));
-            }
-            probabilities<true, kSparse>(f, my_meta, my_j0, rows, p, add, most);
-            if (i > 0) {  // the sums of the tiles before
-#pragma unroll 1
-              for (int d = 0; d < kDim; d += kCols) {
-                tmem_ld_block(o_at + d, f);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) f[k] *= fade[(k >> 1) & 1];
-                tmem_st_block(o_at + d, f);
+                for (int i = 0; i < 8; ++i) e[i] = src[i];
+                x[k] = *reinterpret_cast<const uint4*>(e);
               }
             }
-#pragma unroll 1
-            for (int d = 0; d < part; ++d) {  // and the probabilities of the columns before
-              uint32_t w[8];
-              tmem_ld_pairs(p_at + kCols / 2 * d, w);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-                w[k] = pack_half2(v.x * fade[k & 1], v.y * fade[k & 1]);
-              }
-              tmem_st_pairs(p_at + kCols / 2 * d, w);
-            }
           }
-          rows.sum[0] = __fadd2_rn(rows.sum[0], add[0]);
-          rows.sum[1] = __fadd2_rn(rows.sum[1], add[1]);
-          tmem_st_pairs(p_at + kCols / 2 * part, p);
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const T* const v = reinterpret_cast<const T*>(&x[k]);
+            float top = 0.0F;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(to_f32(v[i])));
+#pragma unroll
+            for (int d = 1; d < kRowLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            const int e = max(-110, min(127, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+            const float down = __uint_as_float(static_cast<uint32_t>(127 + 10 - e) << 23);
+            const int r = (k0 + k) * kRowsAtOnce + lane / kRowLanes, piece = lane % kRowLanes;
+            store16(base + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) + swizzled(row0 + r, piece & 7),
+                    pack_half2(to_f32(v[0]) * down, to_f32(v[4]) * down), pack_half2(to_f32(v[1]) * down, to_f32(v[5]) * down),
+                    pack_half2(to_f32(v[2]) * down, to_f32(v[6]) * down), pack_half2(to_f32(v[3]) * down, to_f32(v[7]) * down));
+            if (piece == 0) row_factor[r] = a.scale * 1.44269504F * __uint_as_float(static_cast<uint32_t>(127 - 10 + e) << 23);
+          }
         }
-        if (!ok) break;
-        tmem_wait_st();
-        tc_fence_before();
+        fence_proxy_async();
+        if (kSparse) tc_fence_before();  // the sums of the segment before have been read
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&p_full[m]);
-          mbar_arrive(&meta_empty[s]);
-        }
-      }
-      // The rows' outputs, through the query tile's shared memory to 16 bytes a lane.
-      if (ok && tiles > 0) ok = mbar_wait(o_full, 0, abort_flag);
-      ok = __all_sync(0xFFFFFFFFu, ok) && !*abort_flag;
-      tc_fence_after();
-      float inv[2], sum[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float l = rows.sum[k].x + rows.sum[k].y;
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-        sum[k] = l;
-        inv[k] = l == 0.0F ? 0.0F : 1.0F / l;
-      }
-#pragma unroll 1
-      for (int d = 0; d < kDim; d += kCols) {
-        float f[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) f[k] = 0.0F;
-        if (ok && tiles > 0) tmem_ld_block(o_at + d, f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float scale = inv[k & 1];
-          T e[2];
-          e[0] = from_f32<T>(!ok ? NAN : sum[k & 1] == 0.0F ? 0.0F : f[2 * k] * scale);
-          e[1] = from_f32<T>(!ok ? NAN : sum[k & 1] == 0.0F ? 0.0F : f[2 * k + 1] * scale);
-          const int r = row0 + 8 * (k & 1) + (lane >> 2), piece = (d >> 3) + (k >> 1);
-          uint32_t v;
-          memcpy(&v, e, 4);
-          *reinterpret_cast<uint32_t*>(smem + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) +
-                                       swizzled(r, piece & 7) + 4 * (lane & 3)) = v;
-        }
-      }
-      __syncwarp();
-      const bool out_aligned = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-#pragma unroll 4
-      for (int k = 0; k < kLoads; ++k) {
-        const int in_warp = k * kRowsAtOnce + lane / kRowLanes, r = m * kRowsTile + row0 + in_warp, piece = lane % kRowLanes;
-        if (r >= row_count) continue;
-        const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
-        const int64_t out_row = (q.row0 + token) * a.heads + head * shared + in_group;
-        const uint4 v = *reinterpret_cast<const uint4*>(smem + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) +
-                                                        swizzled(row0 + in_warp, piece & 7));
-        T* const out = static_cast<T*>(a.out) + out_row * kDim + piece * 8;
-        if (out_aligned) {
-          *reinterpret_cast<uint4*>(out) = v;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) out[i] = reinterpret_cast<const T*>(&v)[i];
-        }
-      }
-      if (a.lse && (lane & 3) == 0) {
+        if (lane == 0 && (!kSparse || w.tiles > 0)) mbar_arrive(q_full);
+
+        Rows rows;
+        int every_first = 0, every_last = 0;
+        Kv4Seen* const row_seen = reinterpret_cast<Kv4Seen*>(smem + L::off_seen) + m * kRowsTile + row0;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int r = m * kRowsTile + row0 + 8 * k + (lane >> 2);
-          if (r >= row_count) continue;
-          const uint32_t token = (block_row0 + r) / shared, in_group = block_row0 + r - token * shared;
-          const float reference = rows.top[k] == -INFINITY ? 0.0F : rows.top[k] - kLift;
-          a.lse[(q.row0 + token) * a.heads + head * shared + in_group] =
-              !ok ? NAN : sum[k] == 0.0F ? -INFINITY : (reference + __log2f(sum[k])) * 0.693147181F;
+          // Rows past the last do as it does: what they compute is not written.
+          const int mine = 8 * k + (lane >> 2), at = min(m * kRowsTile + row0 + mine, w.row_count - 1);
+          const int pos = w.q.pos0 + static_cast<int>((w.block_row0 + at) / shared);
+          rows.factor[k] = make_float2(row_factor[mine], row_factor[mine]);
+          rows.ref[k] = rows.sum[k] = make_float2(0.0F, 0.0F);
+          rows.last[k] = a.causal ? pos : w.q.length - 1;
+          rows.top[k] = -INFINITY;
+          if constexpr (kSparse) {
+            const Kv4Seen seen = kv4_seen(a, w.q, pos - w.q.pos0);
+            every_first = k ? max(every_first, seen.first) : seen.first;
+            every_last = k ? min(every_last, seen.last) : seen.last;
+            row_seen[mine] = seen;  // (four lanes write the same)
+          }
+        }
+        if constexpr (kSparse) __syncwarp();
+        rows.window = a.window > 0 ? a.window : INT_MAX;
+        if constexpr (!kSparse) {
+          every_last = min(rows.last[0], rows.last[1]);
+          every_first = a.window > 0 ? max(0, max(rows.last[0], rows.last[1])) - a.window + 1 : 0;
+        }
+        const uint32_t s_at = tmem + (static_cast<uint32_t>(row0) << 16) + m * 128, o_at = s_at + 256;
+        for (int i = 0; i < w.tiles; ++i) {
+          const int it = kSparse ? w.done + i : i, s = it & 1, j0 = w.tile_start<kSparse>(i);
+          const int im = kSparse ? w.row_done[m] + i : i;
+          ok = ok && mbar_wait(&k_full[s], (it >> 1) & 1, abort_flag) && mbar_wait(&s_half[m], im & 1, abort_flag);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint4 flag = *reinterpret_cast<const uint4*>(flags + 4 * s);
+          const bool masked = __any_sync(0xFFFFFFFFu, (flag.x | flag.y | flag.z | flag.w) != 0u || j0 < every_first ||
+                                                         j0 + kTokens - 1 > every_last);
+          const uint32_t p_at = s_at + s * (kTokens / 2);
+          // A block of 32 columns.  kMode: without masks, with them, or as `masked` says.
+          auto columns = [&](int part, auto mode) {
+            constexpr int kMode = decltype(mode)::value;
+            const bool with_masks = kMode == 2 ? masked : kMode == 1;
+            const int piece = part ^ (2 * s);  // the block of columns
+            const float* const my_meta = meta + s * 3 * kMetaFloats + (4 * piece + (lane & 3)) * kMetaPitch;
+            const int my_j0 = j0 + kCols * piece + 2 * (lane & 3);
+            if (part == kTokens / kCols / 2) {
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], im & 1, abort_flag));
+              if (!ok) return;
+              tc_fence_after();
+            }
+            uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+            if (kSparse && with_masks) {
+              const int j = j0 + kCols * piece;
+              const uint32_t absent = flags[4 * s + piece];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int mine = 8 * k + (lane >> 2);
+                seen[k] = run_bits(row_seen[mine], a.sinks, j);
+                if (tree && j + kCols > w.q.pos0)
+                  seen[k] |= kv4_tree_bits(a, w.q, static_cast<int>((w.block_row0 + min(m * kRowsTile + row0 + mine, w.row_count - 1)) / shared), j);
+                seen[k] = (seen[k] & ~absent) >> (2 * (lane & 3));
+              }
+            }
+            float f[16], most[2];
+            float2 add[2];
+            uint32_t p[8];
+            tmem_ld_block(s_at + kCols * piece, f);
+            if (with_masks) probabilities<true, kSparse>(f, my_meta, my_j0, rows, seen, p, add, most);
+            else probabilities<false, kSparse>(f, my_meta, my_j0, rows, seen, p, add, most);
+            // A row without a reference yet, or one whose reference has become too low: for p vs, or for p, which value
+            // scales near zero let grow unseen by p vs (an infinite p among either).
+            const float weights = fmax3(fmaxf(add[0].x, add[0].y), add[1].x, add[1].y);
+            const bool low = fminf(rows.top[0], rows.top[1]) == -INFINITY || fmaxf(most[0], most[1]) > kMostP || weights > a.most_weight;
+            if (__any_sync(0xFFFFFFFFu, low)) {
+              tmem_wait_st();  // what was written before is read below, the sums of the tiles before too
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], im & 1, abort_flag));
+              if (!ok) return;
+              tc_fence_after();
+              float best[2], fade[2];
+              tmem_ld_block(s_at + kCols * piece, f);
+              references<kSparse>(f, my_meta, my_j0, rows, seen, best);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 1));
+                best[k] = fmaxf(best[k], __shfl_xor_sync(0xFFFFFFFFu, best[k], 2));
+                const float next = fmaxf(rows.top[k], best[k]);
+                fade[k] = fade_to(rows.top[k], next);
+                rows.top[k] = next;
+                const float ref = next == -INFINITY ? 0.0F : kLift - next;
+                rows.ref[k] = make_float2(ref, ref);
+                rows.sum[k] = __fmul2_rn(rows.sum[k], make_float2(fade[k], fade[k]));
+              }
+              probabilities<true, kSparse>(f, my_meta, my_j0, rows, seen, p, add, most);
+              if (i > 0) {  // the sums of the tiles before
+#pragma unroll 1
+                for (int d = 0; d < kDim; d += kCols) {
+                  tmem_ld_block(o_at + d, f);
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) f[k] *= fade[(k >> 1) & 1];
+                  tmem_st_block(o_at + d, f);
+                }
+              }
+#pragma unroll 1
+              for (int d = 0; d < part; ++d) {  // and the probabilities of the columns before
+                uint32_t w[8];
+                tmem_ld_pairs(p_at + kCols / 2 * d, w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+                  w[k] = pack_half2(v.x * fade[k & 1], v.y * fade[k & 1]);
+                }
+                tmem_st_pairs(p_at + kCols / 2 * d, w);
+              }
+            }
+            rows.sum[0] = __fadd2_rn(rows.sum[0], add[0]);
+            rows.sum[1] = __fadd2_rn(rows.sum[1], add[1]);
+            tmem_st_pairs(p_at + kCols / 2 * part, p);
+          };
+          // Blocks in one short loop: its instructions stay near, the other three warps of a scheduler fill its waits.
+          // (Sparse rows' masks are selects in the same steps: as one loop with both, the compiler joined the two, and every
+          // tile paid for them.)
+          if constexpr (!kSparse) {
+#pragma unroll 1
+            for (int part = 0; part < kTokens / kCols && ok; ++part) columns(part, std::integral_constant<int, 2>{});
+          } else if (masked) {
+#pragma unroll 1
+            for (int part = 0; part < kTokens / kCols && ok; ++part) columns(part, std::integral_constant<int, 1>{});
+          } else {
+#pragma unroll 1
+            for (int part = 0; part < kTokens / kCols && ok; ++part) columns(part, std::integral_constant<int, 0>{});
+          }
+          if (!ok) break;
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&meta_empty[s]);
+            if (kSparse && w.tiles_m == 1) mbar_arrive(&meta_empty[s]);
+            mbar_arrive(&p_full[m]);
+          }
+        }
+        // The rows' outputs, through the query tile's shared memory to 16 bytes a lane.
+        if (ok && w.tiles > 0) ok = mbar_wait(o_full, kSparse ? w.segments & 1 : 0, abort_flag);
+        ok = __all_sync(0xFFFFFFFFu, ok) && !*abort_flag;
+        tc_fence_after();
+        float inv[2], sum[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float l = rows.sum[k].x + rows.sum[k].y;
+          l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+          l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+          sum[k] = l;
+          inv[k] = l == 0.0F ? 0.0F : 1.0F / l;
+        }
+        if constexpr (kSparse) {
+          if (!w.whole) {  // a part of a segment: its sums as they are, and their references
+            float* const part = line_parts(a) + (2 * static_cast<int64_t>(blockIdx.x) + (w.tile0 == 0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
+            float* const sums = part + (m * kRowsTile + row0 + (lane >> 2)) * kDim + 2 * (lane & 3);
+#pragma unroll 1
+            for (int d = 0; d < kDim && w.tiles > 0; d += kCols) {
+              float f[16];
+              if (ok) tmem_ld_block(o_at + d, f);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<float2*>(sums + (k & 1) * 8 * kDim + d + 8 * (k >> 1)) = make_float2(f[2 * k], f[2 * k + 1]);
+            }
+            if ((lane & 3) == 0) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                *reinterpret_cast<float2*>(part + kBlockRows * kDim + 2 * (m * kRowsTile + row0 + 8 * k + (lane >> 2))) =
+                    ok ? make_float2(rows.top[k], w.tiles > 0 ? sum[k] : 0.0F) : make_float2(0.0F, NAN);
+            }
+            continue;
+          }
+        }
+#pragma unroll 1
+        for (int d = 0; d < kDim; d += kCols) {
+          float f[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) f[k] = 0.0F;
+          if (ok && w.tiles > 0) tmem_ld_block(o_at + d, f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float scale = inv[k & 1];
+            T e[2];
+            e[0] = from_f32<T>(!ok ? NAN : sum[k & 1] == 0.0F ? 0.0F : f[2 * k] * scale);
+            e[1] = from_f32<T>(!ok ? NAN : sum[k & 1] == 0.0F ? 0.0F : f[2 * k + 1] * scale);
+            const int r = row0 + 8 * (k & 1) + (lane >> 2), piece = (d >> 3) + (k >> 1);
+            uint32_t v;
+            memcpy(&v, e, 4);
+            *reinterpret_cast<uint32_t*>(smem + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) +
+                                         swizzled(r, piece & 7) + 4 * (lane & 3)) = v;
+          }
+        }
+        __syncwarp();
+        const bool out_aligned = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+#pragma unroll 4
+        for (int k = 0; k < kLoads; ++k) {
+          const int in_warp = k * kRowsAtOnce + lane / kRowLanes, r = m * kRowsTile + row0 + in_warp, piece = lane % kRowLanes;
+          if (r >= w.row_count) continue;
+          const uint32_t token = (w.block_row0 + r) / shared, in_group = w.block_row0 + r - token * shared;
+          const int64_t out_row = (w.q.row0 + token) * a.heads + w.head * shared + in_group;
+          const uint4 v = *reinterpret_cast<const uint4*>(smem + L::off_q + m * L::kQBytes + (piece >> 3) * (kRowsTile * 128) +
+                                                          swizzled(row0 + in_warp, piece & 7));
+          T* const out = static_cast<T*>(a.out) + out_row * kDim + piece * 8;
+          if (out_aligned) {
+            *reinterpret_cast<uint4*>(out) = v;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) out[i] = reinterpret_cast<const T*>(&v)[i];
+          }
+        }
+        if (a.lse && (lane & 3) == 0) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int r = m * kRowsTile + row0 + 8 * k + (lane >> 2);
+            if (r >= w.row_count) continue;
+            const uint32_t token = (w.block_row0 + r) / shared, in_group = w.block_row0 + r - token * shared;
+            const float reference = rows.top[k] == -INFINITY ? 0.0F : rows.top[k] - kLift;
+            a.lse[(w.q.row0 + token) * a.heads + w.head * shared + in_group] =
+                !ok ? NAN : sum[k] == 0.0F ? -INFINITY : (reference + __log2f(sum[k])) * 0.693147181F;
+          }
         }
       }
-    }
+    } while (next_list(false));
   } else if (warp < kMmaWarp) {
+    if constexpr (kSparse) registers_inc<88>();
     // =================== unpacking ===================
     // Keys: lane (g, t) takes 16 bytes t (at D = 128) of tokens g, g + 8, .. of its warp's 32.
     const int uw = warp - kUnpackWarp0, g = lane >> 2, t = lane & 3;
@@ -611,10 +890,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
     uint32_t word[4][kWords];
     float ks = 0.0F, vs = 0.0F;
     bool seen = false;
-    int page[2] = {ask_page(tile_start(0) + 32 * uw), ask_page(tile_start(0) + 32 * uw + 16)};
-    auto load_keys = [&](int i) {
-      const int j = tile_start(i) + 32 * uw;
-      const int64_t v[2] = {vector_of(page[0], j), vector_of(page[1], j + 16)};
+    int page[2] = {-1, -1};
+    auto load_keys = [&](const Work& w, int i) {
+      const int j = w.tile_start<kSparse>(i) + 32 * uw;
+      const int64_t v[2] = {vector_of(w, page[0], j), vector_of(w, page[1], j + 16)};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint8_t* src = c.codes[0] + (v[k >> 1] + 8 * (k & 1) + g) * (kDim / 2) + t * (kDim / 8);
@@ -629,22 +908,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
       const int mine = j + lane;
       const int64_t at = (lane < 16 ? v[0] : v[1]) + (lane & 15);
       seen = static_cast<uint32_t>(lane < 16 ? page[0] : page[1]) < static_cast<uint32_t>(c.num_pages) &&
-             (mine >= any_first || (kSparse && mine < a.sinks)) && mine <= any_last;
+             (mine >= w.any_first || (kSparse && mine < a.sinks)) && mine <= w.any_last;
       ks = __ldg(c.scales[0] + at);
       vs = __ldg(c.scales[1] + at);
-      const int next = kSparse ? tile_start(i + 1) + 32 * uw : j + kTokens;
-      page[0] = ask_page(next);
-      page[1] = ask_page(next + 16);
+      const int next = kSparse ? w.tile_start<kSparse>(i + 1) + 32 * uw : j + kTokens;
+      page[0] = ask_page(w, next);
+      page[1] = ask_page(w, next + 16);
     };
     // Values: a lane takes 8 tokens and 8 or 16 dimensions.
     constexpr int kValueWords = kDim / 64;                  // 8-dimension words of a token, per lane
     const int group = (uw >> 1) * 8 + (lane & 7);           // its 8 tokens
     const int piece = (uw & 1) * 4 + (lane >> 3);           // its words: piece * kValueWords and on
     uint32_t value[8][kValueWords];
-    int value_page = ask_page(tile_start(0) + (group >> 1) * 16);
-    auto load_values = [&](int i) {
-      const int j = tile_start(i) + (group >> 1) * 16;
-      const uint8_t* src = c.codes[1] + (vector_of(value_page, j) + 8 * (group & 1)) * (kDim / 2) + piece * (4 * kValueWords);
+    int value_page = -1;
+    auto load_values = [&](const Work& w, int i) {
+      const int j = w.tile_start<kSparse>(i) + (group >> 1) * 16;
+      const uint8_t* src = c.codes[1] + (vector_of(w, value_page, j) + 8 * (group & 1)) * (kDim / 2) + piece * (4 * kValueWords);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if constexpr (kValueWords == 2) {
@@ -654,82 +933,108 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
           value[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * (kDim / 2)));
         }
       }
-      value_page = ask_page(kSparse ? tile_start(i + 1) + (group >> 1) * 16 : j + kTokens);
+      value_page = ask_page(w, kSparse ? w.tile_start<kSparse>(i + 1) + (group >> 1) * 16 : j + kTokens);
     };
-    if (tiles > 0) {
-      load_keys(0);
-      load_values(0);
-    }
-    for (int i = 0; i < tiles; ++i) {
-      const int s = i & 1;
-      const uint32_t parity = ((i >> 1) - 1) & 1;
-      if (i >= kStages) {
-        const bool ok = mbar_wait(&k_empty[s], parity, abort_flag) && mbar_wait(&meta_empty[s], parity, abort_flag);
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      }
-      const uint32_t key_dst = base + L::off_k + s * L::kTileBytes;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int token = 32 * uw + 8 * k + g;
-#pragma unroll
-        for (int j = 0; j < kWords; ++j) {
-          // Lanes two apart lie in the two halves of a row: they take their words in another order, off the same banks.
-          const int jj = kWords == 4 ? j ^ (t & 2) : j;
-          uint32_t w = word[k][j];
-          if constexpr (kWords == 4) w = (t & 2) ? word[k][j ^ 2] : w;
-          const int at = t * kWords + jj;  // word of the row
-          store16(key_dst + (at >> 3) * (kTokens * 128) + swizzled(token, at & 7), codes_exact<0>(w), codes_exact<1>(w),
-                  codes_exact<2>(w), codes_exact<3>(w));
+    bool ok = true;
+    do {
+      for (int segment = 0; segment < count && ok; ++segment) {
+        const Work& w = work(segment);
+        if (w.tiles > 0) {
+          page[0] = ask_page(w, w.tile_start<kSparse>(0) + 32 * uw);
+          page[1] = ask_page(w, w.tile_start<kSparse>(0) + 32 * uw + 16);
+          value_page = ask_page(w, w.tile_start<kSparse>(0) + (group >> 1) * 16);
+          load_keys(w, 0);
+          load_values(w, 0);
         }
-      }
-      float* const ms = meta + s * 3 * kMetaFloats + meta_at(32 * uw + lane);
-      if (seen && vs == 1.0F &&
-          zero_value<kDim>(c.codes[1], pages, c.heads, head, c.page_shift, tile_start(i) + 32 * uw + lane))
-        vs = 0.0F;
-      ms[0] = seen ? ks : 0.0F;
-      ms[kMetaFloats] = seen ? vs : 0.0F;
-      ms[2 * kMetaFloats] = seen ? scale_exponent(vs, a.least_exponent, most_exponent(kLift)) : -INFINITY;
-      const uint32_t all = __ballot_sync(0xFFFFFFFFu, seen);
-      if (lane == 0) flags[4 * s + uw] = ~all;
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[s]);
-      if (i + 1 < tiles) load_keys(i + 1);
+        for (int i = 0; i < w.tiles; ++i) {
+          const int it = kSparse ? w.done + i : i, s = it & 1;
+          const uint32_t parity = ((it >> 1) - 1) & 1;
+          if (it >= kStages) {
+            ok = mbar_wait(&k_empty[s], parity, abort_flag) && mbar_wait(&meta_empty[s], parity, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+          }
+          const uint32_t key_dst = base + L::off_k + s * L::kTileBytes;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int token = 32 * uw + 8 * k + g;
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+              // Lanes two apart lie in the two halves of a row: they take their words in another order, off the same banks.
+              const int jj = kWords == 4 ? j ^ (t & 2) : j;
+              uint32_t w = word[k][j];
+              if constexpr (kWords == 4) w = (t & 2) ? word[k][j ^ 2] : w;
+              const int at = t * kWords + jj;  // word of the row
+              store16(key_dst + (at >> 3) * (kTokens * 128) + swizzled(token, at & 7), codes_exact<0>(w), codes_exact<1>(w),
+                      codes_exact<2>(w), codes_exact<3>(w));
+            }
+          }
+          float* const ms = meta + s * 3 * kMetaFloats + meta_at(32 * uw + lane);
+          if (seen && vs == 1.0F &&
+              zero_value<kDim>(c.codes[1], a.page_table + w.b * a.table_stride, c.heads, w.head, c.page_shift,
+                               w.tile_start<kSparse>(i) + 32 * uw + lane))
+            vs = 0.0F;
+          ms[0] = seen ? ks : 0.0F;
+          ms[kMetaFloats] = seen ? vs : 0.0F;
+          ms[2 * kMetaFloats] = seen ? scale_exponent(vs, a.least_exponent, most_exponent(kLift)) : -INFINITY;
+          const uint32_t all = __ballot_sync(0xFFFFFFFFu, seen);
+          if (lane == 0) flags[4 * s + uw] = ~all;
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&k_full[s]);
+          if (i + 1 < w.tiles) load_keys(w, i + 1);
 
-      if (i >= kStages) {
-        const bool ok = mbar_wait(&v_empty[s], parity, abort_flag);
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      }
-      // Row of a dimension: 64 tokens, 128 bytes; this lane's 8 tokens are one 16-byte chunk.
-      const uint32_t dst = base + L::off_v + s * L::kTileBytes + (group >> 3) * (kDim * 128);
+          if (it >= kStages) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&v_empty[s], parity, abort_flag));
+            if (!ok) break;
+          }
+          // Row of a dimension: 64 tokens, 128 bytes; this lane's 8 tokens are one 16-byte chunk.
+          const uint32_t dst = base + L::off_v + s * L::kTileBytes + (group >> 3) * (kDim * 128);
 #pragma unroll
-      for (int j = 0; j < kValueWords; ++j) {
-        uint32_t x[4], y[4];
+          for (int j = 0; j < kValueWords; ++j) {
+            uint32_t x[4], y[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[k] = __byte_perm(value[2 * k][j], value[2 * k + 1][j], 0x5410);
-          y[k] = __byte_perm(value[2 * k][j], value[2 * k + 1][j], 0x7632);
-        }
-        const int d = (piece * kValueWords + j) * 8, chunk = group & 7;
-        store16(dst + swizzled(d + 0, chunk), codes_exact<0>(x[0]), codes_exact<0>(x[1]), codes_exact<0>(x[2]), codes_exact<0>(x[3]));
-        store16(dst + swizzled(d + 1, chunk), codes_exact<1>(x[0]), codes_exact<1>(x[1]), codes_exact<1>(x[2]), codes_exact<1>(x[3]));
-        store16(dst + swizzled(d + 2, chunk), codes_exact<2>(x[0]), codes_exact<2>(x[1]), codes_exact<2>(x[2]), codes_exact<2>(x[3]));
-        store16(dst + swizzled(d + 3, chunk), codes_exact<3>(x[0]), codes_exact<3>(x[1]), codes_exact<3>(x[2]), codes_exact<3>(x[3]));
-        store16(dst + swizzled(d + 4, chunk), codes_exact<0>(y[0]), codes_exact<0>(y[1]), codes_exact<0>(y[2]), codes_exact<0>(y[3]));
-        store16(dst + swizzled(d + 5, chunk), codes_exact<1>(y[0]), codes_exact<1>(y[1]), codes_exact<1>(y[2]), codes_exact<1>(y[3]));
-        store16(dst + swizzled(d + 6, chunk), codes_exact<2>(y[0]), codes_exact<2>(y[1]), codes_exact<2>(y[2]), codes_exact<2>(y[3]));
-        store16(dst + swizzled(d + 7, chunk), codes_exact<3>(y[0]), codes_exact<3>(y[1]), codes_exact<3>(y[2]), codes_exact<3>(y[3]));
+            for (int k = 0; k < 4; ++k) {
+              x[k] = __byte_perm(value[2 * k][j], value[2 * k + 1][j], 0x5410);
+              y[k] = __byte_perm(value[2 * k][j], value[2 * k + 1][j], 0x7632);
+            }
+            const int d = (piece * kValueWords + j) * 8, chunk = group & 7;
+            store16(dst + swizzled(d + 0, chunk), codes_exact<0>(x[0]), codes_exact<0>(x[1]), codes_exact<0>(x[2]), codes_exact<0>(x[3]));
+            store16(dst + swizzled(d + 1, chunk), codes_exact<1>(x[0]), codes_exact<1>(x[1]), codes_exact<1>(x[2]), codes_exact<1>(x[3]));
+            store16(dst + swizzled(d + 2, chunk), codes_exact<2>(x[0]), codes_exact<2>(x[1]), codes_exact<2>(x[2]), codes_exact<2>(x[3]));
+            store16(dst + swizzled(d + 3, chunk), codes_exact<3>(x[0]), codes_exact<3>(x[1]), codes_exact<3>(x[2]), codes_exact<3>(x[3]));
+            store16(dst + swizzled(d + 4, chunk), codes_exact<0>(y[0]), codes_exact<0>(y[1]), codes_exact<0>(y[2]), codes_exact<0>(y[3]));
+            store16(dst + swizzled(d + 5, chunk), codes_exact<1>(y[0]), codes_exact<1>(y[1]), codes_exact<1>(y[2]), codes_exact<1>(y[3]));
+            store16(dst + swizzled(d + 6, chunk), codes_exact<2>(y[0]), codes_exact<2>(y[1]), codes_exact<2>(y[2]), codes_exact<2>(y[3]));
+            store16(dst + swizzled(d + 7, chunk), codes_exact<3>(y[0]), codes_exact<3>(y[1]), codes_exact<3>(y[2]), codes_exact<3>(y[3]));
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[s]);
+          if (i + 1 < w.tiles) load_values(w, i + 1);
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[s]);
-      if (i + 1 < tiles) load_values(i + 1);
-    }
+      }
+    } while (next_list(false));
     // These warps are done first.
-    if (a.fill)
-      kv4_fill_rows<T>(a, kDim, b, kv4_sequence(a, c.page_shift, b), share, shares, threadIdx.x - kUnpackWarp0 * 32,
-                       (kMmaWarp - kUnpackWarp0) * 32);
-  } else if (warp - kMmaWarp < tiles_m && tiles > 0) {
+    if (a.fill) {
+      constexpr int kFillThreads = (kMmaWarp - kUnpackWarp0) * 32;
+      const int thread = threadIdx.x - kUnpackWarp0 * 32;
+      if constexpr (kSparse) {
+        for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+          kv4_fill_rows<T>(a, kDim, b, kv4_sequence(a, c.page_shift, b), 0, 1, thread, kFillThreads);
+      } else {
+        kv4_fill_rows<T>(a, kDim, only.b, kv4_sequence(a, c.page_shift, only.b), share, shares, thread, kFillThreads);
+      }
+    }
+  } else if (kSparse || (warp - kMmaWarp < only.tiles_m && only.tiles > 0)) {
+    if constexpr (kSparse) {
+      registers_dec<40>();
+      if (warp >= kMmaWarp + 2) {  // fill up the warpgroup
+        while (next_list(true)) {
+        }
+        goto done;
+      }
+    }
     // =================== products of a row tile: one lane issues ===================
     const int m = warp - kMmaWarp;
     const uint32_t leader = elect();
@@ -746,6 +1051,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
         mma_ss(leader, s_tmem + half * (kTokens / 2), q_desc + at, k_desc + (s * L::kTileBytes >> 4) + rows + at, kInstrS, k > 0);
       }
     };
+    // (For both row tiles, where a segment of a line has one.)
+    uint32_t alone = 0;
+    auto commit_both = [&](uint64_t* bar) {
+      mma_commit(leader, bar);
+      if (kSparse) mma_commit(leader & alone, bar);
+    };
     auto first_half = [&](int s) {
       scores(s, s);
       mma_commit(leader, &s_half[m]);
@@ -753,36 +1064,50 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
     auto other_half = [&](int s) {
       scores(s, s ^ 1);
       mma_commit(leader, &s_full[m]);
-      mma_commit(leader, &k_empty[s]);
+      commit_both(&k_empty[s]);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0;
     };
-    bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
-    if (ok) {
-      tc_fence_after();
-      first_half(0);
-      other_half(0);
-    }
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int s = i & 1;
-      const bool more = i + 1 < tiles;
-      // Operands first, which are early: nothing but the products is then between probabilities and scores.
-      ok = wait(&v_full[s], (i >> 1) & 1) && (!more || wait(&k_full[s ^ 1], ((i + 1) >> 1) & 1)) && wait(&p_full[m], i & 1);
-      if (!ok) break;
-      tc_fence_after();
-      if (more) first_half(s ^ 1);
-      const uint32_t p_tmem = s_tmem + s * (kTokens / 2);
+    bool ok = true;
+    do {
+      for (int segment = 0; segment < count && ok; ++segment) {
+        const Work& w = work(segment);
+        if (kSparse && w.tiles == 0) continue;
+        alone = w.tiles_m == 1;
+        ok = wait(q_full, kSparse ? w.segments & 1 : 0);
+        if (kSparse && m >= w.tiles_m) continue;
+        const int start = kSparse ? w.done : 0;
+        ok = ok && wait(&k_full[start & 1], (start >> 1) & 1);
+        if (ok) {
+          tc_fence_after();
+          first_half(start & 1);
+          other_half(start & 1);
+        }
+        for (int i = 0; i < w.tiles && ok; ++i) {
+          const int it = kSparse ? w.done + i : i, s = it & 1;
+          const bool more = i + 1 < w.tiles;
+          // Operands first, which are early: nothing but the products is then between probabilities and scores.
+          ok = wait(&v_full[s], (it >> 1) & 1) && (!more || wait(&k_full[s ^ 1], ((it + 1) >> 1) & 1)) &&
+               wait(&p_full[m], (kSparse ? w.row_done[m] + i : i) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (more) first_half(s ^ 1);
+          const uint32_t p_tmem = s_tmem + s * (kTokens / 2);
 #pragma unroll
-      for (int k = 0; k < kTokens / 16; ++k) {  // 16 tokens
-        const uint32_t at = ((k >> 2) * (kDim * 128) + (k & 3) * 32) >> 4;
-        mma_ts(leader, o_tmem, p_tmem + 8 * (k ^ (4 * s)), v_desc + (s * L::kTileBytes >> 4) + at, kInstrO, i > 0 || k > 0);
+          for (int k = 0; k < kTokens / 16; ++k) {  // 16 tokens
+            const uint32_t at = ((k >> 2) * (kDim * 128) + (k & 3) * 32) >> 4;
+            mma_ts(leader, o_tmem, p_tmem + 8 * (k ^ (4 * s)), v_desc + (s * L::kTileBytes >> 4) + at, kInstrO, i > 0 || k > 0);
+          }
+          commit_both(&v_empty[s]);
+          if (more) other_half(s ^ 1);
+        }
+        if (ok) commit_both(o_full);
       }
-      mma_commit(leader, &v_empty[s]);
-      if (more) other_half(s ^ 1);
-    }
-    if (ok) mma_commit(leader, o_full);
+      __syncwarp();
+    } while (next_list(false));
   }
+done:
   __syncwarp();
   // After a wait was given up, products under way end by themselves: time for that before the tensor memory is freed.
   if (warp >= kMmaWarp && *abort_flag) {
@@ -796,21 +1121,98 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4View c, Kv4At
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// Adds the parts of the segments that a line's ranges cut, a block to an end of a range and a share of the rows: it works
+// where that end is the first one inside its segment, each warp on a row, the parts in their order.
+constexpr int kJoinWarps = 8;
+constexpr int kJoinShares = 16;
+template <class T, int kDim>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4View c, Kv4Attend a, uint32_t shared, int64_t blocks) {
+  constexpr int kPer = kDim / 32;
+#if __CUDA_ARCH__ >= 900
+  cudaGridDependencySynchronize();
+#endif
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t* const starts = static_cast<const int64_t*>(a.workspace);
+  const int64_t total = starts[a.batch], n = ranges(total, blocks), end = blockIdx.x + 1;
+  if (end >= n) return;
+  const int64_t u = range_start(total, end, n);
+  int lo = 0, hi = a.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  const Kv4Sequence q = kv4_sequence(a, c.page_shift, lo);
+  const Line l = line_of(a, q, shared);
+  const int64_t segment = (u - starts[lo]) / l.units, u0 = starts[lo] + segment * l.units;
+  const Work w = segment_of(a, shared, q, l, lo, segment);
+  // Ranges that hold tiles of the segment.
+  const int64_t c0 = range_of(total, u0, n), c1 = range_of(total, u0 + max(1, w.tiles) - 1, n);
+  if (c0 + 1 != end || c1 <= c0) return;
+  const float* const base = line_parts(a);
+  for (int r = blockIdx.y * kJoinWarps + warp; r < w.row_count; r += kJoinShares * kJoinWarps) {
+    float m = -INFINITY, sum = 0.0F, v[kPer];
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) v[d] = 0.0F;
+    for (int64_t k = c0; k <= c1; ++k) {
+      const float* const part = base + (2 * k + (k == c0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
+      const float2 st = *reinterpret_cast<const float2*>(part + kBlockRows * kDim + 2 * r);
+      if (st.y == 0.0F) continue;  // the part's tiles had nothing for the row: its sums may not have been written
+      float x[kPer];
+      if constexpr (kPer == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(part + r * kDim + lane * kPer);
+      else *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(part + r * kDim + lane * kPer);
+      const float next = fmaxf(m, st.x), old = fade_to(m, next), f = fade_to(st.x, next);
+      m = next;
+      sum = sum * old + f * st.y;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) v[d] = v[d] * old + f * x[d];
+    }
+    const float inv = sum == 0.0F ? 0.0F : 1.0F / sum;
+    const uint32_t token = (w.block_row0 + r) / shared, in_group = w.block_row0 + r - token * shared;
+    const int64_t at = (q.row0 + token) * a.heads + w.head * shared + in_group;
+    T* const out = static_cast<T*>(a.out) + at * kDim + lane * kPer;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) out[d] = from_f32<T>(v[d] * inv);
+    if (a.lse && lane == 0) a.lse[at] = sum == 0.0F ? -INFINITY : ((m == -INFINITY ? 0.0F : m - kLift) + __log2f(sum)) * 0.693147181F;
+  }
+}
+
+// Blocks of a line: one an SM, and no more than there can be tiles.
+int64_t line_blocks(const Kv4View& c, const Kv4Attend& a) {
+  const int64_t row_blocks = (static_cast<int64_t>(a.max_rows) * (a.heads / c.heads) + kBlockRows - 1) / kBlockRows;
+  const int64_t tiles = std::max<int64_t>(1, ((static_cast<int64_t>(a.max_pages) << c.page_shift) + kTokens - 1) / kTokens);
+  const int64_t segments = row_blocks * a.batch * c.heads;
+  return segments >= sm_count() ? sm_count() : std::min<int64_t>(sm_count(), segments * tiles);
+}
+
 template <class T, int kDim, bool kSparse>
 void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
   Kv4Attend a = given;
   keep_sums_finite(a, c.page_shift, kLift);
   const int shared = a.heads / c.heads;
   const int64_t row_blocks = (static_cast<int64_t>(a.max_rows) * shared + kBlockRows - 1) / kBlockRows;
-  const int64_t blocks = row_blocks * a.batch * c.heads;
-  if (blocks > INT_MAX) throw InvalidArgument("batch * heads * query rows are too many for one call");
+  const int64_t blocks = kSparse ? line_blocks(c, a) : row_blocks * a.batch * c.heads;
+  if (row_blocks * a.batch * c.heads > INT_MAX) throw InvalidArgument("batch * heads * query rows are too many for one call");
   const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
   allow_dynamic_shared<kv4_chunk_kernel<T, kDim, kSparse>>(Layout<kDim>::kBytes, "shared memory of the chunk attention kernel");
-  kv4_chunk_kernel<T, kDim, kSparse><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
+  kv4_chunk_kernel<T, kDim, kSparse><<<static_cast<unsigned>(blocks), kSparse ? kLineThreads : kThreads, Layout<kDim>::kBytes, stream>>>(
       c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
   count_launch();
   check(cudaGetLastError(), "launch chunk attention kernel");
+  if (!kSparse || blocks == 1) return;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks - 1), kJoinShares);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  check(cudaLaunchKernelEx(&cfg, kv4_chunk_join_kernel<T, kDim>, c, a, static_cast<uint32_t>(shared), blocks),
+        "launch chunk attention join kernel");
+  count_launch();
 }
 
 template <class T>
@@ -824,6 +1226,11 @@ void launch_typed(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
 
 // Head dimension 256 would need 768 columns of tensor memory.
 bool kv4_chunk_supported(const Kv4View& c) { return c.dim <= 128; }
+
+size_t kv4_chunk_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
+  if (a.sinks == 0 && !a.ancestors) return 0;
+  return starts_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(line_blocks(c, a)) * partial_floats(kBlockRows, c.dim);
+}
 
 void launch_kv4_chunk(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
   if (a.type == kElemF16) launch_typed<__half>(c, a, stream);

@@ -183,6 +183,24 @@ __device__ __forceinline__ Kv4Runs kv4_runs(const Kv4Attend& a, int pos0, int st
   return r;
 }
 
+// A line of work units cut into equal ranges.  Of n = min(blocks, total) ranges, range c is
+// [c total / n, (c + 1) total / n): none is empty.  Where sequences start on the line ([batch + 1], the last is its end)
+// lies at the head of a workspace whose partial sums follow.
+__host__ __device__ __forceinline__ size_t starts_bytes(int64_t batch) {
+  return (static_cast<size_t>(batch + 1) * sizeof(int64_t) + 127) & ~static_cast<size_t>(127);
+}
+__device__ __forceinline__ float* line_parts(const Kv4Attend& a) {
+  return reinterpret_cast<float*>(static_cast<char*>(a.workspace) + starts_bytes(a.batch));
+}
+__device__ __forceinline__ int64_t ranges(int64_t total, int64_t blocks) {
+  return total < blocks ? (total > 0 ? total : 1) : blocks;
+}
+__device__ __forceinline__ int64_t range_start(int64_t total, int64_t c, int64_t n) { return c * total / n; }
+// The range that holds unit u.
+__device__ __forceinline__ int64_t range_of(int64_t total, int64_t u, int64_t n) { return ((u + 1) * n - 1) / total; }
+// Partial sums of one segment's rows: rows x dim unnormalised outputs, then (reference, sum) per row.
+__host__ __device__ constexpr int partial_floats(int rows, int dim) { return rows * dim + 2 * rows; }
+
 // A block's `share` of `shares` of rows lo .. hi of an output (`width` elements a row) and of their log-sum-exp (`heads` a row)
 // to one value each.  (Out of line, as seldom run: the kernels' own code then lies together.)
 template <class T>
@@ -270,6 +288,18 @@ void allow_dynamic_shared(int bytes, const char* what) {
   if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
   check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
   done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+inline int sm_count() {
+  static std::atomic<int> known{0};
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    int dev = 0;
+    check(cudaGetDevice(&dev), "get device");
+    check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "SM count");
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 struct W4View {

@@ -150,6 +150,15 @@ def test_sinks_of_many_sequences(batch):
     _run(64, 1, 2, 16, "bf16", [(37 * b) % 900 for b in range(batch)], window=100, sinks=20, seed=batch)
 
 
+@pytest.mark.parametrize("batch,heads,long", [(300, 8, 0), (700, 4, 3000)])
+def test_more_short_sequences_than_a_block_lists_at_once(engine, batch, heads, long):
+    """Hundreds of segments of a tile for each block, and (`long`) a few of many tiles among them."""
+    lengths = [long if long and b % 99 == 7 else (7 * b) % 45 for b in range(batch)]
+    rows = [b % 4 for b in range(batch)]
+    _run(64, heads, 2, 16, "f16", lengths, rows=rows, window=600, sinks=9, seed=batch)
+    _run(64, heads, 2, 16, "f16", lengths, rows=rows, trees=[_tree(r, r) for r in rows], seed=batch)
+
+
 @pytest.mark.parametrize("dtype,dim,shared", [("f16", 64, 1), ("bf16", 128, 4), ("f16", 128, 7), ("bf16", 256, 2)])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (40, 3), (300, 64)])
 def test_trees(engine, dtype, dim, shared, window, sinks):
