@@ -8,6 +8,7 @@
 //   Bound: memory, every element is read and written once.  A block has a few tokens: their sines and cosines are formed
 //   once, in shared memory, for all heads, while the first vectors are on their way.
 #include <algorithm>
+#include <climits>
 
 #include "quant4.cuh"
 #include "rotary.cuh"
@@ -15,9 +16,11 @@
 namespace msb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTurns = 512;  // sines and cosines of a block, at most
-constexpr int kBatch = 4;    // items of a thread on their way together
+// Threads of a block, at most: a vector of 1,024 dimensions has as many pieces at most.
+constexpr int most_threads(int per) { return per == 1 ? 1024 : 256; }
+constexpr int kTurns = 1024;  // sines and cosines of a block, at most
+constexpr int kBatch = 2;     // vectors of a thread on their way together
+constexpr int kHeads = 4;     // of a thread, about
 
 // kPer consecutive elements.
 template <class T, int kPer>
@@ -50,101 +53,102 @@ __device__ __forceinline__ float2 turn(const Rotate& a, int64_t token, int pair)
   return r;
 }
 
-// kPer: elements that a thread has of either half of its pairs (halves), or in all (neighbours): 16 bytes, or, where
-// something does not start on 16 bytes, one pair.
+// How a call's blocks share its vectors: those before `blocks` of the first have queries, the others keys.
+struct Split {
+  int64_t blocks;
+  int tokens[2];      // of a block
+  int head_lanes[2];
+  int pieces;         // of a vector
+  int turning;        // the first of these turn, the others are copied
+};
+// A thread has one piece of one token's vectors, in every `head_lanes`-th head: its sines and cosines stay in registers.
+// kPer: elements of a piece, of either half of its pairs (halves), or in all (neighbours): 16 bytes, or, where something
+// does not start on 16 bytes, one pair.
 template <class T, int kPer, bool kNeighbours>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(Rotate a, int block_tokens, int pieces, int turning) {
-  constexpr int kVec = kNeighbours && kPer == 1 ? 1 : kPer;
+__global__ void __launch_bounds__(most_threads(kPer), kPer == 1 ? 1 : 4) rotate_kernel(const __grid_constant__ Rotate a, const __grid_constant__ Split c) {
+  constexpr bool kTwoParts = !kNeighbours || kPer == 1;   // a piece's elements lie in two places
+  constexpr int kPairs = kTwoParts ? kPer : kPer / 2;     // of a piece
   __shared__ float2 turns[kTurns];
-  const int heads = a.heads[0] + a.heads[1];
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * block_tokens;
+  const int which = blockIdx.x >= c.blocks;
+  const int heads = a.heads[which], head_lanes = c.head_lanes[which], block_tokens = c.tokens[which];
+  const int64_t token0 = (static_cast<int64_t>(blockIdx.x) - (which ? c.blocks : 0)) * block_tokens;
   const int tokens = static_cast<int>(min(static_cast<int64_t>(block_tokens), a.tokens - token0));
-  const int items = tokens * heads * pieces;
-  struct Item {
-    int token, which, head, piece;
-  };
-  auto item_of = [&](int i) {
-    Item r;
-    const int vector = i / pieces;
-    r.piece = i - vector * pieces;
-    r.token = vector / heads;
-    const int head = vector - r.token * heads;
-    r.which = head >= a.heads[0];
-    r.head = r.which ? head - a.heads[0] : head;
-    return r;
-  };
-  // Where a piece's elements start in its vector, and how far its second part lies from its first.  Of the pieces the
-  // first `turning` turn; the others are copied.
-  auto place = [&](int piece) {
-    if (kNeighbours && kPer == 1) return piece < turning ? 2 * piece : 2 * a.half + (piece - turning);
-    if (kNeighbours) return piece * kPer;
-    return piece < turning ? piece * kPer : 2 * a.half + (piece - turning) * kPer;
-  };
-  constexpr bool kTwoParts = !kNeighbours || kPer == 1;
+  const int vector = threadIdx.x / c.pieces, piece = threadIdx.x - vector * c.pieces;
+  const int my_token = vector / head_lanes, head0 = vector - my_token * head_lanes;
+  const bool turns_it = piece < c.turning;
+  const int start = turns_it ? (kTwoParts && kNeighbours ? 2 * piece : piece * kPer) : 2 * a.half + (piece - c.turning) * kPer;
   const int apart = kNeighbours ? 1 : a.half;
-  Piece<T, kVec> x[kBatch][2];
-  auto load = [&](int base) {
+  const T* x = static_cast<const T*>(a.x[which]) + (token0 + my_token) * a.x_token[which] + head0 * a.x_head[which] + start;
+  T* y = static_cast<T*>(a.y[which]) + (token0 + my_token) * a.y_token[which] + head0 * a.y_head[which] + start;
+  const int64_t x_step = head_lanes * a.x_head[which], y_step = head_lanes * a.y_head[which];
+  int left = my_token < tokens ? (heads - head0 + head_lanes - 1) / head_lanes : 0;  // heads of this thread
+  Piece<T, kPer> v[kBatch][2];
+  auto load = [&]() {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int i = base + k * kThreads;
-      if (i >= items) continue;
-      const Item at = item_of(i);
-      const T* p = static_cast<const T*>(a.x[at.which]) + (token0 + at.token) * a.x_token[at.which] +
-                   at.head * a.x_head[at.which] + place(at.piece);
-      load_piece(x[k][0], p);
-      if (kTwoParts && at.piece < turning) load_piece(x[k][1], p + apart);
+      if (k >= left) break;
+      load_piece(v[k][0], x);
+      if (kTwoParts && turns_it) load_piece(v[k][1], x + apart);
+      x += x_step;
     }
   };
-  load(threadIdx.x);
-  for (int i = threadIdx.x; i < tokens * a.half; i += kThreads) {
+  load();
+  for (int i = threadIdx.x; i < tokens * a.half; i += blockDim.x) {
     const int token = i / a.half;
     turns[i] = turn(a, token0 + token, i - token * a.half);
   }
   __syncthreads();
-  for (int base = threadIdx.x; base < items; base += kBatch * kThreads) {
-    if (base != threadIdx.x) load(base);
+  if (left <= 0) return;
+  float2 t[kPairs];
+#pragma unroll
+  for (int e = 0; e < kPairs; ++e) t[e] = turns_it ? turns[my_token * a.half + piece * kPairs + e] : make_float2(1.0F, 0.0F);
+#pragma unroll 1
+  for (;;) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int i = base + k * kThreads;
-      if (i >= items) continue;
-      const Item at = item_of(i);
-      T* p = static_cast<T*>(a.y[at.which]) + (token0 + at.token) * a.y_token[at.which] + at.head * a.y_head[at.which] +
-             place(at.piece);
-      if (at.piece < turning) {
-        if constexpr (kTwoParts) {
+      if (k >= left) break;
+      if (turns_it) {
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            const float2 t = turns[at.token * a.half + at.piece * kVec + e];
-            const float u = to_f32(x[k][0].e[e]), v = to_f32(x[k][1].e[e]);
-            x[k][0].e[e] = from_f32<T>(u * t.x - v * t.y);
-            x[k][1].e[e] = from_f32<T>(u * t.y + v * t.x);
-          }
-          store_piece(p + apart, x[k][1]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kVec; e += 2) {
-            const float2 t = turns[at.token * a.half + (at.piece * kVec + e) / 2];
-            const float u = to_f32(x[k][0].e[e]), v = to_f32(x[k][0].e[e + 1]);
-            x[k][0].e[e] = from_f32<T>(u * t.x - v * t.y);
-            x[k][0].e[e + 1] = from_f32<T>(u * t.y + v * t.x);
-          }
+        for (int e = 0; e < kPairs; ++e) {
+          T& u = kTwoParts ? v[k][0].e[e] : v[k][0].e[2 * e];
+          T& w = kTwoParts ? v[k][1].e[e] : v[k][0].e[2 * e + 1];
+          const float fu = to_f32(u), fw = to_f32(w);
+          u = from_f32<T>(fu * t[e].x - fw * t[e].y);
+          w = from_f32<T>(fu * t[e].y + fw * t[e].x);
         }
+        if (kTwoParts) store_piece(y + apart, v[k][1]);
       }
-      store_piece(p, x[k][0]);
+      store_piece(y, v[k][0]);
+      y += y_step;
     }
+    left -= kBatch;
+    if (left <= 0) return;
+    load();
   }
 }
 
 template <class T, int kPer, bool kNeighbours>
 void launch_pairs(const Rotate& a, cudaStream_t stream) {
-  const int turned = 2 * a.half, heads = a.heads[0] + a.heads[1];
-  const int turning = kNeighbours && kPer > 1 ? turned / kPer : a.half / kPer;
-  const int pieces = turning + (a.dim - turned) / kPer;
-  // As many tokens to a block as give each thread an item of sines or a batch of vectors, whichever is less.
-  const int64_t items = static_cast<int64_t>(heads) * pieces;
-  int block_tokens = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kThreads / a.half, kBatch * kThreads / items)));
-  const int64_t blocks = (a.tokens + block_tokens - 1) / block_tokens;
-  rotate_kernel<T, kPer, kNeighbours><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a, block_tokens, pieces, turning);
+  const int turned = 2 * a.half;
+  Split c{};
+  c.turning = kNeighbours && kPer > 1 ? turned / kPer : a.half / kPer;
+  c.pieces = c.turning + (a.dim - turned) / kPer;
+  // Heads of a thread: some batches; few tokens spread over the SMs, one to a block.
+  const bool few = a.tokens <= 2 * sm_count();
+  constexpr int kWanted = 256;
+  int threads = std::min(kWanted, a.half);
+  int64_t blocks[2];
+  for (int w = 0; w < 2; ++w) {
+    c.head_lanes[w] = std::max(1, std::min(few ? a.heads[w] : (a.heads[w] + kHeads - 1) / kHeads, kWanted / c.pieces));
+    const int per_token = c.pieces * c.head_lanes[w];  // at most most_threads(kPer)
+    c.tokens[w] = few ? 1 : std::max(1, std::min(kWanted / per_token, kTurns / a.half));
+    blocks[w] = a.heads[w] > 0 ? (a.tokens + c.tokens[w] - 1) / c.tokens[w] : 0;
+    if (blocks[w] > 0) threads = std::max(threads, per_token * c.tokens[w]);
+  }
+  if (blocks[0] + blocks[1] > INT_MAX) throw InvalidArgument("tokens are too many for one call");
+  c.blocks = blocks[0];
+  threads = (threads + 31) / 32 * 32;
+  rotate_kernel<T, kPer, kNeighbours><<<static_cast<unsigned>(blocks[0] + blocks[1]), threads, 0, stream>>>(a, c);
 }
 
 template <class T>
