@@ -195,6 +195,8 @@ __device__ __forceinline__ int64_t moved_vector(const Kv4View& c, int64_t slot, 
 __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Move a) {
   const int parts = c.dim / 64 + 1, part = blockIdx.x % parts, which = blockIdx.x / parts, head = blockIdx.y;
   const int64_t slots = c.num_pages << c.page_shift;
+  uint8_t* const codes = which ? c.codes[1] : c.codes[0];
+  float* const scales = which ? c.scales[1] : c.scales[0];
   int64_t to[kMoves];
   uint4 x[kMoves][2];
 #pragma unroll
@@ -207,9 +209,9 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Mo
     to[k] = moved_vector(c, target, head);
     const int64_t from = moved_vector(c, source, head);
     if (part == 0) {
-      x[k][0].x = __float_as_uint(c.scales[which][from]);
+      x[k][0].x = __float_as_uint(scales[from]);
     } else {
-      const uint4* p = reinterpret_cast<const uint4*>(c.codes[which] + from * (c.dim / 2) + (part - 1) * 32);
+      const uint4* p = reinterpret_cast<const uint4*>(codes + from * (c.dim / 2) + (part - 1) * 32);
       x[k][0] = p[0];
       x[k][1] = p[1];
     }
@@ -219,34 +221,78 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Mo
   for (int k = 0; k < kMoves; ++k) {
     if (to[k] < 0) continue;
     if (part == 0) {
-      c.scales[which][to[k]] = __uint_as_float(x[k][0].x);
+      scales[to[k]] = __uint_as_float(x[k][0].x);
     } else {
-      uint4* p = reinterpret_cast<uint4*>(c.codes[which] + to[k] * (c.dim / 2) + (part - 1) * 32);
+      uint4* p = reinterpret_cast<uint4*>(codes + to[k] * (c.dim / 2) + (part - 1) * 32);
       p[0] = x[k][0];
       p[1] = x[k][1];
     }
   }
 }
-// More tokens: out to a workspace, [key or value][head][token] codes, then scales alike, and back in a second launch.
-// A thread has 16 bytes of codes, the first of a vector its scale too.
-template <bool kOut>
+// More tokens: out to a workspace, [key or value][head][token] codes, then scales alike, and back in a second launch, most
+// of it through L2.  A thread has 16 bytes of codes of kManyMoves vectors, asked for together, a vector's first
+// thread its scale too.
+constexpr int kManyMoves = 4;
+template <bool kOut, int kDim>
 __global__ void __launch_bounds__(kThreads) kv4_move_many_kernel(Kv4View c, Kv4Move a) {
-  const int lanes = c.dim / 32, head = blockIdx.y, which = blockIdx.z;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
-  const int lane = threadIdx.x % lanes;
-  if (i >= a.tokens) return;
-  const int64_t slots = c.num_pages << c.page_shift, source = __ldg(a.source + i), target = __ldg(a.target + i);
-  if (source < 0 || source >= slots || target < 0 || target >= slots) return;
-  const int64_t here = moved_vector(c, kOut ? source : target, head);
-  const int64_t there = (static_cast<int64_t>(which) * c.heads + head) * a.tokens + i;
-  uint4* const codes = reinterpret_cast<uint4*>(c.codes[which] + here * (c.dim / 2)) + lane;
-  uint4* const kept = static_cast<uint4*>(a.workspace) + there * lanes + lane;
-  float* const kept_scales = reinterpret_cast<float*>(static_cast<uint4*>(a.workspace) + 2 * c.heads * a.tokens * lanes);
-  if (kOut) *kept = *codes;
-  else *codes = *kept;
-  if (lane != 0) return;
-  if (kOut) kept_scales[there] = c.scales[which][here];
-  else c.scales[which][here] = kept_scales[there];
+  constexpr int kLanes = kDim / 32, kStep = kThreads / kLanes;
+  const int head = blockIdx.y, which = blockIdx.z, lane = threadIdx.x % kLanes;
+  uint8_t* const codes = which ? c.codes[1] : c.codes[0];
+  float* const scales = which ? c.scales[1] : c.scales[0];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kStep * kManyMoves) + threadIdx.x / kLanes;
+  const int64_t slots = c.num_pages << c.page_shift, kept0 = (static_cast<int64_t>(which) * c.heads + head) * a.tokens;
+  uint4* const kept = static_cast<uint4*>(a.workspace) + kept0 * kLanes + lane;
+  float* const kept_scales = reinterpret_cast<float*>(static_cast<uint4*>(a.workspace) + 2 * c.heads * a.tokens * kLanes) + kept0;
+  int64_t here[kManyMoves];  // -1: none
+#pragma unroll
+  for (int k = 0; k < kManyMoves; ++k) {
+    const int64_t i = first + k * kStep;
+    here[k] = -1;
+    if (i >= a.tokens) continue;
+    const int64_t source = __ldg(a.source + i), target = __ldg(a.target + i);
+    if (source < 0 || source >= slots || target < 0 || target >= slots) continue;
+    here[k] = moved_vector(c, kOut ? source : target, head);
+  }
+#if __CUDA_ARCH__ >= 900
+  if (kOut) cudaTriggerProgrammaticLaunchCompletion();
+  else cudaGridDependencySynchronize();
+#endif
+  uint4 x[kManyMoves];
+  float s[kManyMoves];
+#pragma unroll
+  for (int k = 0; k < kManyMoves; ++k) {
+    if (here[k] < 0) continue;
+    const int64_t i = first + k * kStep;
+    x[k] = kOut ? *(reinterpret_cast<const uint4*>(codes + here[k] * (kDim / 2)) + lane) : kept[i * kLanes];
+    if (lane == 0) s[k] = kOut ? scales[here[k]] : kept_scales[i];
+  }
+#pragma unroll
+  for (int k = 0; k < kManyMoves; ++k) {
+    if (here[k] < 0) continue;
+    const int64_t i = first + k * kStep;
+    if (kOut) kept[i * kLanes] = x[k];
+    else *(reinterpret_cast<uint4*>(codes + here[k] * (kDim / 2)) + lane) = x[k];
+    if (lane == 0) (kOut ? kept_scales[i] : scales[here[k]]) = s[k];
+  }
+}
+template <int kDim>
+void launch_move_many(const Kv4View& c, const Kv4Move& a, cudaStream_t stream) {
+  const int64_t per_block = kThreads / (kDim / 32) * kManyMoves;
+  const dim3 blocks(static_cast<unsigned>((a.tokens + per_block - 1) / per_block), static_cast<unsigned>(c.heads), 2);
+  kv4_move_many_kernel<true, kDim><<<blocks, kThreads, 0, stream>>>(c, a);
+  check(cudaGetLastError(), "launch cache move kernel");
+  // The second reads its slots while the first is at work.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = blocks;
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  check(cudaLaunchKernelEx(&cfg, kv4_move_many_kernel<false, kDim>, c, a), "launch cache move kernel");
+  count_launch(2);
 }
 
 template <class T, bool kAligned>
@@ -290,11 +336,9 @@ void launch_kv4_move(const Kv4View& c, const Kv4Move& a, cudaStream_t stream) {
     kv4_move_kernel<<<dim3(2 * (c.dim / 64 + 1), static_cast<unsigned>(c.heads)), kMoveThreads, 0, stream>>>(c, a);
     count_launch();
   } else {
-    const int64_t per_block = kThreads / (c.dim / 32);
-    const dim3 blocks(static_cast<unsigned>((a.tokens + per_block - 1) / per_block), static_cast<unsigned>(c.heads), 2);
-    kv4_move_many_kernel<true><<<blocks, kThreads, 0, stream>>>(c, a);
-    kv4_move_many_kernel<false><<<blocks, kThreads, 0, stream>>>(c, a);
-    count_launch(2);
+    if (c.dim == 64) launch_move_many<64>(c, a, stream);
+    else if (c.dim == 128) launch_move_many<128>(c, a, stream);
+    else launch_move_many<256>(c, a, stream);
   }
   check(cudaGetLastError(), "launch cache move kernel");
 }
