@@ -406,8 +406,8 @@ typedef struct msb_page_table {
 int msb_pages_workspace_bytes(const msb_page_table* table, int64_t rows, int64_t* bytes);
 /* Gives every sequence tokens[b] more tokens (a negative number: none): pages from the stack's top, in the sequences'
  * order, entered in the table; lengths grow.  The rows of the step, `rows` of them, lie in the sequences' order:
- * query_offsets [sequences + 1] their starts (held to `rows`), slots and positions [rows] where each is cached and its
- * place in the sequence.  A sequence whose pages do not fit its table row, whose rows pass `rows`, or that lacks pages
+ * query_offsets [sequences + 1] their starts (held to `rows`), slots and positions [rows] (16-byte aligned) where each is cached
+ * and its place in the sequence.  A sequence whose pages do not fit its table row, whose rows pass `rows`, or that lacks pages
  * where those before it have taken what there is, is refused: it keeps its length, its rows, and those past the last,
  * get -1. */
 int msb_pages_extend_device(const msb_page_table* table, const int32_t* tokens, int64_t rows, int32_t* query_offsets,

@@ -1780,8 +1780,8 @@ int msb_pages_extend_device(const msb_page_table* table, const int32_t* tokens, 
     if (!tokens || !query_offsets || (rows > 0 && (!slots || !positions))) throw InvalidArgument("NULL argument");
     check_address(tokens, 4, "tokens");
     check_address(query_offsets, 4, "query_offsets");
-    check_address(slots, 8, "slots");
-    check_address(positions, 4, "positions");
+    check_address(slots, 16, "slots");
+    check_address(positions, 16, "positions");
     check_pages_workspace(p, rows, workspace, workspace_bytes);
     DeviceGuard g(table->device);
     launch_pages_extend(p, PagesExtend{tokens, rows, query_offsets, slots, positions, workspace},
