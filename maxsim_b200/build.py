@@ -132,7 +132,7 @@ def build_binding() -> Path:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{base / 'include'}",
            f"-I{base / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
            f"-I{sysconfig.get_paths()['include']}", str(BINDING_SRC), "-o", str(tmp), f"-L{base / 'lib'}", f"-L{PKG}",
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING)
     _stamp().parent.mkdir(exist_ok=True)

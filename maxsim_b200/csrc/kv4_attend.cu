@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       row0 = static_cast<int>(segment % w.blocks) * kRows;
     }
     const int all_rows = w.q.rows * line.shared;
+    const bool tree_window = kSparse && a.ancestors && a.window > 0;
 
     // Rows: which tokens they see; lane (g, t) loads row g of each column tile, dimensions t * kDim / 4 and on.
     constexpr int kRaw = kKeyWords * 8 * sizeof(T) / 16;
@@ -361,7 +362,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
         last[nt][k] = INT_MAX;  // rows past the block are not written: no reason to mask for them
         if (rr < all_rows) {
           if constexpr (kSparse) {
-            const Kv4Seen seen = kv4_seen(a, w.q, rr / line.shared);
+            // (Of a tree's rows under a window the first one waits for their masks: below, when the copies are on their way.)
+            const Kv4Seen seen = tree_window ? Kv4Seen{max(0, max(0, w.q.pos0) - a.window), w.q.pos0 - 1} : kv4_seen(a, w.q, rr / line.shared);
             last[nt][k] = seen.last;
             first[nt][k] = seen.first;
           } else {
@@ -443,6 +445,18 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     for (int i = 0; i < kStages - 1; ++i) {
       copy_step(j0 + i * kTile, i, i);
       ask_pages(j0 + (i + 1) * kTile);
+    }
+    if (tree_window) {
+#pragma unroll
+      for (int nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int rr = row0 + nt * 8 + 2 * t + k;
+          if (rr < all_rows) first[nt][k] = kv4_seen(a, w.q, rr / line.shared).first;
+          every_first = max(every_first, first[nt][k]);
+        }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) every_first = max(every_first, __shfl_xor_sync(0xFFFFFFFFu, every_first, d));
     }
     // Queries, while the first copies are on their way.
     uint32_t q[kTiles][2 * kKeyWords][2];

@@ -598,17 +598,28 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
     do {
       for (int segment = 0; segment < count; ++segment) {
         const Work& w = work(segment);
-        if (m >= w.tiles_m) {
-          if constexpr (kSparse) {  // the other row tile's segment: passed together, as a wait may not fall a phase behind
-            if (w.tiles > 0) {
-              if (lane == 0) mbar_arrive(q_full);
-              ok = ok && mbar_wait(o_full, w.segments & 1, abort_flag);
-              ok = __all_sync(0xFFFFFFFFu, ok);
+        const int row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16;  // of the row tile, and its lane of tensor memory
+        if (kSparse ? m * kRowsTile + row0 >= w.row_count : m >= w.tiles_m) {
+          // No rows for this warp.  On a line it passes the segment with the others all the same, as no wait may fall a phase
+          // behind, and arrives for what it does not do (its rows' products are never read): the warps that have rows get
+          // its share of the issue slots.
+          if constexpr (kSparse) {
+            if (w.tiles == 0) continue;
+            if (lane == 0) mbar_arrive(q_full);
+            for (int i = 0; i < w.tiles && m < w.tiles_m && ok; ++i) {
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[m], (w.row_done[m] + i) & 1, abort_flag));
+              if (lane == 0 && ok) {
+                uint64_t* const bar = &meta_empty[(w.done + i) & 1];
+                mbar_arrive(bar);
+                if (w.tiles_m == 1) mbar_arrive(bar);
+                mbar_arrive(&p_full[m]);
+              }
             }
+            ok = ok && mbar_wait(o_full, w.segments & 1, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, ok);
           }
           continue;
         }
-        const int row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16;  // of the row tile, and its lane of tensor memory
         float* const row_factor = reinterpret_cast<float*>(smem + L::off_rows) + m * kRowsTile + row0;
         constexpr int kRowLanes = kDim / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 16 / kRowsAtOnce;
         // The warp's rows of the query tile, 8 dimensions a lane: scaled by a power of two to a maximum in [2^10, 2^11),
