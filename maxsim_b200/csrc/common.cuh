@@ -99,9 +99,44 @@ struct TopkFuse {
   bool done;                    // set when the fused path ran (otherwise the caller selects from scores)
 };
 
+// A launch that may start while the kernel before it on the stream ends: its first blocks are then in place when that one's
+// results are.  The kernel calls wait_for_previous() before it reads or writes any memory, in every thread.  With `cluster`,
+// in clusters of so many blocks.
+template <class... Params, class... Args>
+void launch_early(void (*kernel)(Params...), dim3 blocks, int threads, size_t shared, cudaStream_t stream, int cluster,
+                  const char* what, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = blocks;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  cfg.attrs = attributes;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+  count_launch();
+}
+
 // ---------------------------------------------------------------------------
 // Small device helpers.
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ void wait_for_previous() {
+#if __CUDA_ARCH__ >= 900
+  cudaGridDependencySynchronize();
+#endif
+}
+// From here on the kernel after this one may start; it waits for this one's end before it touches memory.  (After
+// wait_for_previous: no more than one kernel waits beside the one at work.)
+__device__ __forceinline__ void let_next_start() {
+#if __CUDA_ARCH__ >= 900
+  cudaTriggerProgrammaticLaunchCompletion();
+#endif
+}
 __device__ __forceinline__ uint32_t float_to_ordered(float f) {
   uint32_t u = __float_as_uint(f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);

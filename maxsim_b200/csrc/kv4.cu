@@ -194,6 +194,8 @@ __device__ __forceinline__ int64_t moved_vector(const Kv4View& c, int64_t slot, 
 }
 __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Move a) {
   const int parts = c.dim / 64 + 1, part = blockIdx.x % parts, which = blockIdx.x / parts, head = blockIdx.y;
+  wait_for_previous();
+  let_next_start();
   const int64_t slots = c.num_pages << c.page_shift;
   uint8_t* const codes = which ? c.codes[1] : c.codes[0];
   float* const scales = which ? c.scales[1] : c.scales[0];
@@ -243,6 +245,10 @@ __global__ void __launch_bounds__(kThreads) kv4_move_many_kernel(Kv4View c, Kv4M
   const int64_t slots = c.num_pages << c.page_shift, kept0 = (static_cast<int64_t>(which) * c.heads + head) * a.tokens;
   uint4* const kept = static_cast<uint4*>(a.workspace) + kept0 * kLanes + lane;
   float* const kept_scales = reinterpret_cast<float*>(static_cast<uint4*>(a.workspace) + 2 * c.heads * a.tokens * kLanes) + kept0;
+  if (kOut) {  // what the second pass reads before it waits is there when it starts
+    wait_for_previous();
+    let_next_start();
+  }
   int64_t here[kManyMoves];  // -1: none
 #pragma unroll
   for (int k = 0; k < kManyMoves; ++k) {
@@ -253,10 +259,7 @@ __global__ void __launch_bounds__(kThreads) kv4_move_many_kernel(Kv4View c, Kv4M
     if (source < 0 || source >= slots || target < 0 || target >= slots) continue;
     here[k] = moved_vector(c, kOut ? source : target, head);
   }
-#if __CUDA_ARCH__ >= 900
-  if (kOut) cudaTriggerProgrammaticLaunchCompletion();
-  else cudaGridDependencySynchronize();
-#endif
+  if (!kOut) wait_for_previous();
   uint4 x[kManyMoves];
   float s[kManyMoves];
 #pragma unroll
@@ -279,20 +282,9 @@ template <int kDim>
 void launch_move_many(const Kv4View& c, const Kv4Move& a, cudaStream_t stream) {
   const int64_t per_block = kThreads / (kDim / 32) * kManyMoves;
   const dim3 blocks(static_cast<unsigned>((a.tokens + per_block - 1) / per_block), static_cast<unsigned>(c.heads), 2);
-  kv4_move_many_kernel<true, kDim><<<blocks, kThreads, 0, stream>>>(c, a);
-  check(cudaGetLastError(), "launch cache move kernel");
-  // The second reads its slots while the first is at work.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = blocks;
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  check(cudaLaunchKernelEx(&cfg, kv4_move_many_kernel<false, kDim>, c, a), "launch cache move kernel");
-  count_launch(2);
+  launch_early(kv4_move_many_kernel<true, kDim>, blocks, kThreads, 0, stream, 0, "launch cache move kernel", c, a);
+  // The second reads its slots while the first is at work: neither writes them.
+  launch_early(kv4_move_many_kernel<false, kDim>, blocks, kThreads, 0, stream, 0, "launch cache move kernel", c, a);
 }
 
 template <class T, bool kAligned>
@@ -333,14 +325,13 @@ size_t kv4_move_workspace_bytes(const Kv4View& c, int64_t tokens) {
 void launch_kv4_move(const Kv4View& c, const Kv4Move& a, cudaStream_t stream) {
   if (a.tokens <= 0) return;
   if (a.tokens <= kMostMoved) {
-    kv4_move_kernel<<<dim3(2 * (c.dim / 64 + 1), static_cast<unsigned>(c.heads)), kMoveThreads, 0, stream>>>(c, a);
-    count_launch();
+    launch_early(kv4_move_kernel, dim3(2 * (c.dim / 64 + 1), static_cast<unsigned>(c.heads)), kMoveThreads, 0, stream, 0,
+                 "launch cache move kernel", c, a);
   } else {
     if (c.dim == 64) launch_move_many<64>(c, a, stream);
     else if (c.dim == 128) launch_move_many<128>(c, a, stream);
     else launch_move_many<256>(c, a, stream);
   }
-  check(cudaGetLastError(), "launch cache move kernel");
 }
 
 void launch_kv4_append(const Kv4View& c, const Kv4Append& a, cudaStream_t stream) {

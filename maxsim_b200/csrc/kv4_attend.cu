@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
   __shared__ float2 part_stats[kRows];   // of the block, for its cluster
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
 
+  if (kSparse) wait_for_previous();
   const int64_t block = blockIdx.x;
   int64_t unit = 0, unit_end = 1, before = 0;
   int b = 0;
@@ -945,6 +946,12 @@ void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cuda
   static_assert(kShared >= static_cast<int>(sizeof(float)) * kWarps * 8 * kTiles * (kDim + 4), "sums fit the ring");
   if (s.cluster > 0) {
     allow_dynamic_shared<kv4_attend_kernel<T, kDim, kTiles, true, kSparse>>(kShared, "shared memory of the cache attention kernel");
+    if constexpr (kSparse) {
+      launch_early(kv4_attend_kernel<T, kDim, kTiles, true, true>,
+                   dim3(static_cast<unsigned>(static_cast<int64_t>(s.row_blocks) * a.batch * c.heads * s.cluster)), kWarps * 32,
+                   kShared, stream, s.cluster, "launch cache attention kernel", c, a, line);
+      return;
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(s.row_blocks) * a.batch * c.heads * s.cluster));
     cfg.blockDim = dim3(kWarps * 32);
@@ -961,9 +968,14 @@ void launch_shape(const Kv4View& c, const Kv4Attend& given, const Shape& s, cuda
     return;
   }
   allow_dynamic_shared<kv4_attend_kernel<T, kDim, kTiles, false, kSparse>>(kShared, "shared memory of the cache attention kernel");
-  kv4_attend_kernel<T, kDim, kTiles, false, kSparse><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
-  count_launch();
-  check(cudaGetLastError(), "launch cache attention kernel");
+  if constexpr (kSparse) {
+    launch_early(kv4_attend_kernel<T, kDim, kTiles, false, true>, dim3(static_cast<unsigned>(s.blocks)), kWarps * 32, kShared, stream, 0,
+                 "launch cache attention kernel", c, a, line);
+  } else {
+    kv4_attend_kernel<T, kDim, kTiles, false, false><<<static_cast<unsigned>(s.blocks), kWarps * 32, kShared, stream>>>(c, a, line);
+    count_launch();
+    check(cudaGetLastError(), "launch cache attention kernel");
+  }
   if (!needs_join(c, a)) return;
   const int64_t rows = static_cast<int64_t>(a.max_rows) * a.heads;
   const int64_t segments = c.heads * ((static_cast<int64_t>(a.max_rows) * line.shared + line.block_rows - 1) / line.block_rows);

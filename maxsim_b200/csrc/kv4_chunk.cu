@@ -485,9 +485,8 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
   Work only{};
   int share = 0, shares = 1;
   if constexpr (kSparse) {
-#if __CUDA_ARCH__ >= 900
-    cudaTriggerProgrammaticLaunchCompletion();
-#endif
+    wait_for_previous();
+    let_next_start();
     const Place start = find_place(c, a, shared);
     if (threadIdx.x == 0) {
       place = start;
@@ -590,8 +589,12 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
     count = work_count;
     return count > 0;
   };
+  if constexpr (kSparse) {
+    // Of the 24 x 32 x 80 registers that a line's block is launched with: 20 warps' 88 and 4 warps' 40.
+    if (warp >= kMmaWarp) registers_dec<40>();
+    else registers_inc<88>();
+  }
   if (warp < kSoftWarps) {
-    if constexpr (kSparse) registers_inc<88>();
     // =================== softmax: a warp has 16 rows, a thread two of them and a quarter of their columns ===================
     const int m = warp >> 3;
     bool ok = true;
@@ -893,7 +896,6 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
       }
     } while (next_list(false));
   } else if (warp < kMmaWarp) {
-    if constexpr (kSparse) registers_inc<88>();
     // =================== unpacking ===================
     // Keys: lane (g, t) takes 16 bytes t (at D = 128) of tokens g, g + 8, .. of its warp's 32.
     const int uw = warp - kUnpackWarp0, g = lane >> 2, t = lane & 3;
@@ -1037,15 +1039,11 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
         kv4_fill_rows<T>(a, kDim, only.b, kv4_sequence(a, c.page_shift, only.b), share, shares, thread, kFillThreads);
       }
     }
-  } else if (kSparse || (warp - kMmaWarp < only.tiles_m && only.tiles > 0)) {
-    if constexpr (kSparse) {
-      registers_dec<40>();
-      if (warp >= kMmaWarp + 2) {  // fill up the warpgroup
-        while (next_list(true)) {
-        }
-        goto done;
-      }
+  } else if (warp >= kMmaWarp + 2) {
+    // They make a line's block whole warpgroups, and its lists.
+    while (next_list(true)) {
     }
+  } else if (kSparse || (warp - kMmaWarp < only.tiles_m && only.tiles > 0)) {
     // =================== products of a row tile: one lane issues ===================
     const int m = warp - kMmaWarp;
     const uint32_t leader = elect();
@@ -1118,7 +1116,6 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
       __syncwarp();
     } while (next_list(false));
   }
-done:
   __syncwarp();
   // After a wait was given up, products under way end by themselves: time for that before the tensor memory is freed.
   if (warp >= kMmaWarp && *abort_flag) {
@@ -1139,9 +1136,7 @@ constexpr int kJoinShares = 16;
 template <class T, int kDim>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4View c, Kv4Attend a, uint32_t shared, int64_t blocks) {
   constexpr int kPer = kDim / 32;
-#if __CUDA_ARCH__ >= 900
-  cudaGridDependencySynchronize();
-#endif
+  wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t* const starts = static_cast<const int64_t*>(a.workspace);
   const int64_t total = starts[a.batch], n = ranges(total, blocks), end = blockIdx.x + 1;
@@ -1207,23 +1202,18 @@ void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
   const uint64_t starts = reinterpret_cast<uintptr_t>(a.query) | static_cast<uint64_t>(a.q_row_stride) * sizeof(T) |
                           static_cast<uint64_t>(a.q_head_stride) * sizeof(T);
   allow_dynamic_shared<kv4_chunk_kernel<T, kDim, kSparse>>(Layout<kDim>::kBytes, "shared memory of the chunk attention kernel");
-  kv4_chunk_kernel<T, kDim, kSparse><<<static_cast<unsigned>(blocks), kSparse ? kLineThreads : kThreads, Layout<kDim>::kBytes, stream>>>(
-      c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
-  count_launch();
-  check(cudaGetLastError(), "launch chunk attention kernel");
-  if (!kSparse || blocks == 1) return;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks - 1), kJoinShares);
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  check(cudaLaunchKernelEx(&cfg, kv4_chunk_join_kernel<T, kDim>, c, a, static_cast<uint32_t>(shared), blocks),
-        "launch chunk attention join kernel");
-  count_launch();
+  if constexpr (kSparse) {
+    launch_early(kv4_chunk_kernel<T, kDim, true>, dim3(static_cast<unsigned>(blocks)), kLineThreads, Layout<kDim>::kBytes, stream, 0,
+                 "launch chunk attention kernel", c, a, static_cast<uint32_t>(shared), static_cast<int>(row_blocks), (starts & 15) == 0);
+    if (blocks > 1)
+      launch_early(kv4_chunk_join_kernel<T, kDim>, dim3(static_cast<unsigned>(blocks - 1), kJoinShares), kJoinWarps * 32, 0, stream, 0,
+                   "launch chunk attention join kernel", c, a, static_cast<uint32_t>(shared), blocks);
+  } else {
+    kv4_chunk_kernel<T, kDim, false><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
+        c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
+    count_launch();
+    check(cudaGetLastError(), "launch chunk attention kernel");
+  }
 }
 
 template <class T>

@@ -197,6 +197,8 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(Pages p, PagesExtend e
   __shared__ __align__(8) unsigned char plan_memory[(kMost + 1) * 8 + kMost * 8];
   __shared__ Two scratch[kThreads / 32];
   const Plan plan = plan_at(plan_memory, p.sequences);
+  wait_for_previous();
+  let_next_start();
   const int64_t free = free_pages(p);
   const int taken = extend_plan<kThreads>(p, e, plan, scratch, free);
   if constexpr (kCluster) cooperative_groups::this_cluster().sync();
@@ -221,9 +223,8 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(Pages p, PagesExtend e
 }
 __global__ void __launch_bounds__(kMostThreads) extend_plan_kernel(Pages p, PagesExtend e) {
   __shared__ Two scratch[kMostThreads / 32];
-#if __CUDA_ARCH__ >= 900
-  cudaTriggerProgrammaticLaunchCompletion();
-#endif
+  wait_for_previous();
+  let_next_start();
   const Plan plan = plan_at(e.workspace, p.sequences);
   const int64_t free = free_pages(p);
   const int taken = extend_plan<kMostThreads>(p, e, plan, scratch, free);
@@ -232,9 +233,7 @@ __global__ void __launch_bounds__(kMostThreads) extend_plan_kernel(Pages p, Page
 __global__ void __launch_bounds__(kRowThreads) extend_rows_kernel(Pages p, PagesExtend e) {
   __shared__ __align__(8) unsigned char plan_memory[(kSmall + 1) * 8 + kSmall * 8];
   Plan plan = plan_at(e.workspace, p.sequences);
-#if __CUDA_ARCH__ >= 900
-  cudaGridDependencySynchronize();
-#endif
+  wait_for_previous();
   if (p.sequences <= kSmall) {  // all that the plan has, at once
     const Plan here = plan_at(plan_memory, p.sequences);
     for (int b = threadIdx.x; b < p.sequences; b += kRowThreads) {
@@ -315,6 +314,8 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(Pages p, const int32
   __shared__ __align__(8) unsigned char plan_memory[(kMost + 1) * 8 + kMost * 8];
   __shared__ Two scratch[kThreads / 32];
   const Plan plan = plan_at(plan_memory, p.sequences);
+  wait_for_previous();
+  let_next_start();
   const int64_t free = free_pages(p);
   truncate_plan<kThreads>(p, to, plan, scratch, free);
   if constexpr (kCluster) cooperative_groups::this_cluster().sync();
@@ -323,42 +324,17 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(Pages p, const int32
 }
 __global__ void __launch_bounds__(kMostThreads) truncate_plan_kernel(Pages p, const int32_t* to, void* workspace) {
   __shared__ Two scratch[kMostThreads / 32];
-#if __CUDA_ARCH__ >= 900
-  cudaTriggerProgrammaticLaunchCompletion();
-#endif
+  wait_for_previous();
+  let_next_start();
   const Plan plan = plan_at(workspace, p.sequences);
   const int64_t free = free_pages(p);
   truncate_plan<kMostThreads>(p, to, plan, scratch, free);
   truncate_state<kMostThreads>(p, to, plan, free);
 }
 __global__ void __launch_bounds__(kRowThreads) truncate_pages_kernel(Pages p, void* workspace) {
-#if __CUDA_ARCH__ >= 900
-  cudaGridDependencySynchronize();
-#endif
+  wait_for_previous();
   truncate_pages(p, plan_at(workspace, p.sequences), static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x,
                  static_cast<int64_t>(gridDim.x) * kRowThreads);
-}
-
-// A kernel launched while the one before it runs (`cluster` 0), or as a cluster of so many blocks.
-template <class... Args>
-void launch_with(void (*kernel)(Args...), int64_t blocks, int threads, int cluster, cudaStream_t stream, const char* what, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = stream;
-  cudaLaunchAttribute attribute{};
-  if (cluster > 0) {
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = static_cast<unsigned>(cluster);
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  } else {
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-  }
-  cfg.attrs = &attribute;
-  cfg.numAttrs = 1;
-  check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
-  count_launch();
 }
 
 // Ancestors of the nodes of drafted trees: a block a sequence, its parents in shared memory, a thread a node's
@@ -366,6 +342,8 @@ void launch_with(void (*kernel)(Args...), int64_t blocks, int threads, int clust
 constexpr int kTreeThreads = 128;
 __global__ void __launch_bounds__(kTreeThreads) draft_ancestors_kernel(DraftTrees t) {
   __shared__ int16_t parent[kMostTreeRows];
+  wait_for_previous();
+  let_next_start();
   const int b = blockIdx.x;
   // Sequences' rows held to the call's; the rows before the first and after the last, and past the announced number, 0.
   const int64_t lo = max(0, t.offsets[b]), hi = min(static_cast<int64_t>(t.offsets[b + 1]), t.rows);
@@ -411,41 +389,34 @@ constexpr int kClusterThreads = 512;
 constexpr int kCluster = 8;
 
 void launch_pages_extend(const Pages& p, const PagesExtend& e, cudaStream_t stream) {
+  constexpr const char* kWhat = "launch page table kernel";
   if (pages_workspace_bytes(p, e.rows) > 0) {
-    extend_plan_kernel<<<1, kMostThreads, 0, stream>>>(p, e);
-    count_launch();
-    check(cudaGetLastError(), "launch page table kernel");
+    launch_early(extend_plan_kernel, dim3(1), kMostThreads, 0, stream, 0, kWhat, p, e);
     constexpr int kPerBlock = kRowThreads * kRows;
-    if (e.rows > 0) launch_with(extend_rows_kernel, (e.rows + kPerBlock - 1) / kPerBlock, kRowThreads, 0, stream, "launch slot kernel", p, e);
+    if (e.rows > 0)
+      launch_early(extend_rows_kernel, dim3(static_cast<unsigned>((e.rows + kPerBlock - 1) / kPerBlock)), kRowThreads, 0, stream, 0, kWhat, p, e);
   } else if (p.sequences <= kFewThreads && e.rows <= 4 * kFewThreads) {
-    extend_kernel<kFewThreads, false><<<1, kFewThreads, 0, stream>>>(p, e);
-    count_launch();
-    check(cudaGetLastError(), "launch page table kernel");
+    launch_early(extend_kernel<kFewThreads, false>, dim3(1), kFewThreads, 0, stream, 0, kWhat, p, e);
   } else {
-    launch_with(extend_kernel<kClusterThreads, true>, kCluster, kClusterThreads, kCluster, stream, "launch page table kernel", p, e);
+    launch_early(extend_kernel<kClusterThreads, true>, dim3(kCluster), kClusterThreads, 0, stream, kCluster, kWhat, p, e);
   }
 }
 
 void launch_pages_truncate(const Pages& p, const int32_t* to, void* workspace, cudaStream_t stream) {
+  constexpr const char* kWhat = "launch page return kernel";
   if (pages_workspace_bytes(p, 0) > 0) {
-    truncate_plan_kernel<<<1, kMostThreads, 0, stream>>>(p, to, workspace);
-    count_launch();
-    check(cudaGetLastError(), "launch page return kernel");
+    launch_early(truncate_plan_kernel, dim3(1), kMostThreads, 0, stream, 0, kWhat, p, to, workspace);
     const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(512, (p.num_pages + kRowThreads - 1) / kRowThreads));
-    launch_with(truncate_pages_kernel, blocks, kRowThreads, 0, stream, "launch page return kernel", p, workspace);
+    launch_early(truncate_pages_kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, stream, 0, kWhat, p, workspace);
   } else if (p.sequences <= kFewThreads) {
-    truncate_kernel<kFewThreads, false><<<1, kFewThreads, 0, stream>>>(p, to);
-    count_launch();
-    check(cudaGetLastError(), "launch page return kernel");
+    launch_early(truncate_kernel<kFewThreads, false>, dim3(1), kFewThreads, 0, stream, 0, kWhat, p, to);
   } else {
-    launch_with(truncate_kernel<kClusterThreads, true>, kCluster, kClusterThreads, kCluster, stream, "launch page return kernel", p, to);
+    launch_early(truncate_kernel<kClusterThreads, true>, dim3(kCluster), kClusterThreads, 0, stream, kCluster, kWhat, p, to);
   }
 }
 
 void launch_draft_ancestors(const DraftTrees& t, cudaStream_t stream) {
-  draft_ancestors_kernel<<<static_cast<unsigned>(t.batch), kTreeThreads, 0, stream>>>(t);
-  count_launch();
-  check(cudaGetLastError(), "launch draft tree kernel");
+  launch_early(draft_ancestors_kernel, dim3(static_cast<unsigned>(t.batch)), kTreeThreads, 0, stream, 0, "launch draft tree kernel", t);
 }
 
 }  // namespace msb

@@ -69,6 +69,8 @@ __global__ void __launch_bounds__(most_threads(kPer), kPer == 1 ? 1 : 4) rotate_
   constexpr bool kTwoParts = !kNeighbours || kPer == 1;   // a piece's elements lie in two places
   constexpr int kPairs = kTwoParts ? kPer : kPer / 2;     // of a piece
   __shared__ float2 turns[kTurns];
+  wait_for_previous();
+  let_next_start();
   const int which = blockIdx.x >= c.blocks;
   const int heads = a.heads[which], head_lanes = c.head_lanes[which], block_tokens = c.tokens[which];
   const int64_t token0 = (static_cast<int64_t>(blockIdx.x) - (which ? c.blocks : 0)) * block_tokens;
@@ -148,7 +150,8 @@ void launch_pairs(const Rotate& a, cudaStream_t stream) {
   if (blocks[0] + blocks[1] > INT_MAX) throw InvalidArgument("tokens are too many for one call");
   c.blocks = blocks[0];
   threads = (threads + 31) / 32 * 32;
-  rotate_kernel<T, kPer, kNeighbours><<<static_cast<unsigned>(blocks[0] + blocks[1]), threads, 0, stream>>>(a, c);
+  launch_early(rotate_kernel<T, kPer, kNeighbours>, dim3(static_cast<unsigned>(blocks[0] + blocks[1])), threads, 0, stream, 0,
+               "launch rotary kernel", a, c);
 }
 
 template <class T>
@@ -180,8 +183,6 @@ void launch_rotate(const Rotate& a, cudaStream_t stream) {
   if (a.type == kElemF32) launch_typed<float>(a, stream);
   else if (a.type == kElemF16) launch_typed<__half>(a, stream);
   else launch_typed<__nv_bfloat16>(a, stream);
-  count_launch();
-  check(cudaGetLastError(), "launch rotary kernel");
 }
 
 }  // namespace msb
