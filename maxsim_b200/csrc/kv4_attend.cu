@@ -5,6 +5,10 @@
 // sum_j e^(s_j - m) vs_j vc_j / sum_j e^(s_j - m) in one pass with a running reference m, sums in fp32; a row
 // that sees nothing writes zeros and a log-sum-exp of -inf.
 //
+// Sparse rows: with `sinks` a row sees tokens j < sinks past its window too; with masks (a tree of drafted tokens, the
+// sequence's last ones) it sees of these the ones whose bits it has, and all before them, or what the window leaves of them
+// (kv4_seen).
+//
 // kv4_attend_kernel: few rows a sequence (decode, drafted tokens).
 //   Bound: the codes' bytes, D + 8 per token and head; then latency, a warp's chain a step (unpacking, products, maximum,
 //   vote, exponentials, products): of 16 warps an SM it leaves 57% of the issue slots and of the memory's rate used.
@@ -35,9 +39,13 @@
 //   kv4_join_kernel adds in a fixed order; it is launched early (programmatic dependent launch).
 //   Short contexts (shape_of has the rule) take a cluster of 2 to 8 blocks a segment instead, whose parts are
 //   joined over distributed shared memory: one launch.
+//   Sparse rows have instances of their own.  A sequence's units are those over its two runs of tokens, the sinks and the
+//   window's, counted as one (what lies between is never loaded); only steps at a run's end form masks, from a row's bounds
+//   and, over a tree, 32 of its bits at once.
 //   Measured on the device, D = 128, 8 heads, 4 query heads each: 64 sequences of 4,096 tokens 77 us (3.7 TB/s of
 //   codes, 57% of a copy's rate), 2 of 115,000 66 us (3.8 TB/s), 1 of 16,384 17 us, 1 of 1,030 6.9 us; of the first 4 to
-//   5 us are the join and both launches' ends.  D = 256: the first 134 us (4.1 TB/s).
+//   5 us are the join and both launches' ends.  D = 256: the first 134 us (4.1 TB/s).  Sparse rows: 64 sequences of up to
+//   16,384 tokens, the last 4,096 and the first 64 of each seen, 78.5 us (3.2 TB/s); one of 30,001, 1,024 and 4 seen, 7.2 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -1020,6 +1028,22 @@ bool many_rows(const Kv4View& c, const Kv4Attend& a) {
   if (a.engine == 2) return true;
   const int64_t rows = static_cast<int64_t>(a.max_rows) * (a.heads / c.heads);
   const int64_t heads = static_cast<int64_t>(a.batch) * c.heads, sms = sm_count();
+  if (a.sinks > 0 || a.ancestors) {
+    // Sparse rows: either kernel spreads its tiles evenly, so that microseconds follow from their numbers (fitted to trees of
+    // 4 to 64 nodes, 4 query heads a head, contexts of 300 to 16,000 tokens, 2 and 8 heads, 1 to 64 sequences).  This
+    // file's: 10, 0.025 a row block of 16, and 5.8 ns (D = 64: 3.8) a tile of each.  kv4_chunk.cu's: 20, and 17 ns (15) a
+    // tile of each block of 128 rows, 23 (21) of 256, which costs as much as five tiles beside them.  (Measured, in that
+    // order: 16 sequences of 4,000 tokens, 8 heads: 68 and 107 us at 32 rows a head, 118 and 110 at 64, 408 and 151 at
+    // 256; 4 of 16,000: 64 and 93, 106 and 95, 363 and 132; 64 of 300: 55 and 94, 98 and 94, 346 and 129.)
+    int64_t most = static_cast<int64_t>(a.max_pages) << c.page_shift;
+    if (a.window > 0) most = std::min<int64_t>(most, static_cast<int64_t>(a.window) + a.sinks + a.max_rows + 2 * kStep);
+    const double tiles = static_cast<double>((most + kTile - 1) / kTile), blocks = static_cast<double>(heads * ((rows + 15) / 16));
+    const double few = 10.0 + blocks * (0.025 + (c.dim == 64 ? 0.0038 : 0.0058) * tiles);
+    const double tile = rows > 128 ? (c.dim == 64 ? 0.021 : 0.023) : (c.dim == 64 ? 0.015 : 0.017);
+    const double units = static_cast<double>(heads * ((rows + 255) / 256)) * (tiles + 5.0);
+    // (A block has eight of these at least, where a segment has as many.)
+    return 20.0 + tile * std::max(units, static_cast<double>(sms) * std::min(8.0, tiles + 5.0)) < few;
+  }
   const int64_t waves = (heads * ((rows + 255) / 256) + sms - 1) / sms;
   return heads * ((rows + 15) / 16) >= waves * (rows > 128 ? 440 : 350);
 }

@@ -323,6 +323,13 @@ __device__ __forceinline__ Work work_of(const Kv4Attend& a, uint32_t shared, con
 // block.  Every segment of a sequence has as many units as the largest could have tiles, and some for what a segment costs
 // beside its tiles (reading queries, the first tile's chain, writing rows: 12 to 15 us, a tile 3 to 3.5).
 constexpr int kSegmentUnits = 4;
+// Segments are cut where there are fewer than blocks, into ranges of kLeastUnits and more (a part of one has its 12 to 15 us
+// too).  The workspace: the sequences' starts, the line's end, the number of ranges, then the parts.
+constexpr int kLeastUnits = 8;
+__host__ __device__ __forceinline__ size_t line_head_bytes(int64_t batch) { return starts_bytes(batch + 1); }
+__device__ __forceinline__ float* chunk_parts(const Kv4Attend& a) {
+  return reinterpret_cast<float*>(static_cast<char*>(a.workspace) + line_head_bytes(a.batch));
+}
 struct Line {
   int units;   // of a segment
   int blocks;  // row blocks
@@ -403,15 +410,23 @@ __device__ __noinline__ Place find_place(const Kv4View& c, const Kv4Attend& a, u
     if (b >= a.batch) return int64_t{0};
     return line_of(a, kv4_sequence(a, c.page_shift, b), shared).all(c.heads);
   };
-  int64_t total = 0;
-  for (int b = threadIdx.x; b < a.batch; b += kLineThreads) total += units_of(b);
+  __shared__ int64_t segment_sums[kLineThreads / 32];
+  int64_t total = 0, segments = 0;
+  for (int b = threadIdx.x; b < a.batch; b += kLineThreads) {
+    const Line l = line_of(a, kv4_sequence(a, c.page_shift, b), shared);
+    total += l.all(c.heads);
+    segments += static_cast<int64_t>(c.heads) * l.blocks;
+  }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
-  if (lane == 0) sums[warp] = total;
+  for (int d = 16; d > 0; d >>= 1) {
+    total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+    segments += __shfl_xor_sync(0xFFFFFFFFu, segments, d);
+  }
+  if (lane == 0) sums[warp] = total, segment_sums[warp] = segments;
   __syncthreads();
-  total = 0;
-  for (int i = 0; i < kWarps; ++i) total += sums[i];
-  const int64_t n = ranges(total, gridDim.x), c0 = blockIdx.x;
+  total = segments = 0;
+  for (int i = 0; i < kWarps; ++i) total += sums[i], segments += segment_sums[i];
+  const int64_t n = ranges(total, min(static_cast<int64_t>(gridDim.x), max(segments, total / kLeastUnits))), c0 = blockIdx.x;
   Place p{0, 0, 0, 0};
   if (c0 < n) {
     p.unit = range_start(total, c0, n);
@@ -443,7 +458,10 @@ __device__ __noinline__ Place find_place(const Kv4View& c, const Kv4Attend& a, u
       found[1] = b;
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) starts[a.batch] = total;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    starts[a.batch] = total;
+    starts[a.batch + 1] = n;
+  }
   __syncthreads();
   if (p.unit < p.unit_end) {
     p.before = found[0];
@@ -826,7 +844,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
         }
         if constexpr (kSparse) {
           if (!w.whole) {  // a part of a segment: its sums as they are, and their references
-            float* const part = line_parts(a) + (2 * static_cast<int64_t>(blockIdx.x) + (w.tile0 == 0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
+            float* const part = chunk_parts(a) + (2 * static_cast<int64_t>(blockIdx.x) + (w.tile0 == 0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
             float* const sums = part + (m * kRowsTile + row0 + (lane >> 2)) * kDim + 2 * (lane & 3);
 #pragma unroll 1
             for (int d = 0; d < kDim && w.tiles > 0; d += kCols) {
@@ -1134,12 +1152,12 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
 constexpr int kJoinWarps = 8;
 constexpr int kJoinShares = 16;
 template <class T, int kDim>
-__global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4View c, Kv4Attend a, uint32_t shared, int64_t blocks) {
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4View c, Kv4Attend a, uint32_t shared) {
   constexpr int kPer = kDim / 32;
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t* const starts = static_cast<const int64_t*>(a.workspace);
-  const int64_t total = starts[a.batch], n = ranges(total, blocks), end = blockIdx.x + 1;
+  const int64_t total = starts[a.batch], n = starts[a.batch + 1], end = blockIdx.x + 1;
   if (end >= n) return;
   const int64_t u = range_start(total, end, n);
   int lo = 0, hi = a.batch;
@@ -1155,7 +1173,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4View
   // Ranges that hold tiles of the segment.
   const int64_t c0 = range_of(total, u0, n), c1 = range_of(total, u0 + max(1, w.tiles) - 1, n);
   if (c0 + 1 != end || c1 <= c0) return;
-  const float* const base = line_parts(a);
+  const float* const base = chunk_parts(a);
   for (int r = blockIdx.y * kJoinWarps + warp; r < w.row_count; r += kJoinShares * kJoinWarps) {
     float m = -INFINITY, sum = 0.0F, v[kPer];
 #pragma unroll
@@ -1207,7 +1225,7 @@ void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
                  "launch chunk attention kernel", c, a, static_cast<uint32_t>(shared), static_cast<int>(row_blocks), (starts & 15) == 0);
     if (blocks > 1)
       launch_early(kv4_chunk_join_kernel<T, kDim>, dim3(static_cast<unsigned>(blocks - 1), kJoinShares), kJoinWarps * 32, 0, stream, 0,
-                   "launch chunk attention join kernel", c, a, static_cast<uint32_t>(shared), blocks);
+                   "launch chunk attention join kernel", c, a, static_cast<uint32_t>(shared));
   } else {
     kv4_chunk_kernel<T, kDim, false><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
         c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
@@ -1230,7 +1248,7 @@ bool kv4_chunk_supported(const Kv4View& c) { return c.dim <= 128; }
 
 size_t kv4_chunk_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
   if (a.sinks == 0 && !a.ancestors) return 0;
-  return starts_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(line_blocks(c, a)) * partial_floats(kBlockRows, c.dim);
+  return line_head_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(line_blocks(c, a)) * partial_floats(kBlockRows, c.dim);
 }
 
 void launch_kv4_chunk(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
