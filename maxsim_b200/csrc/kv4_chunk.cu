@@ -27,6 +27,15 @@
 //   beside it.  Half of the issue slots are used.  Reading the queries takes 8,000 cycles of a block and writing the rows
 //   5,000.  And the blocks' order: 256 of them start by row block, then by sequence, whatever their length.  Replayed on
 //   148 SMs from these cycles that ends after 153 to 156 us; longest first would end after 116, evenly spread after 105.
+//   Sparse rows (sinks, trees of drafted tokens) have instances of their own, in which a block works through a range of a
+//   line of tiles of all segments (find_place), since segments of 2 to 70 tiles fill 148 SMs badly one to a block (trees:
+//   234 us so, 139 on the line; a part of a segment costs 12 to 15 us beside its tiles, of which the join's read is the
+//   least).  Their softmax warps take 88 registers, from two warps that only make the block whole warpgroups: with 80 a few
+//   words spilled, and as the codes' loads pass through what is left of L1 beside 205 KB of shared memory, every reload went
+//   to L2 (5.3 us a tile of 256 rows where this takes 3.3).  Measured: 16 trees of 25 to 64 nodes after 100 to 8,192 tokens,
+//   32 heads (8 of the cache), D = 128, 139 us with the join; chunks of 512 rows of 4 sequences up to 16,000 tokens, a
+//   window of 2,048 and 100 sinks, 163 us.  A tile takes 6,300 cycles there, 3,400 of them in the columns' loops (exponentials
+//   alone: 2,048); the rest are its products' and barriers' latencies.
 // Every wait is bounded; a block that gives up writes NaN rows.
 #include <algorithm>
 #include <climits>
@@ -342,7 +351,8 @@ __device__ __forceinline__ Line line_of(const Kv4Attend& a, const Kv4Sequence& q
   if (a.window > 0) {
     // A block's rows are those of this many query tokens (of a tree: all see the same tiles); a window that starts up
     // to 15 tokens early, and a tree's that starts one early.
-    const int64_t tokens = a.ancestors ? q.rows + q.left + 1 : min(static_cast<int64_t>(q.rows), static_cast<int64_t>((kBlockRows - 1) / shared + 2));
+    const int64_t tokens = a.ancestors ? static_cast<int64_t>(q.rows) + q.left + 1
+                                       : min(static_cast<int64_t>(q.rows), static_cast<int64_t>((kBlockRows - 1) / shared + 2));
     const int64_t seen = (a.sinks + kTokens - 1) / kTokens + (tokens - 1 + a.window + 14) / kTokens + 1;
     l.units = static_cast<int>(min(static_cast<int64_t>(l.units), seen));
   }
@@ -350,7 +360,8 @@ __device__ __forceinline__ Line line_of(const Kv4Attend& a, const Kv4Sequence& q
   return l;
 }
 // Segment `segment` of a sequence.
-__device__ __forceinline__ Work segment_of(const Kv4Attend& a, uint32_t shared, const Kv4Sequence& q, const Line& l, int b, int64_t segment) {
+__device__ __forceinline__ Work segment_of(const Kv4Attend& a, uint32_t shared, const Kv4Sequence& q, const Line& l, int b,
+                                           int64_t segment) {
   return work_of<true>(a, shared, q, b, static_cast<int>(segment / l.blocks), static_cast<int>(segment % l.blocks));
 }
 // Where a block is on the line.
@@ -489,8 +500,8 @@ __device__ __forceinline__ uint32_t run_bits(const Kv4Seen& run, int sinks, int 
 // has one segment after the other, of the first and the last perhaps a part, whose sums go to the workspace.  Its roles
 // pass from a segment to the next by themselves, as barriers' phases count on.
 template <class T, int kDim, bool kSparse>
-__global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chunk_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ Kv4Attend a, uint32_t shared, int row_blocks,
-                                                                bool aligned) {
+__global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
+    kv4_chunk_kernel(const __grid_constant__ Kv4View c, const __grid_constant__ Kv4Attend a, uint32_t shared, int row_blocks, bool aligned) {
   using L = Layout<kDim>;
   extern __shared__ unsigned char raw_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -747,7 +758,8 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
                 const int mine = 8 * k + (lane >> 2);
                 seen[k] = run_bits(row_seen[mine], a.sinks, j);
                 if (tree && j + kCols > w.q.pos0)
-                  seen[k] |= kv4_tree_bits(a, w.q, static_cast<int>((w.block_row0 + min(m * kRowsTile + row0 + mine, w.row_count - 1)) / shared), j);
+                  seen[k] |= kv4_tree_bits(
+                      a, w.q, static_cast<int>((w.block_row0 + min(m * kRowsTile + row0 + mine, w.row_count - 1)) / shared), j);
                 seen[k] = (seen[k] & ~absent) >> (2 * (lane & 3));
               }
             }
@@ -844,7 +856,8 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1) kv4_chun
         }
         if constexpr (kSparse) {
           if (!w.whole) {  // a part of a segment: its sums as they are, and their references
-            float* const part = chunk_parts(a) + (2 * static_cast<int64_t>(blockIdx.x) + (w.tile0 == 0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
+            float* const part =
+                chunk_parts(a) + (2 * static_cast<int64_t>(blockIdx.x) + (w.tile0 == 0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
             float* const sums = part + (m * kRowsTile + row0 + (lane >> 2)) * kDim + 2 * (lane & 3);
 #pragma unroll 1
             for (int d = 0; d < kDim && w.tiles > 0; d += kCols) {

@@ -10,6 +10,8 @@
 //   Bound: latency.  One block forms the sums (plan); where rows or sequences are many a second kernel with four rows (or a
 //   page given back) to a thread does the rest, launched early, else the same block does it, from shared memory.
 //   A row whose position starts a page enters that page in the table: each new page has one such row.
+//   Measured on the device: a token for each of 64 sequences, and back, 5.9 us; 128,000 rows of 500 sequences in 8,000 new
+//   pages, and back, 12.7 us (launch_pages_extend has what chooses between the forms).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -280,7 +282,8 @@ __device__ __forceinline__ void truncate_plan(const Pages& p, const int32_t* to,
 template <int kThreads>
 __device__ __forceinline__ void truncate_state(const Pages& p, const int32_t* to, const Plan& plan, int64_t free) {
   for (int b = threadIdx.x; b < p.sequences; b += kThreads)
-    p.lengths[b] = b > 0 ? plan.entry[b] : static_cast<int32_t>(max(int64_t{0}, min(static_cast<int64_t>(to[0]), held_length(p, 0))));
+    p.lengths[b] =
+        b > 0 ? plan.entry[b] : static_cast<int32_t>(max(int64_t{0}, min(static_cast<int64_t>(to[0]), held_length(p, 0))));
   if (threadIdx.x == 0) *p.free_count = static_cast<int32_t>(min(free + plan.start[p.sequences], p.num_pages));
 }
 // Page k of those given back goes to entry free + all - 1 - k.  A thread (`first` of `step`) has kRows consecutive ones at a
@@ -379,8 +382,8 @@ size_t pages_workspace_bytes(const Pages& p, int64_t rows) {
   return p.sequences > kSmall || rows > kSmallRows ? plan_bytes(p.sequences) : 0;
 }
 
-// Up to 256 sequences one block of as many threads does it all (extend: up to 1,024 rows): 64 sequences, a token each, and
-// back 8.3 us, of which a cluster's launch would make 10.4.  (How many pages go back the host does not know: some thousand
+// Up to 256 sequences one block of as many threads does it all (extend: up to 1,024 rows): for 64 sequences, a token each,
+// 2 us less a call than a cluster.  (How many pages go back the host does not know: some thousand
 // at once, which end many long sequences, take a block longer, 11 us for 8,000.)  Up to 1,024 sequences and 8,192 rows a
 // cluster: giving back 8,000 pages of 500 sequences 6.9 us.  More, two kernels: 128,000 rows 10 us, which are 21 in a
 // cluster, bound by the loads and stores of its eight SMs.
@@ -394,7 +397,8 @@ void launch_pages_extend(const Pages& p, const PagesExtend& e, cudaStream_t stre
     launch_early(extend_plan_kernel, dim3(1), kMostThreads, 0, stream, 0, kWhat, p, e);
     constexpr int kPerBlock = kRowThreads * kRows;
     if (e.rows > 0)
-      launch_early(extend_rows_kernel, dim3(static_cast<unsigned>((e.rows + kPerBlock - 1) / kPerBlock)), kRowThreads, 0, stream, 0, kWhat, p, e);
+      launch_early(extend_rows_kernel, dim3(static_cast<unsigned>((e.rows + kPerBlock - 1) / kPerBlock)), kRowThreads, 0, stream,
+                   0, kWhat, p, e);
   } else if (p.sequences <= kFewThreads && e.rows <= 4 * kFewThreads) {
     launch_early(extend_kernel<kFewThreads, false>, dim3(1), kFewThreads, 0, stream, 0, kWhat, p, e);
   } else {
@@ -411,7 +415,8 @@ void launch_pages_truncate(const Pages& p, const int32_t* to, void* workspace, c
   } else if (p.sequences <= kFewThreads) {
     launch_early(truncate_kernel<kFewThreads, false>, dim3(1), kFewThreads, 0, stream, 0, kWhat, p, to);
   } else {
-    launch_early(truncate_kernel<kClusterThreads, true>, dim3(kCluster), kClusterThreads, 0, stream, kCluster, kWhat, p, to);
+    launch_early(truncate_kernel<kClusterThreads, true>, dim3(kCluster), kClusterThreads, 0, stream, kCluster, kWhat, p,
+                 to);
   }
 }
 

@@ -6,7 +6,10 @@
 // would be off by 2^-8 of a turn at 10^5).  The nearest quarter turn is taken off in integers; what is left, an eighth
 // of a turn at most, becomes fp32 with all its bits.
 //   Bound: memory, every element is read and written once.  A block has a few tokens: their sines and cosines are formed
-//   once, in shared memory, for all heads, while the first vectors are on their way.
+//   once, in shared memory, for all heads, while the first vectors are on their way.  A thread keeps those of its piece of a
+//   vector in registers and goes through heads; two vectors on their way leave registers for four blocks of 256 threads an
+//   SM (four and one block's worth: 70 us where this takes 57; sines read from shared memory for every vector: 79).
+//   Measured on the device: 16,384 tokens, 32 + 8 heads of 128, bf16, 56 to 57 us, 6.0 TB/s; 64 of them 2.5 us.
 #include <algorithm>
 #include <climits>
 
@@ -65,7 +68,8 @@ struct Split {
 // kPer: elements of a piece, of either half of its pairs (halves), or in all (neighbours): 16 bytes, or, where something
 // does not start on 16 bytes, one pair.
 template <class T, int kPer, bool kNeighbours>
-__global__ void __launch_bounds__(most_threads(kPer), kPer == 1 ? 1 : 4) rotate_kernel(const __grid_constant__ Rotate a, const __grid_constant__ Split c) {
+__global__ void __launch_bounds__(most_threads(kPer), kPer == 1 ? 1 : 4)
+    rotate_kernel(const __grid_constant__ Rotate a, const __grid_constant__ Split c) {
   constexpr bool kTwoParts = !kNeighbours || kPer == 1;   // a piece's elements lie in two places
   constexpr int kPairs = kTwoParts ? kPer : kPer / 2;     // of a piece
   __shared__ float2 turns[kTurns];

@@ -875,3 +875,15 @@ def test_graphs_and_streams():
         torch.cuda.current_stream().wait_stream(s)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for r in results for a, b in zip(r, alone))
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (24, 3)])
+def test_example_answers_with_drafts(window, sinks):
+    """The example runs, keeps one to three tokens a step, and what it keeps is a path of what it drafted."""
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    import answer_with_drafts
+
+    answer, counts = answer_with_drafts.main(prompts=(20, 1, 33), tokens=6, window=window, sinks=sinks)
+    assert answer.shape == (3, 6, 3) and counts.shape == (3, 6)
+    assert ((counts >= 1) & (counts <= 3)).all()
+    assert torch.equal((answer >= 0).sum(dim=2), counts) and ((answer[..., 0] >= 0) & (answer[..., 0] < 1000)).all()
