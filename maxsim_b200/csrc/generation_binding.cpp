@@ -549,6 +549,11 @@ PyObject* rotate(PyObject* const* args, Py_ssize_t n) {
           refuse(std::string(out_names[w]) + " must be " + names[w] + " itself or lie apart from " + names[i]);
         if (i > w && y[i].numel() > 0 && !apart(out, vectors(y[i]))) refuse("out[0] and out[1] must lie apart");
       }
+      int64_t last = 0;
+      for (int64_t d = 0; d < given.dim(); ++d) last += (given.size(d) - 1) * given.stride(d);
+      const char* const p = static_cast<const char*>(given.const_data_ptr());
+      if (p < out.at + span(out) && out.at < p + (last + 1) * static_cast<int64_t>(given.element_size()))
+        refuse(std::string(out_names[w]) + " must lie apart from positions");
     }
   }
   for (int w = 0; w < count; ++w) {

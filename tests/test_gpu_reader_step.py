@@ -668,6 +668,9 @@ def test_rotary_refusals():
     same = torch.empty((5, 2, 64), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError, match="apart"):
         rotary(q[:, :2], k, p, out=(same, same))
+    store = torch.zeros((5, 4, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="apart from positions"):
+        rotary(q, None, store.view(torch.int64).flatten()[:10].view(2, 5), out=(store, None))
     grad = q.clone().requires_grad_()
     with pytest.raises(ValueError, match="gradient"):
         rotary(grad, k, p)
