@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
         for (int i = 0; i < w.tiles; ++i) {
           const int it = kSparse ? w.done + i : i, s = it & 1, j0 = w.tile_start<kSparse>(i);
           const int im = kSparse ? w.row_done[m] + i : i;
-          ok = ok && mbar_wait(&k_full[s], (it >> 1) & 1, abort_flag) && mbar_wait(&s_half[m], im & 1, abort_flag);
+          ok = (!kSparse || ok) && mbar_wait(&k_full[s], (it >> 1) & 1, abort_flag) && mbar_wait(&s_half[m], im & 1, abort_flag);
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -823,22 +823,34 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
           // tile paid for them.)
           if constexpr (!kSparse) {
 #pragma unroll 1
-            for (int part = 0; part < kTokens / kCols && ok; ++part) columns(part, std::integral_constant<int, 2>{});
+            for (int part = 0; part < kTokens / kCols; ++part) {
+              columns(part, std::integral_constant<int, 2>{});
+              if (!ok) break;
+            }
           } else if (masked) {
 #pragma unroll 1
-            for (int part = 0; part < kTokens / kCols && ok; ++part) columns(part, std::integral_constant<int, 1>{});
+            for (int part = 0; part < kTokens / kCols; ++part) {
+              columns(part, std::integral_constant<int, 1>{});
+              if (!ok) break;
+            }
           } else {
 #pragma unroll 1
-            for (int part = 0; part < kTokens / kCols && ok; ++part) columns(part, std::integral_constant<int, 0>{});
+            for (int part = 0; part < kTokens / kCols; ++part) {
+              columns(part, std::integral_constant<int, 0>{});
+              if (!ok) break;
+            }
           }
           if (!ok) break;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&meta_empty[s]);
-            if (kSparse && w.tiles_m == 1) mbar_arrive(&meta_empty[s]);
+            if (kSparse) {  // (a segment's last probabilities end it: what is counted on comes before)
+              mbar_arrive(&meta_empty[s]);
+              if (w.tiles_m == 1) mbar_arrive(&meta_empty[s]);
+            }
             mbar_arrive(&p_full[m]);
+            if (!kSparse) mbar_arrive(&meta_empty[s]);
           }
         }
         // The rows' outputs, through the query tile's shared memory to 16 bytes a lane.
