@@ -618,12 +618,10 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
     count = work_count;
     return count > 0;
   };
-  if constexpr (kSparse) {
-    // Of the 24 x 32 x 80 registers that a line's block is launched with: 20 warps' 88 and 4 warps' 40.
-    if (warp >= kMmaWarp) registers_dec<40>();
-    else registers_inc<88>();
-  }
+  // Of the 24 x 32 x 80 registers that a line's block is launched with: 20 warps' 88 and 4 warps' 40.  (Each role asks for its
+  // own: after a common place the compiler would not know which it has.)
   if (warp < kSoftWarps) {
+    if constexpr (kSparse) registers_inc<88>();
     // =================== softmax: a warp has 16 rows, a thread two of them and a quarter of their columns ===================
     const int m = warp >> 3;
     bool ok = true;
@@ -939,6 +937,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
       }
     } while (next_list(false));
   } else if (warp < kMmaWarp) {
+    if constexpr (kSparse) registers_inc<88>();
     // =================== unpacking ===================
     // Keys: lane (g, t) takes 16 bytes t (at D = 128) of tokens g, g + 8, .. of its warp's 32.
     const int uw = warp - kUnpackWarp0, g = lane >> 2, t = lane & 3;
@@ -1082,82 +1081,85 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
         kv4_fill_rows<T>(a, kDim, only.b, kv4_sequence(a, c.page_shift, only.b), share, shares, thread, kFillThreads);
       }
     }
-  } else if (warp >= kMmaWarp + 2) {
-    // They make a line's block whole warpgroups, and its lists.
-    while (next_list(true)) {
-    }
-  } else if (kSparse || (warp - kMmaWarp < only.tiles_m && only.tiles > 0)) {
-    // =================== products of a row tile: one lane issues ===================
-    const int m = warp - kMmaWarp;
-    const uint32_t leader = elect();
-    constexpr uint32_t kInstrS = (1u << 4) | (static_cast<uint32_t>(kTokens / 2 >> 3) << 17) | (8u << 24);
-    constexpr uint32_t kInstrO = (1u << 4) | (static_cast<uint32_t>(kDim >> 3) << 17) | (8u << 24);
-    const uint32_t s_tmem = tmem + m * 128, o_tmem = s_tmem + 256;
-    const uint64_t q_desc = operand_desc(base + L::off_q + m * L::kQBytes), k_desc = operand_desc(base + L::off_k);
-    const uint64_t v_desc = operand_desc(base + L::off_v);
-    auto scores = [&](int s, int half) {
-#pragma unroll
-      for (int k = 0; k < kDim / 16; ++k) {  // 16 dimensions: 32 bytes of a 128-byte row
-        const uint32_t at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-        const uint32_t rows = half * (kTokens / 2 * 128) >> 4;
-        mma_ss(leader, s_tmem + half * (kTokens / 2), q_desc + at, k_desc + (s * L::kTileBytes >> 4) + rows + at, kInstrS, k > 0);
+  } else {
+    if constexpr (kSparse) registers_dec<40>();
+    if (warp >= kMmaWarp + 2) {
+      // They make a line's block whole warpgroups, and its lists.
+      while (next_list(true)) {
       }
-    };
-    // (For both row tiles, where a segment of a line has one.)
-    uint32_t alone = 0;
-    auto commit_both = [&](uint64_t* bar) {
-      mma_commit(leader, bar);
-      if (kSparse) mma_commit(leader & alone, bar);
-    };
-    auto first_half = [&](int s) {
-      scores(s, s);
-      mma_commit(leader, &s_half[m]);
-    };
-    auto other_half = [&](int s) {
-      scores(s, s ^ 1);
-      mma_commit(leader, &s_full[m]);
-      commit_both(&k_empty[s]);
-    };
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0;
-    };
-    bool ok = true;
-    do {
-      for (int segment = 0; segment < count && ok; ++segment) {
-        const Work& w = work(segment);
-        if (kSparse && w.tiles == 0) continue;
-        alone = w.tiles_m == 1;
-        ok = wait(q_full, kSparse ? w.segments & 1 : 0);
-        if (kSparse && m >= w.tiles_m) continue;
-        const int start = kSparse ? w.done : 0;
-        ok = ok && wait(&k_full[start & 1], (start >> 1) & 1);
-        if (ok) {
-          tc_fence_after();
-          first_half(start & 1);
-          other_half(start & 1);
-        }
-        for (int i = 0; i < w.tiles && ok; ++i) {
-          const int it = kSparse ? w.done + i : i, s = it & 1;
-          const bool more = i + 1 < w.tiles;
-          // Operands first, which are early: nothing but the products is then between probabilities and scores.
-          ok = wait(&v_full[s], (it >> 1) & 1) && (!more || wait(&k_full[s ^ 1], ((it + 1) >> 1) & 1)) &&
-               wait(&p_full[m], (kSparse ? w.row_done[m] + i : i) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (more) first_half(s ^ 1);
-          const uint32_t p_tmem = s_tmem + s * (kTokens / 2);
+    } else if (kSparse || (warp - kMmaWarp < only.tiles_m && only.tiles > 0)) {
+      // =================== products of a row tile: one lane issues ===================
+      const int m = warp - kMmaWarp;
+      const uint32_t leader = elect();
+      constexpr uint32_t kInstrS = (1u << 4) | (static_cast<uint32_t>(kTokens / 2 >> 3) << 17) | (8u << 24);
+      constexpr uint32_t kInstrO = (1u << 4) | (static_cast<uint32_t>(kDim >> 3) << 17) | (8u << 24);
+      const uint32_t s_tmem = tmem + m * 128, o_tmem = s_tmem + 256;
+      const uint64_t q_desc = operand_desc(base + L::off_q + m * L::kQBytes), k_desc = operand_desc(base + L::off_k);
+      const uint64_t v_desc = operand_desc(base + L::off_v);
+      auto scores = [&](int s, int half) {
 #pragma unroll
-          for (int k = 0; k < kTokens / 16; ++k) {  // 16 tokens
-            const uint32_t at = ((k >> 2) * (kDim * 128) + (k & 3) * 32) >> 4;
-            mma_ts(leader, o_tmem, p_tmem + 8 * (k ^ (4 * s)), v_desc + (s * L::kTileBytes >> 4) + at, kInstrO, i > 0 || k > 0);
+        for (int k = 0; k < kDim / 16; ++k) {  // 16 dimensions: 32 bytes of a 128-byte row
+          const uint32_t at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+          const uint32_t rows = half * (kTokens / 2 * 128) >> 4;
+          mma_ss(leader, s_tmem + half * (kTokens / 2), q_desc + at, k_desc + (s * L::kTileBytes >> 4) + rows + at, kInstrS, k > 0);
+        }
+      };
+      // (For both row tiles, where a segment of a line has one.)
+      uint32_t alone = 0;
+      auto commit_both = [&](uint64_t* bar) {
+        mma_commit(leader, bar);
+        if (kSparse) mma_commit(leader & alone, bar);
+      };
+      auto first_half = [&](int s) {
+        scores(s, s);
+        mma_commit(leader, &s_half[m]);
+      };
+      auto other_half = [&](int s) {
+        scores(s, s ^ 1);
+        mma_commit(leader, &s_full[m]);
+        commit_both(&k_empty[s]);
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0;
+      };
+      bool ok = true;
+      do {
+        for (int segment = 0; segment < count && ok; ++segment) {
+          const Work& w = work(segment);
+          if (kSparse && w.tiles == 0) continue;
+          alone = w.tiles_m == 1;
+          ok = wait(q_full, kSparse ? w.segments & 1 : 0);
+          if (kSparse && m >= w.tiles_m) continue;
+          const int start = kSparse ? w.done : 0;
+          ok = ok && wait(&k_full[start & 1], (start >> 1) & 1);
+          if (ok) {
+            tc_fence_after();
+            first_half(start & 1);
+            other_half(start & 1);
           }
-          commit_both(&v_empty[s]);
-          if (more) other_half(s ^ 1);
+          for (int i = 0; i < w.tiles && ok; ++i) {
+            const int it = kSparse ? w.done + i : i, s = it & 1;
+            const bool more = i + 1 < w.tiles;
+            // Operands first, which are early: nothing but the products is then between probabilities and scores.
+            ok = wait(&v_full[s], (it >> 1) & 1) && (!more || wait(&k_full[s ^ 1], ((it + 1) >> 1) & 1)) &&
+                 wait(&p_full[m], (kSparse ? w.row_done[m] + i : i) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (more) first_half(s ^ 1);
+            const uint32_t p_tmem = s_tmem + s * (kTokens / 2);
+#pragma unroll
+            for (int k = 0; k < kTokens / 16; ++k) {  // 16 tokens
+              const uint32_t at = ((k >> 2) * (kDim * 128) + (k & 3) * 32) >> 4;
+              mma_ts(leader, o_tmem, p_tmem + 8 * (k ^ (4 * s)), v_desc + (s * L::kTileBytes >> 4) + at, kInstrO, i > 0 || k > 0);
+            }
+            commit_both(&v_empty[s]);
+            if (more) other_half(s ^ 1);
+          }
+          if (ok) commit_both(o_full);
         }
-        if (ok) commit_both(o_full);
-      }
-      __syncwarp();
-    } while (next_list(false));
+        __syncwarp();
+      } while (next_list(false));
+    }
   }
   __syncwarp();
   // After a wait was given up, products under way end by themselves: time for that before the tensor memory is freed.
