@@ -333,11 +333,26 @@ __device__ __forceinline__ Work work_of(const Kv4Attend& a, uint32_t shared, con
 // beside its tiles (reading queries, the first tile's chain, writing rows: 12 to 15 us, a tile 3 to 3.5).
 constexpr int kSegmentUnits = 4;
 // Segments are cut where there are fewer than blocks, into ranges of kLeastUnits and more (a part of one has its 12 to 15 us
-// too).  The workspace: the sequences' starts, the line's end, the number of ranges, then the parts.
+// too).  The workspace: of each block the segment that starts in its range and ends in another, for the join, then the parts.
 constexpr int kLeastUnits = 8;
-__host__ __device__ __forceinline__ size_t line_head_bytes(int64_t batch) { return starts_bytes(batch + 1); }
-__device__ __forceinline__ float* chunk_parts(const Kv4Attend& a) {
-  return reinterpret_cast<float*>(static_cast<char*>(a.workspace) + line_head_bytes(a.batch));
+struct Cut {
+  int64_t row0;         // of the sequence
+  uint32_t block_row0;
+  int row_count;
+  int head;
+  int parts;            // 0: none
+  int unused[2];
+};
+__host__ __device__ __forceinline__ size_t cut_bytes(int64_t blocks) {
+  return (static_cast<size_t>(blocks) * sizeof(Cut) + 127) & ~static_cast<size_t>(127);
+}
+__device__ __forceinline__ float* chunk_parts(const Kv4Attend& a, int64_t blocks) {
+  return reinterpret_cast<float*>(static_cast<char*>(a.workspace) + cut_bytes(blocks));
+}
+// Quotients of numbers that are mostly below 2^32 (a division in 64 bits takes several hundred cycles of a block's start).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
 struct Line {
   int units;   // of a segment
@@ -362,14 +377,17 @@ __device__ __forceinline__ Line line_of(const Kv4Attend& a, const Kv4Sequence& q
 // Segment `segment` of a sequence.
 __device__ __forceinline__ Work segment_of(const Kv4Attend& a, uint32_t shared, const Kv4Sequence& q, const Line& l, int b,
                                            int64_t segment) {
-  return work_of<true>(a, shared, q, b, static_cast<int>(segment / l.blocks), static_cast<int>(segment % l.blocks));
+  const int64_t head = quotient(segment, l.blocks);
+  return work_of<true>(a, shared, q, b, static_cast<int>(head), static_cast<int>(segment - head * l.blocks));
 }
 // Where a block is on the line.
 struct Place {
   int64_t unit, unit_end, before;  // before: units of the sequences before b
+  int64_t total, ranges;
   int b;
 };
-// The block's next segments, up to `most`, into a list; by one thread.  A part past a segment's tiles is nobody's.
+// The block's next segments, up to `most`, into a list, and the one that is cut at its range's end for the join; by one
+// thread.  A part past a segment's tiles is nobody's.
 __device__ __forceinline__ int next_works(const Kv4View& c, const Kv4Attend& a, uint32_t shared, Place& p, Work* works, int most) {
   int count = 0, done = 0, row_done[2] = {0, 0}, segments = 0;
   const Work* const last_work = works + most - 1;
@@ -389,13 +407,19 @@ __device__ __forceinline__ int next_works(const Kv4View& c, const Kv4Attend& a, 
         q = kv4_sequence(a, c.page_shift, ++p.b);
         l = line_of(a, q, shared);
       }
-      const int64_t inside = p.unit - p.before, segment = inside / l.units;
+      const int64_t inside = p.unit - p.before, segment = quotient(inside, l.units);
       const int first = static_cast<int>(inside - segment * l.units);
       const int last = static_cast<int>(min(static_cast<int64_t>(l.units), first + (p.unit_end - p.unit)));
       p.unit += last - first;
       Work w = segment_of(a, shared, q, l, p.b, segment);
       if (first >= max(1, w.tiles)) continue;
       w.whole = first == 0 && last >= w.tiles;
+      if (first == 0 && !w.whole) {  // its tiles' last unit is so many ranges on
+        const int64_t end = p.before + segment * l.units + w.tiles - 1;
+        const int64_t on = quotient((end + 1) * p.ranges - 1, p.total) - blockIdx.x;
+        static_cast<Cut*>(a.workspace)[blockIdx.x] =
+            Cut{q.row0, w.block_row0, w.row_count, w.head, static_cast<int>(on) + 1, {0, 0}};
+      }
       w.tile0 = first;
       w.tiles = max(0, min(last, w.tiles) - first);
       w.done = done;
@@ -411,7 +435,7 @@ __device__ __forceinline__ int next_works(const Kv4View& c, const Kv4Attend& a, 
   }
   return count;
 }
-// The block's range, by all of its threads; the first block writes the sequences' starts for the join.
+// The block's range, by all of its threads.
 __device__ __noinline__ Place find_place(const Kv4View& c, const Kv4Attend& a, uint32_t shared) {
   __shared__ int64_t sums[kLineThreads / 32];
   __shared__ int64_t found[2];
@@ -438,12 +462,11 @@ __device__ __noinline__ Place find_place(const Kv4View& c, const Kv4Attend& a, u
   total = segments = 0;
   for (int i = 0; i < kWarps; ++i) total += sums[i], segments += segment_sums[i];
   const int64_t n = ranges(total, min(static_cast<int64_t>(gridDim.x), max(segments, total / kLeastUnits))), c0 = blockIdx.x;
-  Place p{0, 0, 0, 0};
+  Place p{0, 0, 0, total, n, 0};
   if (c0 < n) {
-    p.unit = range_start(total, c0, n);
-    p.unit_end = min(range_start(total, c0 + 1, n), total);
+    p.unit = quotient(c0 * total, n);
+    p.unit_end = min(quotient((c0 + 1) * total, n), total);
   }
-  int64_t* const starts = static_cast<int64_t*>(a.workspace);
   int64_t carry = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kLineThreads) {
     const int b = b0 + threadIdx.x;
@@ -463,16 +486,12 @@ __device__ __noinline__ Place find_place(const Kv4View& c, const Kv4Attend& a, u
       carry += sums[i];
     }
     const int64_t before = base + upto - mine;
-    if (blockIdx.x == 0 && b < a.batch) starts[b] = before;
     if (p.unit >= before && p.unit < before + mine) {
       found[0] = before;
       found[1] = b;
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    starts[a.batch] = total;
-    starts[a.batch + 1] = n;
-  }
+  if (threadIdx.x == 0) static_cast<Cut*>(a.workspace)[c0].parts = 0;  // until next_works finds one
   __syncthreads();
   if (p.unit < p.unit_end) {
     p.before = found[0];
@@ -513,15 +532,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
   __shared__ int work_count;
   Work only{};
   int share = 0, shares = 1;
-  if constexpr (kSparse) {
-    wait_for_previous();
-    let_next_start();
-    const Place start = find_place(c, a, shared);
-    if (threadIdx.x == 0) {
-      place = start;
-      works[kList - 1].segments = -1;
-    }
-  } else {
+  if constexpr (!kSparse) {
     // Later row blocks see more tokens under a causal mask: they start first.
     const int64_t per_block = static_cast<int64_t>(a.batch) * c.heads;
     const int block = row_blocks - 1 - static_cast<int>(blockIdx.x / per_block);
@@ -577,6 +588,16 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if constexpr (kSparse) {  // nothing of what is above reads what the kernel before may write
+    wait_for_previous();
+    let_next_start();
+    const Place start = find_place(c, a, shared);
+    if (threadIdx.x == 0) {
+      place = start;
+      works[kList - 1].segments = -1;
+      work_count = next_works(c, a, shared, place, works, kList);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -602,11 +623,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
     return only;
   };
   int count = 1;
-  if constexpr (kSparse) {
-    if (threadIdx.x == 0) work_count = next_works(c, a, shared, place, works, kList);
-    __syncthreads();
-    count = work_count;
-  }
+  if constexpr (kSparse) count = work_count;
   // The next list, after a full one: every role comes here (with the loop over lists around the roles, what one of them
   // needs would be formed before it and held through all).
   auto next_list = [&](bool writes) {
@@ -655,15 +672,25 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
         // The warp's rows of the query tile, 8 dimensions a lane: scaled by a power of two to a maximum in [2^10, 2^11),
         // fp16, in the codes' order.  (In a loop: straight code would be fetched from memory and used once.)
         constexpr int kBatch = kSparse ? kLoads : 4;
+        // (A line's blocks do this for every segment: all loads are asked for at once, and a row is found from the one before.)
+        const int first_row = m * kRowsTile + row0 + lane / kRowLanes;
+        uint32_t token = 0, in_group = 0;
+        if (kSparse) {
+          token = (w.block_row0 + first_row) / shared;
+          in_group = w.block_row0 + first_row - token * shared;
+        }
 #pragma unroll 1
         for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
           uint4 x[kBatch];
 #pragma unroll
           for (int k = 0; k < kBatch; ++k) {
-            const int r = m * kRowsTile + row0 + (k0 + k) * kRowsAtOnce + lane / kRowLanes;
+            const int r = first_row + (k0 + k) * kRowsAtOnce;
             x[k] = make_uint4(0, 0, 0, 0);
+            if (!kSparse) {
+              token = (w.block_row0 + r) / shared;
+              in_group = w.block_row0 + r - token * shared;
+            }
             if (r < w.row_count) {
-              const uint32_t token = (w.block_row0 + r) / shared, in_group = w.block_row0 + r - token * shared;
               const T* src = static_cast<const T*>(a.query) + (w.q.row0 + token) * a.q_row_stride +
                              static_cast<int64_t>(w.head * shared + in_group) * a.q_head_stride + (lane % kRowLanes) * 8;
               if (aligned) {
@@ -674,6 +701,10 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
                 for (int i = 0; i < 8; ++i) e[i] = src[i];
                 x[k] = *reinterpret_cast<const uint4*>(e);
               }
+            }
+            if (kSparse) {
+              in_group += kRowsAtOnce;
+              while (in_group >= shared) in_group -= shared, ++token;
             }
           }
 #pragma unroll
@@ -867,7 +898,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
         if constexpr (kSparse) {
           if (!w.whole) {  // a part of a segment: its sums as they are, and their references
             float* const part =
-                chunk_parts(a) + (2 * static_cast<int64_t>(blockIdx.x) + (w.tile0 == 0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
+                chunk_parts(a, gridDim.x) + (2 * static_cast<int64_t>(blockIdx.x) + (w.tile0 == 0 ? 1 : 0)) * partial_floats(kBlockRows, kDim);
             float* const sums = part + (m * kRowsTile + row0 + (lane >> 2)) * kDim + 2 * (lane & 3);
 #pragma unroll 1
             for (int d = 0; d < kDim && w.tiles > 0; d += kCols) {
@@ -1174,34 +1205,19 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// Adds the parts of the segments that a line's ranges cut, a block to an end of a range and a share of the rows: it works
-// where that end is the first one inside its segment, each warp on a row, the parts in their order.
+// Adds the parts of the segments that a line's ranges cut, a block to a range, in which one starts that ends in another, and a
+// share of its rows: a warp has a row, the parts come in their order.
 constexpr int kJoinWarps = 8;
 constexpr int kJoinShares = 16;
 template <class T, int kDim>
-__global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4View c, Kv4Attend a, uint32_t shared) {
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4Attend a, uint32_t shared, int64_t blocks) {
   constexpr int kPer = kDim / 32;
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t* const starts = static_cast<const int64_t*>(a.workspace);
-  const int64_t total = starts[a.batch], n = starts[a.batch + 1], end = blockIdx.x + 1;
-  if (end >= n) return;
-  const int64_t u = range_start(total, end, n);
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= u) lo = mid;
-    else hi = mid;
-  }
-  const Kv4Sequence q = kv4_sequence(a, c.page_shift, lo);
-  const Line l = line_of(a, q, shared);
-  const int64_t segment = (u - starts[lo]) / l.units, u0 = starts[lo] + segment * l.units;
-  const Work w = segment_of(a, shared, q, l, lo, segment);
-  // Ranges that hold tiles of the segment.
-  const int64_t c0 = range_of(total, u0, n), c1 = range_of(total, u0 + max(1, w.tiles) - 1, n);
-  if (c0 + 1 != end || c1 <= c0) return;
-  const float* const base = chunk_parts(a);
-  for (int r = blockIdx.y * kJoinWarps + warp; r < w.row_count; r += kJoinShares * kJoinWarps) {
+  const Cut w = static_cast<const Cut*>(a.workspace)[blockIdx.x];
+  const int64_t c0 = blockIdx.x, c1 = c0 + w.parts - 1;
+  const float* const base = chunk_parts(a, blocks);
+  for (int r = blockIdx.y * kJoinWarps + warp; r < (w.parts > 1 ? w.row_count : 0); r += kJoinShares * kJoinWarps) {
     float m = -INFINITY, sum = 0.0F, v[kPer];
 #pragma unroll
     for (int d = 0; d < kPer; ++d) v[d] = 0.0F;
@@ -1220,7 +1236,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_chunk_join_kernel(Kv4View
     }
     const float inv = sum == 0.0F ? 0.0F : 1.0F / sum;
     const uint32_t token = (w.block_row0 + r) / shared, in_group = w.block_row0 + r - token * shared;
-    const int64_t at = (q.row0 + token) * a.heads + w.head * shared + in_group;
+    const int64_t at = (w.row0 + token) * a.heads + w.head * shared + in_group;
     T* const out = static_cast<T*>(a.out) + at * kDim + lane * kPer;
 #pragma unroll
     for (int d = 0; d < kPer; ++d) out[d] = from_f32<T>(v[d] * inv);
@@ -1252,7 +1268,7 @@ void launch_dim(const Kv4View& c, const Kv4Attend& given, cudaStream_t stream) {
                  "launch chunk attention kernel", c, a, static_cast<uint32_t>(shared), static_cast<int>(row_blocks), (starts & 15) == 0);
     if (blocks > 1)
       launch_early(kv4_chunk_join_kernel<T, kDim>, dim3(static_cast<unsigned>(blocks - 1), kJoinShares), kJoinWarps * 32, 0, stream, 0,
-                   "launch chunk attention join kernel", c, a, static_cast<uint32_t>(shared));
+                   "launch chunk attention join kernel", a, static_cast<uint32_t>(shared), blocks);
   } else {
     kv4_chunk_kernel<T, kDim, false><<<static_cast<unsigned>(blocks), kThreads, Layout<kDim>::kBytes, stream>>>(
         c, a, shared, static_cast<int>(row_blocks), (starts & 15) == 0);
@@ -1275,7 +1291,7 @@ bool kv4_chunk_supported(const Kv4View& c) { return c.dim <= 128; }
 
 size_t kv4_chunk_workspace_bytes(const Kv4View& c, const Kv4Attend& a) {
   if (a.sinks == 0 && !a.ancestors) return 0;
-  return line_head_bytes(a.batch) + sizeof(float) * 2 * static_cast<size_t>(line_blocks(c, a)) * partial_floats(kBlockRows, c.dim);
+  return cut_bytes(line_blocks(c, a)) + sizeof(float) * 2 * static_cast<size_t>(line_blocks(c, a)) * partial_floats(kBlockRows, c.dim);
 }
 
 void launch_kv4_chunk(const Kv4View& c, const Kv4Attend& a, cudaStream_t stream) {
