@@ -1031,18 +1031,18 @@ bool many_rows(const Kv4View& c, const Kv4Attend& a) {
   if (a.sinks > 0 || a.ancestors) {
     // Sparse rows: either kernel spreads its tiles evenly, so that microseconds follow from their numbers (fitted to trees of
     // 4 to 64 nodes, 4 query heads a head, contexts of 300 to 16,000 tokens, 2 and 8 heads, 1 to 64 sequences).  This
-    // file's: 10, 0.025 a row block of 16, and 5.8 ns (D = 64: 3.8) a tile of each.  kv4_chunk.cu's: 20, and 17 ns (15) a
-    // tile of each block of 128 rows, 23 (21) of 256, which costs as much as five tiles beside them.  (Measured, in that
-    // order: 16 sequences of 4,000 tokens, 8 heads: 68 and 107 us at 32 rows a head, 118 and 110 at 64, 408 and 151 at
-    // 256; 4 of 16,000: 64 and 93, 106 and 95, 363 and 132; 64 of 300: 55 and 94, 98 and 94, 346 and 129.)
+    // file's: 10, 0.025 a row block of 16, and 5.8 ns (D = 64: 3.8) a tile of each.  kv4_chunk.cu's: 13, and 17 ns (15) a
+    // tile of each block of 128 rows, 22 (20) of 256, which costs as much as five tiles beside them.  (Measured, in that
+    // order: 16 sequences of 4,000 tokens, 8 heads: 68 and 94 us at 32 rows a head, 119 and 96 at 64, 409 and 138 at 256;
+    // 4 of 16,000: 64 and 86, 107 and 88, 366 and 120; 64 of 300: 55 and 78, 99 and 79, 347 and 114.)
     int64_t most = static_cast<int64_t>(a.max_pages) << c.page_shift;
     if (a.window > 0) most = std::min<int64_t>(most, static_cast<int64_t>(a.window) + a.sinks + a.max_rows + 2 * kStep);
     const double tiles = static_cast<double>((most + kTile - 1) / kTile), blocks = static_cast<double>(heads * ((rows + 15) / 16));
     const double few = 10.0 + blocks * (0.025 + (c.dim == 64 ? 0.0038 : 0.0058) * tiles);
-    const double tile = rows > 128 ? (c.dim == 64 ? 0.021 : 0.023) : (c.dim == 64 ? 0.015 : 0.017);
+    const double tile = rows > 128 ? (c.dim == 64 ? 0.020 : 0.022) : (c.dim == 64 ? 0.015 : 0.017);
     const double units = static_cast<double>(heads * ((rows + 255) / 256)) * (tiles + 5.0);
     // (A block has eight of these at least, where a segment has as many.)
-    return 20.0 + tile * std::max(units, static_cast<double>(sms) * std::min(8.0, tiles + 5.0)) < few;
+    return 13.0 + tile * std::max(units, static_cast<double>(sms) * std::min(8.0, tiles + 5.0)) < few;
   }
   const int64_t waves = (heads * ((rows + 255) / 256) + sms - 1) / sms;
   return heads * ((rows + 15) / 16) >= waves * (rows > 128 ? 440 : 350);
