@@ -24,7 +24,7 @@
 //   171 us on the device, 173 with the host's call (12 us more before the scores were formed in halves, below).  A
 //   tile of 256 rows takes about 5,000 cycles, of which the exponentials need 2,048 and the products as much: what bounds
 //   it is the softmax warps' chain of loads, conversions and stores, 1,000 cycles and more for 32 columns whatever waits
-//   beside it.  Half of the issue slots are used.  Reading the queries takes 8,000 cycles of a block and writing the rows
+//   beside it.  Half of the issue slots are used.  Reading the queries takes about 7,000 cycles of a block and writing the rows
 //   5,000.  And the blocks' order: 256 of them start by row block, then by sequence, whatever their length.  Replayed on
 //   148 SMs from these cycles that ends after 153 to 156 us; longest first would end after 116, evenly spread after 105.
 //   Sparse rows (sinks, trees of drafted tokens) have instances of their own, in which a block works through a range of a

@@ -216,7 +216,8 @@ class PageTable:
     ``num_pages`` pages.  ``page_table`` int32 ``[max_sequences, max_pages]`` (-1 where there is none) and ``lengths``
     int32 ``[max_sequences]`` are what `Int4KVCache.attend` takes; pages that no sequence owns lie on a stack,
     ``free_pages`` int32 ``[num_pages]`` of which the first ``free_count`` (int32 ``[1]``) are valid.  A page belongs to
-    one sequence.  All four change in place."""
+    one sequence.  All four change in place, so calls on one table must not overlap on the GPU (one stream, or an order
+    between streams)."""
 
     def __init__(self, num_pages, page_size, max_sequences, max_pages, *, device="cuda"):
         _load()

@@ -812,6 +812,50 @@ def test_a_tree_is_checked_and_its_path_kept(window, sinks):
     assert ((last.double() - want_last.double()).abs() <= 2.0**-7 * want_last.double().abs() + 2.0**-9 * 4).all()
 
 
+@pytest.mark.parametrize("tokens", [200, 3000])
+def test_kernels_that_start_early_wait_for_what_they_read(tokens):
+    """A chain of calls whose inputs the kernel just before makes (torch's or this library's), run on and on, gives what it
+    gives with a wait after every call."""
+    heads, dim, page, b = 4, 64, 16, 5
+    pages = -(-tokens // page) + b
+
+    def run(wait):
+        g = torch.Generator(device="cuda").manual_seed(tokens)
+        cache, table, rotary = m.Int4KVCache(2 * pages, page, heads, dim), m.PageTable(2 * pages, page, b, 2 * pages), m.Rotary(dim)
+        share = _int32([tokens // b] * b)
+        most, results = tokens // b, []
+        x = torch.randn((tokens, heads, dim), generator=g, device="cuda").to(torch.bfloat16)
+        parents = torch.arange(-1, most - 1, dtype=torch.int32, device="cuda").repeat(b) if most <= 1024 else None
+        for step in range(6):
+            offsets, slots, positions = table.extend(share, tokens)
+            wait()
+            q, k = rotary(x, x, positions)
+            wait()
+            cache.append(k, q, slots)
+            wait()
+            order = torch.randperm(tokens, generator=g, device="cuda")
+            wait()
+            cache.move(slots[order] * 1, slots.flip(0) + 0)  # the slots come from the kernels just before
+            wait()
+            bits, depths = m.draft_ancestors(parents * 1, offsets, max_query_tokens=most)
+            wait()
+            a = cache.attend(q, table.page_table, table.lengths, query_offsets=offsets, max_query_tokens=most, ancestors=bits)
+            wait()
+            w = cache.attend(a, table.page_table, table.lengths, query_offsets=offsets, max_query_tokens=most, window=20, sinks=3)
+            wait()
+            x = (a + w).clamp(-3, 3)
+            table.truncate(table.lengths - (share - 1 - step))
+            wait()
+            results.append((x, depths, positions, table.lengths.clone()))
+        torch.cuda.synchronize()
+        return [t.clone() for r in results for t in r] + [cache.k_codes, cache.v_scales, table.page_table, table.free_pages]
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(3):
+        for got, w in zip(run(lambda: None), want):
+            assert torch.equal(got, w)
+
+
 def test_graphs_and_streams():
     """The step captured into two graphs that live at once, replayed in turn and with new inputs in place; and calls on
     two streams at once."""
