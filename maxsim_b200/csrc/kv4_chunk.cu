@@ -30,13 +30,13 @@
 //   Sparse rows (sinks, trees of drafted tokens) have instances of their own, in which a block works through a range of a
 //   line of tiles of all segments (find_place), since segments of 2 to 70 tiles fill 148 SMs badly one to a block (trees:
 //   234 us so, 127 on the line; a part of a segment costs about 10 us beside its tiles: reading queries 4, the first tile's
-//   chain, writing 3).  Their softmax warps take 88 registers, from two warps that only make the block whole warpgroups: with
-//   80 a few words spilled, and as the codes' loads pass through what is left of L1 beside 205 KB of shared memory, every
-//   reload went to L2 (5.3 us a tile of 256 rows where this takes 3.3).  Measured: 16 trees of 25 to 64 nodes after 100 to
-//   8,192 tokens, 32 heads (8 of the cache), D = 128, 127 us with the join; chunks of 512 rows of 4 sequences up to 16,000
-//   tokens, a window of 2,048 and 100 sinks, 147 us.  A tile takes 6,300 cycles there, 3,400 of them in the columns' loops
-//   (exponentials alone: 2,048); the rest are its products' and barriers' latencies.  (The next tile's first scores asked for
-//   before the last probabilities are written: 3% slower.)
+//   chain, writing 3).  Their softmax and unpacking warps take 88 registers, from two warps that only make the block whole
+//   warpgroups: with 80 a few words spilled, and as the codes' loads pass through what is left of L1 beside 205 KB of shared
+//   memory, every reload went to L2 (5.3 us a tile of 256 rows where this takes 3.3).  Measured: 16 trees of 25 to 64 nodes
+//   after 100 to 8,192 tokens, 32 heads (8 of the cache), D = 128, 127 us with the join; chunks of 512 rows of 4 sequences up
+//   to 16,000 tokens, a window of 2,048 and 100 sinks, 148 us.  A tile takes 6,300 cycles there, 3,400 of them in the
+//   columns' loops (exponentials alone: 2,048); the rest are its products' and barriers' latencies.  (The next tile's first
+//   scores asked for before the last probabilities are written: 3% slower.)
 // Every wait is bounded; a block that gives up writes NaN rows.
 #include <algorithm>
 #include <climits>
@@ -636,9 +636,9 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
     count = work_count;
     return count > 0;
   };
-  // Of the 24 x 32 x 80 registers that a line's block is launched with: 16 warps' 88, 4 warps' 80 and 4 warps' 48.  (Each role
-  // asks for its own: after a common place the compiler would not know which it has.  88, 88 and 40: 1% slower, as 96, 64
-  // and 32; 88, 72 and 56: 4%.)
+  // Of the 24 x 32 x 80 registers that a line's block is launched with: 20 warps' 88 and 4 warps' 40.  (Each role asks for its
+  // own: after a common place the compiler would not know which it has.  96, 64 and 32: 1% faster with two row tiles, 10%
+  // slower with one, which the unpacking bounds then; 88, 72 and 56: 4% slower.)
   if (warp < kSoftWarps) {
     if constexpr (kSparse) registers_inc<88>();
     // =================== softmax: a warp has 16 rows, a thread two of them and a quarter of their columns ===================
@@ -967,7 +967,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
       }
     } while (next_list(false));
   } else if (warp < kMmaWarp) {
-    if constexpr (kSparse) registers_inc<80>();  // as many as at launch; for the compiler, which else counts on 88
+    if constexpr (kSparse) registers_inc<88>();
     // =================== unpacking ===================
     // Keys: lane (g, t) takes 16 bytes t (at D = 128) of tokens g, g + 8, .. of its warp's 32.
     const int uw = warp - kUnpackWarp0, g = lane >> 2, t = lane & 3;
@@ -1112,7 +1112,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
       }
     }
   } else {
-    if constexpr (kSparse) registers_dec<48>();
+    if constexpr (kSparse) registers_dec<40>();
     if (warp >= kMmaWarp + 2) {
       // They make a line's block whole warpgroups, and its lists.
       while (next_list(true)) {
