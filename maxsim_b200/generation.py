@@ -323,8 +323,9 @@ class Rotary:
     ``rotary_dim / 2 + i`` (``pairs="halves"``) or ``2i`` and ``2i + 1`` (``"neighbours"``).  Pair ``i`` turns by ``position *
     theta ** (-2i / rotary_dim)``, or ``position * frequencies[i]`` where these are given (radians a position).
     ``sections`` says how many pairs go by each axis, one axis by default: consecutive runs, or ``interleaved``, pair
-    ``i`` of ``n`` axes by axis ``i % n`` while ``i < n * sections[i % n]`` and by the first one from there.  Angles are
-    exact at any position: turns are held to 2^-64."""
+    ``i`` of ``n`` axes by axis ``i % n`` while ``i < n * sections[i % n]`` and by the first one from there.  A
+    frequency is a double, held as turns to 2^-64, so that an angle is off by at most ``|position|`` (2^-65 turns and a
+    double's rounding of the frequency) before it becomes fp32: less than fp32 shows up to some 10^8 positions."""
 
     def __init__(self, head_dim, *, sections=None, theta=10000.0, rotary_dim=None, interleaved=False, pairs="halves",
                  frequencies=None, device="cuda"):
