@@ -395,13 +395,27 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
       any_first = min(any_first, __shfl_xor_sync(0xFFFFFFFFu, any_first, d));
     }
 
-    // This warp's steps of 32 tokens, those that some row sees.  (Sparse rows: j0 and upto count the front's tokens and
-    // those from begin on as one run; token_of has the token.)
-    const int gap = kSparse ? w.begin - w.front : 0, base = kSparse ? 0 : w.begin;
-    auto token_of = [&](int j) { return kSparse && j >= w.front ? j + gap : j; };
-    const int upto = min(base + tile1 * kTile, any_last + 1 - gap);
-    int j0 = base + tile0 * kTile + warp * kStep;
-    if (any_first > token_of(j0) && (!kSparse || j0 >= w.front)) j0 += (any_first - token_of(j0)) / kTile * kTile;
+    // This warp's steps of 32 tokens, those that some row sees.
+    const int base = kSparse ? 0 : w.begin;
+    int j0 = base + tile0 * kTile + warp * kStep, upto = any_last + 1;
+    // Sparse rows: j0 and upto count the front's tokens and those from begin on as one run, and leave out the steps between
+    // the sinks and the first token that these rows' windows see.  The sinks may end past the front (which the first row's
+    // window cuts off), never before it; from the warp's first step past them on, token_of adds `gap`.
+    const int past_sinks = kSparse ? (a.sinks + kStep - 1) & ~(kStep - 1) : 0;
+    int gap = 0;
+    if constexpr (kSparse) {
+      const Kv4Runs runs = kv4_runs(a, w.q.pos0, kStep);  // (w's, which would be held through the loop)
+      gap = runs.begin - runs.front;
+      upto = min(tile1 * kTile, upto - gap);
+      const int turn = j0 + (max(0, past_sinks - j0) + kTile - 1) / kTile * kTile;
+      const int more = max(0, any_first - (turn + gap)) / kTile * kTile;
+      gap += more;
+      upto = max(upto - more, min(upto, turn));  // at least the steps over the sinks
+    } else {
+      upto = min(base + tile1 * kTile, upto);
+      if (any_first > j0) j0 += (any_first - j0) / kTile * kTile;
+    }
+    auto token_of = [&](int j) { return kSparse && j >= past_sinks ? j + gap : j; };
 
     const int32_t* pages = a.page_table + b * a.table_stride;
     const bool two_pages = c.page_shift == 4;  // else 32 aligned tokens lie in one

@@ -1,0 +1,77 @@
+"""The serving step's operators where their ranges end: prompts under a window from their first token on, blocks of many small
+segments, masks wider than any tree, arrays between guard words, steps that nothing waits for."""
+
+import pytest
+
+import maxsim_b200 as m
+from maxsim_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_kv4 import DTYPES, _normal, _random_cache, _tables  # noqa: E402
+from test_gpu_reader_step import _check_rows, _int32, engine  # noqa: E402, F401
+
+
+# --------------------------------------------------------------------------- prompts under a window with sinks
+
+def _window_mask(length, rows, window, sinks):
+    """[rows, length]: the last `rows` tokens, each up to its own, the last `window` of these and the first `sinks`."""
+    p, j = torch.arange(length - rows, length).unsqueeze(1), torch.arange(length)
+    return (j <= p) & ((j > p - window) | (j < sinks))
+
+
+def _check_prompts(dim, heads, shared, page, dtype, lengths, rows, window, sinks, seed=0):
+    pages = sum(-(-n // page) for n in lengths) + 2
+    cache, table = _random_cache(pages, page, heads, dim, seed), _tables(lengths, page, pages, seed=seed)
+    offsets = [sum(rows[:b]) for b in range(len(rows) + 1)]
+    query = _normal((offsets[-1], heads * shared, dim), seed + 9, DTYPES[dtype], 1.5)
+    got, lse = cache.attend(query, table, _int32(lengths), query_offsets=_int32(offsets), max_query_tokens=max(rows),
+                            window=window, sinks=sinks, return_lse=True)
+    masks = [_window_mask(n, r, window, sinks) for n, r in zip(lengths, rows)]
+    _check_rows(got, lse, query, cache, table, lengths, offsets, masks, dim**-0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [24, 256, 1024])
+@pytest.mark.parametrize("sinks", [4, 64, 300])
+def test_sinks_of_prompts_from_their_first_token(engine, dim, window, sinks):  # noqa: F811
+    """Rows whose window has left the sinks beside rows whose window is still over them, in one sequence."""
+    _check_prompts(dim, 2, 4, 16, "bf16", [200, 512, 700, 1536], [200, 512, 700, 512], window, sinks, seed=sinks)
+
+
+@pytest.mark.parametrize("dim,heads,shared,length,rows,window,sinks", [
+    (128, 8, 1, 200, 200, 24, 4), (128, 2, 4, 512, 512, 256, 4), (256, 1, 1, 300, 300, 1, 1), (256, 8, 4, 1536, 512, 1024, 4),
+    (64, 1, 4, 2500, 2500, 130, 33), (128, 1, 2, 2500, 1000, 700, 1000), (128, 1, 1, 5000, 5000, 16, 97)])
+def test_sinks_of_one_prompt(dim, heads, shared, length, rows, window, sinks):
+    """One sequence, by the kernel that the sizes choose: a cluster a segment, or ranges that end among the sinks, between
+    them and the window, within it."""
+    _check_prompts(dim, heads, shared, 32, "f16", [length], [rows], window, sinks, seed=length)
+
+
+@pytest.mark.parametrize("window,sinks", [(24, 4), (256, 64)])
+def test_the_example_sees_a_long_prompts_sinks(monkeypatch, window, sinks):
+    """Every layer's attention to prompts of 300 tokens and fewer, in 64 bits."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    import answer_with_drafts
+
+    plain, prompts, seen = m.Int4KVCache.attend, (300, 5, 80), []
+
+    def attend(cache, query, page_table, lengths, **kw):
+        out = plain(cache, query, page_table, lengths, **kw)
+        if kw.get("ancestors") is None:
+            got, lse = plain(cache, query, page_table, lengths, return_lse=True, **kw)
+            assert torch.equal(got, out)
+            offsets = kw["query_offsets"].tolist()
+            masks = [_window_mask(n, n, window, sinks) for n in prompts]
+            _check_rows(got, lse, query, cache, page_table, lengths.tolist(), offsets, masks, query.shape[2]**-0.5)
+            seen.append(offsets)
+        return out
+
+    monkeypatch.setattr(m.Int4KVCache, "attend", attend)
+    answer_with_drafts.main(prompts=prompts, tokens=1, window=window, sinks=sinks)
+    assert seen == [[0, 300, 305, 385]] * 2
