@@ -100,8 +100,9 @@ struct TopkFuse {
 };
 
 // A launch that may start while the kernel before it on the stream ends: its first blocks are then in place when that one's
-// results are.  The kernel calls wait_for_previous() before it reads or writes any memory, in every thread.  With `cluster`,
-// in clusters of so many blocks.
+// results are.  The kernel calls wait_for_previous() before it reads or writes any memory, in every thread, and reads with
+// ordinary loads: memory that the kernel before it writes is not constant during its life.  With `cluster`, in clusters of so
+// many blocks.
 template <class... Params, class... Args>
 void launch_early(void (*kernel)(Params...), dim3 blocks, int threads, size_t shared, cudaStream_t stream, int cluster,
                   const char* what, Args... args) {

@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Mo
     const int64_t i = threadIdx.x + k * kMoveThreads;
     to[k] = -1;
     if (i >= a.tokens) continue;
-    const int64_t source = __ldg(a.source + i), target = __ldg(a.target + i);
+    const int64_t source = a.source[i], target = a.target[i];
     if (source < 0 || source >= slots || target < 0 || target >= slots) continue;
     to[k] = moved_vector(c, target, head);
     const int64_t from = moved_vector(c, source, head);
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) kv4_move_many_kernel(Kv4View c, Kv4M
     const int64_t i = first + k * kStep;
     here[k] = -1;
     if (i >= a.tokens) continue;
-    const int64_t source = __ldg(a.source + i), target = __ldg(a.target + i);
+    const int64_t source = a.source[i], target = a.target[i];
     if (source < 0 || source >= slots || target < 0 || target >= slots) continue;
     here[k] = moved_vector(c, kOut ? source : target, head);
   }

@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
                      static_cast<int64_t>(head * line.shared + r % line.shared) * a.q_head_stride + t * (kDim / 4);
         if (line.aligned) {
 #pragma unroll
-          for (int i = 0; i < kRaw; ++i) raw[nt][i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+          for (int i = 0; i < kRaw; ++i) raw[nt][i] = load_input<kSparse>(reinterpret_cast<const uint4*>(p) + i);
         } else {
           load_scattered(raw[nt], p);
         }
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(kWarps * 32, resident_blocks(kDim, kTiles)) kv
     uint32_t seen_queue = 0;  // two bits a step, the oldest lowest: its 16-token tiles lie on pages of the cache
     auto ask_pages = [&](int j) {
       const int at = token_of(j);
-      next_page[0] = j < upto ? __ldg(pages + (at >> c.page_shift)) : -1;
-      next_page[1] = !two_pages ? next_page[0] : j + 16 < upto ? __ldg(pages + ((at + 16) >> c.page_shift)) : -1;
+      next_page[0] = j < upto ? load_input<kSparse>(pages + (at >> c.page_shift)) : -1;
+      next_page[1] = !two_pages ? next_page[0] : j + 16 < upto ? load_input<kSparse>(pages + ((at + 16) >> c.page_shift)) : -1;
     };
     // Copies the step at j into a stage; tiles without a page copy the cache's first vectors.
     auto copy_step = [&](int j, int stage, int slot) {

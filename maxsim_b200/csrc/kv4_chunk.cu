@@ -278,9 +278,9 @@ __device__ __forceinline__ void references(const float (&f)[16], const float* me
 }
 
 // Whether token j's value is a vector of zeros.  Out of line: in the unpacking warps' loop it cost 5 us of 170.
-template <int kDim>
+template <int kDim, bool kSparse>
 __device__ __noinline__ bool zero_value(const uint8_t* codes, const int32_t* pages, int heads, int head, int page_shift, int j) {
-  const int64_t page = __ldg(pages + (j >> page_shift));
+  const int64_t page = load_input<kSparse>(pages + (j >> page_shift));
   return zero_codes<kDim>(codes + (((page * heads + head) << page_shift) + (j & ((1 << page_shift) - 1))) * (kDim / 2));
 }
 
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
   const int page_mask = (1 << c.page_shift) - 1;
   // Vector of token j's 16-token group on page p (-1: none), and whether the page is the cache's.
   auto ask_page = [&](const Work& w, int j) {
-    return j <= w.any_last ? __ldg(a.page_table + w.b * a.table_stride + (j >> c.page_shift)) : -1;
+    return j <= w.any_last ? load_input<kSparse>(a.page_table + w.b * a.table_stride + (j >> c.page_shift)) : -1;
   };
   auto vector_of = [&](const Work& w, int page, int j) {
     return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages)
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
               const T* src = static_cast<const T*>(a.query) + (w.q.row0 + token) * a.q_row_stride +
                              static_cast<int64_t>(w.head * shared + in_group) * a.q_head_stride + (lane % kRowLanes) * 8;
               if (aligned) {
-                x[k] = __ldg(reinterpret_cast<const uint4*>(src));
+                x[k] = load_input<kSparse>(reinterpret_cast<const uint4*>(src));
               } else {
                 __align__(16) T e[8];
 #pragma unroll
@@ -983,10 +983,10 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
       for (int k = 0; k < 4; ++k) {
         const uint8_t* src = c.codes[0] + (v[k >> 1] + 8 * (k & 1) + g) * (kDim / 2) + t * (kDim / 8);
         if constexpr (kWords == 4) {
-          const uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
+          const uint4 u = load_input<kSparse>(reinterpret_cast<const uint4*>(src));
           word[k][0] = u.x, word[k][1] = u.y, word[k][2] = u.z, word[k][3] = u.w;
         } else {
-          const uint2 u = __ldg(reinterpret_cast<const uint2*>(src));
+          const uint2 u = load_input<kSparse>(reinterpret_cast<const uint2*>(src));
           word[k][0] = u.x, word[k][1] = u.y;
         }
       }
@@ -994,8 +994,8 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
       const int64_t at = (lane < 16 ? v[0] : v[1]) + (lane & 15);
       seen = static_cast<uint32_t>(lane < 16 ? page[0] : page[1]) < static_cast<uint32_t>(c.num_pages) &&
              (mine >= w.any_first || (kSparse && mine < a.sinks)) && mine <= w.any_last;
-      ks = __ldg(c.scales[0] + at);
-      vs = __ldg(c.scales[1] + at);
+      ks = load_input<kSparse>(c.scales[0] + at);
+      vs = load_input<kSparse>(c.scales[1] + at);
       const int next = kSparse ? w.tile_start<kSparse>(i + 1) + 32 * uw : j + kTokens;
       page[0] = ask_page(w, next);
       page[1] = ask_page(w, next + 16);
@@ -1012,10 +1012,10 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if constexpr (kValueWords == 2) {
-          const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + k * (kDim / 2)));
+          const uint2 u = load_input<kSparse>(reinterpret_cast<const uint2*>(src + k * (kDim / 2)));
           value[k][0] = u.x, value[k][1] = u.y;
         } else {
-          value[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * (kDim / 2)));
+          value[k][0] = load_input<kSparse>(reinterpret_cast<const uint32_t*>(src + k * (kDim / 2)));
         }
       }
       value_page = ask_page(w, kSparse ? w.tile_start<kSparse>(i + 1) + (group >> 1) * 16 : j + kTokens);
@@ -1056,7 +1056,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
           }
           float* const ms = meta + s * 3 * kMetaFloats + meta_at(32 * uw + lane);
           if (seen && vs == 1.0F &&
-              zero_value<kDim>(c.codes[1], a.page_table + w.b * a.table_stride, c.heads, w.head, c.page_shift,
+              zero_value<kDim, kSparse>(c.codes[1], a.page_table + w.b * a.table_stride, c.heads, w.head, c.page_shift,
                                w.tile_start<kSparse>(i) + 32 * uw + lane))
             vs = 0.0F;
           ms[0] = seen ? ks : 0.0F;

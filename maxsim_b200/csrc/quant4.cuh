@@ -128,6 +128,15 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Attend& a, int page
   return s;
 }
 
+// A load of what the kernel only reads.  One launched early (launch_early) is resident while the kernel before it may
+// still be writing that: it has ordinary loads, which come after its wait; __ldg is for memory that nothing writes while the
+// kernel lives, whatever it waits for.
+template <bool kEarly, class V>
+__device__ __forceinline__ V load_input(const V* p) {
+  if constexpr (kEarly) return *p;
+  else return __ldg(p);
+}
+
 // What a row sees.  Without masks: tokens first .. last, and those below `sinks` up to last.  With masks (a tree of
 // drafted tokens), a row's bits are the sequence's rows that it sees, n of them; first .. last are the context, what is
 // cached before the sequence's rows, and of it the last window - n.
@@ -149,7 +158,7 @@ __device__ __forceinline__ Kv4Seen kv4_seen(const Kv4Attend& a, const Kv4Sequenc
     const int all = q.rows + q.left;
     int n = 0;
     for (int w = 0; w < a.words && 64 * w < all; ++w) {
-      uint64_t word = static_cast<uint64_t>(__ldg(bits + w));
+      uint64_t word = static_cast<uint64_t>(bits[w]);
       if (all - 64 * w < 64) word &= (uint64_t{1} << (all - 64 * w)) - 1;
       n += __popcll(word);
     }
@@ -163,8 +172,8 @@ __device__ __forceinline__ uint32_t kv4_tree_bits(const Kv4Attend& a, const Kv4S
   if (at <= -32 || at >= all) return 0;
   const uint32_t* words = reinterpret_cast<const uint32_t*>(a.ancestors + (q.row0 + row) * a.ancestors_stride);
   const int w = at >> 5;
-  const uint32_t lo = w >= 0 && w < 2 * a.words ? __ldg(words + w) : 0u;
-  const uint32_t hi = w + 1 < 2 * a.words ? __ldg(words + w + 1) : 0u;
+  const uint32_t lo = w >= 0 && w < 2 * a.words ? words[w] : 0u;
+  const uint32_t hi = w + 1 < 2 * a.words ? words[w + 1] : 0u;
   const uint32_t bits = __funnelshift_r(lo, hi, at & 31);
   return all - at < 32 ? bits & ((1u << (all - at)) - 1) : bits;
 }

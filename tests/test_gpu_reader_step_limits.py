@@ -75,3 +75,57 @@ def test_the_example_sees_a_long_prompts_sinks(monkeypatch, window, sinks):
     monkeypatch.setattr(m.Int4KVCache, "attend", attend)
     answer_with_drafts.main(prompts=prompts, tokens=1, window=window, sinks=sinks)
     assert seen == [[0, 300, 305, 385]] * 2
+
+
+# --------------------------------------------------------------------------- kernels that start early
+
+@pytest.mark.parametrize("dim,most", [(64, 3), (128, 12), (128, 70), (256, 12)])
+def test_inputs_that_the_kernel_before_writes_anew(engine, dim, most):  # noqa: F811
+    """Page table entries, masks, queries and codes at the same addresses step after step, each written by the kernel just
+    before the one that reads it, while that one is already there."""
+    b, heads, kv, page = 9, 8, 2, 16
+    rows, parents = b * most, _int32([-1] + [i // 2 for i in range(most - 1)]).repeat(b)
+    tokens, flat = _int32([most] * b), _int32([-1, *range(most - 1)]).repeat(b)
+    x = _normal((20, rows, heads + 2 * kv, dim), dim + most, torch.bfloat16)
+
+    def run(wait):
+        cache, table, rotary = m.Int4KVCache(400, page, kv, dim), m.PageTable(400, page, b, 40), m.Rotary(dim)
+        query, kept, results = torch.empty((rows, heads, dim), dtype=torch.bfloat16, device="cuda"), torch.empty(0), []
+        before = _int32([5 * i for i in range(b)])
+        _, slots, _ = table.extend(before, 180)
+        cache.append(x[0, :1, :kv].expand(180, kv, dim), x[0, :1, kv:2 * kv].expand(180, kv, dim), slots)
+        for step in range(20):
+            now = x[step]
+            offsets, slots, positions = table.extend(tokens, rows)
+            wait()
+            cache.append(now[:, heads:heads + kv], now[:, heads + kv:], slots)
+            wait()
+            cache.move(slots.flip(0), slots)
+            wait()
+            bits, depths = m.draft_ancestors(parents if step % 2 else flat, offsets, max_query_tokens=most)
+            wait()
+            rotary(now[:, :heads], None, positions, out=(query, None))
+            wait()
+            a = cache.attend(query, table.page_table, table.lengths, query_offsets=offsets, max_query_tokens=most, ancestors=bits)
+            wait()
+            rotary(now[:, :heads], None, depths, out=(query, None))
+            wait()
+            w = cache.attend(query, table.page_table, table.lengths, query_offsets=offsets, max_query_tokens=most, window=9, sinks=4)
+            wait()
+            kept = table.lengths - (tokens - step % 2)  # every second step keeps a token
+            table.truncate(kept)
+            wait()
+            if step % 5 == 4:  # other pages for all
+                table.truncate(torch.zeros_like(tokens))
+                wait()
+                table.extend(kept.flip(0), 400)
+                wait()
+            results += [a, w, table.lengths.clone(), table.page_table.clone()]
+        torch.cuda.synchronize()
+        return results
+
+    want = run(torch.cuda.synchronize)
+    assert not any(torch.isnan(t).any() for t in want)
+    for _ in range(3):
+        for got, w in zip(run(lambda: None), want):
+            assert torch.equal(got, w)
