@@ -1159,7 +1159,11 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
           if (kSparse && w.tiles == 0) continue;
           alone = w.tiles_m == 1;
           ok = wait(q_full, kSparse ? w.segments & 1 : 0);
-          if (kSparse && m >= w.tiles_m) continue;
+          if (kSparse && m >= w.tiles_m) {
+            // Nothing to do but to have seen this phase: the next one's arrivals come after o_full, which waits for this.
+            if (ok && lane == 0) mbar_arrive(o_full);
+            continue;
+          }
           const int start = kSparse ? w.done : 0;
           ok = ok && wait(&k_full[start & 1], (start >> 1) & 1);
           if (ok) {
@@ -1185,7 +1189,7 @@ __global__ void __launch_bounds__(kSparse ? kLineThreads : kThreads, 1)
             commit_both(&v_empty[s]);
             if (more) other_half(s ^ 1);
           }
-          if (ok) commit_both(o_full);
+          if (ok) mma_commit(leader, o_full);
         }
         __syncwarp();
       } while (next_list(false));

@@ -129,3 +129,48 @@ def test_inputs_that_the_kernel_before_writes_anew(engine, dim, most):  # noqa: 
     for _ in range(3):
         for got, w in zip(run(lambda: None), want):
             assert torch.equal(got, w)
+
+
+@pytest.mark.parametrize("dim,shared,batch", [(64, 8, 400), (128, 4, 150), (128, 64, 90)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_segments_of_one_and_two_row_tiles_in_turn(dim, shared, batch, tree):
+    """Dozens of segments for each block of the kernel for many rows, of few tiles of tokens: runs of segments with one
+    tile of rows, where half of the kernel's warps have no products and only keep up, with some of two, of more than 256
+    rows and without tokens among them."""
+    sizes = [1, 2, 3, 1, 1, 128 // shared, 1, 2, 0, 1, 128 // shared + 1, 1, 1, 256 // shared + 1, 1, 2, 256 // shared, 1, 1, 0]
+    rows = [sizes[(7 * b) % 20 if b % 60 < 30 else b % 5] for b in range(batch)]
+    lengths = [max(0, n + [0, 40, 3, 130, 0, 300, 17][b % 7] - (n if b % 23 == 5 else 0)) for b, n in enumerate(rows)]
+    trees = [[(i - 1) // 2 for i in range(n)] for n in rows]
+    pages = sum(-(-n // 16) for n in lengths) + 2
+    cache, table = _random_cache(pages, 16, 2, dim, 3), _tables(lengths, 16, pages, seed=4)
+    offsets = [sum(rows[:b]) for b in range(batch + 1)]
+    query = _normal((offsets[-1], 2 * shared, dim), 5, torch.float16, 1.5)
+    kw = dict(query_offsets=_int32(offsets), max_query_tokens=max(rows), return_lse=True)
+    if tree:
+        kw["ancestors"], _ = m.draft_ancestors(_int32([p for t in trees for p in t]), kw["query_offsets"], max_query_tokens=max(rows))
+        masks = [_tree_mask(n, t) for n, t in zip(lengths, trees)]
+    else:
+        kw.update(window=50, sinks=7)
+        masks = [_window_mask(n, r, 50, 7) for n, r in zip(lengths, rows)]
+    _lib.set_option("kv4_engine", 2)
+    try:
+        results = [cache.attend(query, table, _int32(lengths), **kw) for _ in range(4)]
+    finally:
+        _lib.set_option("kv4_engine", 0)
+    for got, lse in results[1:]:
+        assert torch.equal(got, results[0][0]) and torch.equal(lse, results[0][1])
+    _check_rows(*results[0], query, cache, table, lengths, offsets, masks, dim**-0.5)
+
+
+def _tree_mask(length, parents):
+    """[nodes, length]: all before the nodes, and each node's path."""
+    rows, first = len(parents), length - len(parents)
+    mask = torch.zeros((rows, length), dtype=torch.bool)
+    for i, p in enumerate(parents):
+        if p >= 0:
+            mask[i] = mask[p]
+        elif first > 0:
+            mask[i, :first] = True
+        if first + i >= 0:
+            mask[i, first + i] = True
+    return mask
