@@ -356,8 +356,10 @@ __global__ void __launch_bounds__(kTreeThreads) draft_ancestors_kernel(DraftTree
     parent[i] = static_cast<int16_t>(p >= 0 && p < i ? p : -1);
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < rows * t.words; k += kTreeThreads) {
-    const int i = k / t.words, word = k - i * t.words;
+  // Words with nodes, and those past them (a caller's rows may be wider, up to 2^24 words: their number passes 32 bits).
+  const int words = min(t.words, kMostTreeRows / 64);
+  for (int k = threadIdx.x; k < rows * words; k += kTreeThreads) {
+    const int i = k / words, word = k - i * words;
     uint64_t bits = 0;
     int depth = -1;
     for (int at = i; at >= 0; at = parent[at]) {
@@ -367,6 +369,8 @@ __global__ void __launch_bounds__(kTreeThreads) draft_ancestors_kernel(DraftTree
     t.ancestors[(lo + i) * t.words + word] = static_cast<int64_t>(bits);
     if (word == 0) t.depths[lo + i] = depth;
   }
+  for (int i = threadIdx.x / 32; i < rows; i += kTreeThreads / 32)
+    for (int word = words + threadIdx.x % 32; word < t.words; word += 32) t.ancestors[(lo + i) * t.words + word] = 0;
   auto clear = [&](int64_t from, int64_t to) {
     for (int64_t k = from * t.words + threadIdx.x; k < to * t.words; k += kTreeThreads) t.ancestors[k] = 0;
     for (int64_t i = from + threadIdx.x; i < to; i += kTreeThreads) t.depths[i] = 0;

@@ -174,3 +174,27 @@ def _tree_mask(length, parents):
         if first + i >= 0:
             mask[i, first + i] = True
     return mask
+
+
+# --------------------------------------------------------------------------- masks of drafted trees, from C
+
+def _draft_ancestors(parents, offsets, most, words, ancestors, depths):
+    rows, batch = ancestors.shape[0], offsets.shape[0] - 1
+    _lib.check(_lib.lib.msb_draft_ancestors_device(parents.data_ptr(), rows, offsets.data_ptr(), batch, most, words,
+                                                   ancestors.data_ptr(), depths.data_ptr(), 0,
+                                                   torch.cuda.current_stream().cuda_stream))
+
+
+@pytest.mark.parametrize("rows,words", [(5, 1), (70, 2), (70, 3), (70, 16), (70, 17), (70, 100), (1024, 2**21)])
+def test_masks_wider_than_their_trees(rows, words):
+    """Words past a tree's nodes are 0, however wide the caller's rows are: the last case has 2^31 words, 17 GB."""
+    if 8 * rows * words > torch.cuda.mem_get_info()[0] // 2:
+        pytest.skip("not enough memory")
+    ancestors = torch.full((rows + 1, words), -1, dtype=torch.int64, device="cuda")
+    depths = torch.full((rows + 1,), -1, dtype=torch.int32, device="cuda")
+    parents = torch.tensor([i - 1 if i % 50 else i - 3 for i in range(rows + 1)], dtype=torch.int32, device="cuda")
+    _draft_ancestors(parents, _int32([0, rows]), rows, words, ancestors, depths)
+    want, want_depths = m.draft_ancestors(parents[:rows], _int32([0, rows]), max_query_tokens=rows)
+    held = want.shape[1]
+    assert torch.equal(ancestors[:rows, :held], want) and torch.equal(depths[:rows], want_depths)
+    assert not ancestors[:, held:].any() and not ancestors[rows].any() and depths[rows] == 0
