@@ -377,7 +377,7 @@ int msb_kv4_attend_masked_device(const msb_kv4_cache* cache, const msb_kv4_atten
 /* Masks and depths of the nodes of drafted trees: parents[i] of row i is a row of the same sequence with a lower place
  * (counted from its first row); any other number: the context's last token.  ancestors [rows, words], words at least
  * ceil(max_query_rows / 64): the row's path up, itself among it; depths [rows]: nodes above it.  max_query_rows at most
- * 1024; rows past it of their sequence, and rows that no sequence owns, get 0. */
+ * 1024; rows past it of their sequence, and rows that no sequence owns (all of them where batch is 0), get 0. */
 int msb_draft_ancestors_device(const int32_t* parents, int64_t rows, const int32_t* query_offsets, int32_t batch,
                                int32_t max_query_rows, int32_t words, int64_t* ancestors, int32_t* depths,
                                int32_t device, void* stream);

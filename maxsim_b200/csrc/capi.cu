@@ -1727,12 +1727,19 @@ int msb_draft_ancestors_device(const int32_t* parents, int64_t rows, const int32
     if (max_query_rows > kMostTreeRows) throw InvalidArgument("max_query_rows must be at most 1024");
     if (words < 1 || words < (max_query_rows + 63) / 64) throw InvalidArgument("words must be at least ceil(max_query_rows / 64)");
     if (words > 1 << 24) throw InvalidArgument("words must be at most 2^24");
-    if (rows == 0 || batch == 0) return;
-    if (!parents || !query_offsets || !ancestors || !depths) throw InvalidArgument("NULL argument");
+    if (rows == 0) return;
+    if (!ancestors || !depths || (batch > 0 && (!parents || !query_offsets))) throw InvalidArgument("NULL argument");
     check_address(parents, 4, "parents");
     check_address(query_offsets, 4, "query_offsets");
     check_address(ancestors, 8, "ancestors");
     check_address(depths, 4, "depths");
+    if (batch == 0) {  // no sequence owns a row
+      DeviceGuard g(device);
+      const size_t n = static_cast<size_t>(rows);
+      check(cudaMemsetAsync(ancestors, 0, n * words * sizeof(int64_t), static_cast<cudaStream_t>(stream)), "clear ancestors");
+      check(cudaMemsetAsync(depths, 0, n * sizeof(int32_t), static_cast<cudaStream_t>(stream)), "clear depths");
+      return;
+    }
     DraftTrees t{parents, query_offsets, rows, ancestors, depths, batch, max_query_rows, words};
     DeviceGuard g(device);
     launch_draft_ancestors(t, static_cast<cudaStream_t>(stream));

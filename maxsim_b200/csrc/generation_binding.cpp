@@ -361,10 +361,6 @@ PyObject* draft_ancestors(PyObject* const* args, Py_ssize_t n) {
   const int64_t words = std::max<int64_t>(1, (most + 63) / 64);
   const at::Tensor parents = given.contiguous(), offsets = starts.contiguous();
   at::Tensor ancestors = empty({rows, words}, c10::kLong, device), depths = empty({rows}, c10::kInt, device);
-  if (batch == 0) {
-    ancestors.zero_();
-    depths.zero_();
-  }
   check_status(msb_draft_ancestors_device(parents.const_data_ptr<int32_t>(), rows, offsets.const_data_ptr<int32_t>(),
                                           static_cast<int32_t>(batch), static_cast<int32_t>(most),
                                           static_cast<int32_t>(words), ancestors.mutable_data_ptr<int64_t>(),

@@ -198,3 +198,16 @@ def test_masks_wider_than_their_trees(rows, words):
     held = want.shape[1]
     assert torch.equal(ancestors[:rows, :held], want) and torch.equal(depths[:rows], want_depths)
     assert not ancestors[:, held:].any() and not ancestors[rows].any() and depths[rows] == 0
+
+
+def test_rows_of_no_sequence_at_all():
+    """Without sequences every row's mask and depth is 0, from C as from Python; nothing past the rows is written."""
+    ancestors = torch.full((6, 3), -1, dtype=torch.int64, device="cuda")
+    depths = torch.full((6,), -1, dtype=torch.int32, device="cuda")
+    parents, offsets = _int32([-1, 0, 1, 2, 3]), _int32([0])
+    _draft_ancestors(parents, offsets, 5, 3, ancestors[:5], depths[:5])
+    assert not ancestors[:5].any() and not depths[:5].any() and (ancestors[5] == -1).all() and depths[5] == -1
+    for _ in range(3):  # fresh memory that holds something
+        torch.full((1000,), -1, dtype=torch.int64, device="cuda")
+        bits, depths = m.draft_ancestors(parents, offsets)
+        assert bits.shape == (5, 1) and not bits.any() and not depths.any()

@@ -215,3 +215,10 @@ def test_package_refuses_host_devices_and_bad_sizes():
         m.draft_ancestors(one, one)
     with pytest.raises(TypeError, match="tensor"):
         m.draft_ancestors([0], one)
+
+
+@pytest.mark.parametrize("ancestors,depths,text", [(None, _PTR, "NULL"), (_PTR, None, "NULL"), (_PTR + 4, _PTR, "aligned")])
+def test_draft_ancestors_without_sequences_still_writes(ancestors, depths, text):
+    """Rows that no sequence owns are cleared, so their arrays have to be there; parents and offsets need not."""
+    with pytest.raises(ValueError, match=text):
+        check(lib.msb_draft_ancestors_device(None, 5, None, 0, 3, 1, ancestors, depths, 0, None))
