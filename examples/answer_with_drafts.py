@@ -76,7 +76,7 @@ def main(prompts=(37, 5, 80), tokens=24, layers=2, dim=128, heads=8, kv_heads=2,
     grow = torch.full((batch,), nodes, dtype=torch.int32, device="cuda")
     parents = torch.tensor(PARENTS * batch, dtype=torch.int32, device="cuda")
     first = torch.arange(batch, device="cuda").unsqueeze(1) * nodes  # each sequence's first row
-    place = torch.arange(len(PATH), device="cuda")
+    place, path = torch.arange(len(PATH), device="cuda"), torch.tensor(PATH, device="cuda")
     answer, counts = [], []
     for _ in range(tokens):
         before = table.lengths.clone()
@@ -94,12 +94,11 @@ def main(prompts=(37, 5, 80), tokens=24, layers=2, dim=128, heads=8, kv_heads=2,
         right = torch.stack((says[:, 0] == draft[:, 2], says[:, 2] == draft[:, 4]), dim=1)
         count = 1 + right.int().cumprod(dim=1).sum(dim=1)
         kept = place < count.unsqueeze(1)
-        path = torch.tensor(PATH, device="cuda")
         source = torch.where(kept, slots[first + path], -1)
         for layer in model:
             layer.cache.move(source.flatten(), slots[first + place].flatten())
         table.truncate(before + count.int())
-        answer.append(torch.where(kept, draft[:, PATH], -1))
+        answer.append(torch.where(kept, draft[:, path], -1))
         counts.append(count)
         logits = logits[torch.arange(batch, device="cuda"), path[count - 1]]
     return torch.stack(answer, dim=1), torch.stack(counts, dim=1)

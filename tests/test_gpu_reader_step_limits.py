@@ -211,3 +211,29 @@ def test_rows_of_no_sequence_at_all():
         torch.full((1000,), -1, dtype=torch.int64, device="cuda")
         bits, depths = m.draft_ancestors(parents, offsets)
         assert bits.shape == (5, 1) and not bits.any() and not depths.any()
+
+
+def test_the_examples_steps_wait_for_nothing(monkeypatch):
+    """The host asks for step after step without waiting for the GPU: no copy from pageable memory and no read-back from the
+    first step's table call on."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    import answer_with_drafts
+
+    extend, calls = m.PageTable.extend, []
+
+    def watched(table, tokens, rows):
+        if calls:  # the first call is the prompts'
+            torch.cuda.set_sync_debug_mode("error")
+        calls.append(rows)
+        return extend(table, tokens, rows)
+
+    monkeypatch.setattr(m.PageTable, "extend", watched)
+    try:
+        answer, counts = answer_with_drafts.main(prompts=(20, 1, 33), tokens=5, window=24, sinks=3)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert calls == [54] + [15] * 5
+    assert torch.equal((answer >= 0).sum(dim=2), counts) and ((counts >= 1) & (counts <= 3)).all()
