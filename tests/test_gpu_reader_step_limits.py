@@ -237,3 +237,38 @@ def test_the_examples_steps_wait_for_nothing(monkeypatch):
         torch.cuda.set_sync_debug_mode("default")
     assert calls == [54] + [15] * 5
     assert torch.equal((answer >= 0).sum(dim=2), counts) and ((counts >= 1) & (counts <= 3)).all()
+
+
+# --------------------------------------------------------------------------- page tables
+
+@pytest.mark.parametrize("sequences", [1, 3, 256, 257, 1500])
+@pytest.mark.parametrize("lengths,count,page", [(1 << 30, 1 << 30, -5), (-9, -9, 1 << 30), (63, 6, -(1 << 31)), (64, 0, 7),
+                                                (0, 6, 7), (17, 1 << 30, 1 << 30), (40, 3, 3)])
+def test_page_tables_that_hold_nonsense_keep_to_their_arrays(sequences, lengths, count, page):
+    """Whatever lengths, counts and ids the four arrays hold, nothing beside any of them is written, and what is read of them
+    is theirs: all four lie between guard words, whose values as lengths, counts or ids would show in the results."""
+    guard, gap = 123456789, 512
+    sizes = (4 * sequences, sequences, 6, 1)  # table [sequences, 4], lengths, stack of 6, its count
+    results = []
+    for value in (guard, -guard):
+        store = torch.full((sum(sizes) + gap * 5,), value, dtype=torch.int32, device="cuda")
+        parts, inside, at = [], torch.zeros_like(store, dtype=torch.bool), gap
+        for n, fill in zip(sizes, (page, lengths, page, count)):
+            parts.append(store[at:at + n])
+            parts[-1].fill_(fill)
+            inside[at:at + n] = True
+            at += n + gap
+        table = m.PageTable.from_tensors(parts[0].view(sequences, 4), *parts[1:], page_size=16)
+        tokens = torch.full((sequences,), 7, dtype=torch.int32, device="cuda")
+        seen = []
+        for call in ("extend", "truncate", "extend"):
+            if call == "extend":
+                seen += table.extend(tokens, 7 * sequences)
+                assert ((seen[-1] >= -1) & (seen[-1] < 64)).all()
+            else:
+                table.truncate(torch.full((sequences,), -3, dtype=torch.int32, device="cuda"))
+                assert (table.lengths == 0).all() and 0 <= table.free_count.item() <= 6
+            assert (store[~inside] == value).all()
+            seen += [t.clone() for t in parts]
+        results.append(seen)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
