@@ -73,7 +73,8 @@ int32_t type_id(c10::ScalarType type, bool f32) {
   if (type == c10::kFloat && f32) return MSB_TYPE_F32;
   refuse(std::string("dtype must be ") + (f32 ? "fp32, fp16 or bf16" : "fp16 or bf16") + ", got " + c10::toString(type));
 }
-// (at::empty comes here through two dispatches, 0.15 us a tensor.)
+// (at::empty comes here through two dispatches, 0.15 us a tensor.  Dispatch modes do not see these tensors, nor are they filled
+// where torch fills uninitialised memory: every element of an output is written.)
 at::Tensor empty(c10::IntArrayRef sizes, c10::ScalarType type, c10::Device device) {
   return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }

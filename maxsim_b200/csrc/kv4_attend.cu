@@ -40,12 +40,13 @@
 //   Short contexts (shape_of has the rule) take a cluster of 2 to 8 blocks a segment instead, whose parts are
 //   joined over distributed shared memory: one launch.
 //   Sparse rows have instances of their own.  A sequence's units are those over its two runs of tokens, the sinks and the
-//   window's, counted as one (what lies between is never loaded); only steps at a run's end form masks, from a row's bounds
+//   window's, counted as one (what lies between is never loaded); of these a warp leaves out the steps between the sinks and
+//   what the windows of its own rows see.  Steps that one of the rows does not see whole form masks, from the rows' bounds
 //   and, over a tree, 32 of its bits at once.
 //   Measured on the device, D = 128, 8 heads, 4 query heads each: 64 sequences of 4,096 tokens 77 us (3.7 TB/s of
 //   codes, 57% of a copy's rate), 2 of 115,000 66 us (3.8 TB/s), 1 of 16,384 17 us, 1 of 1,030 6.9 us; of the first 4 to
 //   5 us are the join and both launches' ends.  D = 256: the first 134 us (4.1 TB/s).  Sparse rows: 64 sequences of up to
-//   16,384 tokens, the last 4,096 and the first 64 of each seen, 78.5 us (3.2 TB/s); one of 30,001, 1,024 and 4 seen, 7.2 us.
+//   16,384 tokens, the last 4,096 and the first 64 of each seen, 80 us (3.2 TB/s); one of 30,001, 1,024 and 4 seen, 7.3 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -1051,7 +1052,10 @@ bool many_rows(const Kv4View& c, const Kv4Attend& a) {
     // file's: 10, 0.025 a row block of 16, and 5.8 ns (D = 64: 3.8) a tile of each.  kv4_chunk.cu's: 13, and 17 ns (15) a
     // tile of each block of 128 rows, 22 (20) of 256, which costs as much as five tiles beside them.  (Measured, in that
     // order: 16 sequences of 4,000 tokens, 8 heads: 68 and 94 us at 32 rows a head, 119 and 96 at 64, 409 and 138 at 256;
-    // 4 of 16,000: 64 and 86, 107 and 88, 366 and 120; 64 of 300: 55 and 78, 99 and 79, 347 and 114.)
+    // 4 of 16,000: 64 and 86, 107 and 88, 366 and 120; 64 of 300: 55 and 78, 99 and 79, 347 and 114.)  Prompts of 16 to 2,000
+    // rows under windows of 256 to 4,096, from their first token on or far behind it, end within 1.23 times the better
+    // kernel's time by the same rule: 4 sequences' last 512 of 2,048 tokens, a window of 1,024 and 64 sinks, 342 and 113 us;
+    // one's last 200 of 3,000 48 and 51, and of 2 heads 17 and 48; D = 64, 8 heads: 36 and 45, where it takes the second.
     int64_t most = static_cast<int64_t>(a.max_pages) << c.page_shift;
     if (a.window > 0) most = std::min<int64_t>(most, static_cast<int64_t>(a.window) + a.sinks + a.max_rows + 2 * kStep);
     const double tiles = static_cast<double>((most + kTile - 1) / kTile), blocks = static_cast<double>(heads * ((rows + 15) / 16));

@@ -31,10 +31,10 @@
 //   line of tiles of all segments (find_place), since segments of 2 to 70 tiles fill 148 SMs badly one to a block (trees:
 //   234 us so, 127 on the line; a part of a segment costs about 10 us beside its tiles: reading queries 4, the first tile's
 //   chain, writing 3).  Their softmax and unpacking warps take 88 registers, from two warps that only make the block whole
-//   warpgroups: with 80 a few words spilled, and as the codes' loads pass through what is left of L1 beside 205 KB of shared
-//   memory, every reload went to L2 (5.3 us a tile of 256 rows where this takes 3.3).  Measured: 16 trees of 25 to 64 nodes
+//   warpgroups: with 80 a few words more spilled, and as the codes' loads pass through what is left of L1 beside 205 KB of shared
+//   memory, every reload went to L2 (5.3 us a tile of 256 rows where this takes 3.3; what still spills is 0.4% of the instructions).  Measured: 16 trees of 25 to 64 nodes
 //   after 100 to 8,192 tokens, 32 heads (8 of the cache), D = 128, 127 us with the join; chunks of 512 rows of 4 sequences up
-//   to 16,000 tokens, a window of 2,048 and 100 sinks, 148 us.  A tile takes 6,300 cycles there, 3,400 of them in the
+//   to 16,000 tokens, a window of 2,048 and 100 sinks, 142 us.  A tile takes 6,300 cycles there, 3,400 of them in the
 //   columns' loops (exponentials alone: 2,048); the rest are its products' and barriers' latencies.  (The next tile's first
 //   scores asked for before the last probabilities are written: 3% slower.)
 // Every wait is bounded; a block that gives up writes NaN rows.
